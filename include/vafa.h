@@ -365,6 +365,53 @@ VAFA_API int vafa_absorb_project_f32_bwd(const float *q_raw, const float *W_Q, c
                                          int64_t D_Q, int64_t D_KV, int64_t D_H, void *workspace,
                                          int64_t workspace_bytes, void *stream);
 
+/* ======================================================================== */
+/* Paged key-value cache (bf16 / fp16).  No counterpart in the reference.   */
+/* ======================================================================== */
+
+/* Keys and values of n_seq sequences in pages: token p of sequence b is token
+ * p % page_size of page page_table[b * table_stride + p / page_size].  k and v are
+ * [n_pages, page_size, Hk, D] with the given strides (in elements, multiples of 8;
+ * features contiguous, 16-byte aligned).  page_table (table_width entries a row) and
+ * cache_lens [n_seq] are device int32.  Entries outside [0, n_pages) and positions
+ * outside the table are neither read nor written. */
+typedef struct vafa_paged_cache {
+  void *k, *v;
+  int64_t n_pages, page_size, Hk, D;
+  int64_t k_page, k_token, k_head;
+  int64_t v_page, v_token, v_head;
+  const int32_t *page_table;
+  int64_t table_stride, table_width;
+  const int32_t *cache_lens;
+  int64_t n_seq;
+} vafa_paged_cache;
+
+/* Appends T tokens: token t of sequence b (cu[b] <= t < cu[b + 1]; cu NULL: t = b,
+ * T = n_seq) goes to position cache_lens[b] + t - cu[b].  k and v are [T, Hk, D] and
+ * q [T, H, D] (H = 0: none) with strides in elements, multiples of 8.  inv_freq
+ * [rot / 2] (device fp32; rot even, at most D; 0: no rotation): the feature pairs
+ * (i, i + rot / 2), or (2i, 2i + 1) if interleaved, of k and q turn by position *
+ * inv_freq[i].  Rotated k and v go to the cache, rotated q to q_out [T, H, D].  Tokens
+ * at or past cu[n_seq] are not stored, their rows of q_out are zeros. */
+VAFA_API int vafa_paged_append(const vafa_paged_cache *cache, const void *k, int64_t k_token,
+                               int64_t k_head, const void *v, int64_t v_token, int64_t v_head,
+                               int64_t T, const int32_t *cu, const void *q, int64_t q_token,
+                               int64_t q_head, int64_t H, void *q_out, const float *inv_freq,
+                               int64_t rot, int32_t interleaved, int32_t dtype, void *stream);
+
+/* Attention of one new token per sequence, q [n_seq, H, D] (strides in elements,
+ * multiples of 8) -> out [n_seq, H, D], over the first cache_lens[b] tokens of its
+ * pages (the last `window` of them; 0: all): H / Hk query heads share a key head, D in
+ * {64, 128, 256}.  Scores are scale q.k, then softcap tanh(. / softcap) (0: none), then
+ * minus slopes[h] (device fp32 [H] or NULL) times the key's distance from the last
+ * token.  A sequence without keys gets zeros. */
+VAFA_API int64_t vafa_paged_decode_workspace(const vafa_paged_cache *cache, int64_t H,
+                                             int64_t window);
+VAFA_API int vafa_paged_decode(const vafa_paged_cache *cache, const void *q, int64_t q_token,
+                               int64_t q_head, int64_t H, void *out, float scale, float softcap,
+                               int64_t window, const float *slopes, int32_t dtype,
+                               void *workspace, int64_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

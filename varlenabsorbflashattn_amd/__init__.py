@@ -6,11 +6,15 @@ Drop-in replacements for the reference packages' public APIs:
 * ``triton_target_attn_absorb``: :func:`packed_target_attn`,
   :func:`target_attn_inner`, :func:`prepare_target_attn_indices`
 
+Beside them, for language models: :func:`paged_kv_append` and :func:`paged_decode_attn`
+(a paged key-value cache and the attention of one new token over it).
+
 All compute runs in the in-tree HIP library ``libvafa.so`` (C ABI in
 ``include/vafa.h``); it is loaded on the first call.
 """
 from .varlen import packed_varlen_attn, set_validate_cu_seqlens
 from .absorb import packed_target_attn, prepare_target_attn_indices, target_attn_inner
+from .paged import paged_decode_attn, paged_kv_append
 
 __all__ = [
     "packed_varlen_attn",
@@ -18,5 +22,7 @@ __all__ = [
     "packed_target_attn",
     "prepare_target_attn_indices",
     "target_attn_inner",
+    "paged_kv_append",
+    "paged_decode_attn",
 ]
 __version__ = "0.1.0"

@@ -44,6 +44,14 @@ class PlanInfo(C.Structure):
         "off_fcomb", "n_fcomb", "n_fpart_rows", "max_fcomb_rows", "xcd_heads")]
 
 
+class PagedCache(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p)] + [(n, C.c_int64) for n in (
+        "n_pages", "page_size", "Hk", "D", "k_page", "k_token", "k_head",
+        "v_page", "v_token", "v_head")] + [
+        ("page_table", C.c_void_p), ("table_stride", C.c_int64), ("table_width", C.c_int64),
+        ("cache_lens", C.c_void_p), ("n_seq", C.c_int64)]
+
+
 _lib = None
 _lock = threading.Lock()
 
@@ -53,6 +61,7 @@ _I32 = C.c_int32
 _PI64 = C.POINTER(C.c_int64)
 _PI32 = C.POINTER(C.c_int32)
 _PINFO = C.POINTER(PlanInfo)
+_PCACHE = C.POINTER(PagedCache)
 
 _SIGS = {
     "vafa_version": (C.c_char_p, []),
@@ -102,6 +111,11 @@ _SIGS = {
     "vafa_absorb_fwd_full_workspace": (C.c_int64, [_PINFO, _I64, _I64, _I64]),
     "vafa_absorb_fwd_full": (C.c_int, [_P, _P, _P, _P, _P, _P, _P, _P, _I64, _P, _PINFO, _I64,
                                        _I64, _I64, _I32, C.c_float, _P, _I64, _P]),
+    "vafa_paged_append": (C.c_int, [_PCACHE, _P, _I64, _I64, _P, _I64, _I64, _I64, _P, _P, _I64,
+                                    _I64, _I64, _P, _P, _I64, _I32, _I32, _P]),
+    "vafa_paged_decode_workspace": (C.c_int64, [_PCACHE, _I64, _I64]),
+    "vafa_paged_decode": (C.c_int, [_PCACHE, _P, _I64, _I64, _I64, _P, C.c_float, C.c_float, _I64,
+                                    _P, _I32, _P, _I64, _P]),
 }
 
 EXPORTED = tuple(_SIGS)

@@ -4,6 +4,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include "paged.h"
+
 namespace vafa {
 
 // Lets kernel `fn` be launched with `bytes` of dynamic LDS (above the 64 KB
@@ -105,6 +107,34 @@ struct AbsorbArgs {
   float scale;
 };
 
+// Tokens appended to a paged cache; strides in elements.
+struct AppendArgs {
+  const void *q, *k, *v;  // q: null where H is 0
+  void *q_out, *kc, *vc;
+  const int32_t *cu, *lens;  // cu null: one token per sequence
+  const float *inv_freq;
+  PageMap map;
+  int64_t q_token, q_head, k_token, k_head, v_token, v_head;
+  int64_t k_page, kc_token, kc_head, v_page, vc_token, vc_head;
+  int64_t T;
+  int n_seq, H, Hk, D, rot, interleaved;
+};
+
+// Attention of one new token per sequence over a paged cache.
+struct DecodeArgs {
+  const void *q, *kc, *vc;
+  void *out;
+  const int32_t *lens;
+  const float *slopes;  // or null
+  float *part_o, *part_ml;  // pieces: [slots, 16, D] and [slots, 16, 2]
+  PageMap map;
+  int64_t q_token, q_head;
+  int64_t k_page, kc_token, kc_head, v_page, vc_token, vc_head;
+  int64_t capacity;  // tokens of a sequence's pages
+  int n_seq, H, G, pairs, head_blocks, window;  // window 0: all keys
+  float c, cap2;  // factor on q.k, and cap log2 e (0: none), see paged.hip
+};
+
 // varlen_f32.hip: fp32 varlen on fp32 matrix cores
 bool f32_varlen_mfma_d(int D);      // D in {32, 64, 128, 256}
 bool f32_varlen_bwd_mfma_d(int D);  // D in {32, 64, 128}
@@ -167,6 +197,10 @@ void launch_du_combine(const AbsorbArgs &, hipStream_t);
 // dAX = dO W_V^T, fp32 [T_q, H, F]
 template <typename T>
 void launch_absorb_dax(const AbsorbArgs &, hipStream_t);
+
+// paged.hip (bf16 / f16)
+template <typename T> void launch_paged_append(const AppendArgs &, hipStream_t);
+template <typename T> void launch_paged_decode(const DecodeArgs &, int D, int grid, hipStream_t);
 
 // varlen_mfma.hip (bf16 / f16, D in {32, 64, 128, 256})
 template <typename T, int D> void launch_mfma_varlen_fwd(const VarlenArgs &, hipStream_t);

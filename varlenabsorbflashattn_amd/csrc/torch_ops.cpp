@@ -32,7 +32,8 @@ struct Api {
   X(absorb_bwd) X(absorb_fwd_full_workspace) X(absorb_fwd_full) X(absorb_bwd_full)        \
   X(absorb_bwd_full_workspace)                                                            \
   X(absorb_project_workspace) X(absorb_project_fwd) X(absorb_project_bwd)                 \
-  X(absorb_project_f32_workspace) X(absorb_project_f32_fwd) X(absorb_project_f32_bwd)
+  X(absorb_project_f32_workspace) X(absorb_project_f32_fwd) X(absorb_project_f32_bwd)      \
+  X(paged_append) X(paged_decode_workspace) X(paged_decode)
   VAFA_FNS(VAFA_FN)
 #undef VAFA_FN
 } api;
@@ -246,6 +247,170 @@ absorb_full_bwd(const Tensor &q_raw, const Tensor &W_Q, const Tensor &W_K, const
   return {opt(dq), dX, opt(dwq), opt(dwk), dW_V};
 }
 
+// ---- paged cache: argument checks here, where a call of a few us can afford them ----
+
+void need(bool ok, const char *what, const char *msg) {
+  if (!ok) throw AssertionFailed(std::string(what) + ": " + msg);
+}
+
+// The stride of a dimension as the kernels use it: one of size 1 is never stepped over.
+int64_t stride_of(const Tensor &t, int64_t dim) { return t.size(dim) > 1 ? t.stride(dim) : 0; }
+
+bool rows_ok(const Tensor &t) {
+  bool ok = stride_of(t, t.dim() - 1) <= 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+  for (int64_t d = 0; d + 1 < t.dim(); ++d) ok = ok && stride_of(t, d) % 8 == 0;
+  return ok;
+}
+
+// [T, H, D] as the kernels read it (any token and head stride of whole 16 bytes);
+// other layouts are copied.
+Tensor rows_in(const Tensor &t) {
+  return rows_ok(t) ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+
+void no_grad_only(const char *what, std::initializer_list<Tensor> ts) {
+  if (!at::GradMode::is_enabled()) return;
+  for (const Tensor &t : ts)
+    if (t.defined() && t.requires_grad())
+      throw py::value_error(std::string(what) +
+                            " has no backward: call it under torch.no_grad() or detach its inputs");
+}
+
+vafa_paged_cache cache_of(const char *what, const Tensor &kc, const Tensor &vc,
+                          const Tensor &table, const Tensor &lens) {
+  need(kc.dim() == 4 && vc.sizes() == kc.sizes(), what,
+       "k_cache and v_cache must be [n_pages, page_size, H_k, D] alike");
+  const auto dt = kc.scalar_type();
+  need(dt == at::kHalf || dt == at::kBFloat16, what, "dtype not supported (float16, bfloat16)");
+  need(vc.scalar_type() == dt, what, "k_cache and v_cache must share dtype");
+  need(table.dim() == 2 && lens.dim() == 1 && table.size(0) == lens.size(0), what,
+       "page_table must be [n_seq, pages] and cache_lens [n_seq]");
+  need(table.scalar_type() == at::kInt && lens.scalar_type() == at::kInt, what,
+       "page_table and cache_lens must be int32");
+  need(kc.is_cuda() && vc.device() == kc.device() && table.device() == kc.device() &&
+           lens.device() == kc.device(),
+       what, "requires GPU tensors on one device");
+  if (stride_of(table, 1) > 1 || stride_of(lens, 0) > 1)
+    throw py::value_error(std::string(what) +
+                          ": the rows of page_table and cache_lens must be contiguous");
+  if (!rows_ok(kc) || !rows_ok(vc))
+    throw py::value_error(std::string(what) +
+                          ": the caches must be 16-byte aligned, features contiguous and other "
+                          "strides multiples of 8 elements");
+  for (const Tensor *t : {&kc, &vc})
+    for (int64_t d = 0; d < 4; ++d)
+      if (t->size(d) > 1 && t->stride(d) == 0)
+        throw py::value_error(std::string(what) + ": the caches must not be expanded views");
+  vafa_paged_cache c{};
+  c.k = kc.data_ptr(); c.v = vc.data_ptr();
+  c.n_pages = kc.size(0); c.page_size = kc.size(1); c.Hk = kc.size(2); c.D = kc.size(3);
+  c.k_page = stride_of(kc, 0); c.k_token = stride_of(kc, 1); c.k_head = stride_of(kc, 2);
+  c.v_page = stride_of(vc, 0); c.v_token = stride_of(vc, 1); c.v_head = stride_of(vc, 2);
+  c.page_table = table.data_ptr<int32_t>();
+  c.table_stride = stride_of(table, 0); c.table_width = table.size(1);
+  c.cache_lens = lens.data_ptr<int32_t>(); c.n_seq = lens.size(0);
+  return c;
+}
+
+// [T, heads, D] of the cache's type and device.
+void check_tokens(const char *what, const char *name, const Tensor &t, const Tensor &kc) {
+  if (t.dim() != 3 || t.size(2) != kc.size(3))
+    throw AssertionFailed(std::string(what) + ": " + name + " must be [T, heads, " +
+                          std::to_string(kc.size(3)) + "]");
+  if (t.scalar_type() != kc.scalar_type() || t.device() != kc.device())
+    throw AssertionFailed(std::string(what) + ": " + name +
+                          " must have the cache's dtype and device");
+}
+
+std::optional<Tensor> paged_append(const Tensor &k_in, const Tensor &v_in, const Tensor &kc,
+                                   const Tensor &vc, const Tensor &table, const Tensor &lens,
+                                   const std::optional<Tensor> &cu,
+                                   const std::optional<Tensor> &q_in,
+                                   const std::optional<Tensor> &inv_freq, bool interleaved) {
+  const char *what = "paged_kv_append";
+  no_grad_only(what, {k_in, v_in, kc, vc, q_in.value_or(Tensor()), inv_freq.value_or(Tensor())});
+  const vafa_paged_cache c = cache_of(what, kc, vc, table, lens);
+  check_tokens(what, "k", k_in, kc);
+  check_tokens(what, "v", v_in, kc);
+  need(k_in.size(1) == c.Hk && v_in.sizes() == k_in.sizes(), what,
+       "k and v must be [T, H_k, D] with the cache's heads");
+  const int64_t T = k_in.size(0);
+  if (cu) {
+    need(cu->dim() == 1 && cu->size(0) == c.n_seq + 1, what, "cu_seqlens must be [n_seq + 1]");
+    need(cu->scalar_type() == at::kInt && cu->device() == kc.device(), what,
+         "cu_seqlens must be int32 on the cache's device");
+    if (stride_of(*cu, 0) > 1)
+      throw py::value_error(std::string(what) + ": cu_seqlens must be contiguous");
+  } else {
+    need(T == c.n_seq, what, "without cu_seqlens there must be one token per sequence");
+  }
+  int64_t rot = 0;
+  if (inv_freq) {
+    need(inv_freq->dim() == 1 && 2 * inv_freq->size(0) <= c.D, what,
+         "inv_freq must be [rotated features / 2]");
+    need(inv_freq->scalar_type() == at::kFloat && inv_freq->device() == kc.device(), what,
+         "inv_freq must be float32 on the cache's device");
+    if (stride_of(*inv_freq, 0) > 1)
+      throw py::value_error(std::string(what) + ": inv_freq must be contiguous");
+    rot = 2 * inv_freq->size(0);
+  }
+  int64_t H = 0;
+  if (q_in) {
+    check_tokens(what, "q", *q_in, kc);
+    need(q_in->size(0) == T, what, "q must have as many tokens as k");
+    H = q_in->size(1);
+  }
+  Call call(kc);
+  const Tensor k = rows_in(k_in), v = rows_in(v_in);
+  Tensor q, out;
+  if (q_in) {
+    q = rows_in(*q_in);
+    out = call.empty({T, H, c.D});
+  }
+  check(api.paged_append(&c, ptr(k), stride_of(k, 0), stride_of(k, 1), ptr(v), stride_of(v, 0),
+                         stride_of(v, 1), T, cu ? cu->data_ptr<int32_t>() : nullptr, ptr(q),
+                         q_in ? stride_of(q, 0) : 0, q_in ? stride_of(q, 1) : 0, H, ptr(out),
+                         inv_freq ? f32(*inv_freq) : nullptr, rot, interleaved, dtype_of(kc),
+                         call.stream));
+  for (const Tensor *t : {&kc, &vc})
+    if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+  return q_in ? std::optional<Tensor>(out) : std::nullopt;
+}
+
+// slopes [H] of the distance bias, float32 on q's device.
+const float *slopes_of(const char *what, const std::optional<Tensor> &slopes, int64_t H,
+                       const Tensor &q) {
+  if (!slopes) return nullptr;
+  need(slopes->dim() == 1 && slopes->size(0) == H, what, "alibi_slopes must be [H]");
+  need(slopes->scalar_type() == at::kFloat && slopes->device() == q.device(), what,
+       "alibi_slopes must be float32 on q's device");
+  if (stride_of(*slopes, 0) > 1)
+    throw py::value_error(std::string(what) + ": alibi_slopes must be contiguous");
+  return f32(*slopes);
+}
+
+Tensor paged_decode(const Tensor &q_in, const Tensor &kc, const Tensor &vc, const Tensor &table,
+                    const Tensor &lens, double scale, std::optional<double> softcap,
+                    std::optional<int64_t> window, const std::optional<Tensor> &slopes) {
+  const char *what = "paged_decode_attn";
+  no_grad_only(what, {q_in, kc, vc, slopes.value_or(Tensor())});
+  if (softcap && !(*softcap > 0)) throw py::value_error("softcap must be positive");
+  if (window && *window < 1) throw py::value_error("window must be positive");
+  const vafa_paged_cache c = cache_of(what, kc, vc, table, lens);
+  check_tokens(what, "q", q_in, kc);
+  need(q_in.size(0) == c.n_seq, what, "q must hold one token per sequence");
+  const int64_t H = q_in.size(1);
+  const float *sl = slopes_of(what, slopes, H, q_in);
+  Call call(kc);
+  const Tensor q = rows_in(q_in);
+  Tensor out = call.empty({c.n_seq, H, c.D});
+  void *ws = call.workspace(api.paged_decode_workspace(&c, H, window.value_or(0)));
+  check(api.paged_decode(&c, ptr(q), stride_of(q, 0), stride_of(q, 1), H, ptr(out), (float)scale,
+                         (float)softcap.value_or(0.0), window.value_or(0), sl, dtype_of(kc), ws,
+                         call.ws_bytes(), call.stream));
+  return out;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -271,4 +436,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("absorb_full_bwd", &absorb_full_bwd, no_gil);
   m.def("project_fwd", &project_fwd, no_gil);
   m.def("project_bwd", &project_bwd, no_gil);
+  m.def("paged_append", &paged_append, no_gil);
+  m.def("paged_decode", &paged_decode, no_gil);
 }
