@@ -91,7 +91,7 @@ VAFA_API int vafa_chunk_indices(const int64_t *cu, int64_t n1, int32_t BT, int32
 
 typedef struct vafa_plan_info {
   int64_t magic;          /* VAFA_PLAN_MAGIC */
-  int64_t kind;           /* 1 = varlen, 2 = absorb */
+  int64_t kind;           /* 1 = varlen, 2 = absorb, 3 = masked varlen */
   int64_t n_seg;
   int64_t T_q, T_k, H;
   /* section offsets (in int32 units from the plan start) and item counts */
@@ -153,6 +153,17 @@ VAFA_API int vafa_plan_varlen_balanced(const int64_t *cu_q, const int64_t *cu_k,
 VAFA_API int vafa_plan_absorb(const int64_t *cu_q, const int64_t *cu_k, int64_t n1, int64_t H,
                      int64_t D_KV, int64_t D_H, int32_t *plan, int64_t plan_cap,
                      vafa_plan_info *info);
+
+/* Plan for packed_masked_attn (no counterpart in the reference): H query heads on Hk
+ * key heads.  causal: query i of a segment with nq queries and nk keys has position
+ * p = i + nk - nq and sees key j where j <= p and j > p - window (window 0: no bound),
+ * or j < prefix[segment] (prefix: host int64 [n1 - 1] or NULL).  Not causal: every key
+ * (window 0, prefix NULL).  At most 2^30 tokens.  The same format, kind 3; xcd_heads
+ * holds the parts into which the dK/dV pass divides a key head's query heads. */
+VAFA_API int vafa_plan_masked(const int64_t *cu_q, const int64_t *cu_k, const int64_t *prefix,
+                              int64_t n1, int64_t H, int64_t Hk, int64_t D, int32_t causal,
+                              int64_t window, int32_t *plan, int64_t plan_cap,
+                              vafa_plan_info *info);
 
 /* ======================================================================== */
 /* Device entry points.  plan_dev is the plan copied to device memory.      */
@@ -364,6 +375,31 @@ VAFA_API int vafa_absorb_project_f32_bwd(const float *q_raw, const float *W_Q, c
                                          float *dW_Q, float *dW_K, int64_t T_q, int64_t H,
                                          int64_t D_Q, int64_t D_KV, int64_t D_H, void *workspace,
                                          int64_t workspace_bytes, void *stream);
+
+/* ======================================================================== */
+/* Packed attention with masks, capped scores and distance biases (bf16 /   */
+/* fp16, D in {64, 128, 256}).  No counterpart in the reference.            */
+/* ======================================================================== */
+
+/* q [T_q,H,D], k/v [T_k,Hk,D] contiguous and 16-byte aligned -> o [T_q,H,D],
+ * lse [T_q,H] fp32 log2-domain, under a plan of vafa_plan_masked made with the same H,
+ * Hk, D and window.  Scores are scale q.k, then softcap tanh(. / softcap) (0: none),
+ * then minus slopes[h] (device fp32 [H] or NULL) times |position of the query - key|.
+ * Rows that see no key get zeros (lse -inf). */
+VAFA_API int64_t vafa_masked_fwd_workspace(const vafa_plan_info *info, int64_t D);
+VAFA_API int vafa_masked_fwd(const void *q, const void *k, const void *v, void *o, float *lse,
+                             const int32_t *plan_dev, const vafa_plan_info *info, int64_t Hk,
+                             int64_t D, int32_t dtype, float scale, float softcap, int64_t window,
+                             const float *slopes, void *workspace, int64_t workspace_bytes,
+                             void *stream);
+/* dO [T_q,H,D] -> dq, dk, dv.  Deterministic (no atomics). */
+VAFA_API int64_t vafa_masked_bwd_workspace(const vafa_plan_info *info, int64_t Hk, int64_t D);
+VAFA_API int vafa_masked_bwd(const void *q, const void *k, const void *v, const void *o,
+                             const void *dout, const float *lse, void *dq, void *dk, void *dv,
+                             const int32_t *plan_dev, const vafa_plan_info *info, int64_t Hk,
+                             int64_t D, int32_t dtype, float scale, float softcap, int64_t window,
+                             const float *slopes, void *workspace, int64_t workspace_bytes,
+                             void *stream);
 
 /* ======================================================================== */
 /* Paged key-value cache (bf16 / fp16).  No counterpart in the reference.   */

@@ -1,0 +1,326 @@
+"""Packed attention under a mask on the GPU against the 64-bit oracle, whose bounds count
+the roundings element by element (oracle/masked.py)."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import masked as om
+from varlenabsorbflashattn_amd import (packed_masked_attn, packed_varlen_attn, paged_decode_attn,
+                                       paged_kv_append, set_validate_cu_seqlens)
+from varlenabsorbflashattn_amd.workloads import cu_from_lens
+
+pytestmark = pytest.mark.gpu
+
+U = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+A = {torch.bfloat16: 0.0, torch.float16: 2.0 ** -25}
+BF, HF = torch.bfloat16, torch.float16
+
+
+def f64(t):
+    return None if t is None else t.detach().double().cpu().numpy()
+
+
+def within(name, out, ref, bound):
+    o = f64(out)
+    assert o.shape == ref.shape and np.isfinite(o).all(), name
+    d = np.abs(o - ref)
+    worst = float((d / np.maximum(bound, 1e-300)).max()) if d.size else 0.0
+    print(f"  {name:3s} max {d.max() if d.size else 0.0:.3e}, {worst:.2f} of the bound", flush=True)
+    assert (d <= bound).all(), f"{name}: {worst} times the bound"
+
+
+def inputs(case, ql, kl, H, Hk, D, dt, device, big=1.0):
+    g = torch.Generator(device=device).manual_seed(case)
+
+    def rnd(*s):
+        return torch.randn(*s, generator=g, device=device)
+    q = (big * rnd(sum(ql), H, D)).to(dt)
+    return q, rnd(sum(kl), Hk, D).to(dt), rnd(sum(kl), Hk, D).to(dt), rnd(sum(ql), H, D).to(dt)
+
+
+def step(q, k, v, do, ql, kl, **kw):
+    """(o, dq, dk, dv) of one forward and backward."""
+    x = [t.detach().requires_grad_(True) for t in (q, k, v)]
+    o = packed_masked_attn(*x, cu_seqlens_q=cu_from_lens(ql), cu_seqlens_k=cu_from_lens(kl), **kw)
+    return (o.detach(), *torch.autograd.grad(o, x, do))
+
+
+def compare(got, q, k, v, do, ql, kl, *, scale=None, causal=True, window=None, prefix_lens=None,
+            softcap=None, alibi_slopes=None):
+    ref = om.attention(f64(q), f64(k), f64(v), f64(do), np.cumsum([0] + ql), np.cumsum([0] + kl),
+                       scale if scale is not None else 1 / math.sqrt(q.shape[-1]), causal, window,
+                       prefix_lens, softcap, f64(alibi_slopes), U[q.dtype], A[q.dtype])
+    for (n, (val, bound)), out in zip(ref.items(), got):
+        within(n, out, val, bound)
+
+
+CASES = [
+    # q lens, k lens (None: the same), H, Hk, D, dtype, options
+    ([1], None, 1, 1, 64, BF, {}),
+    ([5, 0, 300, 129, 1], None, 4, 2, 64, BF, {}),
+    ([64, 63, 65, 128, 127, 257], None, 4, 4, 128, HF, {}),
+    ([33, 200], None, 6, 1, 256, BF, {}),
+    ([5, 40, 7, 3], [1, 900, 0, 3], 4, 4, 128, BF, {}),                 # rows without keys
+    ([17, 500], [1000, 700], 8, 2, 128, BF, {"window": 50}),
+    ([300, 33, 1], [300, 500, 2000], 4, 2, 256, HF, {"window": 64, "prefix_lens": [100, 500, 3]}),
+    ([260, 10, 140], [300, 10, 140], 3, 3, 64, BF, {"prefix_lens": [300, 0, 77]}),
+    ([130, 1, 40], [70, 900, 40], 4, 2, 128, HF, {"causal": False}),
+    ([200, 31], None, 10, 2, 128, BF, {"softcap": 5.0}),
+    ([200, 31], None, 4, 2, 256, BF, {"softcap": 30.0, "window": 100}),
+    ([200, 31], None, 5, 1, 64, HF, {"softcap": 1.0}),
+    ([150, 77], [150, 200], 12, 12, 64, BF, {"alibi": True}),
+    ([150, 77], [150, 200], 3, 1, 128, HF, {"alibi": True, "prefix_lens": [40, 200]}),
+    ([150, 77], [150, 200], 4, 4, 256, BF, {"alibi": True, "softcap": 20.0, "window": 33}),
+    ([90, 20], None, 4, 2, 128, BF, {"alibi": True, "softcap": 20.0, "causal": False}),
+    ([90, 20], None, 4, 2, 64, BF, {"scale": -0.3}),
+    ([90, 20], None, 2, 2, 128, HF, {"scale": -0.3, "window": 7}),
+    ([90, 20], None, 2, 1, 128, BF, {"scale": -0.3, "softcap": 2.0}),
+    ([90, 20], None, 2, 1, 64, BF, {"scale": 0.0}),
+    ([70, 9], None, 2, 1, 64, BF, {"window": 1}),                       # itself alone
+    ([3, 1], [6000, 2500], 2, 1, 64, BF, {}),                           # split keys
+    ([40, 16], [5000, 3000], 4, 1, 128, BF, {"window": 1500, "prefix_lens": [700, 0]}),
+    ([100], [4000], 1, 1, 256, HF, {"softcap": 10.0, "alibi": True}),
+    ([1] * 40, [1] * 40, 2, 2, 64, BF, {}),
+    ([600, 700], None, 16, 8, 128, BF, {}),
+]
+
+
+def options(kw, H, device):
+    kw = dict(kw)
+    if kw.pop("alibi", False):
+        kw["alibi_slopes"] = torch.tensor([2.0 ** (-8 * (h + 1) / H) for h in range(H)],
+                                          device=device)
+    if "prefix_lens" in kw:
+        kw["prefix_lens"] = torch.tensor(kw["prefix_lens"], dtype=torch.int32)
+    return kw
+
+
+@pytest.mark.parametrize("case", range(len(CASES)))
+def test_forward_and_backward(device, case):
+    ql, kl, H, Hk, D, dt, opts = CASES[case]
+    kl = kl or ql
+    print(f"[masked] q={ql[:6]} k={kl[:6]} H={H}/{Hk} D={D} {dt} {opts}", flush=True)
+    x = inputs(case, ql, kl, H, Hk, D, dt, device)
+    kw = options(opts, H, device)
+    got = step(*x, ql, kl, **kw)
+    torch.cuda.synchronize()
+    if "prefix_lens" in kw:
+        kw["prefix_lens"] = kw["prefix_lens"].numpy()
+    compare(got, *x, ql, kl, **kw)
+
+
+def test_gradients_against_differences(device):
+    """The gradients of the calls themselves: f(x + e) - f(x - e) in 64 bits from the
+    oracle moves as the GPU's gradients say."""
+    ql, kl, H, Hk, D = [20], [23], 4, 2, 64
+    print("[masked differences]", flush=True)
+    x = inputs(50, ql, kl, H, Hk, D, HF, device)
+    kw = {"softcap": 3.0, "window": 9, "prefix_lens": torch.tensor([4])}
+    got = step(*x, ql, kl, **kw)
+    h = [f64(t) for t in x]
+    g = np.random.default_rng(0)
+    for i, name in enumerate(("dq", "dk", "dv")):
+        e = g.standard_normal(h[i].shape)
+        f = []
+        for sign in (1, -1):
+            y = list(h[:3])
+            y[i] = y[i] + sign * 1e-5 * e
+            o = om.attention(*y, None, [0, 20], [0, 23], 0.125, window=9, prefix=[4], softcap=3.0)
+            f.append((o["o"][0] * h[3]).sum())
+        slope, along = (f[0] - f[1]) / 2e-5, (f64(got[1 + i]) * e).sum()
+        # some 1e3 values with independent errors of a few 2^-11 of their size
+        size = np.linalg.norm(f64(got[1 + i]) * e)
+        print(f"  {name}: {along:.5f} against {slope:.5f}, norm {size:.3f}", flush=True)
+        assert abs(along - slope) <= 8 * 2.0 ** -11 * size
+
+
+def test_large_scores(device):
+    """One-hot rows: scores in the hundreds, where every other probability underflows."""
+    ql = [130, 40]
+    print("[masked large]", flush=True)
+    q, k, v, do = inputs(51, ql, ql, 4, 2, 64, BF, device, big=40.0)
+    with torch.no_grad():
+        o = packed_masked_attn(q, k, v, cu_seqlens_q=cu_from_lens(ql),
+                               cu_seqlens_k=cu_from_lens(ql), scale=1.0)
+    ref = om.attention(f64(q), f64(k), f64(v), None, np.cumsum([0] + ql), np.cumsum([0] + ql), 1.0,
+                       u=U[BF])
+    # scores of up to 2000 summed in fp32 over 64 products: P off by up to 2^-7
+    val, bound = ref["o"]
+    within("o", o, val, bound + 2.0 ** -7 * np.abs(f64(v)).max())
+
+
+def test_not_causal_equals_packed_varlen(device):
+    """Without the causal mask it is packed_varlen_attn, within both operators' roundings;
+    shapes, layouts and lengths given as that operator takes them."""
+    ql, kl = [40, 7], [300, 64]
+    print("[masked varlen]", flush=True)
+    q, k, v, do = inputs(52, ql, kl, 4, 4, 64, BF, device)
+    info = {"q_seqinfo": torch.tensor(ql, device=device), "k_seqinfo": torch.tensor(kl, device=device)}
+    a = packed_masked_attn(q[None], k[None], v[None], causal=False, **info)
+    b = packed_varlen_attn(q[None], k[None], v[None], **info)
+    assert a.shape == b.shape == (1, 47, 4, 64)
+    ref = om.attention(f64(q), f64(k), f64(v), None, np.cumsum([0] + ql), np.cumsum([0] + kl), 0.125,
+                       False, u=U[BF])["o"]
+    within("o", a[0], *ref)
+    within("o", b[0], *ref)
+    # parts of a joint projection, and unaligned rows
+    qkv = torch.randn(47, 12, 64, device=device).to(BF)
+    views = qkv[:, :4], qkv[:, 4:8], qkv[:, 8:]
+    kw = {"cu_seqlens_q": cu_from_lens(ql).to(device), "cu_seqlens_k": cu_from_lens(ql).to(device)}
+    want = packed_masked_attn(*(t.contiguous() for t in views), **kw)
+    assert torch.equal(packed_masked_attn(*views, **kw), want)
+    flat = torch.zeros(47 * 4 * 64 + 1, device=device, dtype=BF)
+    flat[1:] = views[0].flatten()
+    assert torch.equal(packed_masked_attn(flat[1:].view(47, 4, 64), *views[1:], **kw), want)
+
+
+def test_results_repeat(device):
+    """The same bits from call to call, on another stream, and through calls of other
+    lengths in between."""
+    ql, kl = [500, 3, 130], [700, 3000, 130]
+    print("[masked repeat]", flush=True)
+    x = inputs(53, ql, kl, 8, 2, 128, BF, device)
+    first = step(*x, ql, kl, window=600)
+    step(*(t[:200] for t in x), [200], [200])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = step(*x, ql, kl, window=600)
+    again = step(*x, ql, kl, window=600)
+    torch.cuda.synchronize()
+    for a, b, c in zip(first, other, again):
+        assert torch.equal(a, b) and torch.equal(a, c)
+
+
+def test_rows_behind_the_last_segment(device):
+    """With validation off, lengths may cover fewer rows than there are: zeros there."""
+    print("[masked rest]", flush=True)
+    ql = [30, 20]
+    q, k, v, do = inputs(54, [70], [70], 2, 1, 64, BF, device)
+    bad = torch.tensor(float("nan"), device=device).to(BF)
+    q[50:], k[50:], v[50:], do[50:] = bad, bad, bad, bad
+    set_validate_cu_seqlens(False)
+    try:
+        got = step(q, k, v, do, ql, ql)
+    finally:
+        set_validate_cu_seqlens(True)
+    compare([t[:50] for t in got], q[:50], k[:50], v[:50], do[:50], ql, ql)
+    assert not any(t[50:].any() for t in got)
+    with pytest.raises(ValueError, match="must equal total tokens"):
+        step(q, k, v, do, ql, ql)
+
+
+def test_empty_calls(device):
+    print("[masked empty]", flush=True)
+    q = torch.zeros(0, 2, 64, device=device, dtype=BF, requires_grad=True)
+    k = torch.ones(5, 1, 64, device=device, dtype=BF, requires_grad=True)
+    o = packed_masked_attn(q, k, k, cu_seqlens_q=torch.tensor([0, 0]),
+                           cu_seqlens_k=torch.tensor([0, 5]))
+    o.sum().backward()
+    assert o.shape == q.shape and not k.grad.any()
+    q = torch.ones(4, 2, 64, device=device, dtype=BF, requires_grad=True)
+    k = torch.zeros(0, 1, 64, device=device, dtype=BF, requires_grad=True)
+    o = packed_masked_attn(q, k, k, cu_seqlens_q=torch.tensor([0, 4]),
+                           cu_seqlens_k=torch.tensor([0, 0]))
+    o.sum().backward()
+    assert not o.any() and not q.grad.any() and k.grad.shape == k.shape
+
+
+def test_training_step_under_graph_capture(device):
+    """Forward and backward of two lengths in two graphs, replayed alternately with new
+    values; eager work on tensors of its own in between."""
+    print("[masked graph]", flush=True)
+    g = torch.Generator(device=device).manual_seed(55)
+    shapes = [([200, 7, 64], 4, 2, 64, {"softcap": 8.0}), ([90, 300], 4, 1, 128, {"window": 70})]
+    state = []
+    for ql, H, Hk, D, kw in shapes:
+        x = [torch.zeros(sum(ql), n, D, device=device, dtype=BF) for n in (H, Hk, Hk, H)]
+        state.append((x, ql, kw))
+        for t in x:
+            t.copy_(torch.randn(t.shape, generator=g, device=device))
+    graphs = []
+    for x, ql, kw in state:
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            for _ in range(2):
+                step(*x, ql, ql, **kw)
+        torch.cuda.current_stream().wait_stream(side)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step(*x, ql, ql, **kw)
+        graphs.append((graph, out))
+    for i in range(6):
+        (x, ql, kw), (graph, out) = state[i % 2], graphs[i % 2]
+        for t in x:
+            t.copy_(torch.randn(t.shape, generator=g, device=device))
+        want = step(*(t.clone() for t in x), ql, ql, **kw)
+        torch.cuda.synchronize()
+        for t in out:
+            t.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(out, want):
+            assert torch.equal(a, b), i
+
+
+@pytest.mark.parametrize("opts", [{}, {"softcap": 10.0, "window": 40}, {"alibi": True}])
+def test_decode_after_append_matches_the_packed_pass(device, opts):
+    """A prompt through the packed attention and into the cache, then tokens one at a time:
+    the last rows of the packed pass over the whole sequences, within both bounds."""
+    print(f"[masked + paged] {opts}", flush=True)
+    H, Hk, D, page, prompt, new = 8, 2, 128, 16, [37, 100, 1], 4
+    kw = options(opts, H, device)
+    total = [n + new for n in prompt]
+    cu, cu_p = cu_from_lens(total), cu_from_lens(prompt)
+    g = torch.Generator(device=device).manual_seed(56)
+    qkv = torch.randn(sum(total), H + 2 * Hk, D, generator=g, device=device).to(BF)
+    inv = (10000.0 ** (-torch.arange(0, D, 2) / D)).float().to(device)
+    pages = [-(-n // page) for n in total]
+    table = torch.full((3, max(pages)), -1, dtype=torch.int32)
+    order, at = torch.randperm(sum(pages)).int(), 0
+    for b, n in enumerate(pages):
+        table[b, :n] = order[at:at + n]
+        at += n
+    table = table.to(device)
+
+    def caches():
+        return [torch.full((sum(pages), page, Hk, D), float("nan"), device=device).to(BF)
+                for _ in range(2)]
+
+    def parts(x):
+        return x[:, H:H + Hk], x[:, H + Hk:]
+    # the whole sequences at once: rotated q and k for the packed pass
+    zero = torch.zeros(3, dtype=torch.int32, device=device)
+    kc, vc = caches()
+    q = paged_kv_append(*parts(qkv), kc, vc, table, zero, cu_seqlens=cu.to(device), q=qkv[:, :H],
+                        inv_freq=inv)
+    rows = torch.cat([table[b].long()[torch.arange(n, device=device) // page] * page
+                      + torch.arange(n, device=device) % page for b, n in enumerate(total)])
+    k, v = (c.flatten(0, 1)[rows] for c in (kc, vc))
+    assert torch.equal(v, qkv[:, H + Hk:])
+    o = packed_masked_attn(q, k, v, cu_seqlens_q=cu, cu_seqlens_k=cu, **kw)
+    val, bound = om.attention(f64(q), f64(k), f64(v), None, cu.numpy(), cu.numpy(), D ** -0.5,
+                              window=kw.get("window"), softcap=kw.get("softcap"),
+                              slopes=f64(kw.get("alibi_slopes")), u=U[BF])["o"]
+    within("o", o, val, bound)
+    # prompt, then step by step
+    kc2, vc2 = caches()
+    first = torch.cat([torch.arange(cu[b], cu[b] + n) for b, n in enumerate(prompt)]).to(device)
+    paged_kv_append(*parts(qkv[first]), kc2, vc2, table, zero, cu_seqlens=cu_p.to(device),
+                    inv_freq=inv)
+    lens = torch.tensor(prompt, dtype=torch.int32, device=device)
+    for t in range(new):
+        at = (cu[:-1] + torch.tensor(prompt) + t).to(device)
+        x = qkv[at]
+        qs = paged_kv_append(*parts(x), kc2, vc2, table, lens, q=x[:, :H], inv_freq=inv)
+        lens += 1
+        assert torch.equal(qs, q[at])
+        out = paged_decode_attn(qs, kc2, vc2, table, lens, **kw)
+        i = at.cpu().numpy()
+        within("o", out, val[i], bound[i])
+    same = torch.equal(torch.nan_to_num(kc), torch.nan_to_num(kc2))
+    assert same and torch.equal(torch.nan_to_num(vc), torch.nan_to_num(vc2))

@@ -1,0 +1,223 @@
+"""Packed attention under a mask, on the CPU: the plan covers exactly what the mask lets
+through, the calls that are refused, and the oracle against torch and differences."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import masked as om
+from varlenabsorbflashattn_amd import _lib, packed_masked_attn
+
+
+def cu(lens):
+    return np.concatenate([[0], np.cumsum(lens)]).astype(np.int64)
+
+
+def walked(item, window, bn):
+    """Keys that a kernel walks for a forward item (key_walk in csrc/masked.h)."""
+    q0, q1, k0, k1, _, diag, pre, _ = (int(x) for x in item)
+    win0 = q0 + diag - window + 1
+    a1, wl = min(pre, k1), max(win0, k0)
+    if a1 > k0:
+        if wl > a1:
+            return list(range(k0, a1)) + list(range(wl, k1))
+        return list(range(k0, k1))
+    return list(range(wl, k1))
+
+
+CASES = [
+    # q lens, k lens, H, Hk, D, causal, window, prefix
+    ([5, 0, 300, 129], [5, 0, 300, 129], 4, 2, 64, True, 0, None),
+    ([5, 40, 7], [1, 900, 0], 4, 4, 128, True, 0, None),          # rows without keys
+    ([700, 33], [700, 1200], 2, 1, 128, True, 50, None),
+    ([700, 33, 1], [700, 1200, 4000], 8, 2, 256, True, 64, [100, 1200, 3]),
+    ([260, 10], [300, 10], 3, 3, 64, True, 0, [300, 0]),
+    ([130, 1], [70, 5000], 2, 2, 128, False, 0, None),
+    ([1, 16], [20000, 9000], 1, 1, 128, True, 0, None),            # split over keys
+    ([300], [9000], 2, 1, 64, True, 2500, [700]),                  # split across the gap
+    ([2, 1], [0, 0], 1, 1, 64, True, 0, None),
+]
+
+
+@pytest.mark.parametrize("case", range(len(CASES)))
+def test_plan_covers_the_mask(case):
+    ql, kl, H, Hk, D, causal, window, prefix = CASES[case]
+    cq, ck = cu(ql), cu(kl)
+    p = _lib.plan_masked(cq, ck, H, Hk, D, causal, window, prefix)
+    info, win = p.info, window or 1 << 30
+    assert (info.T_q, info.T_k, info.H, info.kind) == (cq[-1], ck[-1], H, 3)
+    assert info.xcd_heads >= 1 and (H // Hk) % info.xcd_heads == 0
+    see = np.zeros((cq[-1], ck[-1]), bool)
+    for s in range(len(ql)):
+        see[cq[s]:cq[s + 1], ck[s]:ck[s + 1]] = om.visible(
+            ql[s], kl[s], causal, window, prefix[s] if prefix else 0)
+    seg = np.searchsorted(cq, np.arange(cq[-1]), side="right") - 1
+    got = np.zeros(see.shape, int)
+    owners = np.zeros(cq[-1], int)
+    prows = set()
+    for it in p.section("fwd"):
+        q0, q1, k0, k1, pbase, diag, pre, owner = (int(x) for x in it)
+        assert 0 <= q0 < q1 <= cq[-1] and 0 <= k0 <= k1 <= ck[-1] and q1 - q0 <= info.q_tile
+        assert len(set(seg[q0:q1])) == 1
+        s = seg[q0]
+        assert diag == ck[s + 1] - cq[s + 1] and ck[s] <= k0 and k1 <= ck[s + 1]
+        assert pre == (ck[s + 1] if not causal else ck[s] + (prefix[s] if prefix else 0))
+        owners[q0:q1] += owner
+        if pbase >= 0:
+            rows = set(range(pbase, pbase + q1 - q0))
+            assert not rows & prows and pbase + q1 - q0 <= info.n_part_rows
+            prows |= rows
+        got[q0:q1, walked(it, win, 64)] += 1
+    assert (owners == 1).all()
+    assert got.max(initial=0) <= 1 and (got[see] == 1).all()
+    # combine items read exactly the split items' rows
+    read = set()
+    for q0, q1, pbase, ns, *_ in p.section("comb").tolist():
+        rows = set(range(pbase, pbase + ns * (q1 - q0)))
+        assert not rows & read
+        read |= rows
+    assert read == prows and len(prows) == info.n_part_rows
+    keys = np.zeros(ck[-1], int)
+    for it in p.section("kv"):
+        k0, k1, q0, q1, diag, pre, *_ = (int(x) for x in it)
+        assert 0 <= k0 < k1 <= ck[-1] and 0 <= q0 <= q1 <= cq[-1] and k1 - k0 <= info.k_tile
+        keys[k0:k1] += 1
+        rows = np.zeros(cq[-1], bool)
+        rows[q0:q1] = True
+        assert not see[~rows, k0:k1].any()
+        assert (seg[q0:q1] == np.searchsorted(ck, k0, side="right") - 1).all()
+    assert (keys == 1).all()
+
+
+def test_plan_refusals():
+    c = cu([4, 4])
+
+    def bad(error, text, *args, **kw):
+        with pytest.raises(error, match=text):
+            _lib.plan_masked(c, c, *args, **kw)
+    bad(AssertionError, "do not divide", 3, 2, 64)
+    bad(AssertionError, "do not divide", 0, 1, 64)
+    bad(ValueError, "belong to the causal", 2, 1, 64, False, 5)
+    bad(ValueError, "belong to the causal", 2, 1, 64, False, 0, [1, 1])
+    bad(ValueError, "window must be positive", 2, 1, 64, True, -1)
+    bad(ValueError, r"prefix_lens\[1\] = 5 of 4", 2, 1, 64, True, 0, [4, 5])
+    bad(ValueError, r"prefix_lens\[0\] = -1", 2, 1, 64, True, 0, [-1, 0])
+    bad(AssertionError, "prefix_lens must be", 2, 1, 64, True, 0, [1])
+    big = np.array([0, (1 << 30) + 1])
+    with pytest.raises(ValueError, match="more than"):
+        _lib.plan_masked(big, big, 1, 1, 64)
+
+
+def test_c_abi_refusals():
+    import ctypes as C
+    L = _lib.lib()
+    p = _lib.plan_masked(cu([4]), cu([4]), 4, 2, 64)
+    other = _lib.plan_varlen(cu([4]), cu([4]), 4, 64)
+    assert L.vafa_masked_fwd_workspace(other.info, 64) == -1
+    assert L.vafa_masked_bwd_workspace(p.info, 3, 64) == -1
+    assert L.vafa_masked_bwd_workspace(p.info, 2, 96) == -1
+    assert L.vafa_varlen_fwd_workspace(p.info, 64) == -1  # and not the other way round
+    need = L.vafa_masked_bwd_workspace(p.info, 2, 64)
+    assert need > 0
+    x = 1 << 20
+    f = [x, x, x, x, x, x, p.info, 2, 64, _lib.DT_BF16, 0.1, 0.0, 0, None, x, 1 << 20, None]
+    b = [x] * 10 + [p.info, 2, 64, _lib.DT_BF16, 0.1, 0.0, 0, None, x, need, None]
+
+    def rc(call, args, at, value):
+        return call(*[value if i == at else y for i, y in enumerate(args)])
+    for at, bad, want in ((0, x + 2, "VALUE"), (7, 3, "ASSERT"), (8, 32, "ASSERT"),
+                          (9, _lib.DT_F32, "ASSERT"), (10, float("nan"), "VALUE"),
+                          (11, -2.0, "VALUE"), (12, -1, "VALUE"), (6, other.info, "VALUE")):
+        assert rc(L.vafa_masked_fwd, f, at, bad) == getattr(_lib, "VAFA_ERR_" + want), at
+    for at, bad, want in ((4, x + 8, "VALUE"), (19, need - 1, "WORKSPACE"), (18, None, "WORKSPACE"),
+                          (18, x + 4, "WORKSPACE"), (15, float("inf"), "VALUE")):
+        assert rc(L.vafa_masked_bwd, b, at, bad) == getattr(_lib, "VAFA_ERR_" + want), at
+    assert C.sizeof(_lib.PagedCache) == 17 * 8
+
+
+def _call(dt=torch.bfloat16, H=4, Hk=2, D=64, **kw):
+    q, k = torch.zeros(6, H, D, dtype=dt), torch.zeros(6, Hk, D, dtype=dt)
+    c = torch.tensor([0, 6], dtype=torch.int32)
+    kw = {"cu_seqlens_q": c, "cu_seqlens_k": c, **kw}
+    return packed_masked_attn(q, k, kw.pop("v", k), **kw)
+
+
+def test_call_refusals():
+    slopes = torch.ones(4)
+    for kw, error, text in (
+            ({"dt": torch.float32}, AssertionError, "dtype"),
+            ({"D": 96}, AssertionError, "head_dim 96"),
+            ({"H": 3}, AssertionError, "do not divide"),
+            ({"v": torch.zeros(6, 2, 64)}, AssertionError, "share dtype"),
+            ({"v": torch.zeros(5, 2, 64, dtype=torch.bfloat16)}, AssertionError, "T_k, H_k"),
+            ({"window": 0}, ValueError, "window must be positive"),
+            ({"softcap": -1.0}, ValueError, "softcap"),
+            ({"softcap": 0.0}, ValueError, "softcap"),
+            ({"softcap": float("inf")}, ValueError, "softcap"),
+            ({"scale": float("nan")}, ValueError, "scale"),
+            ({"causal": False, "window": 3}, ValueError, "belong to the causal"),
+            ({"causal": False, "prefix_lens": torch.tensor([1])}, ValueError, "belong"),
+            ({"alibi_slopes": slopes.double()}, AssertionError, "alibi_slopes"),
+            ({"alibi_slopes": slopes[:3]}, AssertionError, "alibi_slopes"),
+            ({"alibi_slopes": slopes.clone().requires_grad_(True)}, ValueError, "no gradient"),
+            ({"cu_seqlens_q": None}, ValueError, "cu_seqlens_q or q_seqinfo"),
+            ({"cu_seqlens_k": torch.tensor([0, 3, 6])}, AssertionError, "segment count"),
+            ({}, AssertionError, "requires GPU tensors")):
+        with pytest.raises(error, match=text):
+            _call(**kw)
+
+
+def test_oracle_against_autograd():
+    g = torch.Generator().manual_seed(0)
+    H, Hk, D, ql, kl = 4, 2, 8, [5, 9], [5, 12]
+    cq, ck = cu(ql), cu(kl)
+
+    def rnd(*s):
+        return torch.randn(*s, generator=g, dtype=torch.float64)
+    q, k, v, do = rnd(14, H, D), rnd(17, Hk, D), rnd(17, Hk, D), rnd(14, H, D)
+    slopes, cap, window, prefix = [0.5, 0.25, 0.1, 0.0], 2.0, 4, [2, 0]
+    ref = om.attention(*(t.numpy() for t in (q, k, v, do)), cq, ck, 0.7, window=window,
+                       prefix=prefix, softcap=cap, slopes=slopes)
+    x = [t.requires_grad_(True) for t in (q, k, v)]
+    outs = []
+    for s in range(2):
+        for h in range(H):
+            qh, kh, vh = x[0][cq[s]:cq[s + 1], h], x[1][ck[s]:ck[s + 1], h // 2], \
+                x[2][ck[s]:ck[s + 1], h // 2]
+            z = cap * torch.tanh(0.7 * qh @ kh.T / cap)
+            p = torch.arange(ql[s])[:, None] + kl[s] - ql[s]
+            j = torch.arange(kl[s])
+            z = z - slopes[h] * (p - j).abs().double()
+            see = ((j <= p) & (j > p - window)) | (j < prefix[s])
+            outs.append((torch.softmax(z.masked_fill(~see, -math.inf), 1) @ vh, s, h))
+    loss = sum((o * do[cq[s]:cq[s + 1], h]).sum() for o, s, h in outs)
+    for o, s, h in outs:
+        np.testing.assert_allclose(ref["o"][0][cq[s]:cq[s + 1], h], o.detach().numpy(), atol=1e-12)
+    for name, got in zip(("dq", "dk", "dv"), torch.autograd.grad(loss, x)):
+        np.testing.assert_allclose(ref[name][0], got.numpy(), atol=1e-12)
+
+
+def test_oracle_against_differences():
+    g = np.random.default_rng(1)
+    q, k, v, do = (g.standard_normal(s) for s in ((6, 2, 4), (7, 1, 4), (7, 1, 4), (6, 2, 4)))
+    args = (np.array([0, 6]), np.array([0, 7]), -0.4)
+    kw = {"softcap": 1.5, "slopes": [0.3, 0.1], "prefix": [3], "window": 2}
+    ref = om.attention(q, k, v, do, *args, **kw)
+    for name, i in (("dq", 0), ("dk", 1), ("dv", 2)):
+        at, step = (2, 0, 1), 1e-6
+        f = []
+        for sign in (1, -1):
+            x = [t.copy() for t in (q, k, v)]
+            x[i][at] += sign * step
+            f.append((om.attention(*x, None, *args, **kw)["o"][0] * do).sum())
+        assert abs((f[0] - f[1]) / (2 * step) - ref[name][0][at]) < 1e-7
+
+
+def test_oracle_rows_without_keys():
+    g = np.random.default_rng(2)
+    q, k, do = (g.standard_normal(s) for s in ((5, 1, 4), (2, 1, 4), (5, 1, 4)))
+    ref = om.attention(q, k, k, do, np.array([0, 5]), np.array([0, 2]), 1.0, u=0.01)
+    for n in ("o", "dq"):
+        assert not ref[n][0][:3].any() and ref[n][0][3:].any()
+        assert not ref[n][1][:3].any()

@@ -74,6 +74,8 @@ _SIGS = {
     "vafa_plan_varlen": (C.c_int, [_PI64, _PI64, _I64, _I64, _I64, _PI32, _I64, _PINFO]),
     "vafa_plan_varlen_balanced": (C.c_int, [_PI64, _PI64, _I64, _I64, _I64, _PI32, _I64, _PINFO]),
     "vafa_plan_absorb": (C.c_int, [_PI64, _PI64, _I64, _I64, _I64, _I64, _PI32, _I64, _PINFO]),
+    "vafa_plan_masked": (C.c_int, [_PI64, _PI64, _PI64, _I64, _I64, _I64, _I64, _I32, _I64, _PI32,
+                                   _I64, _PINFO]),
     "vafa_varlen_fwd_workspace": (C.c_int64, [_PINFO, _I64]),
     "vafa_varlen_bwd_workspace": (C.c_int64, [_PINFO, _I64]),
     "vafa_absorb_fwd_workspace": (C.c_int64, [_PINFO, _I64, _I64]),
@@ -111,6 +113,12 @@ _SIGS = {
     "vafa_absorb_fwd_full_workspace": (C.c_int64, [_PINFO, _I64, _I64, _I64]),
     "vafa_absorb_fwd_full": (C.c_int, [_P, _P, _P, _P, _P, _P, _P, _P, _I64, _P, _PINFO, _I64,
                                        _I64, _I64, _I32, C.c_float, _P, _I64, _P]),
+    "vafa_masked_fwd_workspace": (C.c_int64, [_PINFO, _I64]),
+    "vafa_masked_bwd_workspace": (C.c_int64, [_PINFO, _I64, _I64]),
+    "vafa_masked_fwd": (C.c_int, [_P, _P, _P, _P, _P, _P, _PINFO, _I64, _I64, _I32, C.c_float,
+                                  C.c_float, _I64, _P, _P, _I64, _P]),
+    "vafa_masked_bwd": (C.c_int, [_P] * 10 + [_PINFO, _I64, _I64, _I32, C.c_float, C.c_float, _I64,
+                                              _P, _P, _I64, _P]),
     "vafa_paged_append": (C.c_int, [_PCACHE, _P, _I64, _I64, _P, _I64, _I64, _I64, _P, _P, _I64,
                                     _I64, _I64, _P, _P, _I64, _I32, _I32, _P]),
     "vafa_paged_decode_workspace": (C.c_int64, [_PCACHE, _I64, _I64]),
@@ -307,6 +315,21 @@ def plan_absorb(cu_q: np.ndarray, cu_k: np.ndarray, H: int, F: int, DH: int) -> 
     return _plan(lib().vafa_plan_absorb, guess, _i64p(a), _i64p(b), a.size, H, F, DH)
 
 
+def plan_masked(cu_q: np.ndarray, cu_k: np.ndarray, H: int, Hk: int, D: int, causal: bool = True,
+                window: int = 0, prefix: Optional[np.ndarray] = None) -> HostPlan:
+    """A plan of packed_masked_attn (window 0: none)."""
+    a = np.ascontiguousarray(cu_q, dtype=np.int64)
+    b = np.ascontiguousarray(cu_k, dtype=np.int64)
+    if a.shape != b.shape:
+        raise AssertionError(f"segment count mismatch: q has {a.size - 1}, k has {b.size - 1}")
+    pre = None if prefix is None else np.ascontiguousarray(prefix, dtype=np.int64)
+    if pre is not None and pre.shape != (a.size - 1,):
+        raise AssertionError(f"prefix_lens must be [{a.size - 1}], got {pre.shape}")
+    guess = 64 + 12 * a.size + int(max(a[-1], 0) + max(b[-1], 0)) // 32 if a.size else 64
+    return _plan(lib().vafa_plan_masked, guess, _i64p(a), _i64p(b),
+                 None if pre is None else _i64p(pre), a.size, H, Hk, D, int(causal), window)
+
+
 # ---- device plans (cached by cu_seqlens content) ------------------------------
 
 class DevicePlan:
@@ -376,8 +399,13 @@ def cached_plan(key: tuple) -> Optional[DevicePlan]:
 def new_plan(key: tuple, cu_q: np.ndarray, cu_k: np.ndarray) -> DevicePlan:
     """Builds and caches the plan of ``key``, from int64 cu_seqlens."""
     kind, dims, device = key[0], key[5], key[6]
-    host = (plan_varlen(cu_q, cu_k, *dims, balanced=True) if kind == "varlen"
-            else plan_absorb(cu_q, cu_k, *dims))
+    if kind == "varlen":
+        host = plan_varlen(cu_q, cu_k, *dims, balanced=True)
+    elif kind == "masked":  # dims end with the prefix lengths as bytes, or None
+        host = plan_masked(cu_q, cu_k, *dims[:-1], None if dims[-1] is None
+                           else np.frombuffer(dims[-1], dtype=np.int64))
+    else:
+        host = plan_absorb(cu_q, cu_k, *dims)
     dp = DevicePlan(host, device)
     with _lock:
         _CACHE[key] = dp

@@ -1,0 +1,196 @@
+// extern "C" entry points of packed_masked_attn: argument checks, workspace carving and
+// kernel dispatch.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+#include <initializer_list>
+
+#include "../../include/vafa.h"
+#include "common.h"
+#include "kernels.h"
+
+namespace vafa {
+int fail(int code, const char *fmt, ...);
+
+namespace {
+
+int check_plan(const vafa_plan_info *info, int64_t Hk, int64_t D) {
+  if (info == nullptr || info->magic != VAFA_PLAN_MAGIC || info->kind != 3)
+    return fail(VAFA_ERR_VALUE, "plan does not belong to this operator");
+  if (D != 64 && D != 128 && D != 256)
+    return fail(VAFA_ERR_ASSERT, "head_dim %lld not supported (64, 128, 256)", (long long)D);
+  if (Hk < 1 || info->H < 1 || info->H % Hk != 0)
+    return fail(VAFA_ERR_ASSERT, "%lld query heads do not divide among %lld key heads",
+                (long long)info->H, (long long)Hk);
+  const int64_t G = info->H / Hk;
+  if (info->xcd_heads < 1 || info->xcd_heads > G)
+    return fail(VAFA_ERR_VALUE, "the plan divides %lld heads into %lld parts", (long long)G,
+                (long long)info->xcd_heads);
+  const bool q_ok =
+      info->q_tile == kVarlenTile || (info->q_tile == kVarlenWideTile && D <= 128);
+  const bool k_ok =
+      info->k_tile == kVarlenTile || (info->k_tile == kVarlenWideTile && D == 128);
+  if (!q_ok || !k_ok)
+    return fail(VAFA_ERR_VALUE, "plan tiles (%lld queries, %lld keys) do not fit head_dim %lld",
+                (long long)info->q_tile, (long long)info->k_tile, (long long)D);
+  return VAFA_OK;
+}
+
+int check_call(const vafa_plan_info *info, int64_t Hk, int64_t D, int32_t dtype, float scale,
+               float softcap, int64_t window, std::initializer_list<const void *> ptrs) {
+  if (int rc = check_plan(info, Hk, D)) return rc;
+  if (dtype != VAFA_BF16 && dtype != VAFA_F16)
+    return fail(VAFA_ERR_ASSERT, "dtype not supported (float16, bfloat16)");
+  if (!std::isfinite(scale)) return fail(VAFA_ERR_VALUE, "scale must be finite");
+  if (!(softcap >= 0.f) || !std::isfinite(softcap))
+    return fail(VAFA_ERR_VALUE, "softcap must be positive and finite");
+  if (window < 0) return fail(VAFA_ERR_VALUE, "window must be positive");
+  for (const void *p : ptrs)
+    if ((uintptr_t)p % 16 != 0) return fail(VAFA_ERR_VALUE, "operands must be 16-byte aligned");
+  return VAFA_OK;
+}
+
+inline int64_t up(int64_t x) { return (x + 255) / 256 * 256; }
+
+struct Ws {
+  float *part_o, *part_lse, *delta, *lse, *part_dk, *part_dv;
+  int64_t bytes;
+};
+
+Ws carve(void *ws, const vafa_plan_info *info, int64_t Hk, int64_t D, bool bwd) {
+  Ws w{};
+  char *base = static_cast<char *>(ws);
+  int64_t used = 0;
+  auto take = [&](int64_t n) {
+    float *p = base != nullptr ? reinterpret_cast<float *>(base + used) : nullptr;
+    used += up(n * 4);
+    return p;
+  };
+  const int64_t rows = info->n_part_rows * info->H;
+  w.part_o = take(rows * D);
+  if (!bwd) {
+    w.part_lse = take(rows);
+  } else {
+    w.delta = take(info->T_q * info->H);
+    w.lse = take(info->T_q * info->H);
+    const int64_t parts = info->xcd_heads > 1 ? info->xcd_heads : 0;
+    w.part_dk = take(parts * info->T_k * Hk * D);
+    w.part_dv = take(parts * info->T_k * Hk * D);
+  }
+  w.bytes = used;
+  return w;
+}
+
+MaskedArgs args_of(const vafa_plan_info *info, const int32_t *plan, int64_t Hk, int64_t D,
+                   float scale, float softcap, int64_t window, const float *slopes) {
+  MaskedArgs a{};
+  a.items = plan + info->off_fwd; a.n_items = info->n_fwd;
+  a.comb_items = plan + info->off_comb; a.n_comb = info->n_comb;
+  a.comb_rows = (int)info->max_comb_rows;
+  a.kv_items = plan + info->off_kv; a.n_kv = info->n_kv;
+  a.T_k = info->T_k;
+  a.H = (int)info->H; a.Hk = (int)Hk; a.D = (int)D;
+  a.q_tile = (int)info->q_tile; a.k_tile = (int)info->k_tile;
+  a.window = (int)(window > 0 ? std::min(window, kMaskedMaxTokens) : kMaskedMaxTokens);
+  a.gsplit = (int)info->xcd_heads;
+  a.slopes = slopes;
+  a.scale = scale;
+  a.c = softcap > 0.f ? 2.f * kLog2e * scale / softcap : scale * kLog2e;
+  a.cap2 = softcap * kLog2e;
+  return a;
+}
+
+int check_ws(int64_t have, const void *ws, int64_t need) {
+  if (have < need || (need > 0 && (ws == nullptr || (uintptr_t)ws % 16 != 0)))
+    return fail(VAFA_ERR_WORKSPACE, "workspace of %lld bytes, %lld needed (16-byte aligned)",
+                (long long)have, (long long)need);
+  return VAFA_OK;
+}
+
+int check_launch(const char *what) {
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess)
+    return fail(VAFA_ERR_RUNTIME, "%s: kernel launch failed: %s", what, hipGetErrorString(e));
+  return VAFA_OK;
+}
+
+template <typename T>
+void fwd(const MaskedArgs &a, hipStream_t st) {
+  if (a.D == 64) launch_masked_fwd<T, 64>(a, st);
+  if (a.D == 128) launch_masked_fwd<T, 128>(a, st);
+  if (a.D == 256) launch_masked_fwd<T, 256>(a, st);
+  launch_lse_combine<T>(a.part_o, a.part_lse, a.o, a.lse, a.comb_items, a.n_comb, a.H, a.D,
+                        a.comb_rows, st);
+}
+
+template <typename T>
+void bwd(const MaskedArgs &a, hipStream_t st) {
+  if (a.D == 64) launch_masked_dq<T, 64>(a, st);
+  if (a.D == 128) launch_masked_dq<T, 128>(a, st);
+  if (a.D == 256) launch_masked_dq<T, 256>(a, st);
+  launch_sum_combine<T>(a.part_o, a.dq, a.comb_items, a.n_comb, a.H, a.D, a.comb_rows, st);
+  if (a.D == 64) launch_masked_dkv<T, 64>(a, st);
+  if (a.D == 128) launch_masked_dkv<T, 128>(a, st);
+  if (a.D == 256) launch_masked_dkv<T, 256>(a, st);
+  launch_masked_group_sum<T>(a, st);
+}
+
+}  // namespace
+}  // namespace vafa
+
+using namespace vafa;
+
+extern "C" {
+
+int64_t vafa_masked_fwd_workspace(const vafa_plan_info *info, int64_t D) {
+  if (check_plan(info, 1, D)) return -1;
+  return carve(nullptr, info, 1, D, false).bytes;
+}
+
+int64_t vafa_masked_bwd_workspace(const vafa_plan_info *info, int64_t Hk, int64_t D) {
+  if (check_plan(info, Hk, D)) return -1;
+  return carve(nullptr, info, Hk, D, true).bytes;
+}
+
+int vafa_masked_fwd(const void *q, const void *k, const void *v, void *o, float *lse,
+                    const int32_t *plan_dev, const vafa_plan_info *info, int64_t Hk, int64_t D,
+                    int32_t dtype, float scale, float softcap, int64_t window, const float *slopes,
+                    void *workspace, int64_t workspace_bytes, void *stream) {
+  if (int rc = check_call(info, Hk, D, dtype, scale, softcap, window, {q, k, v, o})) return rc;
+  const Ws w = carve(workspace, info, Hk, D, false);
+  if (int rc = check_ws(workspace_bytes, workspace, w.bytes)) return rc;
+  MaskedArgs a = args_of(info, plan_dev, Hk, D, scale, softcap, window, slopes);
+  a.q = q; a.k = k; a.v = v; a.o = o; a.lse = lse;
+  a.part_o = w.part_o; a.part_lse = w.part_lse;
+  if (dtype == VAFA_BF16)
+    fwd<bf16>(a, (hipStream_t)stream);
+  else
+    fwd<f16>(a, (hipStream_t)stream);
+  return check_launch("vafa_masked_fwd");
+}
+
+int vafa_masked_bwd(const void *q, const void *k, const void *v, const void *o, const void *dout,
+                    const float *lse, void *dq, void *dk, void *dv, const int32_t *plan_dev,
+                    const vafa_plan_info *info, int64_t Hk, int64_t D, int32_t dtype, float scale,
+                    float softcap, int64_t window, const float *slopes, void *workspace,
+                    int64_t workspace_bytes, void *stream) {
+  if (int rc = check_call(info, Hk, D, dtype, scale, softcap, window,
+                          {q, k, v, o, dout, dq, dk, dv}))
+    return rc;
+  const Ws w = carve(workspace, info, Hk, D, true);
+  if (int rc = check_ws(workspace_bytes, workspace, w.bytes)) return rc;
+  MaskedArgs a = args_of(info, plan_dev, Hk, D, scale, softcap, window, slopes);
+  a.q = q; a.k = k; a.v = v; a.o_in = o; a.dout = dout; a.lse_in = lse;
+  a.dq = dq; a.dk = dk; a.dv = dv;
+  a.part_o = w.part_o; a.delta = w.delta; a.lse = w.lse;
+  a.part_dk = w.part_dk; a.part_dv = w.part_dv;
+  if (dtype == VAFA_BF16)
+    bwd<bf16>(a, (hipStream_t)stream);
+  else
+    bwd<f16>(a, (hipStream_t)stream);
+  return check_launch("vafa_masked_bwd");
+}
+
+}  // extern "C"

@@ -107,6 +107,23 @@ struct AbsorbArgs {
   float scale;
 };
 
+// Packed attention with masks, capped scores and distance biases.
+struct MaskedArgs {
+  const void *q, *k, *v, *o_in, *dout;
+  void *o, *dq, *dk, *dv;
+  float *lse;
+  const float *lse_in, *slopes;  // slopes: or null
+  float *delta;                  // [T_q, H] workspace (backward)
+  float *part_o, *part_lse;      // split partial rows: O (and LSE) or dQ
+  float *part_dk, *part_dv;      // [gsplit, T_k, Hk, D] fp32 where gsplit > 1
+  const int32_t *items, *comb_items, *kv_items;
+  int64_t n_items, n_comb, n_kv;
+  int comb_rows;
+  int64_t T_k;
+  int H, Hk, D, q_tile, k_tile, window, gsplit;
+  float scale, c, cap2;  // c: factor on q.k (masked.h); cap2: cap log2 e, 0 without
+};
+
 // Tokens appended to a paged cache; strides in elements.
 struct AppendArgs {
   const void *q, *k, *v;  // q: null where H is 0
@@ -201,6 +218,13 @@ void launch_absorb_dax(const AbsorbArgs &, hipStream_t);
 // paged.hip (bf16 / f16)
 template <typename T> void launch_paged_append(const AppendArgs &, hipStream_t);
 template <typename T> void launch_paged_decode(const DecodeArgs &, int D, int grid, hipStream_t);
+
+// masked_fwd.hip, masked_bwd.hip (bf16 / f16, D in {64, 128, 256})
+template <typename T, int D> void launch_masked_fwd(const MaskedArgs &, hipStream_t);
+template <typename T, int D> void launch_masked_dq(const MaskedArgs &, hipStream_t);
+template <typename T, int D> void launch_masked_dkv(const MaskedArgs &, hipStream_t);
+// dk = scale * sum, dv = sum of the fp32 partials of gsplit head groups, in order
+template <typename T> void launch_masked_group_sum(const MaskedArgs &, hipStream_t);
 
 // varlen_mfma.hip (bf16 / f16, D in {32, 64, 128, 256})
 template <typename T, int D> void launch_mfma_varlen_fwd(const VarlenArgs &, hipStream_t);

@@ -487,6 +487,142 @@ int vafa_plan_varlen_balanced(const int64_t *cu_q, const int64_t *cu_k, int64_t 
   return plan_varlen(cu_q, cu_k, n1, H, D, true, plan, plan_cap, info);
 }
 
+// Masked varlen plan (packed_masked_attn).  Items name only the keys (queries) that
+// some of their rows see:
+//   fwd section : {q0, q1, k0, k1, pbase, diag, pre, owner}: query row r has position
+//                 r + diag among the absolute keys and sees those in front of `pre`
+//                 and those of its window; between the two ranges nothing of [k0, k1)
+//                 is walked.  pbase as in a varlen plan; owner: 1 for the item that
+//                 holds its rows' first keys.  A tile that sees no key is an item with
+//                 k0 == k1, which writes zeros.
+//   comb section: {q0, q1, pbase, nsplit, seg, 0, 0, 0}.
+//   kv section  : {k0, k1, q0, q1, diag, pre, 0, 0} key tiles with the range of the
+//                 queries that see some of their keys.
+// info->xcd_heads holds the parts into which the query heads of a key head are divided
+// in the dK/dV pass.
+int vafa_plan_masked(const int64_t *cu_q, const int64_t *cu_k, const int64_t *prefix, int64_t n1,
+                     int64_t H, int64_t Hk, int64_t D, int32_t causal, int64_t window,
+                     int32_t *plan, int64_t plan_cap, vafa_plan_info *info) {
+  int rc = check_pair(cu_q, cu_k, n1);
+  if (rc) return rc;
+  if (H < 1 || Hk < 1 || H % Hk != 0 || H > 65536)
+    return fail(VAFA_ERR_ASSERT, "%lld query heads do not divide among %lld key heads",
+                (long long)H, (long long)Hk);
+  if (window < 0) return fail(VAFA_ERR_VALUE, "window must be positive");
+  if (!causal && (window > 0 || prefix != nullptr))
+    return fail(VAFA_ERR_VALUE, "window and prefix_lens belong to the causal mask");
+  // positions and window arithmetic run in 32 bits
+  if (cu_q[n1 - 1] > kMaskedMaxTokens || cu_k[n1 - 1] > kMaskedMaxTokens)
+    return fail(VAFA_ERR_VALUE, "more than %lld tokens", (long long)kMaskedMaxTokens);
+  const int64_t win = window > 0 ? std::min(window, kMaskedMaxTokens) : kMaskedMaxTokens;
+  for (int64_t s = 0; prefix != nullptr && s + 1 < n1; ++s)
+    if (prefix[s] < 0 || prefix[s] > cu_k[s + 1] - cu_k[s])
+      return fail(VAFA_ERR_VALUE, "prefix_lens[%lld] = %lld of %lld keys", (long long)s,
+                  (long long)prefix[s], (long long)(cu_k[s + 1] - cu_k[s]));
+  std::memset(info, 0, sizeof(*info));
+  info->magic = VAFA_PLAN_MAGIC;
+  info->kind = 3;
+  info->n_seg = n1 - 1;
+  info->T_q = cu_q[n1 - 1];
+  info->T_k = cu_k[n1 - 1];
+  info->H = H;
+
+  // keys [lo, hi) that rows [a, b) of segment s see: the prefix' end, and the keys of
+  // [lo, hi) they do not walk in between
+  struct Range {
+    int64_t lo, hi, pre, keys;
+  };
+  auto range_of = [&](int64_t s, int64_t a, int64_t b) {
+    const int64_t ks = cu_k[s], ke = cu_k[s + 1], diag = ke - cu_q[s + 1];
+    Range r;
+    r.pre = causal ? ks + (prefix != nullptr ? prefix[s] : 0) : ke;
+    r.hi = std::max(r.pre, std::min(ke, b + diag));
+    const int64_t first = std::max(ks, a + diag - win + 1);  // of the window
+    r.lo = r.pre > ks ? ks : first;
+    if (r.hi <= r.lo) {
+      r.lo = r.hi = ks;
+    }
+    r.keys = r.hi - r.lo - std::max<int64_t>(0, std::min(first, r.hi) - std::max(r.pre, r.lo));
+    return r;
+  };
+
+  // tiles: wide ones (8 waves) where the launch fills the chip with them
+  auto work_of = [&](int64_t bm, int64_t *items, int64_t *longest) {
+    int64_t keys = 0;
+    *items = *longest = 0;
+    for (int64_t s = 0; s + 1 < n1; ++s)
+      for (int64_t t = cu_q[s]; t < cu_q[s + 1]; t += bm) {
+        const Range r = range_of(s, t, std::min(t + bm, cu_q[s + 1]));
+        keys += r.keys;
+        *longest = std::max(*longest, r.keys);
+        ++*items;
+      }
+    return keys;
+  };
+  const int64_t cus = kVarlenBalance.cus, slots = (D > 128 ? 1 : 2) * cus;
+  int64_t BM = kVarlenTile, BK = kVarlenTile, items, longest;
+  const int64_t keys = work_of(BM, &items, &longest);
+  info->q_tile = BM;
+  info->k_tile = BK;
+  // a chunk of keys per item: the average of the resident workgroups, so that no item
+  // outlasts the rest
+  const int64_t avg = cdiv(keys * H, slots);
+  const int64_t chunk_max = std::max<int64_t>(kMaskedMinChunk, round_up(avg, 64));
+
+  Section fwd, comb, kv;
+  int64_t prow = 0, max_split = 1;
+  for (int64_t s = 0; s + 1 < n1; ++s) {
+    const int64_t q0 = cu_q[s], q1 = cu_q[s + 1], k0 = cu_k[s], k1 = cu_k[s + 1];
+    const int64_t diag = k1 - q1;
+    for (int64_t t = q0; t < q1; t += BM) {
+      const int64_t te = std::min(t + BM, q1), rows = te - t;
+      const Range r = range_of(s, t, te);
+      const int64_t span = r.hi - r.lo;
+      int64_t ns = span > chunk_max + chunk_max / 4 ? cdiv(span, chunk_max) : 1;
+      const int64_t chunk = ns > 1 ? round_up(cdiv(span, ns), 64) : span;
+      if (ns > 1) ns = cdiv(span, chunk);
+      max_split = std::max(max_split, ns);
+      if (ns > 1)
+        comb.push_back(Item{{(int32_t)t, (int32_t)te, (int32_t)prow, (int32_t)ns, (int32_t)s, 0, 0,
+                             0}, 0});
+      for (int64_t j = 0; j < ns; ++j) {
+        const int64_t a = ns > 1 ? r.lo + j * chunk : r.lo;
+        const int64_t b = ns > 1 ? std::min(r.hi, a + chunk) : r.hi;
+        fwd.push_back(Item{{(int32_t)t, (int32_t)te, (int32_t)a, (int32_t)b,
+                            ns > 1 ? (int32_t)(prow + j * rows) : -1, (int32_t)diag,
+                            (int32_t)r.pre, j == 0},
+                           (ns > 1 ? b - a : r.keys) + kVarlenPolicy.item_overhead});
+      }
+      if (ns > 1) prow += ns * rows;
+      if (prow > INT32_MAX) return fail(VAFA_ERR_VALUE, "too many split rows");
+    }
+    const int64_t pre = causal ? k0 + (prefix != nullptr ? prefix[s] : 0) : k1;
+    for (int64_t k = k0; k < k1; k += BK) {
+      const int64_t ke = std::min(k + BK, k1);
+      int64_t a = q0, b = q1;
+      if (k >= pre) {
+        a = std::max(q0, k - diag);
+        b = std::min(q1, ke - 1 + win - diag);
+        if (b < a) a = b = q0;
+      }
+      kv.push_back(Item{{(int32_t)k, (int32_t)ke, (int32_t)a, (int32_t)b, (int32_t)diag,
+                         (int32_t)pre, 0, 0},
+                        (b - a) + kVarlenPolicy.item_overhead});
+    }
+  }
+  sort_lpt(fwd);
+  sort_lpt(kv);
+  comb.keep_order();
+  // parts of a key head's query heads in the dK/dV pass: until every CU has a workgroup
+  int64_t parts = 1;
+  const int64_t G = H / Hk, wgs = (int64_t)kv.items.size() * Hk;
+  while (parts * 2 <= G && G % (parts * 2) == 0 && wgs * parts < slots) parts *= 2;
+  info->xcd_heads = parts;
+  info->n_part_rows = prow;
+  info->max_split = max_split;
+  return emit(fwd, comb, kv, {}, {}, {}, {}, {}, plan, plan_cap, info);
+}
+
 // Absorb plan.  Query rows are (token, head) pairs; one item covers whole
 // tokens [t0, t1) with (t1 - t0) * H <= kAbsorbRows.  A segment's tiles share
 // one split of its key range.

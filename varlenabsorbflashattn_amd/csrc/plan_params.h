@@ -57,6 +57,11 @@ struct VarlenBalance {
   int64_t cus, min_chunk, max_part_bytes;
 };
 constexpr VarlenBalance kVarlenBalance{256, 512, 32 << 20};
+// packed_masked_attn: most tokens of a call (positions, and a position less the window,
+// are 32-bit in the kernels) and the smallest chunk of keys into which a tile's range is
+// split.
+constexpr int64_t kMaskedMaxTokens = int64_t{1} << 30;
+constexpr int64_t kMaskedMinChunk = 512;
 // Absorb forward key splits.  A chunk holds kAbsorbSlack2 / 2 times the
 // average keys per resident forward workgroup (256 CUs x 3 on the MI355X), so
 // large launches stay whole (splitting C5's <= 8192-key samples into 1024-key

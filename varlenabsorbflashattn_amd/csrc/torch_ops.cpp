@@ -33,7 +33,8 @@ struct Api {
   X(absorb_bwd_full_workspace)                                                            \
   X(absorb_project_workspace) X(absorb_project_fwd) X(absorb_project_bwd)                 \
   X(absorb_project_f32_workspace) X(absorb_project_f32_fwd) X(absorb_project_f32_bwd)      \
-  X(paged_append) X(paged_decode_workspace) X(paged_decode)
+  X(paged_append) X(paged_decode_workspace) X(paged_decode) X(masked_fwd_workspace)        \
+  X(masked_fwd) X(masked_bwd_workspace) X(masked_bwd)
   VAFA_FNS(VAFA_FN)
 #undef VAFA_FN
 } api;
@@ -411,6 +412,46 @@ Tensor paged_decode(const Tensor &q_in, const Tensor &kc, const Tensor &vc, cons
   return out;
 }
 
+// Rows that the plan does not reach (possible where validation is off) as zeros.
+void clear_rest(const Tensor &t, int64_t rows) {
+  if (t.size(0) > rows) t.slice(0, rows).zero_();
+}
+
+std::tuple<Tensor, Tensor> masked_fwd(const Tensor &q, const Tensor &k, const Tensor &v,
+                                      const Plan &p, double scale, double softcap, int64_t window,
+                                      const std::optional<Tensor> &slopes) {
+  Call c(q);
+  const int64_t H = q.size(1), D = q.size(2);
+  const float *sl = slopes_of("packed_masked_attn", slopes, H, q);
+  Tensor o = c.like(q), lse = c.empty_f32({q.size(0), H});
+  void *ws = c.workspace(api.masked_fwd_workspace(&p.info, D));
+  check(api.masked_fwd(ptr(q), ptr(k), ptr(v), ptr(o), f32w(lse), p.dev(), &p.info, k.size(1), D,
+                       dtype_of(q), (float)scale, (float)softcap, window, sl, ws, c.ws_bytes(),
+                       c.stream));
+  clear_rest(o, p.info.T_q);
+  return {o, lse};
+}
+
+std::tuple<Tensor, Tensor, Tensor> masked_bwd(const Tensor &q, const Tensor &k, const Tensor &v,
+                                              const Tensor &o, const Tensor &lse, const Tensor &g,
+                                              const Plan &p, double scale, double softcap,
+                                              int64_t window,
+                                              const std::optional<Tensor> &slopes) {
+  Call c(q);
+  const int64_t H = q.size(1), D = q.size(2), Hk = k.size(1);
+  const float *sl = slopes_of("packed_masked_attn", slopes, H, q);
+  const Tensor dout = grad_in(g, q);
+  Tensor dq = c.like(q), dk = c.like(k), dv = c.like(v);
+  void *ws = c.workspace(api.masked_bwd_workspace(&p.info, Hk, D));
+  check(api.masked_bwd(ptr(q), ptr(k), ptr(v), ptr(o), ptr(dout), f32(lse), ptr(dq), ptr(dk),
+                       ptr(dv), p.dev(), &p.info, Hk, D, dtype_of(q), (float)scale, (float)softcap,
+                       window, sl, ws, c.ws_bytes(), c.stream));
+  clear_rest(dq, p.info.T_q);
+  clear_rest(dk, p.info.T_k);
+  clear_rest(dv, p.info.T_k);
+  return {dq, dk, dv};
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -436,6 +477,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("absorb_full_bwd", &absorb_full_bwd, no_gil);
   m.def("project_fwd", &project_fwd, no_gil);
   m.def("project_bwd", &project_bwd, no_gil);
+  m.def("masked_fwd", &masked_fwd, no_gil);
+  m.def("masked_bwd", &masked_bwd, no_gil);
   m.def("paged_append", &paged_append, no_gil);
   m.def("paged_decode", &paged_decode, no_gil);
 }

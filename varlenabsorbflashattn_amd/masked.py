@@ -1,0 +1,148 @@
+"""Packed attention of a language model: causal, windowed and prefix masks on packed
+sequences, grouped key heads, scores capped by a tanh, distance biases; forward and
+backward.  There is no counterpart in the reference, whose packed attention sees every
+key of a segment (:func:`packed_varlen_attn`).
+
+A host plan built from the lengths (cached by content, as for the other packed
+operators) names for every tile of queries the keys that some of its rows see, and for
+every tile of keys the queries that see it; tiles outside the mask are never read.
+"""
+from __future__ import annotations
+
+import math
+from typing import Optional
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib, varlen
+from .varlen import _aligned, _check_tokens, _normalize_qkv, _seqinfo_to_cu_seqlens
+
+
+def _plan_of(q, k, cu_seqlens_q, cu_seqlens_k, causal, window, prefix_lens):
+    """Validation and the device plan.  As for packed_varlen_attn, a cached plan of the
+    same content that covers exactly these tokens passed the checks when it was built."""
+    T_q, H, D = q.shape
+    T_k, Hk = k.shape[:2]
+    cu_q, cu_k = _lib.host_cu_pair(cu_seqlens_q, cu_seqlens_k)
+    prefix = None if prefix_lens is None else _lib.as_host_i64(prefix_lens)
+    if prefix is not None and prefix.shape != (cu_q.size - 1,):
+        raise AssertionError(f"prefix_lens must be [{cu_q.size - 1}], got {prefix.shape}")
+    dims = (H, Hk, D, causal, window, None if prefix is None else prefix.tobytes())
+    key = _lib.plan_key("masked", cu_q, cu_k, dims, q.device)
+    plan = _lib.cached_plan(key) if cu_q.ndim == 1 and cu_k.ndim == 1 else None
+    if plan is not None and plan.T_q == T_q and plan.T_k == T_k:
+        return plan.use()
+    cu_q_h, cu_k_h = _lib.as_host_i64(cu_q), _lib.as_host_i64(cu_k)
+    varlen._validate_cu_seqlens(cu_q_h, cu_seqlens_q.shape, T_q, "cu_seqlens_q")
+    varlen._validate_cu_seqlens(cu_k_h, cu_seqlens_k.shape, T_k, "cu_seqlens_k")
+    if cu_q_h.ndim != 1 or cu_q_h.size < 2:
+        raise ValueError("cu_seqlens_q: must be 1-D with at least 2 elements")
+    if plan is None:
+        plan = _lib.new_plan(key, cu_q_h, cu_k_h)
+    _check_tokens(plan.info, T_q, T_k)
+    return plan.use()
+
+
+class _PackedMaskedAttnFunction(torch.autograd.Function):
+
+    @staticmethod
+    def forward(ctx, q, k, v, cu_seqlens_q, cu_seqlens_k, causal, window, prefix_lens, softcap,
+                alibi_slopes, scale):
+        q, k, v = _aligned(q), _aligned(k), _aligned(v)
+        ops = _lib.ops()
+        plan = _plan_of(q, k, cu_seqlens_q, cu_seqlens_k, causal, window, prefix_lens)
+        o, lse = ops.masked_fwd(q, k, v, plan.native, scale, softcap, window, alibi_slopes)
+        ctx.save_for_backward(q, k, v, o, lse, alibi_slopes)
+        ctx.plan = plan
+        ctx.args = scale, softcap, window
+        return o
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, do):
+        q, k, v, o, lse, slopes = ctx.saved_tensors
+        grads = _lib.ops().masked_bwd(q, k, v, o, lse, do, ctx.plan.use().native, *ctx.args,
+                                      slopes)
+        return *grads, None, None, None, None, None, None, None, None
+
+
+def packed_masked_attn(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    *,
+    cu_seqlens_q: Optional[torch.Tensor] = None,
+    cu_seqlens_k: Optional[torch.Tensor] = None,
+    q_seqinfo: Optional[torch.Tensor] = None,
+    k_seqinfo: Optional[torch.Tensor] = None,
+    causal: bool = True,
+    window: Optional[int] = None,
+    prefix_lens: Optional[torch.Tensor] = None,
+    softcap: Optional[float] = None,
+    alibi_slopes: Optional[torch.Tensor] = None,
+    scale: Optional[float] = None,
+) -> torch.Tensor:
+    """Packed attention under a mask, within each segment.
+
+    ``q`` is ``[T_q, H, D]`` (or ``[1, T_q, H, D]``), ``k`` and ``v`` ``[T_k, H_k, D]``:
+    ``H / H_k`` query heads share a key head; bf16 or fp16, D 64, 128 or 256.  Segments
+    are given as for :func:`packed_varlen_attn`.  The queries of a segment are its last
+    positions: query i of n_q against n_k keys has position ``p = i + n_k - n_q`` and sees
+    key j where ``j <= p``, with ``window`` also ``j > p - window``, or where
+    ``j < prefix_lens[segment]`` (``[n_seg]``); every key with ``causal=False``, which
+    takes neither.  Scores are ``scale * q.k`` (default 1/sqrt(D)), then
+    ``softcap * tanh(. / softcap)``, then minus ``alibi_slopes[h]`` (float32 ``[H]``, no
+    gradient) times ``|p - j|``.  A row that sees no key gets zeros and no gradient.
+    The backward is deterministic.  Segments of at most 2^30 tokens together.
+    """
+    q3, q_was_4d = _normalize_qkv(q, "q")
+    k3, _ = _normalize_qkv(k, "k")
+    v3, _ = _normalize_qkv(v, "v")
+    T_q, H, D = q3.shape
+    T_k, H_k = k3.shape[:2]
+    assert k3.shape == v3.shape == (T_k, H_k, D), \
+        f"k and v must be [T_k, H_k, {D}], got {tuple(k3.shape)} and {tuple(v3.shape)}"
+    assert H_k >= 1 and H % H_k == 0 and H >= 1, \
+        f"{H} query heads do not divide among {H_k} key heads"
+    assert q3.dtype == k3.dtype == v3.dtype, "q/k/v must share dtype"
+    assert q3.dtype in (torch.bfloat16, torch.float16), \
+        f"dtype {q3.dtype} not supported (float16, bfloat16)"
+    assert D in (64, 128, 256), f"head_dim {D} not supported (64, 128, 256)"
+
+    if cu_seqlens_q is None:
+        if q_seqinfo is None:
+            raise ValueError("must provide either cu_seqlens_q or q_seqinfo")
+        cu_seqlens_q = _seqinfo_to_cu_seqlens(q_seqinfo)
+    if cu_seqlens_k is None:
+        if k_seqinfo is None:
+            raise ValueError("must provide either cu_seqlens_k or k_seqinfo")
+        cu_seqlens_k = _seqinfo_to_cu_seqlens(k_seqinfo)
+    n_seg = cu_seqlens_q.numel() - 1
+    assert cu_seqlens_k.numel() - 1 == n_seg, \
+        f"segment count mismatch: q has {n_seg}, k has {cu_seqlens_k.numel() - 1}"
+
+    if window is not None and window < 1:
+        raise ValueError(f"window must be positive, got {window}")
+    if softcap is not None and not (softcap > 0 and math.isfinite(softcap)):
+        raise ValueError(f"softcap must be positive and finite, got {softcap}")
+    if not causal and (window is not None or prefix_lens is not None):
+        raise ValueError("window and prefix_lens belong to the causal mask")
+    if scale is None:
+        scale = 1.0 / math.sqrt(D)
+    if not math.isfinite(scale):
+        raise ValueError(f"scale must be finite, got {scale}")
+    if alibi_slopes is not None:
+        assert alibi_slopes.shape == (H,) and alibi_slopes.dtype == torch.float32, \
+            f"alibi_slopes must be float32 [{H}]"
+        if alibi_slopes.requires_grad and torch.is_grad_enabled():
+            raise ValueError("alibi_slopes get no gradient: detach them")
+        alibi_slopes = alibi_slopes.contiguous()
+    assert q3.is_cuda, "packed_masked_attn requires GPU tensors"
+    assert all(t.device == q3.device for t in (k3, v3, alibi_slopes) if t is not None), \
+        "q/k/v and alibi_slopes must be on the same device"
+
+    o3 = _PackedMaskedAttnFunction.apply(q3, k3, v3, cu_seqlens_q, cu_seqlens_k, bool(causal),
+                                         int(window or 0), prefix_lens, float(softcap or 0.0),
+                                         alibi_slopes, float(scale))
+    return o3.unsqueeze(0) if q_was_4d else o3
