@@ -158,8 +158,9 @@ VAFA_API int vafa_plan_absorb(const int64_t *cu_q, const int64_t *cu_k, int64_t 
  * key heads.  causal: query i of a segment with nq queries and nk keys has position
  * p = i + nk - nq and sees key j where j <= p and j > p - window (window 0: no bound),
  * or j < prefix[segment] (prefix: host int64 [n1 - 1] or NULL).  Not causal: every key
- * (window 0, prefix NULL).  At most 2^30 tokens.  The same format, kind 3; xcd_heads
- * holds the parts into which the dK/dV pass divides a key head's query heads. */
+ * (window 0, prefix NULL).  At most 2^30 tokens.  The same format, kind 3: q_tile rows
+ * are (token, head) pairs of 2^xcd_heads heads that share a key head, kv items may be
+ * divided into parts, whose partial rows (n_fpart_rows) the fcomb items sum. */
 VAFA_API int vafa_plan_masked(const int64_t *cu_q, const int64_t *cu_k, const int64_t *prefix,
                               int64_t n1, int64_t H, int64_t Hk, int64_t D, int32_t causal,
                               int64_t window, int32_t *plan, int64_t plan_cap,
@@ -386,7 +387,7 @@ VAFA_API int vafa_absorb_project_f32_bwd(const float *q_raw, const float *W_Q, c
  * Hk, D and window.  Scores are scale q.k, then softcap tanh(. / softcap) (0: none),
  * then minus slopes[h] (device fp32 [H] or NULL) times |position of the query - key|.
  * Rows that see no key get zeros (lse -inf). */
-VAFA_API int64_t vafa_masked_fwd_workspace(const vafa_plan_info *info, int64_t D);
+VAFA_API int64_t vafa_masked_fwd_workspace(const vafa_plan_info *info, int64_t Hk, int64_t D);
 VAFA_API int vafa_masked_fwd(const void *q, const void *k, const void *v, void *o, float *lse,
                              const int32_t *plan_dev, const vafa_plan_info *info, int64_t Hk,
                              int64_t D, int32_t dtype, float scale, float softcap, int64_t window,

@@ -84,6 +84,13 @@ CASES = [
     ([100], [4000], 1, 1, 256, HF, {"softcap": 10.0, "alibi": True}),
     ([1] * 40, [1] * 40, 2, 2, 64, BF, {}),
     ([600, 700], None, 16, 8, 128, BF, {}),
+    # head sets of 4, 8, 16 and 32 rows, two sets a key head, and a divided dK/dV pass
+    ([50, 301], None, 24, 2, 64, BF, {"alibi": True}),
+    ([50, 31], [200, 31], 8, 1, 128, HF, {"alibi": True, "window": 40}),
+    ([9, 31], [9, 70], 16, 1, 64, BF, {"alibi": True, "softcap": 8.0}),
+    ([1, 0, 37], None, 64, 1, 256, BF, {"alibi": True, "prefix_lens": [1, 0, 5]}),
+    ([1500, 9], None, 16, 2, 64, BF, {}),
+    ([900], None, 8, 1, 256, HF, {"softcap": 9.0}),
 ]
 
 

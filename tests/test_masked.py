@@ -37,6 +37,8 @@ CASES = [
     ([1, 16], [20000, 9000], 1, 1, 128, True, 0, None),            # split over keys
     ([300], [9000], 2, 1, 64, True, 2500, [700]),                  # split across the gap
     ([2, 1], [0, 0], 1, 1, 64, True, 0, None),
+    ([70, 3000, 9], [70, 3000, 40], 24, 2, 128, True, 0, None),    # sets of 4 heads, parts
+    ([2000], [2000], 64, 1, 256, True, 300, [100]),                # sets of 32, parts
 ]
 
 
@@ -47,47 +49,69 @@ def test_plan_covers_the_mask(case):
     p = _lib.plan_masked(cq, ck, H, Hk, D, causal, window, prefix)
     info, win = p.info, window or 1 << 30
     assert (info.T_q, info.T_k, info.H, info.kind) == (cq[-1], ck[-1], H, 3)
-    assert info.xcd_heads >= 1 and (H // Hk) % info.xcd_heads == 0
+    sets = 1 << info.xcd_heads  # heads in the rows of a tile
+    assert (H // Hk) % sets == 0 and sets <= 32 and (sets == 32 or (H // Hk) % (2 * sets) != 0)
     see = np.zeros((cq[-1], ck[-1]), bool)
     for s in range(len(ql)):
         see[cq[s]:cq[s + 1], ck[s]:ck[s + 1]] = om.visible(
             ql[s], kl[s], causal, window, prefix[s] if prefix else 0)
     seg = np.searchsorted(cq, np.arange(cq[-1]), side="right") - 1
-    got = np.zeros(see.shape, int)
-    owners = np.zeros(cq[-1], int)
-    prows = set()
-    for it in p.section("fwd"):
-        q0, q1, k0, k1, pbase, diag, pre, owner = (int(x) for x in it)
-        assert 0 <= q0 < q1 <= cq[-1] and 0 <= k0 <= k1 <= ck[-1] and q1 - q0 <= info.q_tile
-        assert len(set(seg[q0:q1])) == 1
-        s = seg[q0]
-        assert diag == ck[s + 1] - cq[s + 1] and ck[s] <= k0 and k1 <= ck[s + 1]
-        assert pre == (ck[s + 1] if not causal else ck[s] + (prefix[s] if prefix else 0))
-        owners[q0:q1] += owner
-        if pbase >= 0:
-            rows = set(range(pbase, pbase + q1 - q0))
-            assert not rows & prows and pbase + q1 - q0 <= info.n_part_rows
-            prows |= rows
-        got[q0:q1, walked(it, win, 64)] += 1
-    assert (owners == 1).all()
-    assert got.max(initial=0) <= 1 and (got[see] == 1).all()
-    # combine items read exactly the split items' rows
-    read = set()
-    for q0, q1, pbase, ns, *_ in p.section("comb").tolist():
-        rows = set(range(pbase, pbase + ns * (q1 - q0)))
-        assert not rows & read
-        read |= rows
-    assert read == prows and len(prows) == info.n_part_rows
-    keys = np.zeros(ck[-1], int)
+    for items, sums, tile in (("fwd", "comb", info.q_tile), ("dq", "dqc", 128)):
+        got = np.zeros(see.shape, int)
+        owners = np.zeros(cq[-1], int)
+        prows = set()
+        for it in p.section(items):
+            q0, q1, k0, k1, pbase, diag, pre, owner = (int(x) for x in it)
+            assert 0 <= q0 < q1 <= cq[-1] and 0 <= k0 <= k1 <= ck[-1] and (q1 - q0) * sets <= tile
+            assert len(set(seg[q0:q1])) == 1
+            s = seg[q0]
+            assert diag == ck[s + 1] - cq[s + 1] and ck[s] <= k0 and k1 <= ck[s + 1]
+            assert pre == (ck[s + 1] if not causal else ck[s] + (prefix[s] if prefix else 0))
+            owners[q0:q1] += owner
+            if pbase >= 0:
+                rows = set(range(pbase, pbase + q1 - q0))
+                assert not rows & prows and pbase + q1 - q0 <= info.n_part_rows
+                prows |= rows
+            got[q0:q1, walked(it, win, 64)] += 1
+        assert (owners == 1).all()
+        assert got.max(initial=0) <= 1 and (got[see] == 1).all()
+        # the sums read exactly the split items' rows
+        read = set()
+        for q0, q1, pbase, ns, *_ in p.section(sums).tolist():
+            rows = set(range(pbase, pbase + ns * (q1 - q0)))
+            assert not rows & read
+            read |= rows
+        assert read == prows and len(prows) <= info.n_part_rows
+    # every key once, or by all the parts of its tile, which own the rows that are summed
+    keys, prows, parts_of = np.zeros(ck[-1]), {}, {}
     for it in p.section("kv"):
-        k0, k1, q0, q1, diag, pre, *_ = (int(x) for x in it)
+        k0, k1, q0, q1, diag, pre, pbase, part = (int(x) for x in it)
+        part, parts = part >> 16, part & 0xffff
         assert 0 <= k0 < k1 <= ck[-1] and 0 <= q0 <= q1 <= cq[-1] and k1 - k0 <= info.k_tile
-        keys[k0:k1] += 1
+        assert 0 <= part < parts and (pbase >= 0) == (parts > 1)
+        keys[k0:k1] += 1.0 / parts
+        parts_of.setdefault(k0, []).append((part, parts, pbase, k1 - k0))
         rows = np.zeros(cq[-1], bool)
         rows[q0:q1] = True
         assert not see[~rows, k0:k1].any()
         assert (seg[q0:q1] == np.searchsorted(ck, k0, side="right") - 1).all()
-    assert (keys == 1).all()
+    np.testing.assert_allclose(keys, 1.0)
+    sums = {k0: (k1, pbase, n) for k0, k1, pbase, n, *_ in p.section("fcomb").tolist()}
+    used = set()
+    for k0, got in parts_of.items():
+        got.sort()
+        assert [g[0] for g in got] == list(range(got[0][1]))
+        if got[0][1] == 1:
+            assert k0 not in sums
+            continue
+        k1, pbase, n = sums.pop(k0)
+        assert n == got[0][1] and k1 - k0 == got[0][3]
+        for part, _, at, rows in got:
+            assert at == pbase + part * rows
+            new = set(range(at, at + rows))
+            assert not new & used
+            used |= new
+    assert not sums and len(used) == info.n_fpart_rows
 
 
 def test_plan_refusals():
@@ -103,6 +127,7 @@ def test_plan_refusals():
     bad(ValueError, "window must be positive", 2, 1, 64, True, -1)
     bad(ValueError, r"prefix_lens\[1\] = 5 of 4", 2, 1, 64, True, 0, [4, 5])
     bad(ValueError, r"prefix_lens\[0\] = -1", 2, 1, 64, True, 0, [-1, 0])
+    assert _lib.plan_masked(c, c, 40, 1, 64).info.xcd_heads == 3
     bad(AssertionError, "prefix_lens must be", 2, 1, 64, True, 0, [1])
     big = np.array([0, (1 << 30) + 1])
     with pytest.raises(ValueError, match="more than"):
@@ -114,8 +139,9 @@ def test_c_abi_refusals():
     L = _lib.lib()
     p = _lib.plan_masked(cu([4]), cu([4]), 4, 2, 64)
     other = _lib.plan_varlen(cu([4]), cu([4]), 4, 64)
-    assert L.vafa_masked_fwd_workspace(other.info, 64) == -1
+    assert L.vafa_masked_fwd_workspace(other.info, 2, 64) == -1
     assert L.vafa_masked_bwd_workspace(p.info, 3, 64) == -1
+    assert L.vafa_masked_bwd_workspace(p.info, 1, 64) == -1  # built for other sets of heads
     assert L.vafa_masked_bwd_workspace(p.info, 2, 96) == -1
     assert L.vafa_varlen_fwd_workspace(p.info, 64) == -1  # and not the other way round
     need = L.vafa_masked_bwd_workspace(p.info, 2, 64)

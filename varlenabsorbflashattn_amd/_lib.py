@@ -113,7 +113,7 @@ _SIGS = {
     "vafa_absorb_fwd_full_workspace": (C.c_int64, [_PINFO, _I64, _I64, _I64]),
     "vafa_absorb_fwd_full": (C.c_int, [_P, _P, _P, _P, _P, _P, _P, _P, _I64, _P, _PINFO, _I64,
                                        _I64, _I64, _I32, C.c_float, _P, _I64, _P]),
-    "vafa_masked_fwd_workspace": (C.c_int64, [_PINFO, _I64]),
+    "vafa_masked_fwd_workspace": (C.c_int64, [_PINFO, _I64, _I64]),
     "vafa_masked_bwd_workspace": (C.c_int64, [_PINFO, _I64, _I64]),
     "vafa_masked_fwd": (C.c_int, [_P, _P, _P, _P, _P, _P, _PINFO, _I64, _I64, _I32, C.c_float,
                                   C.c_float, _I64, _P, _P, _I64, _P]),

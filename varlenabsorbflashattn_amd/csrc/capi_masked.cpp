@@ -24,15 +24,11 @@ int check_plan(const vafa_plan_info *info, int64_t Hk, int64_t D) {
   if (Hk < 1 || info->H < 1 || info->H % Hk != 0)
     return fail(VAFA_ERR_ASSERT, "%lld query heads do not divide among %lld key heads",
                 (long long)info->H, (long long)Hk);
-  const int64_t G = info->H / Hk;
-  if (info->xcd_heads < 1 || info->xcd_heads > G)
-    return fail(VAFA_ERR_VALUE, "the plan divides %lld heads into %lld parts", (long long)G,
-                (long long)info->xcd_heads);
+  if (info->xcd_heads != masked_set_log2(info->H / Hk))
+    return fail(VAFA_ERR_VALUE, "the plan was built for another number of key heads");
   const bool q_ok =
-      info->q_tile == kVarlenTile || (info->q_tile == kVarlenWideTile && D <= 128);
-  const bool k_ok =
-      info->k_tile == kVarlenTile || (info->k_tile == kVarlenWideTile && D == 128);
-  if (!q_ok || !k_ok)
+      info->q_tile == kVarlenTile || (info->q_tile == kVarlenWideTile && D == 128);
+  if (!q_ok || info->k_tile != kVarlenTile)
     return fail(VAFA_ERR_VALUE, "plan tiles (%lld queries, %lld keys) do not fit head_dim %lld",
                 (long long)info->q_tile, (long long)info->k_tile, (long long)D);
   return VAFA_OK;
@@ -75,9 +71,8 @@ Ws carve(void *ws, const vafa_plan_info *info, int64_t Hk, int64_t D, bool bwd) 
   } else {
     w.delta = take(info->T_q * info->H);
     w.lse = take(info->T_q * info->H);
-    const int64_t parts = info->xcd_heads > 1 ? info->xcd_heads : 0;
-    w.part_dk = take(parts * info->T_k * Hk * D);
-    w.part_dv = take(parts * info->T_k * Hk * D);
+    w.part_dk = take(info->n_fpart_rows * Hk * D);
+    w.part_dv = take(info->n_fpart_rows * Hk * D);
   }
   w.bytes = used;
   return w;
@@ -90,11 +85,12 @@ MaskedArgs args_of(const vafa_plan_info *info, const int32_t *plan, int64_t Hk, 
   a.comb_items = plan + info->off_comb; a.n_comb = info->n_comb;
   a.comb_rows = (int)info->max_comb_rows;
   a.kv_items = plan + info->off_kv; a.n_kv = info->n_kv;
-  a.T_k = info->T_k;
+  a.kvc_items = plan + info->off_fcomb; a.n_kvc = info->n_fcomb;
+  a.kvc_rows = (int)info->max_fcomb_rows;
   a.H = (int)info->H; a.Hk = (int)Hk; a.D = (int)D;
-  a.q_tile = (int)info->q_tile; a.k_tile = (int)info->k_tile;
+  a.q_tile = (int)info->q_tile;
   a.window = (int)(window > 0 ? std::min(window, kMaskedMaxTokens) : kMaskedMaxTokens);
-  a.gsplit = (int)info->xcd_heads;
+  a.lg = masked_set_log2(info->H / Hk);
   a.slopes = slopes;
   a.scale = scale;
   a.c = softcap > 0.f ? 2.f * kLog2e * scale / softcap : scale * kLog2e;
@@ -121,8 +117,7 @@ void fwd(const MaskedArgs &a, hipStream_t st) {
   if (a.D == 64) launch_masked_fwd<T, 64>(a, st);
   if (a.D == 128) launch_masked_fwd<T, 128>(a, st);
   if (a.D == 256) launch_masked_fwd<T, 256>(a, st);
-  launch_lse_combine<T>(a.part_o, a.part_lse, a.o, a.lse, a.comb_items, a.n_comb, a.H, a.D,
-                        a.comb_rows, st);
+  launch_masked_join<T>(a, st);
 }
 
 template <typename T>
@@ -130,11 +125,10 @@ void bwd(const MaskedArgs &a, hipStream_t st) {
   if (a.D == 64) launch_masked_dq<T, 64>(a, st);
   if (a.D == 128) launch_masked_dq<T, 128>(a, st);
   if (a.D == 256) launch_masked_dq<T, 256>(a, st);
-  launch_sum_combine<T>(a.part_o, a.dq, a.comb_items, a.n_comb, a.H, a.D, a.comb_rows, st);
   if (a.D == 64) launch_masked_dkv<T, 64>(a, st);
   if (a.D == 128) launch_masked_dkv<T, 128>(a, st);
   if (a.D == 256) launch_masked_dkv<T, 256>(a, st);
-  launch_masked_group_sum<T>(a, st);
+  launch_masked_sum<T>(a, st);
 }
 
 }  // namespace
@@ -144,9 +138,9 @@ using namespace vafa;
 
 extern "C" {
 
-int64_t vafa_masked_fwd_workspace(const vafa_plan_info *info, int64_t D) {
-  if (check_plan(info, 1, D)) return -1;
-  return carve(nullptr, info, 1, D, false).bytes;
+int64_t vafa_masked_fwd_workspace(const vafa_plan_info *info, int64_t Hk, int64_t D) {
+  if (check_plan(info, Hk, D)) return -1;
+  return carve(nullptr, info, Hk, D, false).bytes;
 }
 
 int64_t vafa_masked_bwd_workspace(const vafa_plan_info *info, int64_t Hk, int64_t D) {
@@ -182,6 +176,9 @@ int vafa_masked_bwd(const void *q, const void *k, const void *v, const void *o, 
   const Ws w = carve(workspace, info, Hk, D, true);
   if (int rc = check_ws(workspace_bytes, workspace, w.bytes)) return rc;
   MaskedArgs a = args_of(info, plan_dev, Hk, D, scale, softcap, window, slopes);
+  a.items = plan_dev + info->off_dq; a.n_items = info->n_dq;
+  a.comb_items = plan_dev + info->off_dqc; a.n_comb = info->n_dqc;
+  a.comb_rows = (int)info->max_dqc_rows;
   a.q = q; a.k = k; a.v = v; a.o_in = o; a.dout = dout; a.lse_in = lse;
   a.dq = dq; a.dk = dk; a.dv = dv;
   a.part_o = w.part_o; a.delta = w.delta; a.lse = w.lse;

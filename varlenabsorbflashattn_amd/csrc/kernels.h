@@ -115,12 +115,12 @@ struct MaskedArgs {
   const float *lse_in, *slopes;  // slopes: or null
   float *delta;                  // [T_q, H] workspace (backward)
   float *part_o, *part_lse;      // split partial rows: O (and LSE) or dQ
-  float *part_dk, *part_dv;      // [gsplit, T_k, Hk, D] fp32 where gsplit > 1
-  const int32_t *items, *comb_items, *kv_items;
-  int64_t n_items, n_comb, n_kv;
-  int comb_rows;
-  int64_t T_k;
-  int H, Hk, D, q_tile, k_tile, window, gsplit;
+  float *part_dk, *part_dv;      // fp32 rows [rows, Hk, D] of divided key tiles
+  const int32_t *items, *comb_items, *kv_items, *kvc_items;
+  int64_t n_items, n_comb, n_kv, n_kvc;
+  int comb_rows, kvc_rows;
+  int H, Hk, D, q_tile, window;
+  int lg;  // log2 of the heads in a set (masked.h)
   float scale, c, cap2;  // c: factor on q.k (masked.h); cap2: cap log2 e, 0 without
 };
 
@@ -221,10 +221,12 @@ template <typename T> void launch_paged_decode(const DecodeArgs &, int D, int gr
 
 // masked_fwd.hip, masked_bwd.hip (bf16 / f16, D in {64, 128, 256})
 template <typename T, int D> void launch_masked_fwd(const MaskedArgs &, hipStream_t);
+// o and lse of split tiles from their partial rows
+template <typename T> void launch_masked_join(const MaskedArgs &, hipStream_t);
 template <typename T, int D> void launch_masked_dq(const MaskedArgs &, hipStream_t);
 template <typename T, int D> void launch_masked_dkv(const MaskedArgs &, hipStream_t);
-// dk = scale * sum, dv = sum of the fp32 partials of gsplit head groups, in order
-template <typename T> void launch_masked_group_sum(const MaskedArgs &, hipStream_t);
+// dq, dk and dv of divided tiles: ordered sums of their fp32 partial rows
+template <typename T> void launch_masked_sum(const MaskedArgs &, hipStream_t);
 
 // varlen_mfma.hip (bf16 / f16, D in {32, 64, 128, 256})
 template <typename T, int D> void launch_mfma_varlen_fwd(const VarlenArgs &, hipStream_t);

@@ -62,14 +62,32 @@ struct ScoreArgs {
 };
 // |c| as the factor of scores that may be -inf: not 0, which would make them NaN (2^-126
 // times a score below 2^100 is 0 beside any other part of the exponent).
-__device__ __forceinline__ float score_factor(float c) { return fmaxf(fabsf(c), 0x1p-126f); }
+__device__ __forceinline__ float score_factor(float c) {
+  // (back to a scalar register: the scalar unit has no float max)
+  return __int_as_float(
+      __builtin_amdgcn_readfirstlane(__float_as_int(fmaxf(fabsf(c), 0x1p-126f))));
+}
 __device__ __forceinline__ float cap_e(float z) {
   return __builtin_amdgcn_rcpf(1.f + fast_exp2(z));
 }
 
-// head h of query heads = (group g, member): consecutive workgroups of an item take the
-// same key head every Hk, so that with Hk a multiple of the XCDs one XCD's L2 serves it
-__device__ __forceinline__ int head_of(int i, int Hk, int G) { return (i % Hk) * G + i / Hk; }
+// Query heads that share a key head are rows of one tile: of the G = H / Hk heads, sets
+// of gp = 2^lg (the largest power of two that divides G, at most 32) lie beside each
+// other in memory, and row r of a tile is head r % gp of token r / gp.  A tile of 128
+// rows then spans 128 / gp tokens: short segments fill it, and the mask's border cuts
+// fewer of its (row, key) pairs.
+struct HeadSets {
+  int H, Hk, lg;
+  __device__ __forceinline__ int sets() const { return H >> lg; }       // of all heads
+  __device__ __forceinline__ int per_key() const { return (H / Hk) >> lg; }
+  // set of workgroup i among an item's: consecutive ones take the same key head every
+  // Hk, so that with Hk a multiple of the XCDs one XCD's L2 serves it
+  __device__ __forceinline__ int set_of(int i) const { return (i % Hk) * per_key() + i / Hk; }
+  // offset of local row r (in heads) from the set's first head of the tile's first token
+  __device__ __forceinline__ int row(int r) const {
+    return (r >> lg) * H + (r & ((1 << lg) - 1));
+  }
+};
 
 }  // namespace
 

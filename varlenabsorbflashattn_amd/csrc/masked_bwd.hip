@@ -4,11 +4,12 @@
 // out as the packed varlen backward (varlen_bwd_mfma.hip):
 //   * dQ, query-major over the forward's items: S^T = K Q^T, dP^T = V dO^T,
 //     dQ^T += K^T dS^T, and delta = rowsum(O dO) for the other kernel;
-//   * dK/dV, key-major: a workgroup owns a key tile of one key head, walks the queries
-//     that see it of every query head that shares the key head (of one of gsplit parts
-//     of them, where a launch has few key tiles: fp32 partials, summed in order), and
-//     accumulates dV^T += dO^T P, dK^T += Q^T dS.
+//   * dK/dV, key-major: a workgroup owns a key tile of one key head, walks blocks of 32
+//     (token, head) rows that see it, of every query head that shares the key head (or a
+//     part of those blocks, where one workgroup's walk would outlast the launch: fp32
+//     partials, summed in order), and accumulates dV^T += dO^T P, dK^T += Q^T dS.
 // With y = cap tanh(z / cap): dz = dx (1 - tanh^2), formed from e of cap_e as 4 e (1 - e).
+#include <algorithm>
 #include <type_traits>
 
 #include "bwd_tiles.h"
@@ -27,7 +28,7 @@ __global__ __launch_bounds__(64 * NW, D >= 256 ? 1 : 2) void masked_dq_kernel(
     const T *__restrict__ dout, const T *__restrict__ o, const float *__restrict__ lse,
     float *__restrict__ delta, float *__restrict__ lse_out, T *__restrict__ dq,
     float *__restrict__ part_dq, const int32_t *__restrict__ items,
-    const float *__restrict__ slopes, ScoreArgs sa, int H, int Hk, int window, float scale) {
+    const float *__restrict__ slopes, ScoreArgs sa, HeadSets hs, int window, float scale) {
   using M = Mfma<T>;
   using S = DqSmem<D>;
   using L = GTile<D>;
@@ -37,19 +38,21 @@ __global__ __launch_bounds__(64 * NW, D >= 256 ? 1 : 2) void masked_dq_kernel(
   extern __shared__ __align__(16) unsigned char smem_raw[];
   T *smem = reinterpret_cast<T *>(smem_raw);
 
-  const int G = H / Hk;
-  const int item = blockIdx.x / H, h = head_of(blockIdx.x % H, Hk, G), hk = h / G;
+  const int H = hs.H, lg = hs.lg, tw = 32 >> lg;  // tokens of a wave
+  const int item = blockIdx.x / hs.sets(), set = hs.set_of(blockIdx.x % hs.sets());
+  const int h0 = set << lg, hk = set / hs.per_key();
   const PlanItem it = load_item(items, item);
   const int q0 = it.v[0], q1 = it.v[1], pbase = it.v[4], diag = it.v[5], pre = it.v[6];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lrow = lane & 31, lhalf = lane >> 5;
-  const int qrow = q0 + wave * 32 + lrow;
-  const bool row_ok = qrow < q1;
-  const bool wave_active = q0 + wave * 32 < q1;
-  const int p = qrow + diag;
-  const int p0 = q0 + wave * 32 + diag;
-  const int p1 = (q0 + wave * 32 + 31 < q1 ? q0 + wave * 32 + 31 : q1 - 1) + diag;
+  const int t0 = q0 + wave * tw;  // the wave's first token
+  const int tok = t0 + (lrow >> lg), h = h0 + (lrow & ((1 << lg) - 1));
+  const bool row_ok = tok < q1;
+  const bool wave_active = t0 < q1;
+  const int p = tok + diag;
+  const int p0 = t0 + diag;
+  const int p1 = (t0 + tw < q1 ? t0 + tw : q1) - 1 + diag;
   const KeyWalk kw = key_walk<kRB>(it.v[2], it.v[3], pre, q0 + diag - window + 1);
 
   constexpr int NS = 32 * NW;  // staging threads per tensor
@@ -62,7 +65,7 @@ __global__ __launch_bounds__(64 * NW, D >= 256 ? 1 : 2) void masked_dq_kernel(
     store_rows<T, D, NS>(stg, stage_k ? ks : ks + S::kKs, st);
   };
   auto load = [&](int j) {
-    load_rows<T, D, NS>(stg, src, walk_key<kRB>(kw, j), walk_end(kw, j), Hk, hk, st);
+    load_rows<T, D, NS>(stg, src, walk_key<kRB>(kw, j), walk_end(kw, j), hs.Hk, hk, st);
   };
   const int nblk = kw.n;
   if (nblk > 0) load(0);
@@ -77,10 +80,11 @@ __global__ __launch_bounds__(64 * NW, D >= 256 ? 1 : 2) void masked_dq_kernel(
   float Dr;
   {
     const int64_t nb = (int64_t)(q1 - q0) * H * D * 2;
-    const rsrc_t rq = make_rsrc(q + (int64_t)q0 * H * D, nb);
-    const rsrc_t rd = make_rsrc(dout + (int64_t)q0 * H * D, nb);
-    const rsrc_t ro = make_rsrc(o + (int64_t)q0 * H * D, nb);
-    const int off = ((wave * 32 + lrow) * H + h) * D * 2 + lhalf * 16;
+    const int64_t base = ((int64_t)q0 * H + h0) * D;
+    const rsrc_t rq = make_rsrc(q + base, nb);
+    const rsrc_t rd = make_rsrc(dout + base, nb);
+    const rsrc_t ro = make_rsrc(o + base, nb);
+    const int off = hs.row(wave * 32 + lrow) * D * 2 + lhalf * 16;
     u32x4 ov[NC];
 #pragma unroll
     for (int cc = 0; cc < NC; ++cc) ov[cc] = buf_load16(ro, off + cc * 32);
@@ -106,11 +110,11 @@ __global__ __launch_bounds__(64 * NW, D >= 256 ? 1 : 2) void masked_dq_kernel(
     Dr = sc + __shfl_xor(sc, 32, 64);
   }
   // rows past q1, and rows that see no key, get LSE = +inf: their P is 0
-  float Lr = row_ok ? lse[(int64_t)qrow * H + h] : __builtin_inff();
+  float Lr = row_ok ? lse[(int64_t)tok * H + h] : __builtin_inff();
   if (Lr == kNegInf) Lr = __builtin_inff();
   if (row_ok && lhalf == 0 && it.v[7] != 0) {  // the item that owns its rows' first keys
-    delta[(int64_t)qrow * H + h] = Dr;
-    lse_out[(int64_t)qrow * H + h] = Lr;
+    delta[(int64_t)tok * H + h] = Dr;
+    lse_out[(int64_t)tok * H + h] = Lr;
   }
   asm volatile("" : "+v"(Lr), "+v"(Dr));
   float slope2 = 0.f;
@@ -232,26 +236,69 @@ __global__ __launch_bounds__(64 * NW, D >= 256 ? 1 : 2) void masked_dq_kernel(
   if (!wave_active) return;
   using RS = RowStore<T, ND>;
   unsigned char *stage = smem_raw + wave * RS::kBytes;
-  const int rows = uniform_clamp(q1 - (q0 + wave * 32), 32);
+  const int rows = uniform_clamp(q1 - t0, tw) << lg;
+  auto off = [&](int r) { return (int64_t)hs.row(r) * D; };
   if (pbase < 0)
-    RS::rows16(acc, [&](float x) { return static_cast<T>(x * scale); }, stage,
-               dq + ((int64_t)(q0 + wave * 32) * H + h) * D, (int64_t)H * D, rows);
+    RS::rows16_at(acc, [&](float x) { return static_cast<T>(x * scale); }, stage,
+                  dq + ((int64_t)t0 * H + h0) * D, off, rows);
   else
-    RS::rows32(acc, scale, stage, part_dq + ((int64_t)(pbase + wave * 32) * H + h) * D,
-               (int64_t)H * D, rows);
+    RS::rows32_at(acc, scale, stage, part_dq + ((int64_t)(pbase + wave * tw) * H + h0) * D, off,
+                  rows);
+}
+
+// LDS-DMA of 32 rows of a head set (tokens from t0 on, rows at or past `rows` read as
+// zero) into a GTile block, as dma_block_rows.
+template <typename T, int D, int NW>
+__device__ __forceinline__ void dma_set_rows(const T *src, int ntok, const HeadSets &hs,
+                                             uint32_t base, int wave, int lane) {
+  using L = GTile<D>;
+  const u32x4 rs = rsrc_words32(src, (uint32_t)(ntok * hs.H * D * 2));
+  if constexpr (D <= 64) {
+    constexpr int kInstr = (L::kElems / 8 + 63) / 64;
+    for (int i = wave; i < kInstr; i += NW) {
+      const int e = (i * 64 + lane) * 8;  // element offset of this lane's 16 bytes
+      const int g = e / L::P2, w = e - g * L::P2;
+      const int j = w / L::P1, wr = w - j * L::P1;
+      if (e < L::kElems && j < 4 && wr < D)
+        lds_dma16(rs, base + i * 1024, (hs.row(4 * g + j) * D + wr) * 2);
+    }
+  } else {
+    constexpr int RPW = kRB / NW;
+    if (lane < D / 8) {
+      int r0 = wave * RPW;
+      asm volatile("" : "+s"(r0));  // the rows' offsets are formed here, not held
+#pragma unroll
+      for (int n = 0; n < RPW; ++n) {
+        int voff;
+        asm volatile("v_add_u32 %0, %1, %2"
+                     : "=v"(voff)
+                     : "s"(hs.row(r0 + n) * D * 2), "v"(lane * 16));
+        lds_dma16(rs, base + L::row(r0 + n) * 2, voff);
+      }
+    }
+  }
 }
 
 // ---- dK / dV -----------------------------------------------------------------------
+// Two buffers of a query block: Q and dO rows, then LSE, delta and (with a bias) the
+// slopes of its rows; and the last DMA instruction's span past its tile.
+template <int D>
+struct MDkvSmem {
+  static constexpr int kQs = GTile<D>::kElems;
+  static constexpr int kVec = 2 * kQs * 2;  // byte offset of the vectors
+  static constexpr int kBufBytes = kVec + 3 * kRB * 4;
+  static constexpr int kBytes = 2 * kBufBytes + 1024;
+};
+
 template <typename T, int D, int NW, bool kCap, bool kBias>
 __global__ __launch_bounds__(64 * NW, D >= 256 && NW < 8 ? 1 : 2) void masked_dkv_kernel(
     const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v,
     const T *__restrict__ dout, const float *__restrict__ lse, const float *__restrict__ delta,
     T *__restrict__ dk, T *__restrict__ dv, float *__restrict__ part_dk,
     float *__restrict__ part_dv, const int32_t *__restrict__ items,
-    const float *__restrict__ slopes, ScoreArgs sa, int H, int Hk, int window, int gsplit,
-    int64_t T_k, float scale) {
+    const float *__restrict__ slopes, ScoreArgs sa, HeadSets hs, int window, float scale) {
   using M = Mfma<T>;
-  using S = DkvSmem<D>;
+  using S = MDkvSmem<D>;
   using L = GTile<D>;
   constexpr int ND = D / 32;
   constexpr int kPre = D >= 128 ? 2 : 4;
@@ -264,12 +311,11 @@ __global__ __launch_bounds__(64 * NW, D >= 256 && NW < 8 ? 1 : 2) void masked_dk
   constexpr bool kLog2 = kCap || kBias;
   extern __shared__ __align__(16) unsigned char smem_raw[];
 
-  const int G = H / Hk;
-  const int item = blockIdx.x / (Hk * gsplit), part = blockIdx.x % (Hk * gsplit);
-  const int hk = part % Hk, gs = part / Hk;
-  const int hg0 = hk * G + G * gs / gsplit, hg1 = hk * G + G * (gs + 1) / gsplit;
+  const int H = hs.H, Hk = hs.Hk, lg = hs.lg, tb = kRB >> lg;  // tokens of a block
+  const int item = blockIdx.x / Hk, hk = blockIdx.x % Hk;
   const PlanItem it = load_item(items, item);
-  const int k0 = it.v[0], k1 = it.v[1], q0 = it.v[2], q1 = it.v[3], diag = it.v[4], pre = it.v[5];
+  const int k0 = it.v[0], k1 = it.v[1], q0 = it.v[2], q1 = it.v[3], diag = it.v[4], pre = it.v[5],
+            pbase = it.v[6];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int kgrp = kShare ? (wave & 3) : wave;
@@ -279,18 +325,31 @@ __global__ __launch_bounds__(64 * NW, D >= 256 && NW < 8 ? 1 : 2) void masked_dk
   const int kw1 = (kw0 + 32 < k1 ? kw0 + 32 : k1) - 1;
   const bool wave_active = kw0 < k1;
 
-  auto issue = [&](int h, int qb, int buf) {
+  auto issue = [&](int set, int qb, int buf) {
     unsigned char *base = smem_raw + buf * S::kBufBytes;
-    dma_block_rows<T, D, NW>(q, qb, q1, H, h, lds_addr(base), wave, lane);
-    dma_block_rows<T, D, NW>(dout, qb, q1, H, h, lds_addr(base + S::kQs * 2), wave, lane);
-    const float *vec = (wave & 1) ? delta : lse;
-    const int rows = uniform_clamp(q1 - qb, kRB);
-    const u32x4 rv = rsrc_words32(vec + (int64_t)qb * H + h, (uint32_t)(rows * H * 4));
-    if (lane < kRB) lds_dma4(rv, lds_addr(base + 2 * S::kQs * 2 + (wave & 1) * kRB * 4), lane * H * 4);
+    const int ntok = uniform_clamp(q1 - qb, tb);
+    const int64_t at = (int64_t)qb * H + (set << lg);
+    dma_set_rows<T, D, NW>(uniform_ptr(q + at * D), ntok, hs, lds_addr(base), wave, lane);
+    dma_set_rows<T, D, NW>(uniform_ptr(dout + at * D), ntok, hs, lds_addr(base + S::kQs * 2), wave,
+                           lane);
+    // LSE, delta and slopes of the rows: a wave each
+    if (wave < 2) {
+      const u32x4 rv = rsrc_words32((wave ? delta : lse) + at, (uint32_t)(ntok * H * 4));
+      if (lane < kRB) lds_dma4(rv, lds_addr(base + S::kVec + wave * kRB * 4), hs.row(lane) * 4);
+    } else if (kBias && wave == 2) {
+      const u32x4 rv = rsrc_words32(slopes + (set << lg), 4u << lg);
+      if (lane < kRB)
+        lds_dma4(rv, lds_addr(base + S::kVec + 2 * kRB * 4), (lane & ((1 << lg) - 1)) * 4);
+    }
   };
-  const int nq = (q1 - q0 + kRB - 1) / kRB;  // query blocks of one head
-  const int nblk = nq * (hg1 - hg0);
-  if (nblk > 0) issue(hg0, q0, 0);
+  // the blocks of the key head's sets, one set after the other; a part of them where the
+  // plan divides a key tile's work (v[7]: part << 16 | parts)
+  const int nq = (q1 - q0 + tb - 1) / tb, nset = hs.per_key();
+  const int64_t all = (int64_t)nq * nset;
+  const int part = it.v[7] >> 16, parts = it.v[7] & 0xffff;
+  const int f0 = (int)(all * part / parts), nblk = (int)(all * (part + 1) / parts) - f0;
+  int set = hk * nset + (nq > 0 ? f0 / nq : 0), qb = q0 + (nq > 0 ? f0 % nq : 0) * tb;
+  if (nblk > 0) issue(set, qb, 0);
 
   uint32_t ksign = 0;  // a negative scale, folded into K's part of the scores
   if constexpr (!kLog2) {
@@ -326,23 +385,22 @@ __global__ __launch_bounds__(64 * NW, D >= 256 && NW < 8 ? 1 : 2) void masked_dk
   const int a_off = L::row(lrow) + lhalf * 8 + dpart * NDO * 32;
   const int t_off = L::row(4 * (lane >> 5) + ((lane & 15) >> 2)) + ((lane >> 4) & 1) * 16 +
                     4 * (lane & 3);
-  int h = hg0, qb = q0;  // of the current block
   auto blk = [&](int j, auto bufc) {
     constexpr int B = decltype(bufc)::value;
-    const int hc = h, qc = qb;
-    qb += kRB;
+    const int qc = qb;  // the block's first token
+    qb += tb;
     if (qb >= q1) {
       qb = q0;
-      ++h;
+      ++set;
     }
     wait_vmcnt<0>();
     __syncthreads();
-    if (j + 1 < nblk) issue(h, qb, 1 - B);
+    if (j + 1 < nblk) issue(set, qb, 1 - B);
     const unsigned char *base = smem_raw + B * S::kBufBytes;
     const lds_cptr<T> qs = as_lds(reinterpret_cast<const T *>(base));
     const lds_cptr<T> ds_ = qs + S::kQs;
-    const float *ls = reinterpret_cast<const float *>(base + 2 * S::kQs * 2);
-    const int p0 = qc + diag, p1 = (qc + kRB < q1 ? qc + kRB : q1) - 1 + diag;
+    const float *ls = reinterpret_cast<const float *>(base + S::kVec);
+    const int p0 = qc + diag, p1 = (qc + tb < q1 ? qc + tb : q1) - 1 + diag;
     const bool active = wave_active && !none_visible(kw0, kw1, p0, p1, pre, window);
     f32x16 s, dp;
     if (active) {
@@ -402,6 +460,8 @@ __global__ __launch_bounds__(64 * NW, D >= 256 && NW < 8 ? 1 : 2) void masked_dk
             s[4 * g + e] += a[e];
             dp[4 * g + e] += b[e];
           }
+          // the partner's registers in two halves: all 32 beside the own 32 would not fit
+          if (g == 1) asm volatile("" : "+v"(s), "+v"(dp)::"memory");
         }
       }
     }
@@ -411,76 +471,93 @@ __global__ __launch_bounds__(64 * NW, D >= 256 && NW < 8 ? 1 : 2) void masked_dk
                                ((i / NDO) >> 1) * 4 * L::P2 + (dpart * NDO + i % NDO) * 32;
         return as_v8<T>(join(lds_tr8<T>(tp), lds_tr8<T>(tp + 2 * L::P2)));
       };
-      typename M::v8 tring[kPre];
+      // register r of a lane is row (lane / 32) * 4 + (r / 4) * 8 + r % 4 of the block.  Of
+      // the rows that the lane's key sees, one bit each: one register, not 16 tokens
+      int ln = lane;
+      asm volatile("" : "+v"(ln));  // formed per block
+      const int row0 = (ln >> 5) * 4, kj = kw0 + (ln & 31);
+      const bool masked = qc + tb > q1 || !all_visible(kw0, kw1, p0, p1, pre, window);
+      uint32_t bits = ~0u;
+      if (masked) {
+        const bool in_pre = kj < pre;
+        const int first = kj - diag - qc, last = first + window;
+        int lo = in_pre || first < 0 ? 0 : first, hi = q1 - qc;  // tokens of the block
+        hi = !in_pre && last < hi ? last : hi;
+        hi = hi < tb ? hi : tb;
+        bits = lo < hi ? (~0u >> (kRB - (hi << lg)) & ~0u << (lo << lg)) >> row0 : 0u;
+      }
+      auto seen = [&](int r) { return (bits >> ((r >> 2) * 8 + (r & 3)) & 1) != 0; };
+      if constexpr (!kLog2) {
+        if (masked) {
 #pragma unroll
-      for (int i = 0; i < kPre; ++i) tring[i] = top(i);
-      // row r of a lane is query q_lane + off(r), its key kw0 + lrow
-      const int q_lane = qc + lhalf * 4;
-      auto off = [](int r) { return (r >> 2) * 8 + (r & 3); };
-      // with a cap, dP - delta is formed (and multiplied by the cap's derivative) here
-      constexpr bool kDeltaHere = kCap && !kDeltaInChain;
-      if constexpr (kLog2) {
-        const float back = (float)(q_lane + diag - kw0 - lrow);
-        float slope2 = 0.f;
-        if constexpr (kBias) slope2 = slopes[hc] * kLog2e;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
+          for (int r = 0; r < 16; ++r) {
+            if (!seen(r)) s[r] = kNegInf;
+            if (r % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+          }
+        }
+      }
+      const int back = qc + diag - kj;
+      // P and dS of register r, in place of the score and of dP (delta - dP with
+      // kDeltaInChain); hidden pairs are masked above, or here where the score is
+      // transformed first
+      auto elem = [&](int r, float lr, float dl, float sl) {
+        float p, d = dp[r];
+        if constexpr (kLog2) {
           float z = s[r] * sa.c;
           if constexpr (kCap) {
             const float e = cap_e(z), e4 = 4.f * e;
             z = __builtin_fmaf(-2.f * sa.cap2, e, sa.cap2);
-            if constexpr (kDeltaHere) dp[r] -= ls[kRB + off(r) + lhalf * 4];
-            dp[r] *= __builtin_fmaf(-e4, e, e4);
+            if constexpr (!kDeltaInChain) d -= dl;
+            d *= __builtin_fmaf(-e4, e, e4);
+          } else {
+            if constexpr (!kDeltaInChain) d -= dl;
           }
-          if constexpr (kBias) z = __builtin_fmaf(-slope2, fabsf(back + (float)off(r)), z);
-          s[r] = z;
+          if constexpr (kBias) {
+            const int t = (row0 + (r >> 2) * 8 + (r & 3)) >> lg;
+            z = __builtin_fmaf(-kLog2e * sl, fabsf((float)(back + t)), z);
+          }
+          p = fast_exp2(z - lr);
+          p = seen(r) ? p : 0.f;
+        } else {
+          p = fast_exp2(__builtin_fmaf(s[r], sa.c, -lr));
+          if constexpr (!kDeltaInChain) d -= dl;
         }
-      }
-      if (qc + kRB > q1 || !all_visible(kw0, kw1, p0, p1, pre, window)) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int qr = q_lane + off(r);
-          if (qr >= q1 || !visible(kw0 + lrow, qr + diag, pre, window)) s[r] = kNegInf;
-        }
-      }
-      auto p_of = [&](float x, float lr) {
-        return fast_exp2(kLog2 ? x - lr : __builtin_fmaf(x, sa.c, -lr));
+        s[r] = p;
+        dp[r] = kDeltaInChain ? -(p * d) : p * d;
       };
-      auto ds_of = [&](float p, float a, float dl) {
-        if constexpr (kDeltaInChain)
-          return -(p * a);
-        else if constexpr (kDeltaHere)
-          return p * a;
-        else
-          return p * (a - dl);
-      };
-      constexpr bool kDl = !kDeltaInChain && !kDeltaHere;
       typename M::v8 pb[2], sb[2];
 #pragma unroll
       for (int g = 0; g < 2; ++g) {
-        const f32x4 Lq = *reinterpret_cast<const f32x4 *>(ls + g * 8 + lhalf * 4);
-        const f32x4 Dl = kDl ? *reinterpret_cast<const f32x4 *>(ls + kRB + g * 8 + lhalf * 4)
-                             : f32x4{0.f, 0.f, 0.f, 0.f};
+        const float *at = ls + g * 8 + lhalf * 4;
+        const f32x4 Lq = *reinterpret_cast<const f32x4 *>(at);
+        f32x4 Dl = f32x4{0.f, 0.f, 0.f, 0.f}, Sl = Dl;
+        if constexpr (!kDeltaInChain) Dl = *reinterpret_cast<const f32x4 *>(at + kRB);
+        if constexpr (kBias) Sl = *reinterpret_cast<const f32x4 *>(at + 2 * kRB);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int r = g * 4 + e;
-          const float p = p_of(s[r], Lq[e]);
-          s[r] = p;
-          dp[r] = ds_of(p, dp[r], Dl[e]);
-        }
+        for (int e = 0; e < 4; ++e) elem(g * 4 + e, Lq[e], Dl[e], Sl[e]);
+        if constexpr (kLog2 || D >= 128) __builtin_amdgcn_sched_barrier(0);
       }
       pb[0] = pack8<T>(s, 0);
       sb[0] = pack8<T>(dp, 0);
+      __builtin_amdgcn_sched_barrier(0);
+      typename M::v8 tring[kPre];
+#pragma unroll
+      for (int i = 0; i < kPre; ++i) tring[i] = top(i);
+      // rows 8..15 under the first half of the chain, which reads rows 0..7 alone
       constexpr int kSteps = 2 * NDO < 8 ? 2 * NDO : 8;
       constexpr int kRowsPer = 8 / kSteps;
       constexpr int kEvery = 2 * NDO / kSteps;
-      auto lse_at = [&](int r) { return ls[(r >> 2) * 8 + lhalf * 4 + (r & 3)]; };
-      auto del_at = [&](int r) {
-        return kDl ? ls[kRB + (r >> 2) * 8 + lhalf * 4 + (r & 3)] : 0.f;
-      };
-      float Ln[kRowsPer], Dn[kRowsPer];
+      auto vec_at = [&](int v, int r) { return ls[v * kRB + (r >> 2) * 8 + lhalf * 4 + (r & 3)]; };
+      float Ln[kRowsPer], Dn[kRowsPer], Sn[kRowsPer];
+      auto next = [&](int r0) {
 #pragma unroll
-      for (int rr = 0; rr < kRowsPer; ++rr) Ln[rr] = lse_at(8 + rr), Dn[rr] = del_at(8 + rr);
+        for (int rr = 0; rr < kRowsPer; ++rr) {
+          Ln[rr] = vec_at(0, r0 + rr);
+          Dn[rr] = kDeltaInChain ? 0.f : vec_at(1, r0 + rr);
+          Sn[rr] = kBias ? vec_at(2, r0 + rr) : 0.f;
+        }
+      };
+      next(8);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int i = 0; i < 4 * NDO; ++i) {
@@ -493,23 +570,12 @@ __global__ __launch_bounds__(64 * NW, D >= 256 && NW < 8 ? 1 : 2) void masked_dk
         if (i + kPre < 4 * NDO) tring[i % kPre] = top(i + kPre);
         if (i < 2 * NDO && i % kEvery == 0) {
           const int g = i / kEvery;
-          float Lc[kRowsPer], Dc[kRowsPer];
+          float Lc[kRowsPer], Dc[kRowsPer], Sc[kRowsPer];
 #pragma unroll
-          for (int rr = 0; rr < kRowsPer; ++rr) {
-            Lc[rr] = Ln[rr], Dc[rr] = Dn[rr];
-            if (g + 1 < kSteps) {
-              const int rn = 8 + (g + 1) * kRowsPer + rr;
-              Ln[rr] = lse_at(rn);
-              Dn[rr] = del_at(rn);
-            }
-          }
+          for (int rr = 0; rr < kRowsPer; ++rr) Lc[rr] = Ln[rr], Dc[rr] = Dn[rr], Sc[rr] = Sn[rr];
+          if (g + 1 < kSteps) next(8 + (g + 1) * kRowsPer);
 #pragma unroll
-          for (int rr = 0; rr < kRowsPer; ++rr) {
-            const int r = 8 + g * kRowsPer + rr;
-            const float p = p_of(s[r], Lc[rr]);
-            s[r] = p;
-            dp[r] = ds_of(p, dp[r], Dc[rr]);
-          }
+          for (int rr = 0; rr < kRowsPer; ++rr) elem(8 + g * kRowsPer + rr, Lc[rr], Dc[rr], Sc[rr]);
           if (g == kSteps - 1) {
             pb[1] = pack8<T>(s, 8);
             sb[1] = pack8<T>(dp, 8);
@@ -530,39 +596,61 @@ __global__ __launch_bounds__(64 * NW, D >= 256 && NW < 8 ? 1 : 2) void masked_dk
   using RS = RowStore<T, NDO>;
   unsigned char *stage = smem_raw + wave * RS::kBytes;
   const int rows = uniform_clamp(k1 - kw0, 32);
-  const int64_t off = ((int64_t)kw0 * Hk + hk) * D + dpart * NDO * 32;
-  if (gsplit == 1) {
+  if (pbase < 0) {
+    const int64_t off = ((int64_t)kw0 * Hk + hk) * D + dpart * NDO * 32;
     RS::rows16(adk, [&](float x) { return static_cast<T>(x * scale); }, stage, dk + off,
                (int64_t)Hk * D, rows);
     RS::rows16(adv, [](float x) { return static_cast<T>(x); }, stage, dv + off, (int64_t)Hk * D,
                rows);
   } else {
-    const int64_t po = (int64_t)gs * T_k * Hk * D + off;
-    RS::rows32(adk, scale, stage, part_dk + po, (int64_t)Hk * D, rows);
-    RS::rows32(adv, 1.f, stage, part_dv + po, (int64_t)Hk * D, rows);
+    const int64_t off = ((int64_t)(pbase + kgrp * 32) * Hk + hk) * D + dpart * NDO * 32;
+    RS::rows32(adk, scale, stage, part_dk + off, (int64_t)Hk * D, rows);
+    RS::rows32(adv, 1.f, stage, part_dv + off, (int64_t)Hk * D, rows);
   }
 }
 
-// dk / dv (blockIdx.y) = sum over the gsplit partials, 8 features per thread.
+// Partial rows of divided tiles to dq, dk and dv, all in one launch (three cost 4 to 8 us
+// more): an item is {r0, r1, pbase, parts}; its rows lie one after another in the
+// output and in each part, so a block adds 2048 neighbouring values, part by part in order.
 template <typename T>
-__global__ __launch_bounds__(256) void masked_group_sum_kernel(const float *part_dk,
-                                                               const float *part_dv, T *dk, T *dv,
-                                                               int64_t n, int gsplit) {
-  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8;
-  if (i >= n) return;
-  const float *src = blockIdx.y ? part_dv : part_dk;
-  f32x4 a = f32x4{0.f, 0.f, 0.f, 0.f}, b = a;
-  for (int g = 0; g < gsplit; ++g) {
-    a += *reinterpret_cast<const f32x4 *>(src + g * n + i);
-    b += *reinterpret_cast<const f32x4 *>(src + g * n + i + 4);
+__global__ __launch_bounds__(256) void masked_sum_kernel(const float *part_dq,
+                                                         const float *part_dk,
+                                                         const float *part_dv, T *dq, T *dk, T *dv,
+                                                         const int32_t *dq_items,
+                                                         const int32_t *kv_items, int n_dq,
+                                                         int n_kv, int HD, int HkD, int chunks) {
+  int y = blockIdx.x / chunks;
+  const float *part = part_dq;
+  T *out = dq;
+  const int32_t *items = dq_items;
+  int w = HD;
+  if (y >= n_dq) {
+    y -= n_dq;
+    const bool v = y >= n_kv;
+    y -= v ? n_kv : 0;
+    part = v ? part_dv : part_dk;
+    out = v ? dv : dk;
+    items = kv_items;
+    w = HkD;
   }
-  typename Mfma<T>::v8 w;
+  const PlanItem it = load_item(items, y);
+  const int64_t n = (int64_t)(it.v[1] - it.v[0]) * w;
+  const int64_t i = ((int64_t)(blockIdx.x % chunks) * 256 + threadIdx.x) * 8;
+  if (i >= n) return;
+  const float *src = part + (int64_t)it.v[2] * w + i;
+  f32x4 a = f32x4{0.f, 0.f, 0.f, 0.f}, b = a;
+#pragma unroll 4
+  for (int j = 0; j < it.v[3]; ++j) {
+    a += *reinterpret_cast<const f32x4 *>(src + j * n);
+    b += *reinterpret_cast<const f32x4 *>(src + j * n + 4);
+  }
+  typename Mfma<T>::v8 x;
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    w[e] = static_cast<T>(a[e]);
-    w[4 + e] = static_cast<T>(b[e]);
+    x[e] = static_cast<T>(a[e]);
+    x[4 + e] = static_cast<T>(b[e]);
   }
-  *reinterpret_cast<typename Mfma<T>::v8 *>((blockIdx.y ? dv : dk) + i) = w;
+  *reinterpret_cast<typename Mfma<T>::v8 *>(out + (int64_t)it.v[0] * w + i) = x;
 }
 
 // Dynamic LDS: the blocks' buffers, or the per-wave row-store regions if those are larger.
@@ -574,7 +662,8 @@ constexpr int masked_dq_lds() {
 template <typename T, int D, int NW>
 constexpr int masked_dkv_lds() {
   constexpr int kStage = NW * RowStore<T, D / 32 / (D >= 256 ? 2 : 1)>::kBytes;
-  constexpr int kBase = dkv_lds_bytes<T, D, NW>();
+  // D = 256: the exchange region behind the buffers
+  constexpr int kBase = MDkvSmem<D>::kBytes + (D >= 256 ? NW * 64 * 32 * 4 : 0);
   return kBase > kStage ? kBase : kStage;
 }
 
@@ -583,20 +672,21 @@ void launch_dq_v(const MaskedArgs &a, hipStream_t st) {
   constexpr auto fn = &masked_dq_kernel<T, D, NW, kCap, kBias>;
   const int smem = masked_dq_lds<T, D, NW>();
   allow_dynamic_lds(reinterpret_cast<const void *>(fn), smem);
-  hipLaunchKernelGGL(fn, dim3((unsigned)(a.n_items * a.H)), dim3(64 * NW), smem, st,
+  hipLaunchKernelGGL(fn, dim3((unsigned)(a.n_items * (a.H >> a.lg))), dim3(64 * NW), smem, st,
                      (const T *)a.q, (const T *)a.k, (const T *)a.v, (const T *)a.dout,
                      (const T *)a.o_in, a.lse_in, a.delta, a.lse, (T *)a.dq, a.part_o, a.items,
-                     a.slopes, ScoreArgs{a.c, a.cap2}, a.H, a.Hk, a.window, a.scale);
+                     a.slopes, ScoreArgs{a.c, a.cap2}, HeadSets{a.H, a.Hk, a.lg}, a.window,
+                     a.scale);
 }
 template <typename T, int D, int NW, bool kCap, bool kBias>
 void launch_dkv_v(const MaskedArgs &a, hipStream_t st) {
   constexpr auto fn = &masked_dkv_kernel<T, D, NW, kCap, kBias>;
   const int smem = masked_dkv_lds<T, D, NW>();
   allow_dynamic_lds(reinterpret_cast<const void *>(fn), smem);
-  hipLaunchKernelGGL(fn, dim3((unsigned)(a.n_kv * a.Hk * a.gsplit)), dim3(64 * NW), smem, st,
+  hipLaunchKernelGGL(fn, dim3((unsigned)(a.n_kv * a.Hk)), dim3(64 * NW), smem, st,
                      (const T *)a.q, (const T *)a.k, (const T *)a.v, (const T *)a.dout, a.lse,
                      a.delta, (T *)a.dk, (T *)a.dv, a.part_dk, a.part_dv, a.kv_items, a.slopes,
-                     ScoreArgs{a.c, a.cap2}, a.H, a.Hk, a.window, a.gsplit, a.T_k, a.scale);
+                     ScoreArgs{a.c, a.cap2}, HeadSets{a.H, a.Hk, a.lg}, a.window, a.scale);
 }
 
 template <typename T, int D, int NW>
@@ -620,32 +710,26 @@ void launch_dkv_nw(const MaskedArgs &a, hipStream_t st) {
 
 template <typename T, int D>
 void launch_masked_dq(const MaskedArgs &a, hipStream_t st) {
-  if (a.n_items == 0) return;
-  if constexpr (D <= 128) {
-    if (a.q_tile == kVarlenWideTile) return launch_dq_nw<T, D, 8>(a, st);
-  }
-  launch_dq_nw<T, D, 4>(a, st);
+  if (a.n_items > 0) launch_dq_nw<T, D, 4>(a, st);
 }
 
 template <typename T, int D>
 void launch_masked_dkv(const MaskedArgs &a, hipStream_t st) {
   if (a.n_kv == 0) return;
-  if constexpr (D == 256) {
-    launch_dkv_nw<T, D, 8>(a, st);
-  } else {
-    if constexpr (D == 128) {
-      if (a.k_tile == kVarlenWideTile) return launch_dkv_nw<T, D, 8>(a, st);
-    }
-    launch_dkv_nw<T, D, 4>(a, st);
-  }
+  launch_dkv_nw<T, D, D == 256 ? 8 : 4>(a, st);
 }
 
 template <typename T>
-void launch_masked_group_sum(const MaskedArgs &a, hipStream_t st) {
-  const int64_t n = a.T_k * a.Hk * a.D;
-  if (a.gsplit == 1 || n == 0) return;
-  hipLaunchKernelGGL((masked_group_sum_kernel<T>), dim3((unsigned)((n / 8 + 255) / 256), 2),
-                     dim3(256), 0, st, a.part_dk, a.part_dv, (T *)a.dk, (T *)a.dv, n, a.gsplit);
+void launch_masked_sum(const MaskedArgs &a, hipStream_t st) {
+  const int64_t n = a.n_comb + 2 * a.n_kvc;
+  if (n == 0) return;
+  const int HD = a.H * a.D, HkD = a.Hk * a.D;
+  const int64_t most = std::max(a.n_comb > 0 ? (int64_t)a.comb_rows * HD : 0,
+                                a.n_kvc > 0 ? (int64_t)a.kvc_rows * HkD : 0);
+  const int64_t chunks = (most + 2047) / 2048;
+  hipLaunchKernelGGL((masked_sum_kernel<T>), dim3((unsigned)(n * chunks)), dim3(256), 0, st,
+                     a.part_o, a.part_dk, a.part_dv, (T *)a.dq, (T *)a.dk, (T *)a.dv, a.comb_items,
+                     a.kvc_items, (int)a.n_comb, (int)a.n_kvc, HD, HkD, (int)chunks);
 }
 
 #define VAFA_INST(T)                                                        \
@@ -655,7 +739,7 @@ void launch_masked_group_sum(const MaskedArgs &a, hipStream_t st) {
   template void launch_masked_dkv<T, 64>(const MaskedArgs &, hipStream_t);  \
   template void launch_masked_dkv<T, 128>(const MaskedArgs &, hipStream_t); \
   template void launch_masked_dkv<T, 256>(const MaskedArgs &, hipStream_t); \
-  template void launch_masked_group_sum<T>(const MaskedArgs &, hipStream_t);
+  template void launch_masked_sum<T>(const MaskedArgs &, hipStream_t);
 VAFA_INST(bf16)
 VAFA_INST(f16)
 #undef VAFA_INST

@@ -3,8 +3,8 @@
 // The layout of products and tiles is that of the packed varlen forward
 // (varlen_mfma.hip): 32 query rows per wave, 64-key tiles staged once per workgroup,
 // S^T = K Q^T, online softmax against a lazily updated running max, O^T += V^T P^T.
-// What differs: H / Hk query heads read one key head; a workgroup walks only the keys
-// that some row of its tile sees (key_walk), a wave skips the tiles that none of its
+// What differs: the rows of a tile are tokens of several query heads that share a key
+// head (HeadSets); a workgroup walks only the keys that some row of its tile sees (key_walk), a wave skips the tiles that none of its
 // rows sees, and only tiles that some row does not see whole are masked.
 #include <type_traits>
 
@@ -143,25 +143,27 @@ __global__ __launch_bounds__(64 * NW, D >= 256 ? 1 : 2) void masked_fwd_kernel(
     const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v,
     T *__restrict__ o, float *__restrict__ lse, float *__restrict__ part_o,
     float *__restrict__ part_lse, const int32_t *__restrict__ items,
-    const float *__restrict__ slopes, ScoreArgs sa, int H, int Hk, int window) {
+    const float *__restrict__ slopes, ScoreArgs sa, HeadSets hs, int window) {
   using M = Mfma<T>;
   constexpr int NC = D / 16, ND = D / 32;
   extern __shared__ __align__(16) unsigned char smem_raw[];
   T *smem = reinterpret_cast<T *>(smem_raw);
 
-  const int G = H / Hk;
-  const int item = blockIdx.x / H, h = head_of(blockIdx.x % H, Hk, G), hk = h / G;
+  const int H = hs.H, lg = hs.lg, tw = 32 >> lg;  // tokens of a wave
+  const int item = blockIdx.x / hs.sets(), set = hs.set_of(blockIdx.x % hs.sets());
+  const int h0 = set << lg, hk = set / hs.per_key();
   const PlanItem it = load_item(items, item);
   const int q0 = it.v[0], q1 = it.v[1], pbase = it.v[4], diag = it.v[5], pre = it.v[6];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lrow = lane & 31, lhalf = lane >> 5;
-  const int qrow = q0 + wave * 32 + lrow;
-  const bool row_ok = qrow < q1;
-  const bool wave_active = q0 + wave * 32 < q1;
-  const int p = qrow + diag;
-  const int p0 = q0 + wave * 32 + diag;  // the wave's first and last position
-  const int p1 = (q0 + wave * 32 + 31 < q1 ? q0 + wave * 32 + 31 : q1 - 1) + diag;
+  const int t0 = q0 + wave * tw;  // the wave's first token
+  const int tok = t0 + (lrow >> lg), h = h0 + (lrow & ((1 << lg) - 1));
+  const bool row_ok = tok < q1;
+  const bool wave_active = t0 < q1;
+  const int p = tok + diag;
+  const int p0 = t0 + diag;  // the wave's first and last position
+  const int p1 = (t0 + tw < q1 ? t0 + tw : q1) - 1 + diag;
   const KeyWalk kw = key_walk<kBN>(it.v[2], it.v[3], pre, q0 + diag - window + 1);
 
   // A negative scale is folded into Q (sign flips are exact) where the running max is
@@ -173,11 +175,11 @@ __global__ __launch_bounds__(64 * NW, D >= 256 ? 1 : 2) void masked_fwd_kernel(
   }
   typename M::v8 qf[NC];
   {
-    const rsrc_t rq = make_rsrc(q + ((int64_t)q0 * H + h) * D, (int64_t)(q1 - q0) * H * D * 2);
-    const int lr = wave * 32 + lrow;
+    const rsrc_t rq = make_rsrc(q + ((int64_t)q0 * H + h0) * D, (int64_t)(q1 - q0) * H * D * 2);
+    const int lr = hs.row(wave * 32 + lrow);
 #pragma unroll
     for (int cc = 0; cc < NC; ++cc) {
-      u32x4 val = buf_load16(rq, (lr * H) * D * 2 + cc * 32 + lhalf * 16);
+      u32x4 val = buf_load16(rq, lr * D * 2 + cc * 32 + lhalf * 16);
 #pragma unroll
       for (int w = 0; w < 4; ++w) val[w] ^= qsign;
       qf[cc] = as_v8<T>(val);
@@ -197,7 +199,7 @@ __global__ __launch_bounds__(64 * NW, D >= 256 ? 1 : 2) void masked_fwd_kernel(
   const int nt = kw.n;
   TileRegs<D, NT> regs;
   auto load = [&](int j) {
-    load_tile<T, D, NT>(regs, k, v, walk_key<kBN>(kw, j), walk_end(kw, j), Hk, hk, tid);
+    load_tile<T, D, NT>(regs, k, v, walk_key<kBN>(kw, j), walk_end(kw, j), hs.Hk, hk, tid);
   };
   if (nt > 0) {
     load(0);
@@ -235,16 +237,65 @@ __global__ __launch_bounds__(64 * NW, D >= 256 ? 1 : 2) void masked_fwd_kernel(
   const float lse_v = l == 0.f ? kNegInf : m_run + fast_log2(l);
   using RS = RowStore<T, ND>;
   unsigned char *stage = smem_raw + wave * RS::kBytes;
-  const int rows = uniform_clamp(q1 - (q0 + wave * 32), 32);
+  const int rows = uniform_clamp(q1 - t0, tw) << lg;
+  auto off = [&](int r) { return (int64_t)hs.row(r) * D; };
   if (pbase < 0) {
-    RS::rows16(acc, [&](float x) { return static_cast<T>(x * inv); }, stage,
-               o + ((int64_t)(q0 + wave * 32) * H + h) * D, (int64_t)H * D, rows);
-    if (row_ok && lhalf == 0) lse[(int64_t)qrow * H + h] = lse_v;
+    RS::rows16_at(acc, [&](float x) { return static_cast<T>(x * inv); }, stage,
+                  o + ((int64_t)t0 * H + h0) * D, off, rows);
+    if (row_ok && lhalf == 0) lse[(int64_t)tok * H + h] = lse_v;
   } else {
-    const int64_t prow = pbase + wave * 32;
-    RS::rows32(acc, inv, stage, part_o + (prow * H + h) * D, (int64_t)H * D, rows);
-    if (row_ok && lhalf == 0) part_lse[(prow + lrow) * H + h] = lse_v;
+    // partial rows lie as the outputs do, token pbase + ... of [rows, H, D]
+    const int64_t prow = pbase + wave * tw;
+    RS::rows32_at(acc, inv, stage, part_o + (prow * H + h0) * D, off, rows);
+    if (row_ok && lhalf == 0) part_lse[(prow + (lrow >> lg)) * H + h] = lse_v;
   }
+}
+
+// Partial rows of split tiles to o and lse: m = max lse_s, w_s = 2^(lse_s - m), O =
+// sum w_s O_s / sum w_s.  An item is {q0, q1, pbase, parts}; its rows lie one after
+// another in the output and in each part: a thread takes 8 neighbouring features, which
+// moved 4.4 TB/s where one wave per row and 4 bytes a lane moved 2.5.
+template <typename T>
+__global__ __launch_bounds__(256) void masked_join_kernel(const float *__restrict__ part_o,
+                                                          const float *__restrict__ part_lse,
+                                                          T *__restrict__ o,
+                                                          float *__restrict__ lse,
+                                                          const int32_t *__restrict__ items, int H,
+                                                          int D, int chunks) {
+  const PlanItem it = load_item(items, blockIdx.x / chunks);
+  const int ns = it.v[3];
+  const int64_t rows = (int64_t)(it.v[1] - it.v[0]) * H;  // (token, head) rows of a part
+  const int64_t i = ((int64_t)(blockIdx.x % chunks) * 256 + threadIdx.x) * 8;
+  const int64_t row = i / D;
+  if (row >= rows) return;
+  const float *ls = part_lse + (int64_t)it.v[2] * H + row;
+  const float *src = part_o + (int64_t)it.v[2] * H * D + i;
+  float m = kNegInf;
+  for (int s = 0; s < ns; ++s) m = fmaxf(m, ls[s * rows]);
+  const float ms = m == kNegInf ? 0.f : m;  // no part sees a key: O = 0, lse = -inf
+  float l = 0.f;
+  f32x4 a = f32x4{0.f, 0.f, 0.f, 0.f}, b = a;
+#pragma unroll 4
+  for (int s = 0; s < ns; ++s) {
+    const float w = fast_exp2(ls[s * rows] - ms);
+    const f32x4 x = *reinterpret_cast<const f32x4 *>(src + s * rows * D);
+    const f32x4 y = *reinterpret_cast<const f32x4 *>(src + s * rows * D + 4);
+    l += w;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      a[e] += w * x[e];
+      b[e] += w * y[e];
+    }
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  typename Mfma<T>::v8 r;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    r[e] = static_cast<T>(a[e] * inv);
+    r[4 + e] = static_cast<T>(b[e] * inv);
+  }
+  *reinterpret_cast<typename Mfma<T>::v8 *>(o + (int64_t)it.v[0] * H * D + i) = r;
+  if (i % D == 0) lse[(int64_t)it.v[0] * H + row] = l == 0.f ? kNegInf : ms + fast_log2(l);
 }
 
 // Dynamic LDS: the K/V buffers, or the per-wave row-store regions if those are larger.
@@ -259,9 +310,10 @@ void launch_v(const MaskedArgs &a, hipStream_t st) {
   constexpr auto fn = &masked_fwd_kernel<T, D, NW, kCap, kBias>;
   const int smem = masked_fwd_lds<T, D, NW>();
   allow_dynamic_lds(reinterpret_cast<const void *>(fn), smem);
-  hipLaunchKernelGGL(fn, dim3((unsigned)(a.n_items * a.H)), dim3(64 * NW), smem, st,
+  hipLaunchKernelGGL(fn, dim3((unsigned)(a.n_items * (a.H >> a.lg))), dim3(64 * NW), smem, st,
                      (const T *)a.q, (const T *)a.k, (const T *)a.v, (T *)a.o, a.lse, a.part_o,
-                     a.part_lse, a.items, a.slopes, ScoreArgs{a.c, a.cap2}, a.H, a.Hk, a.window);
+                     a.part_lse, a.items, a.slopes, ScoreArgs{a.c, a.cap2},
+                     HeadSets{a.H, a.Hk, a.lg}, a.window);
 }
 
 template <typename T, int D, int NW>
@@ -278,16 +330,26 @@ void launch_nw(const MaskedArgs &a, hipStream_t st) {
 template <typename T, int D>
 void launch_masked_fwd(const MaskedArgs &a, hipStream_t st) {
   if (a.n_items == 0) return;
-  if constexpr (D <= 128) {
+  if constexpr (D == 128) {
     if (a.q_tile == kVarlenWideTile) return launch_nw<T, D, 8>(a, st);
   }
   launch_nw<T, D, 4>(a, st);
 }
 
+template <typename T>
+void launch_masked_join(const MaskedArgs &a, hipStream_t st) {
+  if (a.n_comb == 0) return;
+  const int64_t chunks = ((int64_t)a.comb_rows * a.H * a.D + 2047) / 2048;
+  hipLaunchKernelGGL((masked_join_kernel<T>), dim3((unsigned)(a.n_comb * chunks)), dim3(256), 0,
+                     st, a.part_o, a.part_lse, (T *)a.o, a.lse, a.comb_items, a.H, a.D,
+                     (int)chunks);
+}
+
 #define VAFA_INST(T)                                                     \
   template void launch_masked_fwd<T, 64>(const MaskedArgs &, hipStream_t);  \
   template void launch_masked_fwd<T, 128>(const MaskedArgs &, hipStream_t); \
-  template void launch_masked_fwd<T, 256>(const MaskedArgs &, hipStream_t);
+  template void launch_masked_fwd<T, 256>(const MaskedArgs &, hipStream_t); \
+  template void launch_masked_join<T>(const MaskedArgs &, hipStream_t);
 VAFA_INST(bf16)
 VAFA_INST(f16)
 #undef VAFA_INST

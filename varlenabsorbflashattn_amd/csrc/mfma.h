@@ -132,6 +132,12 @@ struct StagedRows {
   static __device__ __forceinline__ void store(const f32x16 (&acc)[NDT], F conv,
                                                unsigned char *stage, O *out,
                                                int64_t row_stride, int rows) {
+    store_at(acc, conv, stage, out, [&](int rr) { return rr * row_stride; }, rows);
+  }
+  // row r at out + off(r)
+  template <typename F, typename R>
+  static __device__ __forceinline__ void store_at(const f32x16 (&acc)[NDT], F conv,
+                                                  unsigned char *stage, O *out, R off, int rows) {
     static_assert(kLanesPerRow >= 1 && kLanesPerRow <= 64 && 64 % kLanesPerRow == 0,
                   "row width");
     const int lane = (int)__builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u));
@@ -153,7 +159,7 @@ struct StagedRows {
       const int rr = s * kRowsPerStep + r0;
       const u32x4 v = *reinterpret_cast<const u32x4 *>(stage + rr * kStride + c * 16);
       if (rr < rows)
-        *reinterpret_cast<u32x4 *>(out + rr * row_stride + c * (16 / (int)sizeof(O))) = v;
+        *reinterpret_cast<u32x4 *>(out + off(rr) + c * (16 / (int)sizeof(O))) = v;
     }
     asm volatile("" ::: "memory");
   }
@@ -175,16 +181,26 @@ struct RowStore {
                                                 int64_t row_stride, int rows) {
     R16::store(acc, conv, stage, out, row_stride, rows);
   }
+  template <typename F, typename R>
+  static __device__ __forceinline__ void rows16_at(const f32x16 (&acc)[ND], F conv,
+                                                   unsigned char *stage, T *out, R off, int rows) {
+    R16::store_at(acc, conv, stage, out, off, rows);
+  }
   // fp32 rows of acc * mul
   static __device__ __forceinline__ void rows32(const f32x16 (&acc)[ND], float mul,
                                                 unsigned char *stage, float *out,
                                                 int64_t row_stride, int rows) {
+    rows32_at(acc, mul, stage, out, [&](int rr) { return rr * row_stride; }, rows);
+  }
+  template <typename R>
+  static __device__ __forceinline__ void rows32_at(const f32x16 (&acc)[ND], float mul,
+                                                   unsigned char *stage, float *out, R off,
+                                                   int rows) {
     constexpr int NH = ND / kHalves;
 #pragma unroll
     for (int hh = 0; hh < kHalves; ++hh)
-      R32::store(*reinterpret_cast<const f32x16(*)[NH]>(&acc[hh * NH]),
-                 [&](float x) { return x * mul; }, stage, out + hh * NH * 32, row_stride,
-                 rows);
+      R32::store_at(*reinterpret_cast<const f32x16(*)[NH]>(&acc[hh * NH]),
+                    [&](float x) { return x * mul; }, stage, out + hh * NH * 32, off, rows);
   }
 };
 

@@ -18,6 +18,7 @@
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
+#include <functional>
 #include <numeric>
 #include <string>
 #include <vector>
@@ -496,10 +497,15 @@ int vafa_plan_varlen_balanced(const int64_t *cu_q, const int64_t *cu_k, int64_t 
 //                 holds its rows' first keys.  A tile that sees no key is an item with
 //                 k0 == k1, which writes zeros.
 //   comb section: {q0, q1, pbase, nsplit, seg, 0, 0, 0}.
-//   kv section  : {k0, k1, q0, q1, diag, pre, 0, 0} key tiles with the range of the
-//                 queries that see some of their keys.
-// info->xcd_heads holds the parts into which the query heads of a key head are divided
-// in the dK/dV pass.
+//   kv section  : {k0, k1, q0, q1, diag, pre, pbase, part << 16 | parts} key tiles with
+//                 the range of the queries that see some of their keys; a tile's blocks
+//                 of 32 rows may be divided into parts, which write fp32 partial rows
+//                 pbase + (key - k0) for every key head.
+//   fcomb section: {k0, k1, pbase, parts, seg, 0, 0, 0}, laid out as the comb items.
+//   dq, dqc     : the dQ pass's items and their sums, as fwd and comb with tiles of
+//                 kVarlenTile rows.
+// Rows of a tile are (token, head) pairs of a head set (masked_set_log2, which
+// info->xcd_heads holds): q_tile rows are q_tile >> k tokens.
 int vafa_plan_masked(const int64_t *cu_q, const int64_t *cu_k, const int64_t *prefix, int64_t n1,
                      int64_t H, int64_t Hk, int64_t D, int32_t causal, int64_t window,
                      int32_t *plan, int64_t plan_cap, vafa_plan_info *info) {
@@ -546,81 +552,178 @@ int vafa_plan_masked(const int64_t *cu_q, const int64_t *cu_k, const int64_t *pr
     return r;
   };
 
-  // tiles: wide ones (8 waves) where the launch fills the chip with them
-  auto work_of = [&](int64_t bm, int64_t *items, int64_t *longest) {
-    int64_t keys = 0;
-    *items = *longest = 0;
-    for (int64_t s = 0; s + 1 < n1; ++s)
-      for (int64_t t = cu_q[s]; t < cu_q[s + 1]; t += bm) {
-        const Range r = range_of(s, t, std::min(t + bm, cu_q[s + 1]));
-        keys += r.keys;
-        *longest = std::max(*longest, r.keys);
-        ++*items;
-      }
-    return keys;
-  };
-  const int64_t cus = kVarlenBalance.cus, slots = (D > 128 ? 1 : 2) * cus;
-  int64_t BM = kVarlenTile, BK = kVarlenTile, items, longest;
-  const int64_t keys = work_of(BM, &items, &longest);
-  info->q_tile = BM;
+  const int lg = masked_set_log2(H / Hk);
+  const int64_t sets = H >> lg, cus = kVarlenBalance.cus;
+  const int64_t slots = (D > 128 ? 1 : D > 64 ? 2 : 3) * cus;  // resident 4-wave workgroups
+  int64_t BK = kVarlenTile;
   info->k_tile = BK;
-  // a chunk of keys per item: the average of the resident workgroups, so that no item
-  // outlasts the rest
-  const int64_t avg = cdiv(keys * H, slots);
-  const int64_t chunk_max = std::max<int64_t>(kMaskedMinChunk, round_up(avg, 64));
-
-  Section fwd, comb, kv;
-  int64_t prow = 0, max_split = 1;
-  for (int64_t s = 0; s + 1 < n1; ++s) {
-    const int64_t q0 = cu_q[s], q1 = cu_q[s + 1], k0 = cu_k[s], k1 = cu_k[s + 1];
-    const int64_t diag = k1 - q1;
-    for (int64_t t = q0; t < q1; t += BM) {
-      const int64_t te = std::min(t + BM, q1), rows = te - t;
-      const Range r = range_of(s, t, te);
-      const int64_t span = r.hi - r.lo;
-      int64_t ns = span > chunk_max + chunk_max / 4 ? cdiv(span, chunk_max) : 1;
-      const int64_t chunk = ns > 1 ? round_up(cdiv(span, ns), 64) : span;
-      if (ns > 1) ns = cdiv(span, chunk);
-      max_split = std::max(max_split, ns);
-      if (ns > 1)
-        comb.push_back(Item{{(int32_t)t, (int32_t)te, (int32_t)prow, (int32_t)ns, (int32_t)s, 0, 0,
-                             0}, 0});
-      for (int64_t j = 0; j < ns; ++j) {
-        const int64_t a = ns > 1 ? r.lo + j * chunk : r.lo;
-        const int64_t b = ns > 1 ? std::min(r.hi, a + chunk) : r.hi;
-        fwd.push_back(Item{{(int32_t)t, (int32_t)te, (int32_t)a, (int32_t)b,
-                            ns > 1 ? (int32_t)(prow + j * rows) : -1, (int32_t)diag,
-                            (int32_t)r.pre, j == 0},
-                           (ns > 1 ? b - a : r.keys) + kVarlenPolicy.item_overhead});
-      }
-      if (ns > 1) prow += ns * rows;
-      if (prow > INT32_MAX) return fail(VAFA_ERR_VALUE, "too many split rows");
+  info->xcd_heads = lg;
+  // (token, head) row blocks that a key tile walks, and its queries
+  const int64_t tb = 32 >> lg, nset = (H / Hk) >> lg;
+  auto queries_of = [&](int64_t s, int64_t k, int64_t ke, int64_t *a, int64_t *b) {
+    const int64_t q0 = cu_q[s], q1 = cu_q[s + 1], diag = cu_k[s + 1] - q1;
+    const int64_t pre = causal ? cu_k[s] + (prefix != nullptr ? prefix[s] : 0) : cu_k[s + 1];
+    *a = q0;
+    *b = q1;
+    if (k >= pre) {
+      *a = std::max(q0, k - diag);
+      *b = std::min(q1, ke - 1 + win - diag);
+      if (*b < *a) *a = *b = q0;
     }
+    return cdiv(*b - *a, tb) * nset;
+  };
+  // tiles of one kind: their keys (blocks), tokens and token count
+  struct Tile {
+    int64_t work, rows;
+  };
+  std::vector<Tile> q128, q256, k128;
+  auto list = [&](int64_t tokens, std::vector<Tile> &v) {
+    for (int64_t s = 0; s + 1 < n1; ++s)
+      for (int64_t t = cu_q[s]; t < cu_q[s + 1]; t += tokens) {
+        const int64_t te = std::min(t + tokens, cu_q[s + 1]);
+        const Range r = range_of(s, t, te);
+        v.push_back({r.hi - r.lo > r.keys ? r.keys : r.hi - r.lo, te - t});
+      }
+  };
+  list(kVarlenTile >> lg, q128);
+  if (D == 128) list(kVarlenWideTile >> lg, q256);
+  for (int64_t s = 0; s + 1 < n1; ++s)
+    for (int64_t k = cu_k[s]; k < cu_k[s + 1]; k += BK) {
+      int64_t a, b;
+      const int64_t ke = std::min(k + BK, cu_k[s + 1]);
+      const int64_t n = queries_of(s, k, ke, &a, &b);
+      k128.push_back({n, ke - k});
+    }
+  // The chunk of work beyond which a tile is divided, and the modelled time with it:
+  // the tiles' pieces dealt longest-first to the resident workgroups (`copies` of each
+  // piece, one per head set, side by side), plus what the partial rows cost.
+  struct Pick {
+    int64_t chunk;
+    double time;
+  };
+  auto pick = [&](const std::vector<Tile> &tiles, int64_t copies, int64_t wgs,
+                  const MaskedModel &m, double launch) {
+    const int64_t groups = std::max<int64_t>(1, wgs / copies);
+    const double rounds = (double)std::max(copies, wgs) / (double)wgs;  // copies > wgs
+    int64_t sum = 0, most = 0;
+    for (const Tile &t : tiles) {
+      sum += t.work;
+      most = std::max(most, t.work);
+    }
+    const int64_t avg = std::max<int64_t>(1, cdiv(sum, groups));
+    Pick best{INT64_MAX, 0.0};
+    std::vector<int64_t> cost;
+    std::vector<double> heap;
+    for (const double f : {0.0, 2.0, 1.5, 1.0, 0.75, 0.5}) {
+      const int64_t chunk =
+          f == 0.0 ? INT64_MAX : std::max(m.min_chunk, round_up((int64_t)(avg * f), m.align));
+      if (f > 0.0 && (chunk >= most || chunk == best.chunk)) continue;
+      cost.clear();
+      double parts = 0.0;
+      for (const Tile &t : tiles) {
+        const int64_t ns = t.work > chunk ? std::min(cdiv(t.work, chunk), kMaskedMaxParts) : 1;
+        for (int64_t j = 0; j < ns; ++j) cost.push_back(t.work / ns + m.item);
+        if (ns > 1) parts += (double)(ns * t.rows);
+      }
+      // many pieces even out by themselves
+      double span = (double)(avg + m.item * (int64_t)cost.size() / groups);
+      if ((int64_t)cost.size() <= 4 * groups) {
+        std::sort(cost.begin(), cost.end(), std::greater<int64_t>());
+        heap.assign(groups, 0.0);
+        for (int64_t c : cost) {
+          std::pop_heap(heap.begin(), heap.end(), std::greater<double>());
+          heap.back() += (double)c;
+          std::push_heap(heap.begin(), heap.end(), std::greater<double>());
+        }
+        span = *std::max_element(heap.begin(), heap.end());
+      } else {
+        span += (double)most / 2;
+      }
+      const double time =
+          span * rounds + (parts > 0.0 ? launch + parts * m.row * (double)copies : 0.0);
+      if (f == 0.0 || time < best.time) best = Pick{chunk, time};
+    }
+    return best;
+  };
+  // a launch of sums in keys (blocks), whose time goes with D
+  const double launch = kMaskedQuery.launch / (double)D, blaunch = kMaskedKeys.launch / (double)D;
+  const Pick p128 = pick(q128, sets, slots, kMaskedQuery, launch);
+  const Pick p256 = D == 128 ? pick(q256, sets, cus, kMaskedQuery, launch) : p128;
+  // The forward's tile: 256 rows (8 waves) read every key tile for twice the rows, where
+  // the model gives up to 5% more for it.  Only at D = 128: at D = 64, where three 4-wave
+  // workgroups share a CU, it gained nothing on 8 x 2048 tokens and lost a third on 24
+  // short sequences (25 -> 38 us); at D = 256 the registers hold one wave per SIMD.
+  const bool wide = D == 128 && p256.time * kMaskedWideGain < p128.time;
+  info->q_tile = wide ? kVarlenWideTile : kVarlenTile;
+  const int64_t blk_max = pick(k128, Hk, slots, kMaskedKeys, blaunch).chunk;
+
+  Section fwd, comb, dq, dqc, kv, kvc;
+  int64_t kprow = 0, max_split = 1;
+  // Query tiles of `tokens` tokens, key ranges beyond chunk_max keys split: their items
+  // and combine items; returns the partial rows.
+  auto query_items = [&](int64_t tokens, int64_t chunk_max, Section &items, Section &sums) {
+    int64_t prow = 0;
+    for (int64_t s = 0; s + 1 < n1; ++s) {
+      const int64_t q0 = cu_q[s], q1 = cu_q[s + 1], diag = cu_k[s + 1] - q1;
+      for (int64_t t = q0; t < q1; t += tokens) {
+        const int64_t te = std::min(t + tokens, q1), rows = te - t;
+        const Range r = range_of(s, t, te);
+        const int64_t span = r.hi - r.lo;
+        int64_t ns = span > chunk_max ? std::min(cdiv(span, chunk_max), kMaskedMaxParts) : 1;
+        const int64_t chunk = ns > 1 ? round_up(cdiv(span, ns), 64) : span;
+        if (ns > 1) {
+          ns = cdiv(span, chunk);
+          sums.push_back(Item{{(int32_t)t, (int32_t)te, (int32_t)prow, (int32_t)ns, (int32_t)s, 0,
+                               0, 0}, 0});
+        }
+        max_split = std::max(max_split, ns);
+        for (int64_t j = 0; j < ns; ++j) {
+          const int64_t a = ns > 1 ? r.lo + j * chunk : r.lo;
+          const int64_t b = ns > 1 ? std::min(r.hi, a + chunk) : r.hi;
+          items.push_back(Item{{(int32_t)t, (int32_t)te, (int32_t)a, (int32_t)b,
+                                ns > 1 ? (int32_t)(prow + j * rows) : -1, (int32_t)diag,
+                                (int32_t)r.pre, j == 0},
+                               (ns > 1 ? b - a : r.keys) + kVarlenPolicy.item_overhead});
+        }
+        if (ns > 1) prow += ns * rows;
+      }
+    }
+    sort_lpt(items);
+    sums.keep_order();
+    return prow;
+  };
+  const int64_t dq_rows = query_items(kVarlenTile >> lg, p128.chunk, dq, dqc);
+  const int64_t fwd_rows = wide ? query_items(kVarlenWideTile >> lg, p256.chunk, fwd, comb)
+                                : query_items(kVarlenTile >> lg, p128.chunk, fwd, comb);
+  if (std::max(fwd_rows, dq_rows) > INT32_MAX) return fail(VAFA_ERR_VALUE, "too many split rows");
+  for (int64_t s = 0; s + 1 < n1; ++s) {
+    const int64_t q1 = cu_q[s + 1], k0 = cu_k[s], k1 = cu_k[s + 1], diag = k1 - q1;
     const int64_t pre = causal ? k0 + (prefix != nullptr ? prefix[s] : 0) : k1;
     for (int64_t k = k0; k < k1; k += BK) {
       const int64_t ke = std::min(k + BK, k1);
-      int64_t a = q0, b = q1;
-      if (k >= pre) {
-        a = std::max(q0, k - diag);
-        b = std::min(q1, ke - 1 + win - diag);
-        if (b < a) a = b = q0;
+      int64_t a, b;
+      const int64_t n = queries_of(s, k, ke, &a, &b);
+      const int64_t parts =
+          n > blk_max ? std::min<int64_t>(cdiv(n, blk_max), kMaskedMaxParts) : 1;
+      if (parts > 1)
+        kvc.push_back(Item{{(int32_t)k, (int32_t)ke, (int32_t)kprow, (int32_t)parts, (int32_t)s, 0,
+                            0, 0}, 0});
+      for (int64_t j = 0; j < parts; ++j) {
+        kv.push_back(Item{{(int32_t)k, (int32_t)ke, (int32_t)a, (int32_t)b, (int32_t)diag,
+                           (int32_t)pre, parts > 1 ? (int32_t)kprow : -1,
+                           (int32_t)(j << 16 | parts)},
+                          n / parts + 2});
+        if (parts > 1) kprow += ke - k;
       }
-      kv.push_back(Item{{(int32_t)k, (int32_t)ke, (int32_t)a, (int32_t)b, (int32_t)diag,
-                         (int32_t)pre, 0, 0},
-                        (b - a) + kVarlenPolicy.item_overhead});
+      if (kprow > INT32_MAX) return fail(VAFA_ERR_VALUE, "too many split rows");
     }
   }
-  sort_lpt(fwd);
   sort_lpt(kv);
-  comb.keep_order();
-  // parts of a key head's query heads in the dK/dV pass: until every CU has a workgroup
-  int64_t parts = 1;
-  const int64_t G = H / Hk, wgs = (int64_t)kv.items.size() * Hk;
-  while (parts * 2 <= G && G % (parts * 2) == 0 && wgs * parts < slots) parts *= 2;
-  info->xcd_heads = parts;
-  info->n_part_rows = prow;
+  kvc.keep_order();
+  info->n_part_rows = std::max(fwd_rows, dq_rows);
+  info->n_fpart_rows = kprow;
   info->max_split = max_split;
-  return emit(fwd, comb, kv, {}, {}, {}, {}, {}, plan, plan_cap, info);
+  return emit(fwd, comb, kv, {}, dq, dqc, {}, kvc, plan, plan_cap, info);
 }
 
 // Absorb plan.  Query rows are (token, head) pairs; one item covers whole

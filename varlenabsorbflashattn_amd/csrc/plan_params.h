@@ -58,10 +58,27 @@ struct VarlenBalance {
 };
 constexpr VarlenBalance kVarlenBalance{256, 512, 32 << 20};
 // packed_masked_attn: most tokens of a call (positions, and a position less the window,
-// are 32-bit in the kernels) and the smallest chunk of keys into which a tile's range is
-// split.
+// are 32-bit in the kernels).
 constexpr int64_t kMaskedMaxTokens = int64_t{1} << 30;
-constexpr int64_t kMaskedMinChunk = 512;
+constexpr int64_t kMaskedMaxParts = 256;
+// The planner's model of a pass's time, in units of one key (query tiles) or one block of
+// 32 rows (key tiles): the smallest chunk and its alignment, what an item costs beside
+// its work, the launch that sums partial rows (times D), and a partial row of one token
+// (or key) and one head set (key head).
+struct MaskedModel {
+  int64_t min_chunk, align, item;
+  double launch, row;
+};
+constexpr MaskedModel kMaskedQuery{512, 64, 150, 48000.0, 0.02};
+constexpr MaskedModel kMaskedKeys{16, 1, 6, 800.0, 2.5e-4};
+constexpr double kMaskedWideGain = 0.95;
+// Query heads that share a key head lie in sets of 2^k rows of a tile (csrc/masked.h):
+// k for G heads a key head.
+inline int masked_set_log2(int64_t G) {
+  int k = 0;
+  while (k < 5 && G % (int64_t{2} << k) == 0) ++k;
+  return k;
+}
 // Absorb forward key splits.  A chunk holds kAbsorbSlack2 / 2 times the
 // average keys per resident forward workgroup (256 CUs x 3 on the MI355X), so
 // large launches stay whole (splitting C5's <= 8192-key samples into 1024-key

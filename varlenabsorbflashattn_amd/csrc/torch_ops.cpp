@@ -424,7 +424,7 @@ std::tuple<Tensor, Tensor> masked_fwd(const Tensor &q, const Tensor &k, const Te
   const int64_t H = q.size(1), D = q.size(2);
   const float *sl = slopes_of("packed_masked_attn", slopes, H, q);
   Tensor o = c.like(q), lse = c.empty_f32({q.size(0), H});
-  void *ws = c.workspace(api.masked_fwd_workspace(&p.info, D));
+  void *ws = c.workspace(api.masked_fwd_workspace(&p.info, k.size(1), D));
   check(api.masked_fwd(ptr(q), ptr(k), ptr(v), ptr(o), f32w(lse), p.dev(), &p.info, k.size(1), D,
                        dtype_of(q), (float)scale, (float)softcap, window, sl, ws, c.ws_bytes(),
                        c.stream));
