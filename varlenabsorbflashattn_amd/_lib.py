@@ -399,13 +399,13 @@ def cached_plan(key: tuple) -> Optional[DevicePlan]:
 def new_plan(key: tuple, cu_q: np.ndarray, cu_k: np.ndarray) -> DevicePlan:
     """Builds and caches the plan of ``key``, from int64 cu_seqlens."""
     kind, dims, device = key[0], key[5], key[6]
-    if kind == "varlen":
-        host = plan_varlen(cu_q, cu_k, *dims, balanced=True)
-    elif kind == "masked":  # dims end with the prefix lengths as bytes, or None
-        host = plan_masked(cu_q, cu_k, *dims[:-1], None if dims[-1] is None
-                           else np.frombuffer(dims[-1], dtype=np.int64))
-    else:
-        host = plan_absorb(cu_q, cu_k, *dims)
+    host = (plan_varlen(cu_q, cu_k, *dims, balanced=True) if kind == "varlen"
+            else plan_absorb(cu_q, cu_k, *dims))
+    return cache_plan(key, host, device)
+
+
+def cache_plan(key: tuple, host: HostPlan, device) -> DevicePlan:
+    """Copies a plan to the device and caches it as ``key``."""
     dp = DevicePlan(host, device)
     with _lock:
         _CACHE[key] = dp

@@ -412,6 +412,15 @@ Tensor paged_decode(const Tensor &q_in, const Tensor &kc, const Tensor &vc, cons
   return out;
 }
 
+// dtype and content of an integer tensor on the host, for a plan's key (tensor.numpy()
+// alone takes 5 to 10 us).
+py::bytes cu_key(const Tensor &t) {
+  if (!t.is_cpu() || !t.is_contiguous()) throw py::value_error("cu_key: a contiguous host tensor");
+  std::string s(1, (char)t.scalar_type());
+  s.append(static_cast<const char *>(t.data_ptr()), (size_t)t.nbytes());
+  return py::bytes(s);
+}
+
 // Rows that the plan does not reach (possible where validation is off) as zeros.
 void clear_rest(const Tensor &t, int64_t rows) {
   if (t.size(0) > rows) t.slice(0, rows).zero_();
@@ -421,6 +430,9 @@ std::tuple<Tensor, Tensor> masked_fwd(const Tensor &q, const Tensor &k, const Te
                                       const Plan &p, double scale, double softcap, int64_t window,
                                       const std::optional<Tensor> &slopes) {
   Call c(q);
+  // evicted from the cache while a kernel of this stream still reads it, the plan keeps
+  // its memory until the stream's work is done
+  p.items.record_stream(c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(q.device().index()).unwrap());
   const int64_t H = q.size(1), D = q.size(2);
   const float *sl = slopes_of("packed_masked_attn", slopes, H, q);
   Tensor o = c.like(q), lse = c.empty_f32({q.size(0), H});
@@ -477,6 +489,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("absorb_full_bwd", &absorb_full_bwd, no_gil);
   m.def("project_fwd", &project_fwd, no_gil);
   m.def("project_bwd", &project_bwd, no_gil);
+  m.def("cu_key", &cu_key);
   m.def("masked_fwd", &masked_fwd, no_gil);
   m.def("masked_bwd", &masked_bwd, no_gil);
   m.def("paged_append", &paged_append, no_gil);

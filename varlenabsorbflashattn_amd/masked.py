@@ -13,35 +13,55 @@ import math
 from typing import Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib, varlen
 from .varlen import _aligned, _check_tokens, _normalize_qkv, _seqinfo_to_cu_seqlens
+
+
+def _host(t, name):
+    """An integer tensor (arrays and lists too) as a contiguous one on the host."""
+    t = torch.as_tensor(t).detach()
+    if t.is_floating_point() or t.is_complex() or t.dtype == torch.bool:
+        raise AssertionError(f"{name} must be integers, got {t.dtype}")
+    return (t if t.device.type == "cpu" else t.cpu()).contiguous()
+
+
+def _host_pair(a, b):
+    """Both cu_seqlens on the host, with one copy for two of one shape on the GPU."""
+    if a is b:
+        h = _host(a, "cu_seqlens_q")
+        return h, h
+    if a.is_cuda and b.is_cuda and a.device == b.device and a.dtype == b.dtype \
+            and a.shape == b.shape and a.dim() == 1:
+        h = _host(torch.stack((a.detach(), b.detach())), "cu_seqlens")
+        return h[0], h[1]
+    return _host(a, "cu_seqlens_q"), _host(b, "cu_seqlens_k")
 
 
 def _plan_of(q, k, cu_seqlens_q, cu_seqlens_k, causal, window, prefix_lens):
     """Validation and the device plan.  As for packed_varlen_attn, a cached plan of the
     same content that covers exactly these tokens passed the checks when it was built."""
     T_q, H, D = q.shape
-    T_k, Hk = k.shape[:2]
-    cu_q, cu_k = _lib.host_cu_pair(cu_seqlens_q, cu_seqlens_k)
-    prefix = None if prefix_lens is None else _lib.as_host_i64(prefix_lens)
-    if prefix is not None and prefix.shape != (cu_q.size - 1,):
-        raise AssertionError(f"prefix_lens must be [{cu_q.size - 1}], got {prefix.shape}")
-    dims = (H, Hk, D, causal, window, None if prefix is None else prefix.tobytes())
-    key = _lib.plan_key("masked", cu_q, cu_k, dims, q.device)
-    plan = _lib.cached_plan(key) if cu_q.ndim == 1 and cu_k.ndim == 1 else None
+    T_k, H_k = k.shape[:2]
+    cu_q, cu_k = _host_pair(cu_seqlens_q, cu_seqlens_k)
+    content = _lib.ops().cu_key
+    prefix = None if prefix_lens is None else _host(prefix_lens, "prefix_lens").to(torch.int64)
+    key = ("masked", content(cu_q), content(cu_k), None if prefix is None else content(prefix),
+           H, H_k, D, causal, window, q.device)
+    plan = _lib.cached_plan(key) if cu_q.dim() == 1 and cu_k.dim() == 1 else None
     if plan is not None and plan.T_q == T_q and plan.T_k == T_k:
-        return plan.use()
+        return plan
     cu_q_h, cu_k_h = _lib.as_host_i64(cu_q), _lib.as_host_i64(cu_k)
-    varlen._validate_cu_seqlens(cu_q_h, cu_seqlens_q.shape, T_q, "cu_seqlens_q")
-    varlen._validate_cu_seqlens(cu_k_h, cu_seqlens_k.shape, T_k, "cu_seqlens_k")
+    varlen._validate_cu_seqlens(cu_q_h, cu_q.shape, T_q, "cu_seqlens_q")
+    varlen._validate_cu_seqlens(cu_k_h, cu_k.shape, T_k, "cu_seqlens_k")
     if cu_q_h.ndim != 1 or cu_q_h.size < 2:
         raise ValueError("cu_seqlens_q: must be 1-D with at least 2 elements")
     if plan is None:
-        plan = _lib.new_plan(key, cu_q_h, cu_k_h)
+        host = _lib.plan_masked(cu_q_h, cu_k_h, H, H_k, D, causal, window,
+                                None if prefix is None else prefix.numpy())
+        plan = _lib.cache_plan(key, host, q.device)
     _check_tokens(plan.info, T_q, T_k)
-    return plan.use()
+    return plan
 
 
 class _PackedMaskedAttnFunction(torch.autograd.Function):
@@ -59,12 +79,10 @@ class _PackedMaskedAttnFunction(torch.autograd.Function):
         return o
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, do):
         q, k, v, o, lse, slopes = ctx.saved_tensors
-        grads = _lib.ops().masked_bwd(q, k, v, o, lse, do, ctx.plan.use().native, *ctx.args,
-                                      slopes)
-        return *grads, None, None, None, None, None, None, None, None
+        return *_lib.ops().masked_bwd(q, k, v, o, lse, do, ctx.plan.native, *ctx.args, slopes), \
+            None, None, None, None, None, None, None, None
 
 
 def packed_masked_attn(
