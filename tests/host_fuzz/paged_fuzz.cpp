@@ -60,39 +60,38 @@ static void lookups(std::mt19937_64 &g) {
 }
 
 static void splits(std::mt19937_64 &g) {
-  const int n = 1 + (int)(g() % 40), pairs = 1 + (int)(g() % 6);
-  const int grid = 1 + (int)(g() % (g() % 2 ? 8 : 600)), window = g() % 3 ? 0 : 1 + (int)(g() % 900);
+  const int n = 1 + (int)(g() % 40);
+  const int chunks = 1 + (int)(g() % (g() % 2 ? 8 : 600)), window = g() % 3 ? 0 : 1 + (int)(g() % 900);
   std::vector<int32_t> tiles(n);
   int32_t total = 0;
   for (auto &t : tiles) {
-    const int32_t len = (int32_t)(g() % 4 == 0 ? 0 : g() % (1u << (1 + g() % 14)));
+    const int32_t len = (int32_t)(g() % 4 == 0 ? 0 : g() % (1u << (1 + g() % 17)));
     t = decode_tiles(len, window);
     const int32_t seen = decode_seen(len, window);
     CHECK(seen <= len && (window == 0 || seen <= window) && (t - 1) * kDecodeTile < seen + (seen == 0) &&
           t * kDecodeTile >= seen);
-    total += t * pairs;
+    total += t;
   }
-  const int32_t per = decode_per(total, grid);
-  CHECK((int64_t)per * grid >= total);
+  const int32_t per = decode_per(total, chunks);
+  CHECK((int64_t)per * chunks >= total);
   if (total == 0) return;
   std::vector<int> covered(total, 0);
   std::set<int64_t> slots, joined;
-  // the workgroups' walk
-  for (int w = 0; w < grid; ++w) {
-    int64_t cur = (int64_t)w * per;
+  // the chunks' walk
+  for (int c = 0; c < chunks; ++c) {
+    int64_t cur = (int64_t)c * per;
     const int64_t end = cur + per < total ? cur + per : total;
     while (cur < end) {
       int32_t t0 = 0, nt = 0;
-      for (int b = 0; b < n && nt == 0; ++b)
-        for (int p = 0; p < pairs && nt == 0; ++p) {
-          if (cur < t0 + tiles[b]) nt = tiles[b];
-          else t0 += tiles[b];
-        }
+      for (int b = 0; b < n && nt == 0; ++b) {
+        if (cur < t0 + tiles[b]) nt = tiles[b];
+        else t0 += tiles[b];
+      }
       const int64_t stop = t0 + nt < end ? t0 + nt : end;
       for (int64_t t = cur; t < stop; ++t) ++covered[t];
       if (stop - cur < nt) {
-        const int64_t s = decode_slot(w, t0, per);
-        CHECK(s >= 0 && s < 2 * grid && slots.insert(s).second);
+        const int64_t s = decode_slot(c, t0, per);
+        CHECK(s >= 0 && s < 2 * chunks && slots.insert(s).second);
       }
       cur = stop;
     }
@@ -100,15 +99,14 @@ static void splits(std::mt19937_64 &g) {
   for (int c : covered) CHECK(c == 1);
   // the join
   int32_t t0 = 0;
-  for (int b = 0; b < n; ++b)
-    for (int p = 0; p < pairs; ++p) {
-      if (tiles[b] > 0) {
-        const int g0 = t0 / per, g1 = (t0 + tiles[b] - 1) / per;
-        if (g0 != g1)
-          for (int w = g0; w <= g1; ++w) CHECK(joined.insert(decode_slot(w, t0, per)).second);
-      }
-      t0 += tiles[b];
+  for (int b = 0; b < n; ++b) {
+    if (tiles[b] > 0) {
+      const int g0 = t0 / per, g1 = (t0 + tiles[b] - 1) / per;
+      if (g0 != g1)
+        for (int c = g0; c <= g1; ++c) CHECK(joined.insert(decode_slot(c, t0, per)).second);
     }
+    t0 += tiles[b];
+  }
   CHECK(slots == joined);
 }
 

@@ -120,10 +120,12 @@ def test_refused_by_the_c_abi():
                           (4, 0, {"table_width": (1 << 31) - 1, "page_size": 1 << 20,
                                   "n_seq": 4096})):
         assert L.vafa_paged_decode_workspace(cache(**kw), H, window) == -1
-    need = L.vafa_paged_decode_workspace(cache(), 4, 0)
+    # short sequences need no partial results
+    assert L.vafa_paged_decode_workspace(cache(), 4, 0) == 0
+    need = L.vafa_paged_decode_workspace(cache(table_width=100), 4, 0)
     assert need > 0
     x = 1 << 24
-    dec = [cache(), x, 256, 64, 4, x, 0.125, 0.0, 0, None, _lib.DT_BF16, x, need, None]
+    dec = [cache(table_width=100), x, 256, 64, 4, x, 0.125, 0.0, 0, None, _lib.DT_BF16, x, need, None]
 
     def rc(at, value, call=L.vafa_paged_decode, args=dec):
         return call(*[value if i == at else y for i, y in enumerate(args)])

@@ -143,12 +143,14 @@ struct DecodeArgs {
   void *out;
   const int32_t *lens;
   const float *slopes;  // or null
-  float *part_o, *part_ml;  // pieces: [slots, 16, D] and [slots, 16, 2]
+  float *part_o, *part_ml;  // pieces: [slots, pairs, 16, D] and [.., 16, 2]
   PageMap map;
   int64_t q_token, q_head;
   int64_t k_page, kc_token, kc_head, v_page, vc_token, vc_head;
   int64_t capacity;  // tokens of a sequence's pages
   int n_seq, H, G, pairs, head_blocks, window;  // window 0: all keys
+  int chunks;  // parts of the axis of all sequences' tiles
+  int direct;  // a chunk is one sequence: no partial results
   float c, cap2;  // factor on q.k, and cap log2 e (0: none), see paged.hip
 };
 
@@ -217,7 +219,7 @@ void launch_absorb_dax(const AbsorbArgs &, hipStream_t);
 
 // paged.hip (bf16 / f16)
 template <typename T> void launch_paged_append(const AppendArgs &, hipStream_t);
-template <typename T> void launch_paged_decode(const DecodeArgs &, int D, int grid, hipStream_t);
+template <typename T> void launch_paged_decode(const DecodeArgs &, int D, hipStream_t);
 
 // masked_fwd.hip, masked_bwd.hip (bf16 / f16, D in {64, 128, 256})
 template <typename T, int D> void launch_masked_fwd(const MaskedArgs &, hipStream_t);

@@ -56,10 +56,11 @@ VAFA_HD int32_t page_of(const PageMap &m, int64_t b, int32_t pos, const PageSlot
 }
 
 // ---- decoding attention: tiles of kDecodeTile keys ------------------------------
-// The tiles of all (sequence, key head, head block) pairs in that order form one
-// axis; workgroup g of `grid` takes the tiles [g * per, (g + 1) * per) of it.
+// The tiles of all sequences, one after another, form one axis, of which chunk c takes
+// the tiles [c * per, (c + 1) * per).  A workgroup walks one chunk for one pair (key head,
+// block of kDecodeRows query heads).
 constexpr int kDecodeTile = 128;
-constexpr int kDecodeRows = 16;  // query heads of one pair (a head block)
+constexpr int kDecodeRows = 16;
 
 // Keys of a sequence that its new token sees, and their tiles.
 VAFA_HD int32_t decode_seen(int32_t len, int32_t window) {
@@ -69,14 +70,14 @@ VAFA_HD int32_t decode_tiles(int32_t len, int32_t window) {
   const int32_t n = decode_seen(len, window);
   return n / kDecodeTile + (n % kDecodeTile != 0);
 }
-VAFA_HD int32_t decode_per(int32_t total, int32_t grid) {
-  return total / grid + (total % grid != 0);
+VAFA_HD int32_t decode_per(int32_t total, int32_t chunks) {
+  return total / chunks + (total % chunks != 0);
 }
-// Partial result of the piece that workgroup g forms of a pair whose tiles start
-// at t0 of the axis: its first piece has slot 2 g, its last 2 g + 1 (pieces
-// between them are whole pairs and need none).
-VAFA_HD int64_t decode_slot(int32_t g, int32_t t0, int32_t per) {
-  return 2 * (int64_t)g + ((int64_t)g * per < t0 ? 1 : 0);
+// Partial result of the piece that chunk c holds of a sequence whose tiles start at t0
+// of the axis: its first piece has slot 2 c, its last 2 c + 1 (pieces between them are
+// whole sequences and need none).
+VAFA_HD int64_t decode_slot(int32_t c, int32_t t0, int32_t per) {
+  return 2 * (int64_t)c + ((int64_t)c * per < t0 ? 1 : 0);
 }
 
 }  // namespace vafa
