@@ -177,6 +177,20 @@ def test_call_refusals():
             ({"H": 3}, AssertionError, "do not divide"),
             ({"v": torch.zeros(6, 2, 64)}, AssertionError, "share dtype"),
             ({"v": torch.zeros(5, 2, 64, dtype=torch.bfloat16)}, AssertionError, "T_k, H_k"),
+            ({"v": torch.zeros(6, 128, dtype=torch.bfloat16)}, ValueError, "got 2-D"),
+            ({"v": torch.zeros(2, 6, 2, 64, dtype=torch.bfloat16)}, ValueError, "batch=1"),
+            ({"alibi_slopes": slopes.double()}, AssertionError, "alibi_slopes"),
+            ({"alibi_slopes": slopes[:3]}, AssertionError, "alibi_slopes"),
+            ({"alibi_slopes": slopes.clone().requires_grad_(True)}, ValueError, "no gradient"),
+            ({}, AssertionError, "requires GPU tensors")):
+        with pytest.raises(error, match=text):
+            _call(**kw)
+
+
+def test_option_refusals():
+    from varlenabsorbflashattn_amd import masked
+    c = torch.tensor([0, 6], dtype=torch.int32)
+    for kw, error, text in (
             ({"window": 0}, ValueError, "window must be positive"),
             ({"softcap": -1.0}, ValueError, "softcap"),
             ({"softcap": 0.0}, ValueError, "softcap"),
@@ -184,14 +198,25 @@ def test_call_refusals():
             ({"scale": float("nan")}, ValueError, "scale"),
             ({"causal": False, "window": 3}, ValueError, "belong to the causal"),
             ({"causal": False, "prefix_lens": torch.tensor([1])}, ValueError, "belong"),
-            ({"alibi_slopes": slopes.double()}, AssertionError, "alibi_slopes"),
-            ({"alibi_slopes": slopes[:3]}, AssertionError, "alibi_slopes"),
-            ({"alibi_slopes": slopes.clone().requires_grad_(True)}, ValueError, "no gradient"),
             ({"cu_seqlens_q": None}, ValueError, "cu_seqlens_q or q_seqinfo"),
-            ({"cu_seqlens_k": torch.tensor([0, 3, 6])}, AssertionError, "segment count"),
-            ({}, AssertionError, "requires GPU tensors")):
+            ({"cu_seqlens_k": None}, ValueError, "cu_seqlens_k or k_seqinfo"),
+            ({"cu_seqlens_k": torch.tensor([0, 3, 6])}, AssertionError, "segment count")):
+        args = {"cu_seqlens_q": c, "cu_seqlens_k": c, "q_seqinfo": None, "k_seqinfo": None,
+                "causal": True, "window": None, "prefix_lens": None, "softcap": None,
+                "scale": None, **kw}
         with pytest.raises(error, match=text):
-            _call(**kw)
+            masked._check_options(64, **args)
+
+
+def test_lengths_on_the_host():
+    from varlenabsorbflashattn_amd import masked
+    for bad in (torch.zeros(3), torch.zeros(3, dtype=torch.bool)):
+        with pytest.raises(AssertionError, match="must be integers"):
+            masked._host(bad, "prefix_lens")
+    assert masked._host(torch.arange(8)[::2], "x").is_contiguous()
+    a = torch.tensor([0, 3], dtype=torch.int32)
+    key = _lib.ops().cu_key
+    assert key(a) == key(a.clone()) != key(a.long()) and key(a) != key(a + 1)
 
 
 def test_oracle_against_autograd():

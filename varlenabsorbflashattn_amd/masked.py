@@ -15,7 +15,7 @@ from typing import Optional
 import torch
 
 from . import _lib, varlen
-from .varlen import _aligned, _check_tokens, _normalize_qkv, _seqinfo_to_cu_seqlens
+from .varlen import _check_tokens, _seqinfo_to_cu_seqlens
 
 
 def _host(t, name):
@@ -64,25 +64,33 @@ def _plan_of(q, k, cu_seqlens_q, cu_seqlens_k, causal, window, prefix_lens):
     return plan
 
 
-class _PackedMaskedAttnFunction(torch.autograd.Function):
+def _check_options(D, cu_seqlens_q, cu_seqlens_k, q_seqinfo, k_seqinfo, causal, window,
+                   prefix_lens, softcap, scale):
+    """cu_seqlens and the options as the kernels take them (window and softcap 0: none)."""
+    if cu_seqlens_q is None:
+        if q_seqinfo is None:
+            raise ValueError("must provide either cu_seqlens_q or q_seqinfo")
+        cu_seqlens_q = _seqinfo_to_cu_seqlens(q_seqinfo)
+    if cu_seqlens_k is None:
+        if k_seqinfo is None:
+            raise ValueError("must provide either cu_seqlens_k or k_seqinfo")
+        cu_seqlens_k = _seqinfo_to_cu_seqlens(k_seqinfo)
+    n_seg = cu_seqlens_q.numel() - 1
+    assert cu_seqlens_k.numel() - 1 == n_seg, \
+        f"segment count mismatch: q has {n_seg}, k has {cu_seqlens_k.numel() - 1}"
 
-    @staticmethod
-    def forward(ctx, q, k, v, cu_seqlens_q, cu_seqlens_k, causal, window, prefix_lens, softcap,
-                alibi_slopes, scale):
-        q, k, v = _aligned(q), _aligned(k), _aligned(v)
-        ops = _lib.ops()
-        plan = _plan_of(q, k, cu_seqlens_q, cu_seqlens_k, causal, window, prefix_lens)
-        o, lse = ops.masked_fwd(q, k, v, plan.native, scale, softcap, window, alibi_slopes)
-        ctx.save_for_backward(q, k, v, o, lse, alibi_slopes)
-        ctx.plan = plan
-        ctx.args = scale, softcap, window
-        return o
-
-    @staticmethod
-    def backward(ctx, do):
-        q, k, v, o, lse, slopes = ctx.saved_tensors
-        return *_lib.ops().masked_bwd(q, k, v, o, lse, do, ctx.plan.native, *ctx.args, slopes), \
-            None, None, None, None, None, None, None, None
+    if window is not None and window < 1:
+        raise ValueError(f"window must be positive, got {window}")
+    if softcap is not None and not (softcap > 0 and math.isfinite(softcap)):
+        raise ValueError(f"softcap must be positive and finite, got {softcap}")
+    if not causal and (window is not None or prefix_lens is not None):
+        raise ValueError("window and prefix_lens belong to the causal mask")
+    if scale is None:
+        scale = 1.0 / math.sqrt(D)
+    if not math.isfinite(scale):
+        raise ValueError(f"scale must be finite, got {scale}")
+    return (cu_seqlens_q, cu_seqlens_k, bool(causal), int(window or 0), float(softcap or 0.0),
+            float(scale))
 
 
 def packed_masked_attn(
@@ -114,53 +122,12 @@ def packed_masked_attn(
     gradient) times ``|p - j|``.  A row that sees no key gets zeros and no gradient.
     The backward is deterministic.  Segments of at most 2^30 tokens together.
     """
-    q3, q_was_4d = _normalize_qkv(q, "q")
-    k3, _ = _normalize_qkv(k, "k")
-    v3, _ = _normalize_qkv(v, "v")
-    T_q, H, D = q3.shape
-    T_k, H_k = k3.shape[:2]
-    assert k3.shape == v3.shape == (T_k, H_k, D), \
-        f"k and v must be [T_k, H_k, {D}], got {tuple(k3.shape)} and {tuple(v3.shape)}"
-    assert H_k >= 1 and H % H_k == 0 and H >= 1, \
-        f"{H} query heads do not divide among {H_k} key heads"
-    assert q3.dtype == k3.dtype == v3.dtype, "q/k/v must share dtype"
-    assert q3.dtype in (torch.bfloat16, torch.float16), \
-        f"dtype {q3.dtype} not supported (float16, bfloat16)"
-    assert D in (64, 128, 256), f"head_dim {D} not supported (64, 128, 256)"
+    ops = _lib.ops()
+    q3, k3, v3 = ops.masked_operands(q, k, v, alibi_slopes)
 
-    if cu_seqlens_q is None:
-        if q_seqinfo is None:
-            raise ValueError("must provide either cu_seqlens_q or q_seqinfo")
-        cu_seqlens_q = _seqinfo_to_cu_seqlens(q_seqinfo)
-    if cu_seqlens_k is None:
-        if k_seqinfo is None:
-            raise ValueError("must provide either cu_seqlens_k or k_seqinfo")
-        cu_seqlens_k = _seqinfo_to_cu_seqlens(k_seqinfo)
-    n_seg = cu_seqlens_q.numel() - 1
-    assert cu_seqlens_k.numel() - 1 == n_seg, \
-        f"segment count mismatch: q has {n_seg}, k has {cu_seqlens_k.numel() - 1}"
-
-    if window is not None and window < 1:
-        raise ValueError(f"window must be positive, got {window}")
-    if softcap is not None and not (softcap > 0 and math.isfinite(softcap)):
-        raise ValueError(f"softcap must be positive and finite, got {softcap}")
-    if not causal and (window is not None or prefix_lens is not None):
-        raise ValueError("window and prefix_lens belong to the causal mask")
-    if scale is None:
-        scale = 1.0 / math.sqrt(D)
-    if not math.isfinite(scale):
-        raise ValueError(f"scale must be finite, got {scale}")
-    if alibi_slopes is not None:
-        assert alibi_slopes.shape == (H,) and alibi_slopes.dtype == torch.float32, \
-            f"alibi_slopes must be float32 [{H}]"
-        if alibi_slopes.requires_grad and torch.is_grad_enabled():
-            raise ValueError("alibi_slopes get no gradient: detach them")
-        alibi_slopes = alibi_slopes.contiguous()
-    assert q3.is_cuda, "packed_masked_attn requires GPU tensors"
-    assert all(t.device == q3.device for t in (k3, v3, alibi_slopes) if t is not None), \
-        "q/k/v and alibi_slopes must be on the same device"
-
-    o3 = _PackedMaskedAttnFunction.apply(q3, k3, v3, cu_seqlens_q, cu_seqlens_k, bool(causal),
-                                         int(window or 0), prefix_lens, float(softcap or 0.0),
-                                         alibi_slopes, float(scale))
-    return o3.unsqueeze(0) if q_was_4d else o3
+    cu_seqlens_q, cu_seqlens_k, causal, window, softcap, scale = _check_options(
+        q3.shape[2], cu_seqlens_q, cu_seqlens_k, q_seqinfo, k_seqinfo, causal, window, prefix_lens,
+        softcap, scale)
+    plan = _plan_of(q3, k3, cu_seqlens_q, cu_seqlens_k, causal, window, prefix_lens)
+    o3 = ops.masked_attn(q3, k3, v3, plan.native, scale, softcap, window, alibi_slopes)
+    return o3.unsqueeze(0) if q.dim() == 4 else o3
