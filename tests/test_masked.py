@@ -122,6 +122,7 @@ def test_plan_refusals():
             _lib.plan_masked(c, c, *args, **kw)
     bad(AssertionError, "do not divide", 3, 2, 64)
     bad(AssertionError, "do not divide", 0, 1, 64)
+    bad(ValueError, "more than 4096 query heads", 8192, 8, 64)
     bad(ValueError, "belong to the causal", 2, 1, 64, False, 5)
     bad(ValueError, "belong to the causal", 2, 1, 64, False, 0, [1, 1])
     bad(ValueError, "window must be positive", 2, 1, 64, True, -1)
@@ -154,7 +155,7 @@ def test_c_abi_refusals():
         return call(*[value if i == at else y for i, y in enumerate(args)])
     for at, bad, want in ((0, x + 2, "VALUE"), (7, 3, "ASSERT"), (8, 32, "ASSERT"),
                           (9, _lib.DT_F32, "ASSERT"), (10, float("nan"), "VALUE"),
-                          (11, -2.0, "VALUE"), (12, -1, "VALUE"), (6, other.info, "VALUE")):
+                          (11, -2.0, "VALUE"), (11, 1e-40, "VALUE"), (12, -1, "VALUE"), (6, other.info, "VALUE")):
         assert rc(L.vafa_masked_fwd, f, at, bad) == getattr(_lib, "VAFA_ERR_" + want), at
     for at, bad, want in ((4, x + 8, "VALUE"), (19, need - 1, "WORKSPACE"), (18, None, "WORKSPACE"),
                           (18, x + 4, "WORKSPACE"), (15, float("inf"), "VALUE")):

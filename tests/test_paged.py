@@ -133,7 +133,8 @@ def test_refused_by_the_c_abi():
     assert rc(12, need - 1) == _lib.VAFA_ERR_WORKSPACE
     assert rc(11, None) == _lib.VAFA_ERR_WORKSPACE
     assert rc(10, _lib.DT_F32) == _lib.VAFA_ERR_ASSERT
-    for at, bad in ((1, x + 2), (2, 100), (6, float("nan")), (7, -1.0), (7, float("inf")), (8, -1)):
+    for at, bad in ((1, x + 2), (2, 100), (6, float("nan")), (7, -1.0), (7, float("inf")), (7, 1e-40),
+                    (8, -1)):
         assert rc(at, bad) == _lib.VAFA_ERR_VALUE, at
     app = [cache(), x, 128, 64, x, 128, 64, 3, None, x, 256, 64, 4, x, x, 64, 0, _lib.DT_BF16, None]
     for at, bad in ((1, x + 8), (2, 4), (5, -8), (7, 4), (7, -1), (9, x + 2), (12, -1), (15, 63),

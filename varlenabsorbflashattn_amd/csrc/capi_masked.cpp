@@ -21,6 +21,8 @@ int check_plan(const vafa_plan_info *info, int64_t Hk, int64_t D) {
     return fail(VAFA_ERR_VALUE, "plan does not belong to this operator");
   if (D != 64 && D != 128 && D != 256)
     return fail(VAFA_ERR_ASSERT, "head_dim %lld not supported (64, 128, 256)", (long long)D);
+  if (info->H > kMaskedMaxHeads)
+    return fail(VAFA_ERR_VALUE, "more than %lld query heads", (long long)kMaskedMaxHeads);
   if (Hk < 1 || info->H < 1 || info->H % Hk != 0)
     return fail(VAFA_ERR_ASSERT, "%lld query heads do not divide among %lld key heads",
                 (long long)info->H, (long long)Hk);
@@ -42,6 +44,8 @@ int check_call(const vafa_plan_info *info, int64_t Hk, int64_t D, int32_t dtype,
   if (!std::isfinite(scale)) return fail(VAFA_ERR_VALUE, "scale must be finite");
   if (!(softcap >= 0.f) || !std::isfinite(softcap))
     return fail(VAFA_ERR_VALUE, "softcap must be positive and finite");
+  if (softcap > 0.f && !std::isfinite(2.f * kLog2e * scale / softcap))
+    return fail(VAFA_ERR_VALUE, "scale / softcap is not finite");
   if (window < 0) return fail(VAFA_ERR_VALUE, "window must be positive");
   for (const void *p : ptrs)
     if ((uintptr_t)p % 16 != 0) return fail(VAFA_ERR_VALUE, "operands must be 16-byte aligned");

@@ -99,7 +99,7 @@ int plan_decode(const vafa_paged_cache *c, int64_t H, int64_t window, DecodePlan
   const int64_t keys = window > 0 ? std::min(cap, window) : cap;
   const int64_t most = (keys + kDecodeTile - 1) / kDecodeTile;  // tiles of a sequence
   const int64_t tiles = c->n_seq * most;
-  if (tiles > INT32_MAX / 2 || c->n_seq * H > INT32_MAX / 2)
+  if (tiles > INT32_MAX / 2 || (c->n_seq + 8) * std::max(H, p->pairs) > INT32_MAX / 2)
     return fail(VAFA_ERR_VALUE, "paged_decode_attn: page_table addresses too many keys (%lld tiles)",
                 (long long)tiles);
   p->direct = most <= kDecodeDirect;
@@ -177,6 +177,8 @@ int vafa_paged_decode(const vafa_paged_cache *c, const void *q, int64_t q_token,
   if (!std::isfinite(scale)) return fail(VAFA_ERR_VALUE, "%s: scale must be finite", what);
   if (!(softcap >= 0.f) || !std::isfinite(softcap))
     return fail(VAFA_ERR_VALUE, "%s: softcap must be positive and finite", what);
+  if (softcap > 0.f && !std::isfinite(2.f * kLog2e * scale / softcap))
+    return fail(VAFA_ERR_VALUE, "%s: scale / softcap is not finite", what);
   if (int rc = check_rows(what, "q", q, q_token, q_head)) return rc;
   if (int rc = check_rows(what, "out", out, 0, 0)) return rc;
   if (p.bytes > 0 &&

@@ -39,7 +39,7 @@ __device__ __forceinline__ TokenAt token_at(const AppendArgs &a, int t, int lane
     b = seq_of(a.cu, a.n_seq, t, lane);
     if (b < a.n_seq) i = t - a.cu[b];
   }
-  if (b >= a.n_seq) return at;
+  if (b >= a.n_seq || i < 0) return at;  // (i < 0: a token in front of cu[0])
   const int64_t pos = (int64_t)a.lens[b] + i;
   if (pos < 0 || pos > INT32_MAX) return at;
   at.pos = (int)pos;

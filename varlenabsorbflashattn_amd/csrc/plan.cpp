@@ -18,6 +18,7 @@
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
+#include <exception>
 #include <functional>
 #include <numeric>
 #include <string>
@@ -506,14 +507,16 @@ int vafa_plan_varlen_balanced(const int64_t *cu_q, const int64_t *cu_k, int64_t 
 //                 kVarlenTile rows.
 // Rows of a tile are (token, head) pairs of a head set (masked_set_log2, which
 // info->xcd_heads holds): q_tile rows are q_tile >> k tokens.
-int vafa_plan_masked(const int64_t *cu_q, const int64_t *cu_k, const int64_t *prefix, int64_t n1,
-                     int64_t H, int64_t Hk, int64_t D, int32_t causal, int64_t window,
-                     int32_t *plan, int64_t plan_cap, vafa_plan_info *info) {
+static int plan_masked(const int64_t *cu_q, const int64_t *cu_k, const int64_t *prefix, int64_t n1,
+                       int64_t H, int64_t Hk, int64_t D, int32_t causal, int64_t window,
+                       int32_t *plan, int64_t plan_cap, vafa_plan_info *info) {
   int rc = check_pair(cu_q, cu_k, n1);
   if (rc) return rc;
-  if (H < 1 || Hk < 1 || H % Hk != 0 || H > 65536)
+  if (H < 1 || Hk < 1 || H % Hk != 0)
     return fail(VAFA_ERR_ASSERT, "%lld query heads do not divide among %lld key heads",
                 (long long)H, (long long)Hk);
+  if (H > kMaskedMaxHeads)
+    return fail(VAFA_ERR_VALUE, "more than %lld query heads", (long long)kMaskedMaxHeads);
   if (window < 0) return fail(VAFA_ERR_VALUE, "window must be positive");
   if (!causal && (window > 0 || prefix != nullptr))
     return fail(VAFA_ERR_VALUE, "window and prefix_lens belong to the causal mask");
@@ -724,6 +727,16 @@ int vafa_plan_masked(const int64_t *cu_q, const int64_t *cu_k, const int64_t *pr
   info->n_fpart_rows = kprow;
   info->max_split = max_split;
   return emit(fwd, comb, kv, {}, dq, dqc, {}, kvc, plan, plan_cap, info);
+}
+
+int vafa_plan_masked(const int64_t *cu_q, const int64_t *cu_k, const int64_t *prefix, int64_t n1,
+                     int64_t H, int64_t Hk, int64_t D, int32_t causal, int64_t window,
+                     int32_t *plan, int64_t plan_cap, vafa_plan_info *info) {
+  try {
+    return plan_masked(cu_q, cu_k, prefix, n1, H, Hk, D, causal, window, plan, plan_cap, info);
+  } catch (const std::exception &e) {  // out of memory: no exception leaves a C entry
+    return fail(VAFA_ERR_RUNTIME, "vafa_plan_masked: %s", e.what());
+  }
 }
 
 // Absorb plan.  Query rows are (token, head) pairs; one item covers whole

@@ -60,6 +60,8 @@ constexpr VarlenBalance kVarlenBalance{256, 512, 32 << 20};
 // packed_masked_attn: most tokens of a call (positions, and a position less the window,
 // are 32-bit in the kernels).
 constexpr int64_t kMaskedMaxTokens = int64_t{1} << 30;
+// Query heads: 256 rows of them lie within 2^31 bytes at D = 256.
+constexpr int64_t kMaskedMaxHeads = 4096;
 constexpr int64_t kMaskedMaxParts = 256;
 // The planner's model of a pass's time, in units of one key (query tiles) or one block of
 // 32 rows (key tiles): the smallest chunk and its alignment, what an item costs beside
@@ -69,8 +71,13 @@ struct MaskedModel {
   int64_t min_chunk, align, item;
   double launch, row;
 };
-constexpr MaskedModel kMaskedQuery{512, 64, 150, 48000.0, 0.02};
-constexpr MaskedModel kMaskedKeys{16, 1, 6, 800.0, 2.5e-4};
+// Forward + backward, us, with launch and row terms of 48000 / 0.02 (keys) and 800 / 2.5e-4
+// (blocks) -> these: 24 sequences of at most 933 tokens, 12 heads of 64 112 -> 97, 16 of at
+// most 2387, 16 heads of 128 on 4 335 -> 329, 64 of at most 4002 on them 1234 -> 1205, a
+// forward of 8 x 100..512 queries against 4k..29k keys 685 -> 671; 8 x 2048, 16 heads of 64
+// on 4, 386 -> 392.  Without any splits the first three take 120, 374 and 1352.
+constexpr MaskedModel kMaskedQuery{512, 64, 150, 24000.0, 0.02};
+constexpr MaskedModel kMaskedKeys{16, 1, 6, 400.0, 1.2e-4};
 constexpr double kMaskedWideGain = 0.95;
 // Query heads that share a key head lie in sets of 2^k rows of a tile (csrc/masked.h):
 // k for G heads a key head.
