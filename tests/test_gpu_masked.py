@@ -331,3 +331,94 @@ def test_decode_after_append_matches_the_packed_pass(device, opts):
         within("o", out, val[i], bound[i])
     same = torch.equal(torch.nan_to_num(kc), torch.nan_to_num(kc2))
     assert same and torch.equal(torch.nan_to_num(vc), torch.nan_to_num(vc2))
+
+
+def test_shared_and_expanded_keys(device):
+    """Keys that one tensor gives to two segments, values expanded over the key heads: the
+    copies' gradients add up in the leaf."""
+    print("[masked expanded]", flush=True)
+    n, H, Hk, D = 40, 4, 2, 64
+    q, k, v, do = inputs(57, [2 * n], [n], H, Hk, D, HF, device)
+    x = [t.detach().requires_grad_(True) for t in (q, k, v[:, :1])]
+    kk, vv = torch.cat([x[1], x[1]]), x[2].expand(n, Hk, D).repeat(2, 1, 1)
+    cu = cu_from_lens([n, n])
+    o = packed_masked_attn(x[0], kk, vv, cu_seqlens_q=cu, cu_seqlens_k=cu)
+    dq, dk, dv = torch.autograd.grad(o, x, do)
+    ref = om.attention(f64(q), f64(kk), f64(vv), f64(do), [0, n, 2 * n], [0, n, 2 * n], D ** -0.5,
+                       u=U[HF], a=A[HF])
+    within("dq", dq, *ref["dq"])
+    val, bound = (np.add(x[:n], x[n:]) for x in ref["dk"])
+    u = U[HF]  # torch adds the two in fp16 again
+    within("dk", dk, val, bound + u * np.abs(val) + A[HF])
+    val, bound = (x.reshape(2, n, Hk, D).sum((0, 2))[:, None] for x in ref["dv"])
+    mag = np.abs(ref["dv"][0]).reshape(2, n, Hk, D).sum((0, 2))[:, None]
+    within("dv", dv, val, bound + 3 * (u * mag + A[HF]))
+
+
+def test_needs_grad_of_some(device):
+    """Gradients of k and v alone, of q alone, and a second derivative refused."""
+    print("[masked some]", flush=True)
+    ql = [70]
+    x = inputs(58, ql, ql, 4, 2, 64, BF, device)
+    want = step(*x, ql, ql)
+    cu = cu_from_lens(ql)
+    for need in ((0,), (1, 2), (2,)):
+        y = [t.detach().requires_grad_(i in need) for i, t in enumerate(x[:3])]
+        o = packed_masked_attn(*y, cu_seqlens_q=cu, cu_seqlens_k=cu)
+        got = torch.autograd.grad(o, [y[i] for i in need], x[3])
+        for i, t in zip(need, got):
+            assert torch.equal(t, want[1 + i])
+    y = [t.detach().requires_grad_(True) for t in x[:3]]
+    o = packed_masked_attn(*y, cu_seqlens_q=cu, cu_seqlens_k=cu)
+    g, = torch.autograd.grad(o, y[:1], x[3], create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(g.sum(), y[1])
+
+
+def test_two_threads(device):
+    """Calls of different lengths from two threads, each on a stream of its own."""
+    import threading
+    print("[masked threads]", flush=True)
+    cases = []
+    for i, (ql, kw) in enumerate((([200, 50], {"window": 60}), ([90, 300], {"softcap": 4.0}))):
+        x = inputs(59 + i, ql, ql, 4, 2, 64, BF, device)
+        cases.append((x, ql, kw, step(*x, ql, ql, **kw)))
+    torch.cuda.synchronize()
+    errors = []
+
+    def work(x, ql, kw, want):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(20):
+                    got = step(*x, ql, ql, **kw)
+                torch.cuda.current_stream().synchronize()
+            for a, b in zip(got, want):
+                assert torch.equal(a, b)
+        except BaseException as e:
+            errors.append(e)
+    threads = [threading.Thread(target=work, args=c) for c in cases]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+
+
+def test_past_4_gib(device):
+    """Tensors of more than 4 GiB: the last segment, a copy of the first, gives its bits."""
+    n, seg, H, D = 2200, 512, 16, 128
+    print(f"[masked far] {n} x {seg} tokens, {n * seg * H * D * 2 / 2 ** 30:.1f} GiB each",
+          flush=True)
+    g = torch.Generator(device=device).manual_seed(60)
+    x = []
+    for _ in range(4):
+        t = torch.empty(n * seg, H, D, device=device, dtype=BF)
+        t.view(n, seg * H * D).copy_(torch.randn(1, seg * H * D, generator=g, device=device))
+        x.append(t)
+    lens = [seg] * n
+    got = step(*x, lens, lens, window=100)
+    near = step(*(t[:seg] for t in x), [seg], [seg], window=100)
+    for far, one in zip(got, near):
+        assert torch.equal(far[-seg:], one) and torch.equal(far[:seg], one)
+    small = [t[:seg, :2] for t in x]
+    compare([t[:, :2] for t in near], *small, [seg], [seg], window=100)

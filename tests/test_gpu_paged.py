@@ -382,3 +382,75 @@ def test_empty_calls(device):
     out = paged_decode_attn(torch.ones(3, 2, 64, device=device, dtype=torch.bfloat16), kc, kc,
                             torch.zeros(3, 0, dtype=torch.int32, device=device), lens + 5)
     assert not out.any()
+
+
+def test_caches_past_4_gib(device):
+    """Pages beyond 4 GiB of a cache hold and give the same bits as near ones."""
+    page, Hk, D, H, dt = 256, 2, 128, 8, torch.bfloat16
+    N = (5 << 30) // (page * Hk * D * 2)
+    print(f"[far pages] {N} pages", flush=True)
+    g = torch.Generator(device=device).manual_seed(12)
+    kc = torch.zeros(N, page, Hk, D, device=device, dtype=dt)
+    vc = torch.zeros_like(kc)
+    x = torch.randn(700, H + 2 * Hk, D, generator=g, device=device).to(dt)
+    inv = (10000.0 ** (-torch.arange(0, D, 2) / D)).float().to(device)
+    outs = []
+    for pages in ([0, 1, 2], [N - 1, N - 3, N - 2]):
+        table = torch.tensor([pages], dtype=torch.int32, device=device)
+        zero = torch.zeros(1, dtype=torch.int32, device=device)
+        q = paged_kv_append(x[:, H:H + Hk], x[:, H + Hk:], kc, vc, table, zero,
+                            cu_seqlens=torch.tensor([0, 700], dtype=torch.int32, device=device),
+                            q=x[:, :H], inv_freq=inv)
+        out = paged_decode_attn(q[-1:], kc, vc, table, zero + 700)
+        outs.append((q, out, kc[pages].clone(), vc[pages].clone()))
+    for a, b in zip(*outs):
+        assert torch.equal(a, b)
+    assert not kc[3:N - 3].any()
+    q, out = outs[0][:2]
+    ref = op.decode(f64(q[-1:]), f64(kc[:3]), f64(vc[:3]), np.array([[0, 1, 2]]), [700], D ** -0.5)
+    close_decode(out, *ref)
+
+
+def test_two_threads(device):
+    """Decoding from two threads, each on a stream of its own."""
+    import threading
+    print("[decode threads]", flush=True)
+    work, errors = [], []
+    for case in (5, 9):
+        lens, q, kc, vc, table, slopes, kw = decode_case(case, device)
+        args = (q, kc, vc, table.to(device), torch.tensor(lens, dtype=torch.int32, device=device))
+        work.append((args, kw, None if slopes is None else slopes.to(device),
+                     paged_decode_attn(*args, alibi_slopes=None if slopes is None
+                                       else slopes.to(device), **kw)))
+    torch.cuda.synchronize()
+
+    def run(args, kw, slopes, want):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(50):
+                    out = paged_decode_attn(*args, alibi_slopes=slopes, **kw)
+                torch.cuda.current_stream().synchronize()
+            assert torch.equal(out, want)
+        except BaseException as e:
+            errors.append(e)
+    threads = [threading.Thread(target=run, args=w) for w in work]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+
+
+def test_tokens_in_front_of_the_first_sequence(device):
+    """cu_seqlens that does not start at 0: the tokens in front belong to no sequence."""
+    print("[append cu]", flush=True)
+    kc = torch.zeros(2, 16, 1, 64, device=device, dtype=torch.bfloat16)
+    vc = torch.zeros_like(kc)
+    k = torch.ones(5, 1, 64, device=device, dtype=torch.bfloat16)
+    table = torch.tensor([[1]], dtype=torch.int32, device=device)
+    q = paged_kv_append(k, k, kc, vc, table, torch.tensor([4], dtype=torch.int32, device=device),
+                        cu_seqlens=torch.tensor([3, 5], dtype=torch.int32, device=device), q=k)
+    assert not q[:3].any() and q[3:].all()
+    want = torch.zeros(16, dtype=torch.bool)
+    want[4:6] = True
+    assert torch.equal(kc[1, :, 0].any(-1).cpu(), want) and not kc[0].any()
