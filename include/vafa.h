@@ -386,21 +386,22 @@ VAFA_API int vafa_absorb_project_f32_bwd(const float *q_raw, const float *W_Q, c
  * lse [T_q,H] fp32 log2-domain, under a plan of vafa_plan_masked made with the same H,
  * Hk, D and window.  Scores are scale q.k, then softcap tanh(. / softcap) (0: none),
  * then minus slopes[h] (device fp32 [H] or NULL) times |position of the query - key|.
- * Rows that see no key get zeros (lse -inf). */
+ * Rows that see no key get zeros (lse -inf).  o_lo: T_q * H * D bytes for the backward,
+ * which hold more bits of o in an order of their own, or NULL. */
 VAFA_API int64_t vafa_masked_fwd_workspace(const vafa_plan_info *info, int64_t Hk, int64_t D);
-VAFA_API int vafa_masked_fwd(const void *q, const void *k, const void *v, void *o, float *lse,
-                             const int32_t *plan_dev, const vafa_plan_info *info, int64_t Hk,
-                             int64_t D, int32_t dtype, float scale, float softcap, int64_t window,
-                             const float *slopes, void *workspace, int64_t workspace_bytes,
-                             void *stream);
+VAFA_API int vafa_masked_fwd(const void *q, const void *k, const void *v, void *o, void *o_lo,
+                             float *lse, const int32_t *plan_dev, const vafa_plan_info *info,
+                             int64_t Hk, int64_t D, int32_t dtype, float scale, float softcap,
+                             int64_t window, const float *slopes, void *workspace,
+                             int64_t workspace_bytes, void *stream);
 /* dO [T_q,H,D] -> dq, dk, dv.  Deterministic (no atomics). */
 VAFA_API int64_t vafa_masked_bwd_workspace(const vafa_plan_info *info, int64_t Hk, int64_t D);
 VAFA_API int vafa_masked_bwd(const void *q, const void *k, const void *v, const void *o,
-                             const void *dout, const float *lse, void *dq, void *dk, void *dv,
-                             const int32_t *plan_dev, const vafa_plan_info *info, int64_t Hk,
-                             int64_t D, int32_t dtype, float scale, float softcap, int64_t window,
-                             const float *slopes, void *workspace, int64_t workspace_bytes,
-                             void *stream);
+                             const void *o_lo, const void *dout, const float *lse, void *dq,
+                             void *dk, void *dv, const int32_t *plan_dev,
+                             const vafa_plan_info *info, int64_t Hk, int64_t D, int32_t dtype,
+                             float scale, float softcap, int64_t window, const float *slopes,
+                             void *workspace, int64_t workspace_bytes, void *stream);
 
 /* ======================================================================== */
 /* Paged key-value cache (bf16 / fp16).  No counterpart in the reference.   */

@@ -422,3 +422,26 @@ def test_past_4_gib(device):
         assert torch.equal(far[-seg:], one) and torch.equal(far[:seg], one)
     small = [t[:seg, :2] for t in x]
     compare([t[:, :2] for t in near], *small, [seg], [seg], window=100)
+
+
+@pytest.mark.parametrize("ql,kl,H,Hk,D,dt", [([200, 7, 33], None, 4, 2, 64, BF),
+                                             ([130, 1, 61], None, 6, 1, 128, HF),
+                                             ([100], [4000], 2, 1, 128, BF),
+                                             ([90, 21], [90, 3500], 2, 2, 256, HF)])
+def test_gradients_of_rows_that_few_keys_carry(device, ql, kl, H, Hk, D, dt):
+    """Steep distance biases: dP - delta is far below either, so that O's rounding in delta
+    alone would put dQ and dK 3 to 8 u off.  What stays is the rounding of dS for the
+    product and that of the result, independent and of at most u / sqrt(3) each in the mean:
+    0.82 u of the norm."""
+    print(f"[masked steep] {ql} {kl} {H}/{Hk} x {D} {dt}", flush=True)
+    kl = kl or ql
+    x = inputs(61, ql, kl, H, Hk, D, dt, device)
+    slopes = torch.linspace(4.0, 7.0, H, device=device)
+    got = step(*x, ql, kl, alibi_slopes=slopes)
+    ref = om.attention(*(f64(t) for t in x), np.cumsum([0] + ql), np.cumsum([0] + kl), D ** -0.5,
+                       slopes=f64(slopes), u=U[dt], a=A[dt])
+    for name, out in zip(("o", "dq", "dk", "dv"), got):
+        val = ref[name][0]
+        off = np.linalg.norm(f64(out) - val) / np.linalg.norm(val)
+        print(f"  {name:3s} {off / U[dt]:.2f} u", flush=True)
+        assert off < U[dt], (name, off)

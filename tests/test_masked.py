@@ -148,17 +148,19 @@ def test_c_abi_refusals():
     need = L.vafa_masked_bwd_workspace(p.info, 2, 64)
     assert need > 0
     x = 1 << 20
-    f = [x, x, x, x, x, x, p.info, 2, 64, _lib.DT_BF16, 0.1, 0.0, 0, None, x, 1 << 20, None]
-    b = [x] * 10 + [p.info, 2, 64, _lib.DT_BF16, 0.1, 0.0, 0, None, x, need, None]
+    f = [x, x, x, x, x, x, x, p.info, 2, 64, _lib.DT_BF16, 0.1, 0.0, 0, None, x, 1 << 20, None]
+    b = [x] * 11 + [p.info, 2, 64, _lib.DT_BF16, 0.1, 0.0, 0, None, x, need, None]
 
     def rc(call, args, at, value):
         return call(*[value if i == at else y for i, y in enumerate(args)])
-    for at, bad, want in ((0, x + 2, "VALUE"), (7, 3, "ASSERT"), (8, 32, "ASSERT"),
-                          (9, _lib.DT_F32, "ASSERT"), (10, float("nan"), "VALUE"),
-                          (11, -2.0, "VALUE"), (11, 1e-40, "VALUE"), (12, -1, "VALUE"), (6, other.info, "VALUE")):
+    for at, bad, want in ((0, x + 2, "VALUE"), (8, 3, "ASSERT"), (9, 32, "ASSERT"),
+                          (10, _lib.DT_F32, "ASSERT"), (11, float("nan"), "VALUE"),
+                          (11, 3e38, "VALUE"), (12, -2.0, "VALUE"), (12, 1e-40, "VALUE"),
+                          (12, 3e5, "VALUE"), (13, -1, "VALUE"), (7, other.info, "VALUE")):
         assert rc(L.vafa_masked_fwd, f, at, bad) == getattr(_lib, "VAFA_ERR_" + want), at
-    for at, bad, want in ((4, x + 8, "VALUE"), (19, need - 1, "WORKSPACE"), (18, None, "WORKSPACE"),
-                          (18, x + 4, "WORKSPACE"), (15, float("inf"), "VALUE")):
+    for at, bad, want in ((5, x + 8, "VALUE"), (4, None, "VALUE"), (20, need - 1, "WORKSPACE"),
+                          (19, None, "WORKSPACE"), (19, x + 4, "WORKSPACE"),
+                          (16, float("inf"), "VALUE")):
         assert rc(L.vafa_masked_bwd, b, at, bad) == getattr(_lib, "VAFA_ERR_" + want), at
     assert C.sizeof(_lib.PagedCache) == 17 * 8
 
@@ -196,6 +198,9 @@ def test_option_refusals():
             ({"softcap": -1.0}, ValueError, "softcap"),
             ({"softcap": 0.0}, ValueError, "softcap"),
             ({"softcap": float("inf")}, ValueError, "softcap"),
+            ({"softcap": 1e-50}, ValueError, "softcap"),
+            ({"softcap": 2e4}, ValueError, "softcap"),
+            ({"window": 1.5}, ValueError, "window must be positive and whole"),
             ({"scale": float("nan")}, ValueError, "scale"),
             ({"causal": False, "window": 3}, ValueError, "belong to the causal"),
             ({"causal": False, "prefix_lens": torch.tensor([1])}, ValueError, "belong"),

@@ -91,7 +91,7 @@ def test_refused_types_and_devices(call):
 
 
 def test_refused_decode_options():
-    for kw in ({"softcap": 0.0}, {"softcap": -1.0}, {"softcap": float("nan")}):
+    for kw in ({"softcap": 0.0}, {"softcap": -1.0}, {"softcap": float("nan")}, {"softcap": 1e-50}):
         with pytest.raises(ValueError, match="softcap must be positive"):
             _decode(_args(), **kw)
     for w in (0, -3):
@@ -134,7 +134,7 @@ def test_refused_by_the_c_abi():
     assert rc(11, None) == _lib.VAFA_ERR_WORKSPACE
     assert rc(10, _lib.DT_F32) == _lib.VAFA_ERR_ASSERT
     for at, bad in ((1, x + 2), (2, 100), (6, float("nan")), (7, -1.0), (7, float("inf")), (7, 1e-40),
-                    (8, -1)):
+                    (7, 2e4), (6, 3e38), (8, -1)):
         assert rc(at, bad) == _lib.VAFA_ERR_VALUE, at
     app = [cache(), x, 128, 64, x, 128, 64, 3, None, x, 256, 64, 4, x, x, 64, 0, _lib.DT_BF16, None]
     for at, bad in ((1, x + 8), (2, 4), (5, -8), (7, 4), (7, -1), (9, x + 2), (12, -1), (15, 63),
@@ -142,6 +142,12 @@ def test_refused_by_the_c_abi():
         assert rc(at, bad, L.vafa_paged_append, app) == _lib.VAFA_ERR_VALUE, at
     assert rc(0, cache(D=60), L.vafa_paged_append, app) == _lib.VAFA_ERR_ASSERT
     assert "head_dim 60" in _lib.last_error()
+    # more blocks of 256 threads than a launch can have
+    big = list(app)
+    big[0], big[7], big[8] = cache(n_seq=1 << 20), (1 << 31) - 1, x
+    assert L.vafa_paged_append(*big) == _lib.VAFA_ERR_VALUE and "too many" in _lib.last_error()
+    assert rc(0, cache(n_seq=1 << 18, table_width=1), L.vafa_paged_decode,
+              dec[:4] + [128] + dec[5:]) == _lib.VAFA_ERR_VALUE
     # nothing to do: no launch
     app[7], app[8] = 0, x
     assert L.vafa_paged_append(*app) == _lib.VAFA_OK

@@ -115,9 +115,9 @@ _SIGS = {
                                        _I64, _I64, _I32, C.c_float, _P, _I64, _P]),
     "vafa_masked_fwd_workspace": (C.c_int64, [_PINFO, _I64, _I64]),
     "vafa_masked_bwd_workspace": (C.c_int64, [_PINFO, _I64, _I64]),
-    "vafa_masked_fwd": (C.c_int, [_P, _P, _P, _P, _P, _P, _PINFO, _I64, _I64, _I32, C.c_float,
+    "vafa_masked_fwd": (C.c_int, [_P] * 7 + [_PINFO, _I64, _I64, _I32, C.c_float,
                                   C.c_float, _I64, _P, _P, _I64, _P]),
-    "vafa_masked_bwd": (C.c_int, [_P] * 10 + [_PINFO, _I64, _I64, _I32, C.c_float, C.c_float, _I64,
+    "vafa_masked_bwd": (C.c_int, [_P] * 11 + [_PINFO, _I64, _I64, _I32, C.c_float, C.c_float, _I64,
                                               _P, _P, _I64, _P]),
     "vafa_paged_append": (C.c_int, [_PCACHE, _P, _I64, _I64, _P, _I64, _I64, _I64, _P, _P, _I64,
                                     _I64, _I64, _P, _P, _I64, _I32, _I32, _P]),

@@ -41,9 +41,10 @@ int check_call(const vafa_plan_info *info, int64_t Hk, int64_t D, int32_t dtype,
   if (int rc = check_plan(info, Hk, D)) return rc;
   if (dtype != VAFA_BF16 && dtype != VAFA_F16)
     return fail(VAFA_ERR_ASSERT, "dtype not supported (float16, bfloat16)");
-  if (!std::isfinite(scale)) return fail(VAFA_ERR_VALUE, "scale must be finite");
-  if (!(softcap >= 0.f) || !std::isfinite(softcap))
-    return fail(VAFA_ERR_VALUE, "softcap must be positive and finite");
+  if (!std::isfinite(scale * kLog2e)) return fail(VAFA_ERR_VALUE, "scale must be finite");
+  if (!softcap_ok(softcap))
+    return fail(VAFA_ERR_VALUE, "softcap must be positive, from %g to %g", (double)kMinSoftcap,
+                (double)kMaxSoftcap);
   if (softcap > 0.f && !std::isfinite(2.f * kLog2e * scale / softcap))
     return fail(VAFA_ERR_VALUE, "scale / softcap is not finite");
   if (window < 0) return fail(VAFA_ERR_VALUE, "window must be positive");
@@ -109,6 +110,22 @@ int check_ws(int64_t have, const void *ws, int64_t need) {
   return VAFA_OK;
 }
 
+// Blocks of every launch (rows of sums by 2048 values).
+int check_grids(const MaskedArgs &a, const vafa_plan_info *info, bool bwd) {
+  const int64_t sets = a.H >> a.lg, HD = (int64_t)a.H * a.D, HkD = (int64_t)a.Hk * a.D;
+  auto chunks = [](int64_t values) { return (values + 2047) / 2048; };
+  bool ok = grid_ok(a.n_items * sets, !bwd && a.q_tile == kVarlenWideTile ? 512 : 256);
+  if (bwd)
+    ok = ok && grid_ok(a.n_kv * a.Hk, a.D == 256 ? 512 : 256) &&
+         grid_ok((a.n_comb + 2 * a.n_kvc) *
+                     std::max(chunks(a.comb_rows * HD), chunks(a.kvc_rows * HkD)), 256);
+  else
+    ok = ok && grid_ok(a.n_comb * chunks(a.comb_rows * HD), 256);
+  return ok ? VAFA_OK
+            : fail(VAFA_ERR_VALUE, "more tiles than a launch can have (%lld segments, %lld tokens)",
+                   (long long)info->n_seg, (long long)std::max(info->T_q, info->T_k));
+}
+
 int check_launch(const char *what) {
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess)
@@ -121,7 +138,9 @@ void fwd(const MaskedArgs &a, hipStream_t st) {
   if (a.D == 64) launch_masked_fwd<T, 64>(a, st);
   if (a.D == 128) launch_masked_fwd<T, 128>(a, st);
   if (a.D == 256) launch_masked_fwd<T, 256>(a, st);
-  launch_masked_join<T>(a, st);
+  if (a.D == 64) launch_masked_join<T, 64>(a, st);
+  if (a.D == 128) launch_masked_join<T, 128>(a, st);
+  if (a.D == 256) launch_masked_join<T, 256>(a, st);
 }
 
 template <typename T>
@@ -152,16 +171,18 @@ int64_t vafa_masked_bwd_workspace(const vafa_plan_info *info, int64_t Hk, int64_
   return carve(nullptr, info, Hk, D, true).bytes;
 }
 
-int vafa_masked_fwd(const void *q, const void *k, const void *v, void *o, float *lse,
-                    const int32_t *plan_dev, const vafa_plan_info *info, int64_t Hk, int64_t D,
-                    int32_t dtype, float scale, float softcap, int64_t window, const float *slopes,
-                    void *workspace, int64_t workspace_bytes, void *stream) {
-  if (int rc = check_call(info, Hk, D, dtype, scale, softcap, window, {q, k, v, o})) return rc;
+int vafa_masked_fwd(const void *q, const void *k, const void *v, void *o, void *o_lo,
+                    float *lse, const int32_t *plan_dev, const vafa_plan_info *info, int64_t Hk,
+                    int64_t D, int32_t dtype, float scale, float softcap, int64_t window,
+                    const float *slopes, void *workspace, int64_t workspace_bytes, void *stream) {
+  if (int rc = check_call(info, Hk, D, dtype, scale, softcap, window, {q, k, v, o, o_lo}))
+    return rc;
   const Ws w = carve(workspace, info, Hk, D, false);
   if (int rc = check_ws(workspace_bytes, workspace, w.bytes)) return rc;
   MaskedArgs a = args_of(info, plan_dev, Hk, D, scale, softcap, window, slopes);
-  a.q = q; a.k = k; a.v = v; a.o = o; a.lse = lse;
+  a.q = q; a.k = k; a.v = v; a.o = o; a.o_lo = (uint8_t *)o_lo; a.lse = lse;
   a.part_o = w.part_o; a.part_lse = w.part_lse;
+  if (int rc = check_grids(a, info, false)) return rc;
   if (dtype == VAFA_BF16)
     fwd<bf16>(a, (hipStream_t)stream);
   else
@@ -169,24 +190,27 @@ int vafa_masked_fwd(const void *q, const void *k, const void *v, void *o, float 
   return check_launch("vafa_masked_fwd");
 }
 
-int vafa_masked_bwd(const void *q, const void *k, const void *v, const void *o, const void *dout,
-                    const float *lse, void *dq, void *dk, void *dv, const int32_t *plan_dev,
-                    const vafa_plan_info *info, int64_t Hk, int64_t D, int32_t dtype, float scale,
-                    float softcap, int64_t window, const float *slopes, void *workspace,
-                    int64_t workspace_bytes, void *stream) {
+int vafa_masked_bwd(const void *q, const void *k, const void *v, const void *o,
+                    const void *o_lo, const void *dout, const float *lse, void *dq, void *dk,
+                    void *dv, const int32_t *plan_dev, const vafa_plan_info *info, int64_t Hk,
+                    int64_t D, int32_t dtype, float scale, float softcap, int64_t window,
+                    const float *slopes, void *workspace, int64_t workspace_bytes, void *stream) {
   if (int rc = check_call(info, Hk, D, dtype, scale, softcap, window,
-                          {q, k, v, o, dout, dq, dk, dv}))
+                          {q, k, v, o, o_lo, dout, dq, dk, dv}))
     return rc;
+  if (o_lo == nullptr && info->T_q > 0)
+    return fail(VAFA_ERR_VALUE, "the backward needs the forward's o_lo");
   const Ws w = carve(workspace, info, Hk, D, true);
   if (int rc = check_ws(workspace_bytes, workspace, w.bytes)) return rc;
   MaskedArgs a = args_of(info, plan_dev, Hk, D, scale, softcap, window, slopes);
   a.items = plan_dev + info->off_dq; a.n_items = info->n_dq;
   a.comb_items = plan_dev + info->off_dqc; a.n_comb = info->n_dqc;
   a.comb_rows = (int)info->max_dqc_rows;
-  a.q = q; a.k = k; a.v = v; a.o_in = o; a.dout = dout; a.lse_in = lse;
+  a.q = q; a.k = k; a.v = v; a.o_in = o; a.o_lo_in = (const uint8_t *)o_lo; a.dout = dout; a.lse_in = lse;
   a.dq = dq; a.dk = dk; a.dv = dv;
   a.part_o = w.part_o; a.delta = w.delta; a.lse = w.lse;
   a.part_dk = w.part_dk; a.part_dv = w.part_dv;
+  if (int rc = check_grids(a, info, true)) return rc;
   if (dtype == VAFA_BF16)
     bwd<bf16>(a, (hipStream_t)stream);
   else

@@ -99,8 +99,8 @@ int plan_decode(const vafa_paged_cache *c, int64_t H, int64_t window, DecodePlan
   const int64_t keys = window > 0 ? std::min(cap, window) : cap;
   const int64_t most = (keys + kDecodeTile - 1) / kDecodeTile;  // tiles of a sequence
   const int64_t tiles = c->n_seq * most;
-  if (tiles > INT32_MAX / 2 || (c->n_seq + 8) * std::max(H, p->pairs) > INT32_MAX / 2)
-    return fail(VAFA_ERR_VALUE, "paged_decode_attn: page_table addresses too many keys (%lld tiles)",
+  if (tiles > INT32_MAX / 2 || !grid_ok((c->n_seq + kXcds) * std::max(H, p->pairs), 256))
+    return fail(VAFA_ERR_VALUE, "paged_decode_attn: too many sequences or keys (%lld tiles)",
                 (long long)tiles);
   p->direct = most <= kDecodeDirect;
   p->chunks = p->direct ? c->n_seq
@@ -143,6 +143,8 @@ int vafa_paged_append(const vafa_paged_cache *c, const void *k, int64_t k_token,
     if (int rc = check_rows(what, "q", q, q_token, q_head)) return rc;
     if (int rc = check_rows(what, "q_out", q_out, 0, 0)) return rc;
   }
+  if (!grid_ok(std::max(T, T * ((H + 2 * c->Hk) * (c->D / 16)) / 256 + 1), 256))
+    return fail(VAFA_ERR_VALUE, "%s: %lld tokens are too many for a call", what, (long long)T);
   if (T == 0) return VAFA_OK;
   AppendArgs a{};
   a.q = q; a.k = k; a.v = v; a.q_out = q_out; a.kc = c->k; a.vc = c->v;
@@ -174,9 +176,11 @@ int vafa_paged_decode(const vafa_paged_cache *c, const void *q, int64_t q_token,
   if (int rc = check_dtype(what, dtype)) return rc;
   DecodePlan p;
   if (int rc = plan_decode(c, H, window, &p)) return rc;
-  if (!std::isfinite(scale)) return fail(VAFA_ERR_VALUE, "%s: scale must be finite", what);
-  if (!(softcap >= 0.f) || !std::isfinite(softcap))
-    return fail(VAFA_ERR_VALUE, "%s: softcap must be positive and finite", what);
+  if (!std::isfinite(scale * kLog2e))
+    return fail(VAFA_ERR_VALUE, "%s: scale must be finite", what);
+  if (!softcap_ok(softcap))
+    return fail(VAFA_ERR_VALUE, "%s: softcap must be positive, from %g to %g", what,
+                (double)kMinSoftcap, (double)kMaxSoftcap);
   if (softcap > 0.f && !std::isfinite(2.f * kLog2e * scale / softcap))
     return fail(VAFA_ERR_VALUE, "%s: scale / softcap is not finite", what);
   if (int rc = check_rows(what, "q", q, q_token, q_head)) return rc;

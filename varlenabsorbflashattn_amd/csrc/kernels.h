@@ -111,6 +111,8 @@ struct AbsorbArgs {
 struct MaskedArgs {
   const void *q, *k, *v, *o_in, *dout;
   void *o, *dq, *dk, *dv;
+  uint8_t *o_lo;  // a byte per element of o (masked.h), or null
+  const uint8_t *o_lo_in;
   float *lse;
   const float *lse_in, *slopes;  // slopes: or null
   float *delta;                  // [T_q, H] workspace (backward)
@@ -224,7 +226,7 @@ template <typename T> void launch_paged_decode(const DecodeArgs &, int D, hipStr
 // masked_fwd.hip, masked_bwd.hip (bf16 / f16, D in {64, 128, 256})
 template <typename T, int D> void launch_masked_fwd(const MaskedArgs &, hipStream_t);
 // o and lse of split tiles from their partial rows
-template <typename T> void launch_masked_join(const MaskedArgs &, hipStream_t);
+template <typename T, int D> void launch_masked_join(const MaskedArgs &, hipStream_t);
 template <typename T, int D> void launch_masked_dq(const MaskedArgs &, hipStream_t);
 template <typename T, int D> void launch_masked_dkv(const MaskedArgs &, hipStream_t);
 // dq, dk and dv of divided tiles: ordered sums of their fp32 partial rows

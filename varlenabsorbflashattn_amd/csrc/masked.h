@@ -6,6 +6,8 @@
 // pre is the segment's end.  The score z = scale q.k passes through cap tanh(z / cap)
 // (kCap) and loses slope |p - j| (kBias); everything runs in the log2 domain.
 #pragma once
+#include <type_traits>
+
 #include "mfma.h"
 
 namespace vafa {
@@ -88,6 +90,36 @@ struct HeadSets {
     return (r >> lg) * H + (r & ((1 << lg) - 1));
   }
 };
+
+// delta = rowsum(O dO) takes O better than 16 bits: where few keys carry a row, dP - delta
+// is small beside either, and O's rounding shows in the gradients (distance biases of 4
+// to 7 a step: dQ and dK 1.7e-2 of their norm off in bf16, 2.2e-3 so; uniform scores 2.45e-3
+// and 2.35e-3).  It costs 2 to 3% of a training step.  A byte per element holds the distance of the fp32 value's bits from those of the rounded one, in units of
+// 2^kLoShift: 8 more bits of the significand, at any scale.
+template <typename T>
+constexpr int kLoShift = std::is_same_v<T, bf16> ? 8 : 5;
+
+template <typename T>
+__device__ __forceinline__ uint32_t lo_byte(float x) {
+  constexpr int S = kLoShift<T>;
+  int d = __float_as_int(x) - __float_as_int(to_f(static_cast<T>(x)));
+  d = (d + (1 << (S - 1))) >> S;  // (beyond a byte: half a step up, fp16's subnormals)
+  return (uint32_t)(d < -128 ? -128 : (d > 127 ? 127 : d)) & 255u;
+}
+template <typename T>
+__device__ __forceinline__ float with_lo(T h, uint32_t word, int byte) {
+  const int d = (int)(word << (24 - 8 * byte)) >> 24;
+  return __int_as_float(__float_as_int(to_f(h)) + (d << kLoShift<T>));
+}
+
+// Where the 8 bytes of features [16 c + 8 half, + 8) of row r lie: the rows that a wave
+// takes, `rows` of the tokens from t0 on and one set, are one block, ordered by c, row
+// and half, so that the forward writes and dQ reads whole lines.
+template <int D>
+__device__ __forceinline__ int64_t lo_at(const HeadSets &hs, int64_t t0, int set, int rows, int r,
+                                         int c, int half) {
+  return (t0 * hs.H + (int64_t)set * rows) * D + ((int64_t)c * rows + r) * 16 + half * 8;
+}
 
 }  // namespace
 

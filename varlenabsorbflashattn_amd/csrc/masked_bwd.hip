@@ -25,8 +25,8 @@ namespace {
 template <typename T, int D, int NW, bool kCap, bool kBias>
 __global__ __launch_bounds__(64 * NW, D >= 256 ? 1 : 2) void masked_dq_kernel(
     const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v,
-    const T *__restrict__ dout, const T *__restrict__ o, const float *__restrict__ lse,
-    float *__restrict__ delta, float *__restrict__ lse_out, T *__restrict__ dq,
+    const T *__restrict__ dout, const T *__restrict__ o, const uint8_t *__restrict__ o_lo,
+    const float *__restrict__ lse, float *__restrict__ delta, float *__restrict__ lse_out, T *__restrict__ dq,
     float *__restrict__ part_dq, const int32_t *__restrict__ items,
     const float *__restrict__ slopes, ScoreArgs sa, HeadSets hs, int window, float scale) {
   using M = Mfma<T>;
@@ -85,9 +85,17 @@ __global__ __launch_bounds__(64 * NW, D >= 256 ? 1 : 2) void masked_dq_kernel(
     const rsrc_t rd = make_rsrc(dout + base, nb);
     const rsrc_t ro = make_rsrc(o + base, nb);
     const int off = hs.row(wave * 32 + lrow) * D * 2 + lhalf * 16;
+    const int rows = uniform_clamp(q1 - t0, tw) << lg;
     u32x4 ov[NC];
+    u32x2 lo[NC];
 #pragma unroll
-    for (int cc = 0; cc < NC; ++cc) ov[cc] = buf_load16(ro, off + cc * 32);
+    for (int cc = 0; cc < NC; ++cc) {
+      ov[cc] = buf_load16(ro, off + cc * 32);
+      lo[cc] = u32x2{0u, 0u};
+      if (row_ok)
+        lo[cc] = *reinterpret_cast<const u32x2 *>(
+            o_lo + lo_at<D>(hs, t0, set, rows, lrow, cc, lhalf));
+    }
 #pragma unroll
     for (int cc = 0; cc < NC; ++cc) {
       u32x4 a = buf_load16(rq, off + cc * 32), b = buf_load16(rd, off + cc * 32);
@@ -104,7 +112,7 @@ __global__ __launch_bounds__(64 * NW, D >= 256 ? 1 : 2) void masked_dq_kernel(
       const T *x = reinterpret_cast<const T *>(&ov[cc]);
       float a = 0.f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) a = __builtin_fmaf(to_f(x[e]), to_f(dof[cc][e]), a);
+      for (int e = 0; e < 8; ++e) a = __builtin_fmaf(with_lo(x[e], lo[cc][e >> 2], e & 3), to_f(dof[cc][e]), a);
       sc += a;
     }
     Dr = sc + __shfl_xor(sc, 32, 64);
@@ -674,9 +682,9 @@ void launch_dq_v(const MaskedArgs &a, hipStream_t st) {
   allow_dynamic_lds(reinterpret_cast<const void *>(fn), smem);
   hipLaunchKernelGGL(fn, dim3((unsigned)(a.n_items * (a.H >> a.lg))), dim3(64 * NW), smem, st,
                      (const T *)a.q, (const T *)a.k, (const T *)a.v, (const T *)a.dout,
-                     (const T *)a.o_in, a.lse_in, a.delta, a.lse, (T *)a.dq, a.part_o, a.items,
-                     a.slopes, ScoreArgs{a.c, a.cap2}, HeadSets{a.H, a.Hk, a.lg}, a.window,
-                     a.scale);
+                     (const T *)a.o_in, a.o_lo_in, a.lse_in, a.delta, a.lse, (T *)a.dq, a.part_o,
+                     a.items, a.slopes, ScoreArgs{a.c, a.cap2}, HeadSets{a.H, a.Hk, a.lg},
+                     a.window, a.scale);
 }
 template <typename T, int D, int NW, bool kCap, bool kBias>
 void launch_dkv_v(const MaskedArgs &a, hipStream_t st) {

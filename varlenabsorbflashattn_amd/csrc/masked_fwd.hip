@@ -141,8 +141,8 @@ __device__ __forceinline__ void masked_tile(const T *ks, const T *vs,
 template <typename T, int D, int NW, bool kCap, bool kBias>
 __global__ __launch_bounds__(64 * NW, D >= 256 ? 1 : 2) void masked_fwd_kernel(
     const T *__restrict__ q, const T *__restrict__ k, const T *__restrict__ v,
-    T *__restrict__ o, float *__restrict__ lse, float *__restrict__ part_o,
-    float *__restrict__ part_lse, const int32_t *__restrict__ items,
+    T *__restrict__ o, uint8_t *__restrict__ o_lo, float *__restrict__ lse,
+    float *__restrict__ part_o, float *__restrict__ part_lse, const int32_t *__restrict__ items,
     const float *__restrict__ slopes, ScoreArgs sa, HeadSets hs, int window) {
   using M = Mfma<T>;
   constexpr int NC = D / 16, ND = D / 32;
@@ -240,6 +240,24 @@ __global__ __launch_bounds__(64 * NW, D >= 256 ? 1 : 2) void masked_fwd_kernel(
   const int rows = uniform_clamp(q1 - t0, tw) << lg;
   auto off = [&](int r) { return (int64_t)hs.row(r) * D; };
   if (pbase < 0) {
+    if (o_lo != nullptr && row_ok) {
+      uint8_t *at = o_lo + lo_at<D>(hs, t0, set, rows, lrow, 0, lhalf);
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        // this lane's features 16 c + 4 lhalf + {0..3, 8..11}; with the words of the row's
+        // other lane they are 16 c + 8 lhalf + {0..7}
+        uint32_t w0 = 0u, w1 = 0u;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          w0 |= lo_byte<T>(acc[c >> 1][(c & 1) * 8 + e] * inv) << e * 8;
+          w1 |= lo_byte<T>(acc[c >> 1][(c & 1) * 8 + 4 + e] * inv) << e * 8;
+        }
+        asm volatile("s_nop 1\n\tv_permlane32_swap_b32 %0, %1\n\ts_nop 1" : "+v"(w0), "+v"(w1));
+        *reinterpret_cast<u32x2 *>(at) = u32x2{w0, w1};
+        at += rows * 16;
+        asm volatile("" : "+v"(at));  // one address at a time: D = 256 has no registers for 16
+      }
+    }
     RS::rows16_at(acc, [&](float x) { return static_cast<T>(x * inv); }, stage,
                   o + ((int64_t)t0 * H + h0) * D, off, rows);
     if (row_ok && lhalf == 0) lse[(int64_t)tok * H + h] = lse_v;
@@ -255,13 +273,12 @@ __global__ __launch_bounds__(64 * NW, D >= 256 ? 1 : 2) void masked_fwd_kernel(
 // sum w_s O_s / sum w_s.  An item is {q0, q1, pbase, parts}; its rows lie one after
 // another in the output and in each part: a thread takes 8 neighbouring features, which
 // moved 4.4 TB/s where one wave per row and 4 bytes a lane moved 2.5.
-template <typename T>
-__global__ __launch_bounds__(256) void masked_join_kernel(const float *__restrict__ part_o,
-                                                          const float *__restrict__ part_lse,
-                                                          T *__restrict__ o,
-                                                          float *__restrict__ lse,
-                                                          const int32_t *__restrict__ items, int H,
-                                                          int D, int chunks) {
+template <typename T, int D>
+__global__ __launch_bounds__(256) void masked_join_kernel(
+    const float *__restrict__ part_o, const float *__restrict__ part_lse, T *__restrict__ o,
+    uint8_t *__restrict__ o_lo, float *__restrict__ lse, const int32_t *__restrict__ items,
+    HeadSets hs, int chunks) {
+  const int H = hs.H;
   const PlanItem it = load_item(items, blockIdx.x / chunks);
   const int ns = it.v[3];
   const int64_t rows = (int64_t)(it.v[1] - it.v[0]) * H;  // (token, head) rows of a part
@@ -289,10 +306,21 @@ __global__ __launch_bounds__(256) void masked_join_kernel(const float *__restric
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
   typename Mfma<T>::v8 r;
+  u32x2 lo{0u, 0u};
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     r[e] = static_cast<T>(a[e] * inv);
     r[4 + e] = static_cast<T>(b[e] * inv);
+    lo[0] |= lo_byte<T>(a[e] * inv) << e * 8;
+    lo[1] |= lo_byte<T>(b[e] * inv) << e * 8;
+  }
+  if (o_lo != nullptr) {
+    const int lg = hs.lg, tw = 32 >> lg, f = (int)(i % D);
+    const int tok = (int)(row / H), h = (int)(row % H);
+    const int w0 = tok / tw * tw, left = it.v[1] - it.v[0] - w0;  // the wave's first token
+    *reinterpret_cast<u32x2 *>(
+        o_lo + lo_at<D>(hs, it.v[0] + w0, h >> lg, (left < tw ? left : tw) << lg,
+                        ((tok - w0) << lg) + (h & ((1 << lg) - 1)), f / 16, f / 8 & 1)) = lo;
   }
   *reinterpret_cast<typename Mfma<T>::v8 *>(o + (int64_t)it.v[0] * H * D + i) = r;
   if (i % D == 0) lse[(int64_t)it.v[0] * H + row] = l == 0.f ? kNegInf : ms + fast_log2(l);
@@ -311,8 +339,8 @@ void launch_v(const MaskedArgs &a, hipStream_t st) {
   const int smem = masked_fwd_lds<T, D, NW>();
   allow_dynamic_lds(reinterpret_cast<const void *>(fn), smem);
   hipLaunchKernelGGL(fn, dim3((unsigned)(a.n_items * (a.H >> a.lg))), dim3(64 * NW), smem, st,
-                     (const T *)a.q, (const T *)a.k, (const T *)a.v, (T *)a.o, a.lse, a.part_o,
-                     a.part_lse, a.items, a.slopes, ScoreArgs{a.c, a.cap2},
+                     (const T *)a.q, (const T *)a.k, (const T *)a.v, (T *)a.o, a.o_lo, a.lse,
+                     a.part_o, a.part_lse, a.items, a.slopes, ScoreArgs{a.c, a.cap2},
                      HeadSets{a.H, a.Hk, a.lg}, a.window);
 }
 
@@ -336,22 +364,24 @@ void launch_masked_fwd(const MaskedArgs &a, hipStream_t st) {
   launch_nw<T, D, 4>(a, st);
 }
 
-template <typename T>
+template <typename T, int D>
 void launch_masked_join(const MaskedArgs &a, hipStream_t st) {
   if (a.n_comb == 0) return;
-  const int64_t chunks = ((int64_t)a.comb_rows * a.H * a.D + 2047) / 2048;
-  hipLaunchKernelGGL((masked_join_kernel<T>), dim3((unsigned)(a.n_comb * chunks)), dim3(256), 0,
-                     st, a.part_o, a.part_lse, (T *)a.o, a.lse, a.comb_items, a.H, a.D,
-                     (int)chunks);
+  const int64_t chunks = ((int64_t)a.comb_rows * a.H * D + 2047) / 2048;
+  hipLaunchKernelGGL((masked_join_kernel<T, D>), dim3((unsigned)(a.n_comb * chunks)), dim3(256),
+                     0, st, a.part_o, a.part_lse, (T *)a.o, a.o_lo, a.lse, a.comb_items,
+                     HeadSets{a.H, a.Hk, a.lg}, (int)chunks);
 }
 
-#define VAFA_INST(T)                                                     \
-  template void launch_masked_fwd<T, 64>(const MaskedArgs &, hipStream_t);  \
-  template void launch_masked_fwd<T, 128>(const MaskedArgs &, hipStream_t); \
-  template void launch_masked_fwd<T, 256>(const MaskedArgs &, hipStream_t); \
-  template void launch_masked_join<T>(const MaskedArgs &, hipStream_t);
-VAFA_INST(bf16)
-VAFA_INST(f16)
+#define VAFA_INST(T, D)                                                   \
+  template void launch_masked_fwd<T, D>(const MaskedArgs &, hipStream_t); \
+  template void launch_masked_join<T, D>(const MaskedArgs &, hipStream_t);
+VAFA_INST(bf16, 64)
+VAFA_INST(bf16, 128)
+VAFA_INST(bf16, 256)
+VAFA_INST(f16, 64)
+VAFA_INST(f16, 128)
+VAFA_INST(f16, 256)
 #undef VAFA_INST
 
 }  // namespace vafa

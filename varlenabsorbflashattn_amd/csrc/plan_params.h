@@ -63,6 +63,16 @@ constexpr int64_t kMaskedMaxTokens = int64_t{1} << 30;
 // Query heads: 256 rows of them lie within 2^31 bytes at D = 256.
 constexpr int64_t kMaskedMaxHeads = 4096;
 constexpr int64_t kMaskedMaxParts = 256;
+// Caps of scores: tanh comes as 1 - 2 e with e exact to a few 2^-24 of 1 (csrc/masked.h), so
+// that a capped score is exact to softcap times that, 1e-3 at the largest cap.
+constexpr float kMinSoftcap = 1e-6f, kMaxSoftcap = 1e4f;
+inline bool softcap_ok(float cap) {
+  return cap == 0.f || (cap >= kMinSoftcap && cap <= kMaxSoftcap);
+}
+// A launch's threads are counted in 32 bits.
+inline bool grid_ok(int64_t blocks, int64_t threads) {
+  return blocks <= (int64_t)UINT32_MAX / threads;
+}
 // The planner's model of a pass's time, in units of one key (query tiles) or one block of
 // 32 rows (key tiles): the smallest chunk and its alignment, what an item costs beside
 // its work, the launch that sums partial rows (times D), and a partial row of one token

@@ -395,7 +395,9 @@ Tensor paged_decode(const Tensor &q_in, const Tensor &kc, const Tensor &vc, cons
                     std::optional<int64_t> window, const std::optional<Tensor> &slopes) {
   const char *what = "paged_decode_attn";
   no_grad_only(what, {q_in, kc, vc, slopes.value_or(Tensor())});
-  if (softcap && !(*softcap > 0)) throw py::value_error("softcap must be positive");
+  // (1e-50 would be 0 in 32 bits, which means none)
+  if (softcap && !(*softcap > 0 && (float)*softcap > 0.f))
+    throw py::value_error("softcap must be positive");
   if (window && *window < 1) throw py::value_error("window must be positive");
   const vafa_paged_cache c = cache_of(what, kc, vc, table, lens);
   check_tokens(what, "q", q_in, kc);
@@ -462,26 +464,30 @@ std::tuple<Tensor, Tensor, Tensor> masked_operands(const Tensor &q_in, const Ten
   return {q, k, v};
 }
 
-std::tuple<Tensor, Tensor> masked_fwd(const Tensor &q, const Tensor &k, const Tensor &v,
-                                      const Plan &p, double scale, double softcap, int64_t window,
-                                      const std::optional<Tensor> &slopes) {
+// o, its low bytes (train) and LSE.
+std::tuple<Tensor, Tensor, Tensor> masked_fwd(const Tensor &q, const Tensor &k, const Tensor &v,
+                                              const Plan &p, double scale, double softcap,
+                                              int64_t window,
+                                              const std::optional<Tensor> &slopes, bool train) {
   Call c(q);
   // evicted from the cache while a kernel of this stream still reads it, the plan keeps
   // its memory until the stream's work is done
   p.items.record_stream(c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(q.device().index()).unwrap());
   const int64_t H = q.size(1), D = q.size(2);
   const float *sl = slopes_of("packed_masked_attn", slopes, H, q);
-  Tensor o = c.like(q), lse = c.empty_f32({q.size(0), H});
+  Tensor o = c.like(q), lse = c.empty_f32({q.size(0), H}), lo;
+  if (train) lo = at::empty(q.sizes(), q.options().dtype(at::kByte));
   void *ws = c.workspace(api.masked_fwd_workspace(&p.info, k.size(1), D));
-  check(api.masked_fwd(ptr(q), ptr(k), ptr(v), ptr(o), f32w(lse), p.dev(), &p.info, k.size(1), D,
-                       dtype_of(q), (float)scale, (float)softcap, window, sl, ws, c.ws_bytes(),
-                       c.stream));
+  check(api.masked_fwd(ptr(q), ptr(k), ptr(v), ptr(o), ptr(lo), f32w(lse), p.dev(), &p.info,
+                       k.size(1), D, dtype_of(q), (float)scale, (float)softcap, window, sl, ws,
+                       c.ws_bytes(), c.stream));
   clear_rest(o, p.info.T_q);
-  return {o, lse};
+  return {o, lo, lse};
 }
 
 std::tuple<Tensor, Tensor, Tensor> masked_bwd(const Tensor &q, const Tensor &k, const Tensor &v,
-                                              const Tensor &o, const Tensor &lse, const Tensor &g,
+                                              const Tensor &o, const Tensor &lo,
+                                              const Tensor &lse, const Tensor &g,
                                               const Plan &p, double scale, double softcap,
                                               int64_t window,
                                               const std::optional<Tensor> &slopes) {
@@ -491,9 +497,9 @@ std::tuple<Tensor, Tensor, Tensor> masked_bwd(const Tensor &q, const Tensor &k, 
   const Tensor dout = grad_in(g, q);
   Tensor dq = c.like(q), dk = c.like(k), dv = c.like(v);
   void *ws = c.workspace(api.masked_bwd_workspace(&p.info, Hk, D));
-  check(api.masked_bwd(ptr(q), ptr(k), ptr(v), ptr(o), ptr(dout), f32(lse), ptr(dq), ptr(dk),
-                       ptr(dv), p.dev(), &p.info, Hk, D, dtype_of(q), (float)scale, (float)softcap,
-                       window, sl, ws, c.ws_bytes(), c.stream));
+  check(api.masked_bwd(ptr(q), ptr(k), ptr(v), ptr(o), ptr(lo), ptr(dout), f32(lse), ptr(dq),
+                       ptr(dk), ptr(dv), p.dev(), &p.info, Hk, D, dtype_of(q), (float)scale,
+                       (float)softcap, window, sl, ws, c.ws_bytes(), c.stream));
   clear_rest(dq, p.info.T_q);
   clear_rest(dk, p.info.T_k);
   clear_rest(dv, p.info.T_k);
@@ -511,8 +517,8 @@ struct MaskedAttn : torch::autograd::Function<MaskedAttn> {
   static Tensor forward(torch::autograd::AutogradContext *ctx, const Tensor &q, const Tensor &k,
                         const Tensor &v, const Plan &p, double scale, double softcap,
                         int64_t window, const std::optional<Tensor> &slopes) {
-    auto [o, lse] = masked_fwd(q, k, v, p, scale, softcap, window, slopes);
-    ctx->save_for_backward({q, k, v, o, lse, slopes.value_or(Tensor())});
+    auto [o, lo, lse] = masked_fwd(q, k, v, p, scale, softcap, window, slopes, true);
+    ctx->save_for_backward({q, k, v, o, lo, lse, slopes.value_or(Tensor())});
     ctx->saved_data["plan"] = c10::IValue::make_capsule(c10::make_intrusive<PlanHolder>(p));
     ctx->saved_data["scale"] = scale;
     ctx->saved_data["softcap"] = softcap;
@@ -524,9 +530,9 @@ struct MaskedAttn : torch::autograd::Function<MaskedAttn> {
     const auto saved = ctx->get_saved_variables();
     const auto holder = ctx->saved_data["plan"].toCapsule();
     const Plan &p = static_cast<PlanHolder *>(holder.get())->plan;
-    const Tensor &sl = saved[5];
-    auto [dq, dk, dv] = masked_bwd(saved[0], saved[1], saved[2], saved[3], saved[4], grads[0], p,
-                                   ctx->saved_data["scale"].toDouble(),
+    const Tensor &sl = saved[6];
+    auto [dq, dk, dv] = masked_bwd(saved[0], saved[1], saved[2], saved[3], saved[4], saved[5],
+                                   grads[0], p, ctx->saved_data["scale"].toDouble(),
                                    ctx->saved_data["softcap"].toDouble(),
                                    ctx->saved_data["window"].toInt(),
                                    sl.defined() ? std::optional<Tensor>(sl) : std::nullopt);
@@ -539,7 +545,7 @@ Tensor masked_attn(const Tensor &q, const Tensor &k, const Tensor &v, const Plan
   if (at::GradMode::is_enabled() &&
       (q.requires_grad() || k.requires_grad() || v.requires_grad()))
     return MaskedAttn::apply(q, k, v, p, scale, softcap, window, slopes);
-  return std::get<0>(masked_fwd(q, k, v, p, scale, softcap, window, slopes));
+  return std::get<0>(masked_fwd(q, k, v, p, scale, softcap, window, slopes, false));
 }
 
 }  // namespace

@@ -79,17 +79,18 @@ def _check_options(D, cu_seqlens_q, cu_seqlens_k, q_seqinfo, k_seqinfo, causal, 
     assert cu_seqlens_k.numel() - 1 == n_seg, \
         f"segment count mismatch: q has {n_seg}, k has {cu_seqlens_k.numel() - 1}"
 
-    if window is not None and window < 1:
-        raise ValueError(f"window must be positive, got {window}")
-    if softcap is not None and not (softcap > 0 and math.isfinite(softcap)):
-        raise ValueError(f"softcap must be positive and finite, got {softcap}")
+    if window is not None and (window < 1 or window != int(window)):
+        raise ValueError(f"window must be positive and whole, got {window}")
+    if softcap is not None and not 1e-6 <= softcap <= 1e4:
+        raise ValueError(f"softcap must be positive, from 1e-6 to 1e4, got {softcap}")
     if not causal and (window is not None or prefix_lens is not None):
         raise ValueError("window and prefix_lens belong to the causal mask")
     if scale is None:
         scale = 1.0 / math.sqrt(D)
     if not math.isfinite(scale):
         raise ValueError(f"scale must be finite, got {scale}")
-    return (cu_seqlens_q, cu_seqlens_k, bool(causal), int(window or 0), float(softcap or 0.0),
+    return (cu_seqlens_q, cu_seqlens_k, bool(causal), min(int(window or 0), 1 << 31),
+            float(softcap or 0.0),
             float(scale))
 
 
@@ -118,9 +119,15 @@ def packed_masked_attn(
     key j where ``j <= p``, with ``window`` also ``j > p - window``, or where
     ``j < prefix_lens[segment]`` (``[n_seg]``); every key with ``causal=False``, which
     takes neither.  Scores are ``scale * q.k`` (default 1/sqrt(D)), then
-    ``softcap * tanh(. / softcap)``, then minus ``alibi_slopes[h]`` (float32 ``[H]``, no
-    gradient) times ``|p - j|``.  A row that sees no key gets zeros and no gradient.
-    The backward is deterministic.  Segments of at most 2^30 tokens together.
+    ``softcap * tanh(. / softcap)`` (1e-6 to 1e4), then minus ``alibi_slopes[h]`` (float32
+    ``[H]``, no gradient) times ``|p - j|``.  A row that sees no key gets zeros and no
+    gradient.  The backward is deterministic.  At most 2^30 tokens and 4096 heads.
+
+    Keys that no query sees are not used, whatever they hold.  One that some query sees
+    must be finite in ``k`` and ``v``: rows that do not see it weigh it with 0, and 0
+    times an infinity is NaN, as in ``softmax(.) @ v``; the same holds for rows of ``q``
+    and of the gradient in the backward.  Lengths on the GPU are read back, which waits for
+    the GPU and which no graph capture allows: pass them on the host there.
     """
     ops = _lib.ops()
     q3, k3, v3 = ops.masked_operands(q, k, v, alibi_slopes)

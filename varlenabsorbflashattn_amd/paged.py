@@ -42,7 +42,8 @@ def paged_kv_append(
     ``q`` ``[T, H, D]`` turn by position * inv_freq[i] on the way, or the pairs
     ``(2i, 2i + 1)`` if ``interleaved``; further features stay.  Returns ``q`` rotated, or
     None without it.  Tokens behind the last sequence are not stored and their rows of
-    the result are zeros.  Two tokens that share a place in the cache leave either there.
+    the result are zeros.  Of two tokens that share a place in the cache, each 16 bytes
+    there are of either.  D: multiples of 8 up to 1024.
     Forward only.
     """
     return _lib.ops().paged_append(k, v, k_cache, v_cache, page_table, cache_lens, cu_seqlens, q,
@@ -65,9 +66,9 @@ def paged_decode_attn(
     ``cache_lens[b]`` tokens of its pages (its own among them).
 
     ``H / H_k`` query heads share a key head; D is 64, 128 or 256.  Scores are
-    ``scale * q.k`` (default 1/sqrt(D)), then ``softcap * tanh(. / softcap)``, then minus
-    ``alibi_slopes[h]`` (float32 ``[H]``) times the key's distance; ``window`` keeps the
-    last that many keys.  :func:`packed_masked_attn` applies the same to whole sequences.
+    ``scale * q.k`` (default 1/sqrt(D)), then ``softcap * tanh(. / softcap)`` (1e-6 to 1e4), then
+    minus ``alibi_slopes[h]`` (float32 ``[H]``) times the key's distance; ``window`` keeps
+    the last that many keys.  :func:`packed_masked_attn` applies the same to whole sequences.
     A sequence without keys gets zeros.  Forward only.
     """
     if scale is None:
