@@ -445,3 +445,31 @@ def test_gradients_of_rows_that_few_keys_carry(device, ql, kl, H, Hk, D, dt):
         off = np.linalg.norm(f64(out) - val) / np.linalg.norm(val)
         print(f"  {name:3s} {off / U[dt]:.2f} u", flush=True)
         assert off < U[dt], (name, off)
+
+
+def test_many_tiny_segments(device):
+    """20000 segments of one token: each gets its own value, dQ and dK are zeros and dV the sum
+    over the heads that share it (small whole numbers: exact)."""
+    print("[masked tiny]", flush=True)
+    n, H, Hk, D = 20000, 6, 3, 64
+    g = torch.Generator(device=device).manual_seed(62)
+    q, k, v = (torch.randn(n, h, D, generator=g, device=device).to(BF).requires_grad_(True)
+               for h in (H, Hk, Hk))
+    do = torch.randint(-8, 9, (n, H, D), generator=g, device=device).to(BF)
+    cu = torch.arange(n + 1)
+    o = packed_masked_attn(q, k, v, cu_seqlens_q=cu, cu_seqlens_k=cu, window=3)
+    dq, dk, dv = torch.autograd.grad(o, (q, k, v), do)
+    assert torch.equal(o, v.repeat_interleave(H // Hk, dim=1))
+    assert torch.equal(dv, do.view(n, Hk, H // Hk, D).sum(2))
+    # dP - delta: two fp32 sums of the same 64 products, each off by at most 66 roundings
+    off = 2 * 66 * 2.0 ** -24 * (do.float() * o.float()).abs().sum(-1).max() * D ** -0.5 * 1.01
+    assert dq.abs().max() <= off * k.abs().max()
+    assert dk.abs().max() <= off * q.abs().max() * (H // Hk)
+
+
+@pytest.mark.parametrize("H,Hk,D", [(4096, 1, 64), (4096, 4096, 64), (96, 32, 256)])
+def test_most_heads(device, H, Hk, D):
+    print(f"[masked heads] {H}/{Hk} x {D}", flush=True)
+    ql, kl = [5, 2], [5, 40]
+    x = inputs(63, ql, kl, H, Hk, D, HF, device)
+    compare(step(*x, ql, kl), *x, ql, kl)

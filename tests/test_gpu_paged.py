@@ -454,3 +454,18 @@ def test_tokens_in_front_of_the_first_sequence(device):
     want = torch.zeros(16, dtype=torch.bool)
     want[4:6] = True
     assert torch.equal(kc[1, :, 0].any(-1).cpu(), want) and not kc[0].any()
+
+
+@pytest.mark.parametrize("H,Hk", [(1024, 1), (1024, 1024), (130, 2)])
+def test_decode_many_heads(device, H, Hk):
+    """Several blocks of 16 heads a key head; as many key heads as there can be."""
+    print(f"[decode heads] {H}/{Hk}", flush=True)
+    D, page, lens, dt = 64, 16, [700, 0, 33], torch.float16
+    g = torch.Generator(device=device).manual_seed(13)
+    kc, vc = (torch.randn(50, page, Hk, D, generator=g, device=device).to(dt) for _ in range(2))
+    q = torch.randn(3, H, D, generator=g, device=device).to(dt)
+    table = torch.arange(3 * 44, dtype=torch.int32).view(3, 44) % 50
+    out = paged_decode_attn(q, kc, vc, table.to(device),
+                            torch.tensor(lens, dtype=torch.int32, device=device), window=650)
+    ref = op.decode(f64(q), f64(kc), f64(vc), table.numpy(), lens, D ** -0.5, window=650)
+    close_decode(out, *ref)
