@@ -383,7 +383,7 @@ VAFA_API int vafa_absorb_project_f32_bwd(const float *q_raw, const float *W_Q, c
 /* ======================================================================== */
 
 /* q [T_q,H,D], k/v [T_k,Hk,D] contiguous and 16-byte aligned -> o [T_q,H,D],
- * lse [T_q,H] fp32 log2-domain, under a plan of vafa_plan_masked made with the same H,
+ * lse [T_q,H] fp32 log2-domain or NULL, under a plan of vafa_plan_masked made with the same H,
  * Hk, D and window.  Scores are scale q.k, then softcap tanh(. / softcap) (0: none),
  * then minus slopes[h] (device fp32 [H] or NULL) times |position of the query - key|.
  * Rows that see no key get zeros (lse -inf).  o_lo: T_q * H * D bytes for the backward,

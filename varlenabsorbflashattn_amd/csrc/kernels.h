@@ -113,7 +113,7 @@ struct MaskedArgs {
   void *o, *dq, *dk, *dv;
   uint8_t *o_lo;  // a byte per element of o (masked.h), or null
   const uint8_t *o_lo_in;
-  float *lse;
+  float *lse;                    // forward: or null
   const float *lse_in, *slopes;  // slopes: or null
   float *delta;                  // [T_q, H] workspace (backward)
   float *part_o, *part_lse;      // split partial rows: O (and LSE) or dQ

@@ -260,7 +260,7 @@ __global__ __launch_bounds__(64 * NW, D >= 256 ? 1 : 2) void masked_fwd_kernel(
     }
     RS::rows16_at(acc, [&](float x) { return static_cast<T>(x * inv); }, stage,
                   o + ((int64_t)t0 * H + h0) * D, off, rows);
-    if (row_ok && lhalf == 0) lse[(int64_t)tok * H + h] = lse_v;
+    if (lse != nullptr && row_ok && lhalf == 0) lse[(int64_t)tok * H + h] = lse_v;
   } else {
     // partial rows lie as the outputs do, token pbase + ... of [rows, H, D]
     const int64_t prow = pbase + wave * tw;
@@ -323,7 +323,8 @@ __global__ __launch_bounds__(256) void masked_join_kernel(
                         ((tok - w0) << lg) + (h & ((1 << lg) - 1)), f / 16, f / 8 & 1)) = lo;
   }
   *reinterpret_cast<typename Mfma<T>::v8 *>(o + (int64_t)it.v[0] * H * D + i) = r;
-  if (i % D == 0) lse[(int64_t)it.v[0] * H + row] = l == 0.f ? kNegInf : ms + fast_log2(l);
+  if (lse != nullptr && i % D == 0)
+    lse[(int64_t)it.v[0] * H + row] = l == 0.f ? kNegInf : ms + fast_log2(l);
 }
 
 // Dynamic LDS: the K/V buffers, or the per-wave row-store regions if those are larger.

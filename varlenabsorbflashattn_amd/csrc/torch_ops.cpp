@@ -464,7 +464,7 @@ std::tuple<Tensor, Tensor, Tensor> masked_operands(const Tensor &q_in, const Ten
   return {q, k, v};
 }
 
-// o, its low bytes (train) and LSE.
+// o, and for a backward its low bytes and LSE.
 std::tuple<Tensor, Tensor, Tensor> masked_fwd(const Tensor &q, const Tensor &k, const Tensor &v,
                                               const Plan &p, double scale, double softcap,
                                               int64_t window,
@@ -475,8 +475,11 @@ std::tuple<Tensor, Tensor, Tensor> masked_fwd(const Tensor &q, const Tensor &k, 
   p.items.record_stream(c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(q.device().index()).unwrap());
   const int64_t H = q.size(1), D = q.size(2);
   const float *sl = slopes_of("packed_masked_attn", slopes, H, q);
-  Tensor o = c.like(q), lse = c.empty_f32({q.size(0), H}), lo;
-  if (train) lo = at::empty(q.sizes(), q.options().dtype(at::kByte));
+  Tensor o = c.like(q), lo, lse;
+  if (train) {
+    lo = at::empty(q.sizes(), q.options().dtype(at::kByte));
+    lse = c.empty_f32({q.size(0), H});
+  }
   void *ws = c.workspace(api.masked_fwd_workspace(&p.info, k.size(1), D));
   check(api.masked_fwd(ptr(q), ptr(k), ptr(v), ptr(o), ptr(lo), f32w(lse), p.dev(), &p.info,
                        k.size(1), D, dtype_of(q), (float)scale, (float)softcap, window, sl, ws,
