@@ -232,6 +232,7 @@ __global__ __launch_bounds__(64 * NW, D >= 256 ? 1 : 2) void masked_dq_kernel(
   };
   using I0 = std::integral_constant<int, 0>;
   using I1 = std::integral_constant<int, 1>;
+  // (one body for both buffers at D = 256: 581 -> 626 us of forward and backward)
   if constexpr (D >= 128) {
     for (int j = 0; j < nblk; j += 2) {
       block(j, I0{});
@@ -393,8 +394,7 @@ __global__ __launch_bounds__(64 * NW, D >= 256 && NW < 8 ? 1 : 2) void masked_dk
   const int a_off = L::row(lrow) + lhalf * 8 + dpart * NDO * 32;
   const int t_off = L::row(4 * (lane >> 5) + ((lane & 15) >> 2)) + ((lane >> 4) & 1) * 16 +
                     4 * (lane & 3);
-  auto blk = [&](int j, auto bufc) {
-    constexpr int B = decltype(bufc)::value;
+  auto blk = [&](int j, int B) {
     const int qc = qb;  // the block's first token
     qb += tb;
     if (qb >= q1) {
@@ -593,10 +593,7 @@ __global__ __launch_bounds__(64 * NW, D >= 256 && NW < 8 ? 1 : 2) void masked_dk
       }
     }
   };
-  for (int j = 0; j < nblk; j += 2) {
-    blk(j, std::integral_constant<int, 0>{});
-    if (j + 1 < nblk) blk(j + 1, std::integral_constant<int, 1>{});
-  }
+  for (int j = 0; j < nblk; ++j) blk(j, j & 1);
   wait_vmcnt<0>();
 
   __syncthreads();
