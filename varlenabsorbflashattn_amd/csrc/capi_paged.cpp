@@ -75,8 +75,8 @@ struct DecodePlan {
   bool direct = false;
 };
 
-// Workgroups resident on the GPU, by registers: 3, 2 or 1 on each of 256 CUs.
-int64_t decode_wgs(int64_t D) { return D == 64 ? 768 : D == 128 ? 512 : 256; }
+// Workgroups resident on the GPU, by registers: 3 (D = 64) or 2 on each of 256 CUs.
+int64_t decode_wgs(int64_t D) { return D == 64 ? 768 : 512; }
 // Sequences of at most this many tiles are not divided: a workgroup each, and no launch
 // that joins (4 sequences of up to 500 keys: 9.5 -> 6.1 us; 8 of 1000, 8 tiles, the other way round
 // 14 -> 26).

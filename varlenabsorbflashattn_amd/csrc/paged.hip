@@ -227,10 +227,10 @@ __global__ __launch_bounds__(256) void paged_append_pairs_kernel(AppendArgs a) {
 //     each 32); C row (l / 16) * 4 + r;
 //   O^T += V^T P^T over 32 keys: the lane's 8 probabilities are the B operand as they
 //     are when slot (l / 16) * 8 + t is key 16 (t / 4) + (l / 16) * 4 + t % 4; V^T in
-//     that order comes from transposing reads.
-// A wave takes 32 of a tile's 128 keys through registers (the next tile's are on their
-// way meanwhile) and its own LDS rows, and shares nothing with the other waves before the
-// piece's end: no barrier in the loop.  Memory-bound, the products are far from their
+//     that order comes from transposing reads (over 16 keys: 4 of each, 16x16x16).
+// A wave takes 32 of a tile's 128 keys, in one step or two, through registers (the next
+// step's are on their way meanwhile) and its own LDS rows, and shares nothing with the
+// other waves before the piece's end: no barrier in the loop.  Memory-bound, the products are far from their
 // rate even with one head.  What a byte costs: rows are loaded whole (16 lanes a row at
 // D = 128) and without keeping them in the caches.  32 heads of 128 on 8 key heads, 64
 // sequences of 1k to 32k keys in pages of 16 (2.37 GB), us: K straight into A operands
@@ -238,15 +238,23 @@ __global__ __launch_bounds__(256) void paged_append_pairs_kernel(AppendArgs a) {
 // keeping them 391, 6.1 TB/s (without keeping them but by 64 bytes 525: the other half
 // of a 128-byte line is read again).  Three waves per SIMD by smaller registers 533.
 template <typename T>
-struct Mfma16;
+struct Mfma16;  // mma: 32 keys or features, mma4: 16 keys
 template <>
 struct Mfma16<bf16> {
+  typedef __attribute__((__vector_size__(4 * sizeof(short)))) short s16x4;
+  static __device__ __forceinline__ f32x4 mma4(u32x2 a, bf16x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s16x4, a),
+                                                     __builtin_bit_cast(s16x4, b), c, 0, 0, 0);
+  }
   static __device__ __forceinline__ f32x4 mma(bf16x8 a, bf16x8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
   }
 };
 template <>
 struct Mfma16<f16> {
+  static __device__ __forceinline__ f32x4 mma4(u32x2 a, f16x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(f16x4, a), b, c, 0, 0, 0);
+  }
   static __device__ __forceinline__ f32x4 mma(f16x8 a, f16x8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
   }
@@ -256,7 +264,13 @@ template <int D>
 struct DecodeSmem {
   static constexpr int kVS = D + 8;   // K and V row stride (elements)
   static constexpr int kOS = D + 4;   // row stride of the waves' outputs (floats)
-  static constexpr int kV = 4 * 64 * kVS * 2;
+  // 16-key groups of a wave's step: by 16 at D = 256, where 32 leave one workgroup on a CU
+  // and nothing in flight while it stores its rows (32 sequences of 500 to 8192 keys, 8
+  // key heads, 138 -> 115 us); by 32 below (by 16, and more workgroups for it: D = 128 391
+  // -> 406 us, D = 64 170 -> 182)
+  static constexpr int kGroups = D >= 256 ? 1 : 2;
+  static constexpr int kRows = 16 * kGroups;
+  static constexpr int kV = 4 * 2 * kRows * kVS * 2;
   static constexpr int kO = 4 * kDecodeRows * kOS * 4;
   static constexpr int kML = kV > kO ? kV : kO;  // then m, l of each wave and row
   static constexpr int kBytes = kML + 2 * 4 * kDecodeRows * 4;
@@ -305,17 +319,19 @@ __device__ __forceinline__ void find_seq(const DecodeArgs &a, int at, int lane, 
 }
 
 template <typename T, int D>
-__global__ __launch_bounds__(256, D >= 256 ? 1 : (D == 128 ? 2 : 3)) void paged_decode_kernel(DecodeArgs a) {
+__global__ __launch_bounds__(256, D >= 128 ? 2 : 3) void paged_decode_kernel(DecodeArgs a) {
   using M = Mfma16<T>;
   using S = DecodeSmem<D>;
   using v8 = typename Mfma<T>::v8;
   constexpr int NC = D / 32, ND = D / 16;
   constexpr int kLanes = D / 8, kRows = 64 / kLanes;  // of a row, and rows of an instruction
+  constexpr int KG = S::kGroups, NI = S::kRows / kRows;  // instructions of a step's K rows
+  constexpr int kSteps = 2 / KG;                         // of a tile
   extern __shared__ __align__(16) unsigned char smem[];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l16 = lane & 15, lg = lane >> 4;
-  T *ks = reinterpret_cast<T *>(smem) + wave * 64 * S::kVS, *vs = ks + 32 * S::kVS;
+  T *ks = reinterpret_cast<T *>(smem) + wave * 2 * S::kRows * S::kVS, *vs = ks + S::kRows * S::kVS;
 
   // the pairs of a chunk on one XCD: they read whole token rows of the pages together
   const int group = blockIdx.x / (kXcds * a.pairs), within = blockIdx.x % (kXcds * a.pairs);
@@ -370,29 +386,33 @@ __global__ __launch_bounds__(256, D >= 256 ? 1 : (D == 128 ? 2 : 3)) void paged_
     float slope2 = 0.f;
     if (a.slopes != nullptr) slope2 = a.slopes[h0 + (l16 < rows ? l16 : 0)] * kLog2e;
 
-    // this lane's two keys of the wave's 32 in tile t: page and token in it
+    // this lane's key of each group of step u (of the wave's 32 keys in tile u / kSteps):
+    // page and token in it
     struct Keys {
-      int id[2], slot[2];
+      int id[KG], slot[KG];
     };
-    auto keys_of = [&](int t) {
+    auto keys_at = [&](int u) {  // the step's first key
+      return lo + u / kSteps * kDecodeTile + wave * 32 + u % kSteps * S::kRows;
+    };
+    auto keys_of = [&](int u) {
       Keys k;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int key = lo + t * kDecodeTile + wave * 32 + 16 * i + l16;
+      for (int i = 0; i < KG; ++i) {
+        const int t = u / kSteps, key = keys_at(u) + 16 * i + l16;
         const PageSlot s = page_slot(a.map, key);
         k.id[i] = t < t0 + run && key < len ? page_of(a.map, b, key, s) : -1;
         k.slot[i] = s.slot;
       }
       return k;
     };
-    // the wave's 32 rows of K and V by whole rows: instruction i takes the rows i * kRows +
+    // the step's rows of K and V by whole rows: instruction i takes the rows i * kRows +
     // lane / kLanes, whose places the lanes that looked them up hand over
-    u32x4 kr[2 * NC], vr[2 * NC];
+    u32x4 kr[NI], vr[NI];
     auto load = [&](const Keys &k) {
 #pragma unroll
-      for (int i = 0; i < 2 * NC; ++i) {
+      for (int i = 0; i < NI; ++i) {
         const int row = i * kRows + lane / kLanes;
-        // (the rows of one instruction lie in one half of the 32)
+        // (the rows of one instruction lie in one group)
         const int id = __shfl(k.id[i * kRows / 16], row & 15, 64);
         const int slot = __shfl(k.slot[i * kRows / 16], row & 15, 64);
         const int64_t ko = id >= 0 ? id * a.k_page + slot * a.kc_token : 0;
@@ -406,34 +426,37 @@ __global__ __launch_bounds__(256, D >= 256 ? 1 : (D == 128 ? 2 : 3)) void paged_
 #pragma unroll
     for (int i = 0; i < ND; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
     float m_run = -kHuge, l_run = 0.f;
-    Keys now = keys_of(t0);
+    const int u0 = t0 * kSteps, u1 = (t0 + run) * kSteps;
+    Keys now = keys_of(u0);
     load(now);
-    Keys next = keys_of(t0 + 1);
-    for (int t = t0; t < t0 + run; ++t) {
-      // which of the 32 keys there are (bit: key)
-      const uint32_t ok = (uint32_t)(__builtin_amdgcn_ballot_w64(now.id[0] >= 0) & 0xffffu) |
-                          (uint32_t)(__builtin_amdgcn_ballot_w64(now.id[1] >= 0) & 0xffffu) << 16;
-      if (ok != 0xffffffffu) {
+    Keys next = keys_of(u0 + 1);
+    for (int u = u0; u < u1; ++u) {
+      // which of the step's keys there are (bit: key)
+      uint32_t ok = 0;
+#pragma unroll
+      for (int i = 0; i < KG; ++i)
+        ok |= (uint32_t)(__builtin_amdgcn_ballot_w64(now.id[i] >= 0) & 0xffffu) << 16 * i;
+      if (ok != 0xffffffffu >> (32 - S::kRows)) {
         // values of absent keys are whatever the cache holds: zeros instead, so that
         // their zero probabilities do not meet infinities
 #pragma unroll
-        for (int i = 0; i < 2 * NC; ++i)
+        for (int i = 0; i < NI; ++i)
           if (!(ok >> (i * kRows + lane / kLanes) & 1)) vr[i] = u32x4{0, 0, 0, 0};
       }
 #pragma unroll
-      for (int i = 0; i < 2 * NC; ++i) {
+      for (int i = 0; i < NI; ++i) {
         const int at = (i * kRows + lane / kLanes) * S::kVS + lane % kLanes * 8;
         *reinterpret_cast<u32x4 *>(ks + at) = kr[i];
         *reinterpret_cast<u32x4 *>(vs + at) = vr[i];
       }
       now = next;
-      if (t + 1 < t0 + run) {
+      if (u + 1 < u1) {
         load(now);
-        next = keys_of(t + 2);
+        next = keys_of(u + 2);
       }
-      f32x4 s[2];
+      f32x4 s[KG];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
+      for (int i = 0; i < KG; ++i) {
         s[i] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int c = 0; c < NC; ++c)
@@ -442,26 +465,28 @@ __global__ __launch_bounds__(256, D >= 256 ? 1 : (D == 128 ? 2 : 3)) void paged_
                         qf[c], s[i]);
       }
       // scores in the log2 domain; C row (key) 16 i + lg * 4 + r
-      float y[8], mx = kNegInf;
+      float y[4 * KG], mx = kNegInf;
+      const int back = len - 1 - keys_at(u);
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+      for (int i = 0; i < KG; ++i)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const int row = 16 * i + lg * 4 + r;
           float z = s[i][r] * a.c;
           if (a.cap2 > 0.f) z = a.cap2 * (1.f - 2.f * __builtin_amdgcn_rcpf(1.f + fast_exp2(z)));
           if (a.slopes != nullptr)
-            z -= slope2 * (float)(len - 1 - (lo + t * kDecodeTile + wave * 32 + row));
+            z -= slope2 * (float)(back - row);
           y[4 * i + r] = ok >> row & 1 ? z : kNegInf;
           mx = fmaxf(mx, y[4 * i + r]);
         }
       mx = max_xor32(max_xor16(mx));
       const float m_new = fmaxf(m_run, mx), alpha = fast_exp2(m_run - m_new);
       m_run = m_new;
-      v8 p;
+      typedef __attribute__((__vector_size__(4 * KG * sizeof(T)))) T VP;
+      VP p;
       float ps = 0.f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
+      for (int e = 0; e < 4 * KG; ++e) {
         const float x = fast_exp2(y[e] - m_run);
         // the sum takes the probabilities as rounded for the product
         p[e] = static_cast<T>(x);
@@ -473,7 +498,10 @@ __global__ __launch_bounds__(256, D >= 256 ? 1 : (D == 128 ? 2 : 3)) void paged_
 #pragma unroll
         for (int r = 0; r < 4; ++r) acc[i][r] *= alpha;
         const T *tr = vs + (lg * 4 + (l16 >> 2)) * S::kVS + 16 * i + 4 * (l16 & 3);
-        acc[i] = M::mma(as_v8<T>(join(lds_tr16(tr), lds_tr16(tr + 16 * S::kVS))), p, acc[i]);
+        if constexpr (KG == 2)
+          acc[i] = M::mma(as_v8<T>(join(lds_tr16(tr), lds_tr16(tr + 16 * S::kVS))), p, acc[i]);
+        else
+          acc[i] = M::mma4(lds_tr16(tr), p, acc[i]);
       }
     }
     l_run += __shfl_xor(l_run, 16, 64);
