@@ -325,7 +325,10 @@ def plan_masked(cu_q: np.ndarray, cu_k: np.ndarray, H: int, Hk: int, D: int, cau
     pre = None if prefix is None else np.ascontiguousarray(prefix, dtype=np.int64)
     if pre is not None and pre.shape != (a.size - 1,):
         raise AssertionError(f"prefix_lens must be [{a.size - 1}], got {pre.shape}")
-    guess = 64 + 12 * a.size + int(max(a[-1], 0) + max(b[-1], 0)) // 32 if a.size else 64
+    # a tile of queries holds 128 rows of up to 32 heads that share a key head
+    G = H // Hk if H > 0 and Hk > 0 else 1
+    rows = max(int(a[-1]), 0) * min(G & -G, 32) + max(int(b[-1]), 0) if a.size else 0
+    guess = 64 + 12 * a.size + rows // 32
     return _plan(lib().vafa_plan_masked, guess, _i64p(a), _i64p(b),
                  None if pre is None else _i64p(pre), a.size, H, Hk, D, int(causal), window)
 

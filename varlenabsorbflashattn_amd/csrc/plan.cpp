@@ -632,11 +632,19 @@ static int plan_masked(const int64_t *cu_q, const int64_t *cu_k, const int64_t *
       double span = (double)(avg + m.item * (int64_t)cost.size() / groups);
       if ((int64_t)cost.size() <= 4 * groups) {
         std::sort(cost.begin(), cost.end(), std::greater<int64_t>());
+        // each piece to the group with the least so far, the root of a heap: its new load
+        // sinks to its place
         heap.assign(groups, 0.0);
         for (int64_t c : cost) {
-          std::pop_heap(heap.begin(), heap.end(), std::greater<double>());
-          heap.back() += (double)c;
-          std::push_heap(heap.begin(), heap.end(), std::greater<double>());
+          const double load = heap[0] + (double)c;
+          int64_t at = 0;
+          for (int64_t kid = 1; kid < groups; kid = 2 * at + 1) {
+            if (kid + 1 < groups && heap[kid + 1] < heap[kid]) ++kid;
+            if (load <= heap[kid]) break;
+            heap[at] = heap[kid];
+            at = kid;
+          }
+          heap[at] = load;
         }
         span = *std::max_element(heap.begin(), heap.end());
       } else {
