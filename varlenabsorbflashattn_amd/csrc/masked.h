@@ -51,8 +51,20 @@ __device__ __forceinline__ bool none_visible(int j0, int j1, int p0, int p1, int
 __device__ __forceinline__ bool all_visible(int j0, int j1, int p0, int p1, int pre, int window) {
   return j1 < pre || (j1 <= p0 && j0 > p1 - window);
 }
-__device__ __forceinline__ bool visible(int j, int p, int pre, int window) {
-  return j < pre || (j <= p && j > p - window);
+// The keys [j, j + 64) that the row at position p sees, a bit each, those from `end` on not
+// among them: once per tile, and then two instructions per score (where_bit) in place of
+// four comparisons and a choice.
+__device__ __forceinline__ uint64_t ones(int n) {  // the lowest n bits, none below 0
+  return n <= 0 ? 0 : (n >= 64 ? ~uint64_t{0} : (uint64_t{1} << n) - 1);
+}
+__device__ __forceinline__ uint64_t seen_keys(int j, int end, int p, int pre, int window) {
+  const int last = p + 1 < end ? p + 1 : end;
+  return ones((pre < end ? pre : end) - j) | (ones(last - j) & ~ones(p - j - window + 1));
+}
+// x where bit i is set, else y.
+__device__ __forceinline__ float where_bit(uint32_t bits, int i, float x, float y) {
+  const uint32_t m = (uint32_t)__builtin_amdgcn_sbfe((int)bits, i, 1);
+  return __uint_as_float((__float_as_uint(x) & m) | (__float_as_uint(y) & ~m));
 }
 
 // Factors of the score transforms.  tanh(x) = 1 - 2 e with e = 1 / (1 + 2^(2 x log2 e)),

@@ -205,11 +205,9 @@ __global__ __launch_bounds__(64 * NW, D >= 256 ? 1 : 2) void masked_dq_kernel(
         }
       }
       if (masked) {
+        const uint32_t seen = (uint32_t)seen_keys(k_lane, ke, p, pre, window);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int j2 = k_lane + off(r);
-          if (j2 >= ke || !visible(j2, p, pre, window)) s[r] = kNegInf;
-        }
+        for (int r = 0; r < 16; ++r) s[r] = where_bit(seen, off(r), s[r], kNegInf);
       }
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
@@ -494,12 +492,12 @@ __global__ __launch_bounds__(64 * NW, D >= 256 && NW < 8 ? 1 : 2) void masked_dk
         hi = hi < tb ? hi : tb;
         bits = lo < hi ? (~0u >> (kRB - (hi << lg)) & ~0u << (lo << lg)) >> row0 : 0u;
       }
-      auto seen = [&](int r) { return (bits >> ((r >> 2) * 8 + (r & 3)) & 1) != 0; };
+      auto row_bit = [](int r) { return (r >> 2) * 8 + (r & 3); };
       if constexpr (!kLog2) {
         if (masked) {
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
-            if (!seen(r)) s[r] = kNegInf;
+            s[r] = where_bit(bits, row_bit(r), s[r], kNegInf);
             if (r % 4 == 3) __builtin_amdgcn_sched_barrier(0);
           }
         }
@@ -525,7 +523,7 @@ __global__ __launch_bounds__(64 * NW, D >= 256 && NW < 8 ? 1 : 2) void masked_dk
             z = __builtin_fmaf(-kLog2e * sl, fabsf((float)(back + t)), z);
           }
           p = fast_exp2(z - lr);
-          p = seen(r) ? p : 0.f;
+          p = where_bit(bits, row_bit(r), p, 0.f);
         } else {
           p = fast_exp2(__builtin_fmaf(s[r], sa.c, -lr));
           if constexpr (!kDeltaInChain) d -= dl;

@@ -67,13 +67,12 @@ __device__ __forceinline__ void masked_tile(const T *ks, const T *vs,
       }
   }
   if (masked) {
+    const uint64_t seen = seen_keys(k_lane, k_end, p, pre, window);
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int j = k_lane + off(kt, r);
-        if (j >= k_end || !visible(j, p, pre, window)) s[kt][r] = kNegInf;
-      }
+      for (int r = 0; r < 16; ++r)
+        s[kt][r] = where_bit((uint32_t)(seen >> 32 * kt), off(0, r), s[kt][r], kNegInf);
   }
   const float c = kLog2 ? 1.f : sa.c;
   typename M::v8 pb[2][2];
