@@ -473,3 +473,30 @@ def test_most_heads(device, H, Hk, D):
     ql, kl = [5, 2], [5, 40]
     x = inputs(63, ql, kl, H, Hk, D, HF, device)
     compare(step(*x, ql, kl), *x, ql, kl)
+
+
+@pytest.mark.parametrize("seed", range(16))
+def test_random_masks(device, seed):
+    rng = np.random.RandomState(100 + seed)
+    D, dt = (64, 128, 256)[seed % 3], (BF, HF)[seed % 2]
+    Hk = int(rng.choice([1, 2, 3]))
+    H = Hk * int(rng.choice([1, 2, 3, 4, 8]))
+    n = int(rng.randint(1, 6))
+    ql = [int(x) for x in rng.randint(0, 200, n)]
+    kl = [int(x) for x in (rng.randint(0, 400, n) if rng.rand() < 0.5 else ql)]
+    kw = {}
+    if rng.rand() < 0.7:
+        kw["window"] = int(rng.choice([1, 2, 31, 64, 65, 150]))
+    if rng.rand() < 0.6:
+        kw["prefix_lens"] = [int(rng.randint(0, k + 1)) for k in kl]
+    if rng.rand() < 0.3:
+        kw["softcap"] = float(rng.choice([2.0, 30.0]))
+    if rng.rand() < 0.3:
+        kw["alibi_slopes"] = torch.linspace(0.01, 0.5, H, device=device)
+    print(f"[masked random {seed}] {ql} {kl} {H}/{Hk} x {D} {dt} {kw}", flush=True)
+    if sum(ql) == 0 or sum(kl) == 0:
+        ql, kl = ql + [3], kl + [4]
+        if "prefix_lens" in kw:
+            kw["prefix_lens"] = kw["prefix_lens"] + [1]
+    x = inputs(200 + seed, ql, kl, H, Hk, D, dt, device)
+    compare(step(*x, ql, kl, **kw), *x, ql, kl, **kw)
