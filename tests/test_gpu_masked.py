@@ -500,3 +500,29 @@ def test_random_masks(device, seed):
             kw["prefix_lens"] = kw["prefix_lens"] + [1]
     x = inputs(200 + seed, ql, kl, H, Hk, D, dt, device)
     compare(step(*x, ql, kl, **kw), *x, ql, kl, **kw)
+
+
+@pytest.mark.parametrize("D,dt,opts", [(64, BF, {}), (128, HF, {"softcap": 20.0}), (256, BF, {}),
+                                       (128, BF, {"alibi": True}), (64, HF, {"softcap": 5.0})])
+def test_unseen_keys_and_rows_without_keys_hold_anything(device, D, dt, opts):
+    """NaN and infinities in keys that no query sees (in front of the window) and in queries
+    and gradients of rows that see no key change nothing: zeros come out for them."""
+    print(f"[masked unseen] {D} {dt} {opts}", flush=True)
+    opts = dict(opts)
+    H, Hk, w = 4, 2, 40
+    ql, kl = [70, 100, 150], [300, 100, 90]  # 60 rows of the last segment see nothing
+    x = inputs(64, ql, kl, H, Hk, D, dt, device)
+    if opts.pop("alibi", False):
+        opts["alibi_slopes"] = torch.linspace(0.1, 0.4, H, device=device)
+    k_dead = slice(0, 300 - 70 - w + 1)
+    q_dead = slice(170, 170 + 60)
+    want, got = [t.clone() for t in x], [t.clone() for t in x]
+    for i, s in ((0, q_dead), (3, q_dead), (1, k_dead), (2, k_dead)):
+        want[i][s] = 0
+        got[i][s] = float("nan") if i != 2 else float("inf")
+    a, b = (step(*y, ql, kl, window=w, **opts) for y in (got, want))
+    for name, s, t in zip(("o", "dq", "dk", "dv"), a, b):
+        assert torch.isfinite(s).all(), name
+        assert torch.equal(s, t), name
+    assert not a[0][q_dead].any() and not a[1][q_dead].any()
+    assert not a[2][k_dead].any() and not a[3][k_dead].any()

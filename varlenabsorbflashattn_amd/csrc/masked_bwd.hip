@@ -119,7 +119,13 @@ __global__ __launch_bounds__(64 * NW, D >= 256 ? 1 : 2) void masked_dq_kernel(
   }
   // rows past q1, and rows that see no key, get LSE = +inf: their P is 0
   float Lr = row_ok ? lse[(int64_t)tok * H + h] : __builtin_inff();
-  if (Lr == kNegInf) Lr = __builtin_inff();
+  const bool dead = !row_ok || Lr == kNegInf;
+  if (wave_any(dead)) {  // whatever such a row and its gradient hold, a factor 0 meets no NaN
+    if (dead) Lr = __builtin_inff(), Dr = 0.f;
+#pragma unroll
+    for (int cc = 0; cc < NC; ++cc)
+      if (dead) qf[cc] = dof[cc] = as_v8<T>(u32x4{0u, 0u, 0u, 0u});
+  }
   if (row_ok && lhalf == 0 && it.v[7] != 0) {  // the item that owns its rows' first keys
     delta[(int64_t)tok * H + h] = Dr;
     lse_out[(int64_t)tok * H + h] = Lr;
@@ -381,6 +387,14 @@ __global__ __launch_bounds__(64 * NW, D >= 256 && NW < 8 ? 1 : 2) void masked_dk
         for (int w = 0; w < 4; ++w) b[w] ^= 0x80008000u;
       }
       vf[cc] = as_v8<T>(b);
+    }
+    // a key that no query sees gets zeros, whatever it holds
+    const int kj = kw0 + lrow, from = kj - diag, to = from + window;
+    const bool seen = kj < pre || (from > q0 ? from : q0) < (to < q1 ? to : q1);
+    if (wave_any(!seen)) {
+#pragma unroll
+      for (int cc = 0; cc < NCS; ++cc)
+        if (!seen) kf[cc] = vf[cc] = as_v8<T>(u32x4{0u, 0u, 0u, 0u});
     }
   }
   f32x16 adk[NDO], adv[NDO];

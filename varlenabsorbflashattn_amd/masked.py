@@ -123,10 +123,11 @@ def packed_masked_attn(
     ``[H]``, no gradient) times ``|p - j|``.  A row that sees no key gets zeros and no
     gradient.  The backward is deterministic.  At most 2^30 tokens and 4096 heads.
 
-    Keys that no query sees are not used, whatever they hold.  One that some query sees
-    must be finite in ``k`` and ``v``: rows that do not see it weigh it with 0, and 0
-    times an infinity is NaN, as in ``softmax(.) @ v``; the same holds for rows of ``q``
-    and of the gradient in the backward.  Lengths on the GPU are read back, which waits for
+    Keys that no query sees, and queries that see no key, may hold anything: zeros come
+    out for them.  A key that some query sees must be finite in ``k`` and ``v``: rows that
+    do not see it may weigh it with 0, and 0 times an infinity is NaN, as in
+    ``softmax(.) @ v``; the same holds for rows of ``q`` and of the gradient in the
+    backward.  Lengths on the GPU are read back, which waits for
     the GPU and which no graph capture allows: pass them on the host there.
     """
     ops = _lib.ops()
