@@ -469,3 +469,21 @@ def test_decode_many_heads(device, H, Hk):
                             torch.tensor(lens, dtype=torch.int32, device=device), window=650)
     ref = op.decode(f64(q), f64(kc), f64(vc), table.numpy(), lens, D ** -0.5, window=650)
     close_decode(out, *ref)
+
+
+def test_expanded_features_are_copied(device):
+    """Rows of one repeated feature (stride 0) are laid out before a kernel reads them."""
+    print("[expanded]", flush=True)
+    lens, q, kc, vc, table, slopes, kw = decode_case(0, device)
+    args = (kc, vc, table.to(device), torch.tensor(lens, dtype=torch.int32, device=device))
+    n, H, D = q.shape
+    wide = torch.randn(n, H, 8, device=device).to(q.dtype)[..., :1].expand(n, H, D)
+    assert wide.stride(2) == 0
+    assert torch.equal(paged_decode_attn(wide, *args), paged_decode_attn(wide.contiguous(), *args))
+    k = wide[:, :1].expand(n, kc.shape[2], D)
+    got = paged_kv_append(k, k, kc.clone(), vc.clone(), *args[2:], q=wide)
+    assert torch.equal(got, wide)
+    k1, v1, k2, v2 = (t.clone() for t in (kc, vc, kc, vc))
+    paged_kv_append(k, k, k1, v1, *args[2:])
+    paged_kv_append(k.contiguous(), k.contiguous(), k2, v2, *args[2:])
+    assert torch.equal(k1, k2) and torch.equal(v1, v2)

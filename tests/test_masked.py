@@ -278,3 +278,8 @@ def test_oracle_rows_without_keys():
     for n in ("o", "dq"):
         assert not ref[n][0][:3].any() and ref[n][0][3:].any()
         assert not ref[n][1][:3].any()
+
+
+def test_expanded_slopes_are_refused():
+    with pytest.raises(ValueError, match="alibi_slopes must be contiguous"):
+        _call(alibi_slopes=torch.ones(1).expand(4))

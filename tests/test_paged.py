@@ -170,3 +170,33 @@ def test_oracle_decode_against_softmax():
     keep = np.concatenate([k[2], k[3]])[:, 0], np.concatenate([v[2], v[3]])[:, 0]
     P = torch.softmax(torch.from_numpy(0.5 * q[0] @ keep[0].T), 1).numpy()
     np.testing.assert_allclose(out[0], P @ keep[1], rtol=1e-12)
+
+
+@pytest.mark.parametrize("call", [_append, _decode])
+@pytest.mark.parametrize("name,shape", [("page_table", (3, 2)), ("cache_lens", (3,))])
+def test_expanded_index_tensors_are_refused(call, name, shape):
+    """One element stands for a row: the kernels would read behind it."""
+    a = _args()
+    a[name] = torch.zeros(1, dtype=torch.int32).expand(shape)
+    with pytest.raises(ValueError, match="must be contiguous"):
+        call(a)
+    # rows that all sequences share are whole rows
+    a["page_table"], a["cache_lens"] = torch.zeros(1, 2, dtype=torch.int32).expand(3, 2), \
+        torch.zeros(3, dtype=torch.int32)
+    with pytest.raises(AssertionError, match="requires GPU tensors"):
+        call(a)
+
+
+def test_expanded_vectors_are_refused():
+    one = torch.ones(1)
+    for kw, text in (({"cu_seqlens": torch.zeros(1, dtype=torch.int32).expand(4)}, "cu_seqlens"),
+                     ({"inv_freq": one.expand(32)}, "inv_freq")):
+        with pytest.raises(ValueError, match=text + " must be contiguous"):
+            _append(_args(), **kw)
+    with pytest.raises(ValueError, match="alibi_slopes must be contiguous"):
+        _decode(_args(), alibi_slopes=one.expand(4))
+    # one head, one frequency: any stride
+    for call, kw in ((_append, {"inv_freq": torch.ones(4)[::4]}),
+                     (_decode, {"alibi_slopes": torch.ones(4)[::4]})):
+        with pytest.raises(AssertionError, match="requires GPU tensors"):
+            call(_args(H=1, Hk=1), **kw)

@@ -257,8 +257,12 @@ void need(bool ok, const char *what, const char *msg) {
 // The stride of a dimension as the kernels use it: one of size 1 is never stepped over.
 int64_t stride_of(const Tensor &t, int64_t dim) { return t.size(dim) > 1 ? t.stride(dim) : 0; }
 
+// Neighbours in memory along a dimension, which the kernels read as such: an expanded
+// dimension (stride 0) holds one element where they would read size of them.
+bool dense(const Tensor &t, int64_t dim) { return t.size(dim) <= 1 || t.stride(dim) == 1; }
+
 bool rows_ok(const Tensor &t) {
-  bool ok = stride_of(t, t.dim() - 1) <= 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+  bool ok = dense(t, t.dim() - 1) && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
   for (int64_t d = 0; d + 1 < t.dim(); ++d) ok = ok && stride_of(t, d) % 8 == 0;
   return ok;
 }
@@ -277,6 +281,11 @@ void no_grad_only(const char *what, std::initializer_list<Tensor> ts) {
                             " has no backward: call it under torch.no_grad() or detach its inputs");
 }
 
+// (last of the checks: the others refuse the same calls without a GPU)
+void on_gpu(const char *what, const Tensor &t) {
+  need(t.is_cuda(), what, "requires GPU tensors on one device");
+}
+
 vafa_paged_cache cache_of(const char *what, const Tensor &kc, const Tensor &vc,
                           const Tensor &table, const Tensor &lens) {
   need(kc.dim() == 4 && vc.sizes() == kc.sizes(), what,
@@ -288,10 +297,7 @@ vafa_paged_cache cache_of(const char *what, const Tensor &kc, const Tensor &vc,
        "page_table must be [n_seq, pages] and cache_lens [n_seq]");
   need(table.scalar_type() == at::kInt && lens.scalar_type() == at::kInt, what,
        "page_table and cache_lens must be int32");
-  need(kc.is_cuda() && vc.device() == kc.device() && table.device() == kc.device() &&
-           lens.device() == kc.device(),
-       what, "requires GPU tensors on one device");
-  if (stride_of(table, 1) > 1 || stride_of(lens, 0) > 1)
+  if (!dense(table, 1) || !dense(lens, 0))
     throw py::value_error(std::string(what) +
                           ": the rows of page_table and cache_lens must be contiguous");
   if (!rows_ok(kc) || !rows_ok(vc))
@@ -302,6 +308,9 @@ vafa_paged_cache cache_of(const char *what, const Tensor &kc, const Tensor &vc,
     for (int64_t d = 0; d < 4; ++d)
       if (t->size(d) > 1 && t->stride(d) == 0)
         throw py::value_error(std::string(what) + ": the caches must not be expanded views");
+  need(vc.device() == kc.device() && table.device() == kc.device() &&
+           lens.device() == kc.device(),
+       what, "requires GPU tensors on one device");
   vafa_paged_cache c{};
   c.k = kc.data_ptr(); c.v = vc.data_ptr();
   c.n_pages = kc.size(0); c.page_size = kc.size(1); c.Hk = kc.size(2); c.D = kc.size(3);
@@ -340,7 +349,7 @@ std::optional<Tensor> paged_append(const Tensor &k_in, const Tensor &v_in, const
     need(cu->dim() == 1 && cu->size(0) == c.n_seq + 1, what, "cu_seqlens must be [n_seq + 1]");
     need(cu->scalar_type() == at::kInt && cu->device() == kc.device(), what,
          "cu_seqlens must be int32 on the cache's device");
-    if (stride_of(*cu, 0) > 1)
+    if (!dense(*cu, 0))
       throw py::value_error(std::string(what) + ": cu_seqlens must be contiguous");
   } else {
     need(T == c.n_seq, what, "without cu_seqlens there must be one token per sequence");
@@ -351,7 +360,7 @@ std::optional<Tensor> paged_append(const Tensor &k_in, const Tensor &v_in, const
          "inv_freq must be [rotated features / 2]");
     need(inv_freq->scalar_type() == at::kFloat && inv_freq->device() == kc.device(), what,
          "inv_freq must be float32 on the cache's device");
-    if (stride_of(*inv_freq, 0) > 1)
+    if (!dense(*inv_freq, 0))
       throw py::value_error(std::string(what) + ": inv_freq must be contiguous");
     rot = 2 * inv_freq->size(0);
   }
@@ -361,6 +370,7 @@ std::optional<Tensor> paged_append(const Tensor &k_in, const Tensor &v_in, const
     need(q_in->size(0) == T, what, "q must have as many tokens as k");
     H = q_in->size(1);
   }
+  on_gpu(what, kc);
   Call call(kc);
   const Tensor k = rows_in(k_in), v = rows_in(v_in);
   Tensor q, out;
@@ -385,7 +395,7 @@ const float *slopes_of(const char *what, const std::optional<Tensor> &slopes, in
   need(slopes->dim() == 1 && slopes->size(0) == H, what, "alibi_slopes must be [H]");
   need(slopes->scalar_type() == at::kFloat && slopes->device() == q.device(), what,
        "alibi_slopes must be float32 on q's device");
-  if (stride_of(*slopes, 0) > 1)
+  if (!dense(*slopes, 0))
     throw py::value_error(std::string(what) + ": alibi_slopes must be contiguous");
   return f32(*slopes);
 }
@@ -404,6 +414,7 @@ Tensor paged_decode(const Tensor &q_in, const Tensor &kc, const Tensor &vc, cons
   need(q_in.size(0) == c.n_seq, what, "q must hold one token per sequence");
   const int64_t H = q_in.size(1);
   const float *sl = slopes_of(what, slopes, H, q_in);
+  on_gpu(what, kc);
   Call call(kc);
   const Tensor q = rows_in(q_in);
   Tensor out = call.empty({c.n_seq, H, c.D});
