@@ -139,3 +139,75 @@ def test_varlen_training_step_under_graph_capture(device):
         assert torch.equal(o_static, o_e)
         for a, b in ((q.grad, qe.grad), (k.grad, ke.grad), (v.grad, ve.grad)):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("op", ["masked", "varlen", "absorb"])
+def test_recorded_plans_outlive_the_cache(device, op):
+    """A graph's launches read their plan in every replay: it stays where it is when calls of
+    many other lengths push it out of the plan cache and take freed memory."""
+    import gc
+    import weakref
+
+    from varlenabsorbflashattn_amd import _lib, packed_masked_attn
+    g = torch.Generator(device=device).manual_seed(8)
+
+    def rnd(*shape):
+        return torch.randn(*shape, generator=g, device=device).to(torch.bfloat16)
+
+    def call(lens, tensors, grad):
+        c = cu_from_lens(lens)
+        x = [t.detach().requires_grad_(True) for t in tensors[:3]]
+        if op == "masked":
+            o = packed_masked_attn(*x, cu_seqlens_q=c, cu_seqlens_k=c, window=90)
+        elif op == "varlen":
+            o = packed_varlen_attn(*x, cu_seqlens_q=c, cu_seqlens_k=c)
+        else:
+            if tuple(lens) not in index:
+                cd = c.to(device)
+                index[tuple(lens)] = (cd, *prepare_target_attn_indices(cd, cd))
+            i = index[tuple(lens)]
+            o = target_attn_inner(*x, i[0], i[0], 0.25, *i[1:], validate=False)
+        return [o.detach(), *torch.autograd.grad(o, x, grad)] if grad is not None else [o.detach()]
+
+    def operands(T):
+        if op == "absorb":
+            return [rnd(T, 2, 64) * 0.1, rnd(T, 64), rnd(64, 2, 32) * 0.1], rnd(T, 2, 32)
+        return [rnd(T, 2, 64) for _ in range(3)], rnd(T, 2, 64)
+
+    index = {}
+    lens = [200, 33, 7]
+    x, do = operands(sum(lens))
+    print(f"[{op} recorded plan]", flush=True)
+    before = set(_lib._CACHE)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call(lens, x, do)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    key, = set(_lib._CACHE) - before
+    items = weakref.ref(_lib._CACHE[key].items)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call(lens, x, do)
+    want = [t.clone() for t in call(lens, x, do)]
+    torch.cuda.synchronize()
+    with torch.no_grad():
+        for n in range(_lib._CACHE_MAX + 1):
+            y, _ = operands(5 + n)
+            call([5 + n], y, None)
+    torch.cuda.synchronize()
+    gc.collect()
+    assert key not in _lib._CACHE
+    assert items() is not None  # before any replay
+    rest = [torch.full((n,), -1, dtype=torch.int32, device=device) for n in (64, 256, 1024)] * 8
+    torch.cuda.synchronize()
+    for i in range(3):
+        for t in out:
+            t.fill_(float("nan"))
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(out, want):
+            assert torch.equal(a, b), i
+    assert all(bool((t == -1).all()) for t in rest)

@@ -336,7 +336,8 @@ def plan_masked(cu_q: np.ndarray, cu_k: np.ndarray, H: int, Hk: int, D: int, cau
 # ---- device plans (cached by cu_seqlens content) ------------------------------
 
 class DevicePlan:
-    """A plan on the device.  ``native`` is the handle the host module takes;
+    """A plan on the device.  ``native`` is the handle the host module takes (which keeps
+    the items of plans that a graph capture recorded);
     ``keys_ok`` remembers that every segment with queries has keys (a property
     of the cu_seqlens the plan was built from)."""
 

@@ -13,8 +13,10 @@
 #include <torch/extension.h>
 
 #include <initializer_list>
+#include <mutex>
 #include <string>
 #include <tuple>
+#include <unordered_map>
 #include <vector>
 
 #include "../../include/vafa.h"
@@ -61,17 +63,6 @@ void check(int rc) {
   throw std::runtime_error("vafa error " + std::to_string(rc) + ": " + msg);
 }
 
-// A device plan: its items and info struct.
-struct Plan {
-  Tensor items;
-  vafa_plan_info info;
-  Plan(Tensor t, const std::string &bytes) : items(std::move(t)) {
-    TORCH_CHECK(bytes.size() == sizeof(info), "plan info of ", bytes.size(), " bytes");
-    std::memcpy(&info, bytes.data(), sizeof(info));
-  }
-  const int32_t *dev() const { return items.data_ptr<int32_t>(); }
-};
-
 int32_t dtype_of(const Tensor &t) {
   switch (t.scalar_type()) {
     case at::kFloat: return VAFA_F32;
@@ -103,6 +94,33 @@ struct Call {
   int64_t ws_bytes() const { return ws.defined() ? ws.numel() : 0; }
 };
 
+// A device plan: its items and info struct.
+struct Plan {
+  Tensor items;
+  vafa_plan_info info;
+  Plan(Tensor t, const std::string &bytes) : items(std::move(t)) {
+    TORCH_CHECK(bytes.size() == sizeof(info), "plan info of ", bytes.size(), " bytes");
+    std::memcpy(&info, bytes.data(), sizeof(info));
+  }
+  // The items as a launch of call c reads them.  A launch that a graph records reads them
+  // again in every replay, without a call that could look the plan up: such a plan stays for
+  // the process's life (32 bytes an item), whatever the cache and the autograd nodes drop.
+  const int32_t *dev(const Call &c) const {
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    const bool known =
+        hipStreamIsCapturing(static_cast<hipStream_t>(c.stream), &status) == hipSuccess;
+    if (!known) (void)hipGetLastError();  // not this call's error
+    if (!known || status != hipStreamCaptureStatusNone) {
+      static std::mutex lock;
+      // (never destroyed: at exit the GPU may be gone before it)
+      static auto *kept = new std::unordered_map<const void *, Tensor>;
+      const std::lock_guard<std::mutex> hold(lock);
+      kept->emplace(items.unsafeGetTensorImpl(), items);
+    }
+    return items.data_ptr<int32_t>();
+  }
+};
+
 void *ptr(const Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
 const float *f32(const Tensor &t) { return static_cast<const float *>(ptr(t)); }
 float *f32w(const Tensor &t) { return static_cast<float *>(ptr(t)); }
@@ -122,7 +140,7 @@ std::tuple<Tensor, Tensor> varlen_fwd(const Tensor &q, const Tensor &k, const Te
   const int64_t D = q.size(2);
   Tensor o = c.like(q), lse = c.empty_f32({q.size(0), q.size(1)});
   void *ws = c.workspace(api.varlen_fwd_workspace(&p.info, D));
-  check(api.varlen_fwd(ptr(q), ptr(k), ptr(v), ptr(o), f32w(lse), p.dev(), &p.info, D, dtype_of(q),
+  check(api.varlen_fwd(ptr(q), ptr(k), ptr(v), ptr(o), f32w(lse), p.dev(c), &p.info, D, dtype_of(q),
                        (float)scale, ws, c.ws_bytes(), c.stream));
   return {o, lse};
 }
@@ -136,7 +154,7 @@ std::tuple<Tensor, Tensor, Tensor> varlen_bwd(const Tensor &q, const Tensor &k, 
   Tensor dq = c.like(q), dk = c.like(k), dv = c.like(v);
   void *ws = c.workspace(api.varlen_bwd_workspace(&p.info, D));
   check(api.varlen_bwd(ptr(q), ptr(k), ptr(v), ptr(o), ptr(dout), f32(lse), ptr(dq), ptr(dk),
-                       ptr(dv), p.dev(), &p.info, D, dtype_of(q), (float)scale, ws, c.ws_bytes(),
+                       ptr(dv), p.dev(c), &p.info, D, dtype_of(q), (float)scale, ws, c.ws_bytes(),
                        c.stream));
   return {dq, dk, dv};
 }
@@ -147,7 +165,7 @@ std::tuple<Tensor, Tensor> absorb_fwd(const Tensor &u, const Tensor &X, const Te
   const int64_t T_q = u.size(0), H = u.size(1), F = u.size(2), DH = W_V.size(2);
   Tensor O = c.empty({T_q, H, DH}), lse = c.empty_f32({T_q, H});
   void *ws = c.workspace(api.absorb_fwd_workspace(&p.info, F, DH));
-  check(api.absorb_fwd(ptr(u), ptr(X), ptr(W_V), ptr(O), f32w(lse), p.dev(), &p.info, F, DH,
+  check(api.absorb_fwd(ptr(u), ptr(X), ptr(W_V), ptr(O), f32w(lse), p.dev(c), &p.info, F, DH,
                        dtype_of(u), (float)scale, ws, c.ws_bytes(), c.stream));
   return {O, lse};
 }
@@ -161,7 +179,7 @@ std::tuple<Tensor, Tensor, Tensor> absorb_bwd(const Tensor &u, const Tensor &X, 
   Tensor du = c.like(u), dX = c.like(X), dW = c.like(W_V);
   void *ws = c.workspace(api.absorb_bwd_workspace(&p.info, F, DH));
   check(api.absorb_bwd(ptr(u), ptr(X), ptr(W_V), ptr(O), ptr(dO), f32(lse), ptr(du), ptr(dX),
-                       ptr(dW), p.dev(), &p.info, F, DH, dtype_of(u), (float)scale, ws,
+                       ptr(dW), p.dev(c), &p.info, F, DH, dtype_of(u), (float)scale, ws,
                        c.ws_bytes(), c.stream));
   return {du, dX, dW};
 }
@@ -177,7 +195,7 @@ std::tuple<Tensor, Tensor, Tensor> absorb_full_fwd(const Tensor &q_raw, const Te
   Tensor q_proj = c.empty({T_q, H * DH}), O = c.empty({T_q, H, DH}), lse = c.empty_f32({T_q, H});
   void *ws = c.workspace(api.absorb_fwd_full_workspace(&p.info, DQ, F, DH));
   check(api.absorb_fwd_full(ptr(q_raw), ptr(X), ptr(W_Q), ptr(W_K), ptr(W_V), ptr(q_proj), ptr(O),
-                            f32w(lse), T_q, p.dev(), &p.info, DQ, F, DH, dtype_of(q_raw),
+                            f32w(lse), T_q, p.dev(c), &p.info, DQ, F, DH, dtype_of(q_raw),
                             (float)scale, ws, c.ws_bytes(), c.stream));
   return {q_proj, O, lse};
 }
@@ -242,7 +260,7 @@ absorb_full_bwd(const Tensor &q_raw, const Tensor &W_Q, const Tensor &W_K, const
   void *ws = c.workspace(api.absorb_bwd_full_workspace(&p.info, T_q, DQ, F, DH));
   check(api.absorb_bwd_full(ptr(q_raw), ptr(X), ptr(W_Q), ptr(W_K), ptr(W_V), ptr(q_proj), ptr(O),
                             ptr(dO), f32(lse), ptr(dq), ptr(dX), ptr(dwq), ptr(dwk), ptr(dW_V),
-                            T_q, p.dev(), &p.info, DQ, F, DH, dtype_of(q_raw), (float)scale, ws,
+                            T_q, p.dev(c), &p.info, DQ, F, DH, dtype_of(q_raw), (float)scale, ws,
                             c.ws_bytes(), c.stream));
   auto opt = [](const Tensor &t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; };
   return {opt(dq), dX, opt(dwq), opt(dwk), dW_V};
@@ -492,7 +510,7 @@ std::tuple<Tensor, Tensor, Tensor> masked_fwd(const Tensor &q, const Tensor &k, 
     lse = c.empty_f32({q.size(0), H});
   }
   void *ws = c.workspace(api.masked_fwd_workspace(&p.info, k.size(1), D));
-  check(api.masked_fwd(ptr(q), ptr(k), ptr(v), ptr(o), ptr(lo), f32w(lse), p.dev(), &p.info,
+  check(api.masked_fwd(ptr(q), ptr(k), ptr(v), ptr(o), ptr(lo), f32w(lse), p.dev(c), &p.info,
                        k.size(1), D, dtype_of(q), (float)scale, (float)softcap, window, sl, ws,
                        c.ws_bytes(), c.stream));
   clear_rest(o, p.info.T_q);
@@ -512,7 +530,7 @@ std::tuple<Tensor, Tensor, Tensor> masked_bwd(const Tensor &q, const Tensor &k, 
   Tensor dq = c.like(q), dk = c.like(k), dv = c.like(v);
   void *ws = c.workspace(api.masked_bwd_workspace(&p.info, Hk, D));
   check(api.masked_bwd(ptr(q), ptr(k), ptr(v), ptr(o), ptr(lo), ptr(dout), f32(lse), ptr(dq),
-                       ptr(dk), ptr(dv), p.dev(), &p.info, Hk, D, dtype_of(q), (float)scale,
+                       ptr(dk), ptr(dv), p.dev(c), &p.info, Hk, D, dtype_of(q), (float)scale,
                        (float)softcap, window, sl, ws, c.ws_bytes(), c.stream));
   clear_rest(dq, p.info.T_q);
   clear_rest(dk, p.info.T_k);
