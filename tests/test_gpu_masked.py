@@ -526,3 +526,38 @@ def test_unseen_keys_and_rows_without_keys_hold_anything(device, D, dt, opts):
         assert torch.equal(s, t), name
     assert not a[0][q_dead].any() and not a[1][q_dead].any()
     assert not a[2][k_dead].any() and not a[3][k_dead].any()
+
+
+def test_second_derivatives_are_refused(device):
+    """With create_graph a gradient is no constant: what would need a second derivative
+    raises, also inside a sum with terms that have one."""
+    print("[masked second]", flush=True)
+    ql = [40, 9]
+    x = inputs(65, ql, ql, 4, 2, 64, BF, device)
+    want = step(*x, ql, ql)
+    cu = cu_from_lens(ql)
+    y = [t.detach().requires_grad_(True) for t in x[:3]]
+    w = torch.ones(4, 1, device=device, dtype=BF, requires_grad=True)
+    o = packed_masked_attn(*y, cu_seqlens_q=cu, cu_seqlens_k=cu)
+    grads = torch.autograd.grad(o, y, x[3], create_graph=True)
+    for a, b in zip(grads, want[1:]):
+        assert a.requires_grad and torch.equal(a, b)
+    refused = pytest.raises(RuntimeError, match="packed_masked_attn has no second derivative")
+    for at in range(3):
+        with refused:
+            (o.float().sum() + grads[at].float().square().sum()).backward(retain_graph=True)
+        for i in range(3):
+            with refused:
+                torch.autograd.grad(grads[at].sum(), y[i], allow_unused=True, retain_graph=True)
+    # an upstream gradient that requires one; products of constants keep their derivatives
+    do = x[3].detach().requires_grad_(True)
+    o = packed_masked_attn(*y, cu_seqlens_q=cu, cu_seqlens_k=cu)
+    g, = torch.autograd.grad(o, y[:1], do, create_graph=True)
+    with refused:
+        torch.autograd.grad(g.sum(), do, retain_graph=True)
+    d, = torch.autograd.grad((g * w).sum(), w)
+    assert torch.equal(d, torch.autograd.grad((want[1] * w).sum(), w)[0])
+    # without create_graph, constants as before
+    y = [t.detach().requires_grad_(True) for t in x[:3]]
+    packed_masked_attn(*y, cu_seqlens_q=cu, cu_seqlens_k=cu).backward(x[3])
+    assert not any(t.grad.requires_grad for t in y)

@@ -10,6 +10,8 @@
 // 50 us: 4 sequences 73 -> 62, 16 absorb samples 84 -> 85.
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <dlfcn.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/extension.h>
 
 #include <initializer_list>
@@ -563,11 +565,18 @@ struct MaskedAttn : torch::autograd::Function<MaskedAttn> {
     const auto holder = ctx->saved_data["plan"].toCapsule();
     const Plan &p = static_cast<PlanHolder *>(holder.get())->plan;
     const Tensor &sl = saved[6];
-    auto [dq, dk, dv] = masked_bwd(saved[0], saved[1], saved[2], saved[3], saved[4], saved[5],
-                                   grads[0], p, ctx->saved_data["scale"].toDouble(),
-                                   ctx->saved_data["softcap"].toDouble(),
-                                   ctx->saved_data["window"].toInt(),
-                                   sl.defined() ? std::optional<Tensor>(sl) : std::nullopt);
+    Tensor dq, dk, dv;
+    std::tie(dq, dk, dv) =
+        masked_bwd(saved[0], saved[1], saved[2], saved[3], saved[4], saved[5], grads[0], p,
+                   ctx->saved_data["scale"].toDouble(), ctx->saved_data["softcap"].toDouble(),
+                   ctx->saved_data["window"].toInt(),
+                   sl.defined() ? std::optional<Tensor>(sl) : std::nullopt);
+    if (at::GradMode::is_enabled()) {  // create_graph: the gradients depend on these four
+      const auto no_second = std::make_shared<torch::autograd::Error>(
+          "packed_masked_attn has no second derivative",
+          torch::autograd::collect_next_edges(saved[0], saved[1], saved[2], grads[0]));
+      for (Tensor *t : {&dq, &dk, &dv}) torch::autograd::set_history(*t, no_second);
+    }
     return {dq, dk, dv, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
   }
 };

@@ -121,7 +121,8 @@ def packed_masked_attn(
     takes neither.  Scores are ``scale * q.k`` (default 1/sqrt(D)), then
     ``softcap * tanh(. / softcap)`` (1e-6 to 1e4), then minus ``alibi_slopes[h]`` (float32
     ``[H]``, no gradient) times ``|p - j|``.  A row that sees no key gets zeros and no
-    gradient.  The backward is deterministic.  At most 2^30 tokens and 4096 heads.
+    gradient.  The backward is deterministic; a second derivative raises.  At most 2^30 tokens
+    and 4096 heads.
 
     Keys that no query sees, and queries that see no key, may hold anything: zeros come
     out for them.  A key that some query sees must be finite in ``k`` and ``v``: rows that
