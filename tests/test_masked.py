@@ -283,3 +283,28 @@ def test_oracle_rows_without_keys():
 def test_expanded_slopes_are_refused():
     with pytest.raises(ValueError, match="alibi_slopes must be contiguous"):
         _call(alibi_slopes=torch.ones(1).expand(4))
+
+
+def test_tangents_and_traces_are_refused():
+    """Derivatives and traces that would lose the call without a word."""
+    import torch.autograd.forward_ad as fw
+    q, k = torch.zeros(6, 4, 64, dtype=torch.bfloat16), torch.zeros(6, 2, 64, dtype=torch.bfloat16)
+    c, slopes = torch.tensor([0, 6], dtype=torch.int32), torch.ones(4)
+    args = [q, k, k.clone(), slopes]
+
+    def call(q, k, v, slopes):
+        return packed_masked_attn(q, k, v, cu_seqlens_q=c, cu_seqlens_k=c, alibi_slopes=slopes)
+    for at in range(4):
+        for grad in (True, False):
+            with fw.dual_level(), torch.set_grad_enabled(grad):
+                x = [fw.make_dual(t, torch.ones_like(t)) if i == at else t
+                     for i, t in enumerate(args)]
+                with pytest.raises(ValueError, match="no forward-mode derivative"):
+                    call(*x)
+                x = [fw.unpack_dual(t).primal for t in x]
+                with pytest.raises(AssertionError, match="requires GPU tensors"):
+                    call(*x)
+    with pytest.raises(ValueError, match="cannot be traced"):
+        torch.jit.trace(call, tuple(args))
+    with pytest.raises(AssertionError, match="requires GPU tensors"):
+        call(*args)

@@ -200,3 +200,18 @@ def test_expanded_vectors_are_refused():
                      (_decode, {"alibi_slopes": torch.ones(4)[::4]})):
         with pytest.raises(AssertionError, match="requires GPU tensors"):
             call(_args(H=1, Hk=1), **kw)
+
+
+@pytest.mark.parametrize("call,names", [(_append, ("q", "k", "v", "k_cache", "v_cache")),
+                                        (_decode, ("q", "k_cache", "v_cache"))])
+def test_tangents_and_traces_are_refused(call, names):
+    import torch.autograd.forward_ad as fw
+    for name in names:
+        a = _args()
+        with fw.dual_level(), torch.no_grad():
+            a[name] = fw.make_dual(a[name], torch.ones_like(a[name]))
+            with pytest.raises(ValueError, match="no forward-mode derivative"):
+                call(a)
+    a = _args()
+    with pytest.raises(ValueError, match="cannot be traced"):
+        torch.jit.trace(lambda q: call({**a, "q": q}), (a["q"],))

@@ -12,6 +12,7 @@
 #include <dlfcn.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 
 #include <initializer_list>
@@ -293,7 +294,20 @@ Tensor rows_in(const Tensor &t) {
   return rows_ok(t) ? t : t.clone(at::MemoryFormat::Contiguous);
 }
 
+// Forward-mode derivatives and traces follow torch's own operations, of which a call here
+// shows them none but the allocation of its output: the tangent would be dropped, and the
+// trace would return memory that nothing wrote.
+void direct_only(const char *what, std::initializer_list<Tensor> ts) {
+  if (torch::jit::tracer::isTracing())
+    throw py::value_error(std::string(what) + " cannot be traced by torch.jit");
+  for (const Tensor &t : ts)
+    if (t.defined() && t._fw_grad(0).defined())
+      throw py::value_error(std::string(what) +
+                            " has no forward-mode derivative: unpack its dual tensors first");
+}
+
 void no_grad_only(const char *what, std::initializer_list<Tensor> ts) {
+  direct_only(what, ts);
   if (!at::GradMode::is_enabled()) return;
   for (const Tensor &t : ts)
     if (t.defined() && t.requires_grad())
@@ -476,6 +490,7 @@ std::tuple<Tensor, Tensor, Tensor> masked_operands(const Tensor &q_in, const Ten
     return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 != 0 ? t.clone() : t;
   };
   const char *what = "packed_masked_attn";
+  direct_only(what, {q_in, k_in, v_in, slopes.value_or(Tensor())});
   const Tensor q = rows(q_in, "q"), k = rows(k_in, "k"), v = rows(v_in, "v");
   const int64_t H = q.size(1), D = q.size(2), Hk = k.size(1);
   need(k.size(2) == D && v.sizes() == k.sizes(), what, "k and v must be [T_k, H_k, D] alike");
