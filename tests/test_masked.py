@@ -308,3 +308,18 @@ def test_tangents_and_traces_are_refused():
         torch.jit.trace(call, tuple(args))
     with pytest.raises(AssertionError, match="requires GPU tensors"):
         call(*args)
+
+
+def test_missing_pointers_are_refused_by_the_c_abi():
+    L = _lib.lib()
+    p = _lib.plan_masked(cu([4]), cu([4]), 4, 2, 64)
+    ws = max(L.vafa_masked_fwd_workspace(p.info, 2, 64), L.vafa_masked_bwd_workspace(p.info, 2, 64))
+    x = 1 << 20
+    f = [x, x, x, x, x, x, x, p.info, 2, 64, _lib.DT_BF16, 0.1, 0.0, 0, None, x, ws, None]
+    b = [x] * 11 + [p.info, 2, 64, _lib.DT_BF16, 0.1, 0.0, 0, None, x, ws, None]
+    for call, args, required in ((L.vafa_masked_fwd, f, (0, 1, 2, 3, 6)),
+                                 (L.vafa_masked_bwd, b, range(11))):
+        for at in required:
+            rc = call(*[None if i == at else y for i, y in enumerate(args)])
+            assert rc == _lib.VAFA_ERR_VALUE, (call, at)
+            assert at == 4 or "NULL" in _lib.last_error()

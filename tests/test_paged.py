@@ -215,3 +215,30 @@ def test_tangents_and_traces_are_refused(call, names):
     a = _args()
     with pytest.raises(ValueError, match="cannot be traced"):
         torch.jit.trace(lambda q: call({**a, "q": q}), (a["q"],))
+
+
+def test_missing_pointers_are_refused_by_the_c_abi():
+    """NULL where there is something to read or write is an error, not an access."""
+    import ctypes as C
+    L = _lib.lib()
+
+    def cache(**kw):
+        c = {"k": 1 << 20, "v": 1 << 21, "n_pages": 5, "page_size": 16, "Hk": 2, "D": 64,
+             "k_page": 2048, "k_token": 128, "k_head": 64, "v_page": 2048, "v_token": 128,
+             "v_head": 64, "page_table": 1 << 22, "table_stride": 2, "table_width": 2,
+             "cache_lens": 1 << 23, "n_seq": 3, **kw}
+        return C.byref(_lib.PagedCache(**c))
+    x = 1 << 24
+    dec = [cache(), x, 256, 64, 4, x, 0.125, 0.0, 0, None, _lib.DT_BF16, None, 0, None]
+    app = [cache(), x, 128, 64, x, 128, 64, 3, None, x, 256, 64, 4, x, x, 64, 0, _lib.DT_BF16, None]
+    for call, args, at in ((L.vafa_paged_decode, dec, (1, 5)),
+                           (L.vafa_paged_append, app, (1, 4, 9, 13, 14))):
+        bad = [(i, None) for i in at] + [(0, cache(**{n: None})) for n in
+                                         ("k", "v", "page_table", "cache_lens")]
+        for i, value in bad:
+            rc = call(*[value if j == i else y for j, y in enumerate(args)])
+            assert rc == _lib.VAFA_ERR_VALUE and "NULL" in _lib.last_error(), (call, i)
+    for c in (cache(table_stride=-2),):
+        assert L.vafa_paged_decode_workspace(c, 4, 0) == -1
+        assert L.vafa_paged_append(c, *app[1:]) == _lib.VAFA_ERR_VALUE
+        assert "entries" in _lib.last_error()

@@ -53,6 +53,12 @@ int check_call(const vafa_plan_info *info, int64_t Hk, int64_t D, int32_t dtype,
   return VAFA_OK;
 }
 
+int check_given(const char *what, std::initializer_list<const void *> ptrs) {
+  for (const void *p : ptrs)
+    if (p == nullptr) return fail(VAFA_ERR_VALUE, "%s: a required pointer is NULL", what);
+  return VAFA_OK;
+}
+
 inline int64_t up(int64_t x) { return (x + 255) / 256 * 256; }
 
 struct Ws {
@@ -177,6 +183,11 @@ int vafa_masked_fwd(const void *q, const void *k, const void *v, void *o, void *
                     const float *slopes, void *workspace, int64_t workspace_bytes, void *stream) {
   if (int rc = check_call(info, Hk, D, dtype, scale, softcap, window, {q, k, v, o, o_lo}))
     return rc;
+  const char *what = "vafa_masked_fwd";
+  if (info->T_q > 0)
+    if (int rc = check_given(what, {q, o, plan_dev})) return rc;
+  if (info->T_k > 0)
+    if (int rc = check_given(what, {k, v})) return rc;
   const Ws w = carve(workspace, info, Hk, D, false);
   if (int rc = check_ws(workspace_bytes, workspace, w.bytes)) return rc;
   MaskedArgs a = args_of(info, plan_dev, Hk, D, scale, softcap, window, slopes);
@@ -187,7 +198,7 @@ int vafa_masked_fwd(const void *q, const void *k, const void *v, void *o, void *
     fwd<bf16>(a, (hipStream_t)stream);
   else
     fwd<f16>(a, (hipStream_t)stream);
-  return check_launch("vafa_masked_fwd");
+  return check_launch(what);
 }
 
 int vafa_masked_bwd(const void *q, const void *k, const void *v, const void *o,
@@ -198,8 +209,13 @@ int vafa_masked_bwd(const void *q, const void *k, const void *v, const void *o,
   if (int rc = check_call(info, Hk, D, dtype, scale, softcap, window,
                           {q, k, v, o, o_lo, dout, dq, dk, dv}))
     return rc;
+  const char *what = "vafa_masked_bwd";
   if (o_lo == nullptr && info->T_q > 0)
     return fail(VAFA_ERR_VALUE, "the backward needs the forward's o_lo");
+  if (info->T_q > 0)
+    if (int rc = check_given(what, {q, o, dout, lse, dq, plan_dev})) return rc;
+  if (info->T_k > 0)
+    if (int rc = check_given(what, {k, v, dk, dv, plan_dev})) return rc;
   const Ws w = carve(workspace, info, Hk, D, true);
   if (int rc = check_ws(workspace_bytes, workspace, w.bytes)) return rc;
   MaskedArgs a = args_of(info, plan_dev, Hk, D, scale, softcap, window, slopes);
@@ -215,7 +231,7 @@ int vafa_masked_bwd(const void *q, const void *k, const void *v, const void *o,
     bwd<bf16>(a, (hipStream_t)stream);
   else
     bwd<f16>(a, (hipStream_t)stream);
-  return check_launch("vafa_masked_bwd");
+  return check_launch(what);
 }
 
 }  // extern "C"

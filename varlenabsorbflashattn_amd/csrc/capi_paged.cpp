@@ -5,6 +5,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
+#include <initializer_list>
 
 #include "../../include/vafa.h"
 #include "common.h"
@@ -23,9 +24,9 @@ int check_cache(const char *what, const vafa_paged_cache *c) {
   if (c->page_size < 1 || c->page_size > INT32_MAX || c->n_pages < 1 || c->n_pages > INT32_MAX)
     return fail(VAFA_ERR_VALUE, "%s: a cache of %lld pages of %lld tokens", what,
                 (long long)c->n_pages, (long long)c->page_size);
-  if (c->table_width < 0 || c->table_width > INT32_MAX)
-    return fail(VAFA_ERR_VALUE, "%s: page_table with rows of %lld entries", what,
-                (long long)c->table_width);
+  if (c->table_width < 0 || c->table_width > INT32_MAX || c->table_stride < 0)
+    return fail(VAFA_ERR_VALUE, "%s: page_table with rows of %lld entries, %lld apart", what,
+                (long long)c->table_width, (long long)c->table_stride);
   const int64_t strides[] = {c->k_page, c->k_token, c->k_head, c->v_page, c->v_token, c->v_head};
   for (int64_t s : strides)
     if (s < 0 || s % 8 != 0)
@@ -42,6 +43,20 @@ int check_rows(const char *what, const char *name, const void *p, int64_t token,
                 "%s: %s must be 16-byte aligned with strides that are multiples of 8 elements",
                 what, name);
   return VAFA_OK;
+}
+
+int check_given(const char *what, std::initializer_list<const void *> ptrs) {
+  for (const void *p : ptrs)
+    if (p == nullptr) return fail(VAFA_ERR_VALUE, "%s: a required pointer is NULL", what);
+  return VAFA_OK;
+}
+
+// The cache's pointers, where there are tokens to store or read.
+int check_pointers(const char *what, const vafa_paged_cache *c) {
+  if (int rc = check_given(what, {c->k, c->v})) return rc;
+  if (c->n_seq == 0) return VAFA_OK;
+  if (int rc = check_given(what, {c->cache_lens})) return rc;
+  return c->table_width > 0 ? check_given(what, {c->page_table}) : VAFA_OK;
 }
 
 int check_dtype(const char *what, int32_t dtype) {
@@ -146,6 +161,12 @@ int vafa_paged_append(const vafa_paged_cache *c, const void *k, int64_t k_token,
   if (!grid_ok(std::max(T, T * ((H + 2 * c->Hk) * (c->D / 16)) / 256 + 1), 256))
     return fail(VAFA_ERR_VALUE, "%s: %lld tokens are too many for a call", what, (long long)T);
   if (T == 0) return VAFA_OK;
+  if (int rc = check_pointers(what, c)) return rc;
+  if (int rc = check_given(what, {k, v})) return rc;
+  if (H > 0)
+    if (int rc = check_given(what, {q, q_out})) return rc;
+  if (rot > 0)
+    if (int rc = check_given(what, {inv_freq})) return rc;
   AppendArgs a{};
   a.q = q; a.k = k; a.v = v; a.q_out = q_out; a.kc = c->k; a.vc = c->v;
   a.cu = cu; a.lens = c->cache_lens; a.inv_freq = inv_freq;
@@ -190,6 +211,8 @@ int vafa_paged_decode(const vafa_paged_cache *c, const void *q, int64_t q_token,
     return fail(VAFA_ERR_WORKSPACE, "workspace of %lld bytes, %lld needed (16-byte aligned)",
                 (long long)workspace_bytes, (long long)p.bytes);
   if (c->n_seq == 0) return VAFA_OK;
+  if (int rc = check_pointers(what, c)) return rc;
+  if (int rc = check_given(what, {q, out})) return rc;
   DecodeArgs a{};
   a.q = q; a.kc = c->k; a.vc = c->v; a.out = out; a.lens = c->cache_lens; a.slopes = slopes;
   a.part_o = (float *)workspace;
