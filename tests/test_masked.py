@@ -323,3 +323,17 @@ def test_missing_pointers_are_refused_by_the_c_abi():
             rc = call(*[None if i == at else y for i, y in enumerate(args)])
             assert rc == _lib.VAFA_ERR_VALUE, (call, at)
             assert at == 4 or "NULL" in _lib.last_error()
+
+
+def test_prefix_lens_of_another_shape_are_refused_behind_a_cached_plan():
+    from varlenabsorbflashattn_amd import masked
+    q, k, c = torch.zeros(9, 2, 64), torch.zeros(9, 1, 64), cu([4, 5])
+    c = torch.from_numpy(c)
+
+    def plan(prefix):
+        return masked._plan_of(q, k, c, c, True, 0, prefix)
+    want = plan(torch.tensor([1, 3]))
+    for bad in (torch.tensor([[1, 3]]), torch.tensor([[1], [3]]), torch.tensor([1, 3, 0])):
+        with pytest.raises(AssertionError, match=r"prefix_lens must be \[2\]"):
+            plan(bad)
+    assert plan(torch.tensor([1, 3], dtype=torch.int32)) is want

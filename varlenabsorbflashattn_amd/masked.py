@@ -46,6 +46,8 @@ def _plan_of(q, k, cu_seqlens_q, cu_seqlens_k, causal, window, prefix_lens):
     cu_q, cu_k = _host_pair(cu_seqlens_q, cu_seqlens_k)
     content = _lib.ops().cu_key
     prefix = None if prefix_lens is None else _host(prefix_lens, "prefix_lens").to(torch.int64)
+    if prefix is not None and prefix.shape != (cu_q.numel() - 1,):  # (the key holds content alone)
+        raise AssertionError(f"prefix_lens must be [{cu_q.numel() - 1}], got {tuple(prefix.shape)}")
     key = ("masked", content(cu_q), content(cu_k), None if prefix is None else content(prefix),
            H, H_k, D, causal, window, q.device)
     plan = _lib.cached_plan(key) if cu_q.dim() == 1 and cu_k.dim() == 1 else None
