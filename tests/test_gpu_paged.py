@@ -487,3 +487,73 @@ def test_expanded_features_are_copied(device):
     paged_kv_append(k, k, k1, v1, *args[2:])
     paged_kv_append(k.contiguous(), k.contiguous(), k2, v2, *args[2:])
     assert torch.equal(k1, k2) and torch.equal(v1, v2)
+
+
+def chunks_of(H, kc, table, window):
+    """Parts of the tiles' axis in a call, from the workspace of their two pieces each."""
+    import ctypes as C
+
+    from varlenabsorbflashattn_amd import _lib
+    n_pages, page, Hk, D = kc.shape
+    c = _lib.PagedCache(k=1 << 20, v=1 << 20, n_pages=n_pages, page_size=page, Hk=Hk, D=D,
+                        k_page=8, k_token=8, k_head=8, v_page=8, v_token=8, v_head=8,
+                        page_table=1 << 20, table_stride=table.shape[1],
+                        table_width=table.shape[1], cache_lens=1 << 20, n_seq=len(table))
+    pairs = Hk * -(-H // Hk // 16)
+    size = _lib.lib().vafa_paged_decode_workspace(C.byref(c), H, window or 0)
+    return size // (2 * pairs * 16 * (4 * D + 8))
+
+
+SPLIT = [
+    # lens, H, Hk, D, page, softcap, window, dtype; tiles of 128 keys, several in each chunk
+    ([20000, 9000, 12345, 3], 48, 8, 128, 32, None, None, torch.float16),
+    ([20000, 9000, 12345, 3], 48, 8, 128, 32, None, None, torch.bfloat16),
+    ([5000, 800, 16000, 0, 129], 32, 16, 64, 16, None, 6000, torch.bfloat16),
+    ([3000, 33, 5000, 1000], 24, 24, 256, 64, 30.0, None, torch.float16),
+    ([257, 6000, 1, 2100, 2100], 160, 5, 128, 128, None, None, torch.float16),
+]
+
+
+@pytest.mark.parametrize("case", range(len(SPLIT)))
+def test_decode_of_sequences_cut_anywhere(device, case):
+    """Chunks that end one sequence and begin the next: a sequence's first piece is then a
+    chunk's second partial result.  The bound per element would hide a lost tile of a long
+    sequence, so each sequence is held to a 2-norm as well.  There the roundings are
+    independent: of P for the product (with |v - o| for |v|, as their sum is the
+    denominator) at most u / sqrt(3) in the mean, and of the result as much: 0.82 u."""
+    lens, H, Hk, D, page, cap, window, dt = SPLIT[case]
+    print(f"[decode cut] {SPLIT[case]}", flush=True)
+    g = torch.Generator(device=device).manual_seed(case + 31)
+    table, N = pages_for(g, lens, page)
+    kc, vc = cache_pair(g, N, page, Hk, D, dt, device, "plain")
+    q = torch.randn(len(lens), H, D, generator=g, device=device).to(dt)
+    tiles = [-(-min(n, window or n) // 128) for n in lens]
+    per = -(-sum(tiles) // chunks_of(H, kc, table, window))
+    base = np.cumsum([0] + tiles)
+    second = [b for b, n in enumerate(tiles)
+              if n and base[b] % per and base[b] // per != (base[b + 1] - 1) // per]
+    print(f"  {per} tiles a chunk, sequences from {base[:-1].tolist()}", flush=True)
+    assert per >= 2 and second
+    kw = {"softcap": cap, "window": window}
+    out = paged_decode_attn(q, kc, vc, table.to(device),
+                            torch.tensor(lens, dtype=torch.int32, device=device), **kw)
+    args = f64(q), f64(kc), f64(vc)
+    ref = op.decode(*args, table.numpy(), lens, D ** -0.5, **kw)
+    close_decode(out, *ref)
+    got, u = f64(out), U[dt]
+
+    def off(x, b):
+        return np.linalg.norm(x[b] - ref[0][b]) / np.linalg.norm(ref[0][b]) / u
+    for b, n in enumerate(lens):
+        if n:
+            print(f"  sequence {b}: {off(got, b):.2f} u", flush=True)
+            assert off(got, b) < 1.0, b
+    # what one tile less would do
+    lost = table.numpy().copy()
+    for b, n in enumerate(lens):
+        at = (n - 1) // 128 // 2 * (128 // page)
+        lost[b, at:at + 128 // page] = -1
+    short = op.decode(*args, lost, lens, D ** -0.5, **kw)[0]
+    for b in second:
+        if tiles[b] > 1 and (not window or lens[b] <= window):
+            assert off(short, b) > 8.0, b
