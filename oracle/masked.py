@@ -42,11 +42,20 @@ def attention(q, k, v, do, cu_q, cu_k, scale, causal=True, window=None, prefix=N
 
     ``u`` is half a step of the type relative to a value, ``a`` half its smallest step.
     The bounds count, element by element: the rounding of P and of dS for the products
-    (u each, and a), the sum of the rounded P (u, in o and through the LSE in P), O's
-    rounding inside delta (u |o||dO|), the fp32 sums behind the scores (2^-12 of P and
-    of P (|dP| + |delta|)), and the output's own rounding (u, a).
+    (u each, and a), the sum of the rounded P (u, in o and through the LSE in P), the fp32
+    sums behind the scores (2^-12 of P and of P (|dP| + |delta|)), and the output's own
+    rounding (u, a).  delta = o.dO meets the rounding of P in o, u sum P |dP - delta| (the
+    denominator is the sum of the same rounded P, so v enters as v - o); o itself comes with
+    eight more bits than the type holds, off by at most one of their steps, 2^-7 u |o|, or
+    by a below fp16's smallest normal value; it and dP are fp32 sums of D products.
+
+    P, dS and a bf16 output below 2^-126, fp32's smallest normal value, may come out as 0:
+    each is then off by less than that, so P by f = 2^-126 in what it multiplies, |v|, |dO|
+    and |dP - delta|, dS by f |scale| and the output by f.  (Keys whose distance bias is above
+    87 hold nothing else.)
     """
     H, Hk, eps = q.shape[1], k.shape[1], 2.0 ** -12
+    f = 2.0 ** -126 if u else 0.0
     G = H // Hk
     names = ["o"] if do is None else ["o", "dq", "dk", "dv"]
     shapes = [q.shape] if do is None else [q.shape, q.shape, k.shape, v.shape]
@@ -63,21 +72,25 @@ def attention(q, k, v, do, cu_q, cu_k, scale, causal=True, window=None, prefix=N
             o = P @ vh
             val["o"][sq, h] = o
             flat = np.divide(2 * a, l, out=np.zeros_like(l), where=l > 0)
-            err["o"][sq, h] = (2 * u + eps) * (P @ np.abs(vh)) + flat * (see @ np.abs(vh))
+            err["o"][sq, h] = (2 * u + eps) * (P @ np.abs(vh)) + (flat + f) * (see @ np.abs(vh))
             if do is None:
                 continue
             d = do[sq, h]
             dP, delta = d @ vh.T, (d * o).sum(1, keepdims=True)
             dS = P * (dP - delta) * grad * scale
             # error of dS: its factors', delta's, its own rounding
-            c = abs(scale)
-            E = (3 * u + eps) * np.abs(dS) + c * P * grad * (
-                u * (np.abs(o) * np.abs(d)).sum(1, keepdims=True)) \
-                + c * eps * P * (np.abs(dP) + np.abs(delta)) + c * a * see
+            c, sums = abs(scale), (q.shape[2] + 1) * 2.0 ** -24 if u else 0.0
+            e_delta = u * (P * np.abs(dP - delta)).sum(1, keepdims=True) \
+                + (2.0 ** -7 * u + sums) * (np.abs(o) * np.abs(d)).sum(1, keepdims=True) \
+                + a * np.abs(d).sum(1, keepdims=True)
+            E = (3 * u + eps) * np.abs(dS) \
+                + c * P * grad * (e_delta + sums * (np.abs(d) @ np.abs(vh).T)) \
+                + c * eps * P * (np.abs(dP) + np.abs(delta)) \
+                + c * (a + f + f * np.abs(dP - delta) * grad) * see
             val["dq"][sq, h] = dS @ kh
             err["dq"][sq, h] = E @ np.abs(kh)
             val["dk"][sk, g] += dS.T @ qh
             err["dk"][sk, g] += E.T @ np.abs(qh)
             val["dv"][sk, g] += P.T @ d
-            err["dv"][sk, g] += (2 * u + eps) * (P.T @ np.abs(d)) + a * (see.T @ np.abs(d))
-    return {n: (val[n], err[n] + u * np.abs(val[n]) + a) for n in names}
+            err["dv"][sk, g] += (2 * u + eps) * (P.T @ np.abs(d)) + (a + f) * (see.T @ np.abs(d))
+    return {n: (val[n], err[n] + u * np.abs(val[n]) + a + f * (val[n] != 0)) for n in names}

@@ -561,3 +561,17 @@ def test_second_derivatives_are_refused(device):
     y = [t.detach().requires_grad_(True) for t in x[:3]]
     packed_masked_attn(*y, cu_seqlens_q=cu, cu_seqlens_k=cu).backward(x[3])
     assert not any(t.grad.requires_grad for t in y)
+
+
+@pytest.mark.parametrize("ql,kl,H,Hk,D,dt", [([200, 7, 33], None, 4, 2, 64, BF),
+                                             ([130, 1, 61], None, 6, 1, 128, HF),
+                                             ([100], [4000], 2, 1, 128, BF),
+                                             ([90, 21], [90, 3500], 2, 2, 256, HF)])
+def test_elements_of_rows_that_few_keys_carry(device, ql, kl, H, Hk, D, dt):
+    """Steep distance biases, element by element: the bounds there are below what delta from
+    o in the type's own bits would give (tests/test_masked.py)."""
+    print(f"[masked steep elements] {ql} {kl} {H}/{Hk} x {D} {dt}", flush=True)
+    kl = kl or ql
+    x = inputs(66, ql, kl, H, Hk, D, dt, device)
+    slopes = torch.linspace(4.0, 7.0, H, device=device)
+    compare(step(*x, ql, kl, alibi_slopes=slopes), *x, ql, kl, alibi_slopes=slopes)

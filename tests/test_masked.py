@@ -337,3 +337,30 @@ def test_prefix_lens_of_another_shape_are_refused_behind_a_cached_plan():
         with pytest.raises(AssertionError, match=r"prefix_lens must be \[2\]"):
             plan(bad)
     assert plan(torch.tensor([1, 3], dtype=torch.int32)) is want
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+def test_bounds_tell_how_many_bits_of_o_delta_takes(dt):
+    """Rows that few keys carry (steep distance biases): delta from o as the type holds it is
+    outside the bounds, delta from eight more bits inside, each beside exact arithmetic."""
+    u, a = {torch.bfloat16: (2.0 ** -8, 0.0), torch.float16: (2.0 ** -11, 2.0 ** -25)}[dt]
+    g = torch.Generator().manual_seed(3)
+    n, H, D = 60, 2, 64
+    q, k, v, do = (torch.randn(n, H, D, generator=g).to(dt).double().numpy() for _ in range(4))
+    at, slopes = np.array([0, n]), [4.0, 7.0]
+    ref = om.attention(q, k, v, do, at, at, D ** -0.5, slopes=slopes, u=u, a=a)
+
+    def gradients(bits):
+        m, e = np.frexp(ref["o"][0])
+        o = np.ldexp(np.round(m * 2.0 ** bits) / 2.0 ** bits, e)
+        dq, dk = np.zeros_like(q), np.zeros_like(k)
+        for h in range(H):
+            P, _, _ = om._head(q[:, h], k[:, h], D ** -0.5, True, None, 0, None, slopes[h])
+            dS = P * (do[:, h] @ v[:, h].T - (do[:, h] * o[:, h]).sum(1, keepdims=True)) * D ** -0.5
+            dq[:, h], dk[:, h] = dS @ k[:, h], dS.T @ q[:, h]
+        return dq, dk
+    digits = 8 if dt == torch.bfloat16 else 11
+    for bits, inside in ((digits, False), (digits + 8, True)):
+        for name, x in zip(("dq", "dk"), gradients(bits)):
+            val, bound = ref[name]
+            assert bool((np.abs(x - val) <= bound).all()) == inside, (bits, name)
