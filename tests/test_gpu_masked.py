@@ -575,3 +575,74 @@ def test_elements_of_rows_that_few_keys_carry(device, ql, kl, H, Hk, D, dt):
     x = inputs(66, ql, kl, H, Hk, D, dt, device)
     slopes = torch.linspace(4.0, 7.0, H, device=device)
     compare(step(*x, ql, kl, alibi_slopes=slopes), *x, ql, kl, alibi_slopes=slopes)
+
+
+def test_prompt_behind_a_cached_prefix(device):
+    """Several new tokens behind what the cache holds: appended, the sequences' keys and
+    values gathered from their pages, and the packed pass over more keys than queries.  Its
+    rows are those of a pass over the whole sequences."""
+    H, Hk, D, page, past, new = 4, 2, 64, 16, [70, 0, 33], [40, 25, 1]
+    print(f"[masked prefix cache] {past} + {new}", flush=True)
+    total = [a + b for a, b in zip(past, new)]
+    g = torch.Generator(device=device).manual_seed(67)
+    qkv = torch.randn(sum(total), H + 2 * Hk, D, generator=g, device=device).to(HF)
+    pages = [-(-n // page) for n in total]
+    table = torch.full((3, max(pages)), -1, dtype=torch.int32)
+    order = torch.randperm(sum(pages), generator=torch.Generator().manual_seed(67)).int()
+    for b, n in enumerate(pages):
+        table[b, :n] = order[sum(pages[:b]):sum(pages[:b + 1])]
+    page_table = table.to(device)
+    # a joint allocation: keys and values of a page beside each other
+    both = torch.full((sum(pages), 2, page, Hk, D), float("nan"), device=device).to(HF)
+    k_cache, v_cache = both[:, 0], both[:, 1]
+    inv = (10000.0 ** (-torch.arange(0, D, 2) / D)).float().to(device)
+    seq = torch.repeat_interleave(torch.arange(3), torch.tensor(total))
+    pos = torch.cat([torch.arange(n) for n in total])
+    old = (pos < torch.tensor(past)[seq]).to(device)
+    lens = torch.zeros(3, dtype=torch.int32, device=device)
+    qs = []
+    for rows, n in ((old, past), (~old, new)):
+        x = qkv[rows]
+        qs.append(paged_kv_append(x[:, H:H + Hk], x[:, H + Hk:], k_cache, v_cache, page_table, lens,
+                                  cu_seqlens=cu_from_lens(n).int().to(device), q=x[:, :H],
+                                  inv_freq=inv))
+        lens += torch.tensor(n, dtype=torch.int32, device=device)
+    b, pos = seq.to(device), pos.to(device)
+    at = page_table[b, pos // page].long()
+    k, v = k_cache[at, pos % page], v_cache[at, pos % page]
+    assert torch.equal(v, qkv[:, H + Hk:])
+    kw = {"window": 50, "softcap": 20.0}
+    o = packed_masked_attn(qs[1], k, v, cu_seqlens_q=cu_from_lens(new),
+                           cu_seqlens_k=cu_from_lens(total), **kw)
+    q = torch.empty_like(qkv[:, :H])
+    q[old], q[~old] = qs
+    val, bound = om.attention(f64(q), f64(k), f64(v), None, np.cumsum([0] + total),
+                              np.cumsum([0] + total), D ** -0.5, u=U[HF], a=A[HF], **kw)["o"]
+    keep = (~old).cpu().numpy()
+    within("o", o, val[keep], bound[keep])
+
+
+def test_saved_tensors_elsewhere(device):
+    """Gradients with the saved tensors kept on the host, and recomputed by checkpointing."""
+    from torch.utils.checkpoint import checkpoint
+    print("[masked saved]", flush=True)
+    ql = [90, 31]
+    x = inputs(68, ql, ql, 4, 2, 128, BF, device)
+    slopes = torch.linspace(0.1, 0.4, 4, device=device)
+    kw = {"window": 40, "alibi_slopes": slopes}
+    want = step(*x, ql, ql, **kw)
+
+    def call(q, k, v):
+        return packed_masked_attn(q, k, v, cu_seqlens_q=cu_from_lens(ql),
+                                  cu_seqlens_k=cu_from_lens(ql), **kw)
+    y = [t.detach().requires_grad_(True) for t in x[:3]]
+    with torch.autograd.graph.save_on_cpu():
+        o = call(*y)
+    for a, b in zip((o, *torch.autograd.grad(o, y, x[3])), want):
+        assert torch.equal(a, b)
+    for reentrant in (False, True):
+        y = [t.detach().requires_grad_(True) for t in x[:3]]
+        o = checkpoint(call, *y, use_reentrant=reentrant)
+        o.backward(x[3])
+        for a, b in zip((o, *(t.grad for t in y)), want):
+            assert torch.equal(a, b)

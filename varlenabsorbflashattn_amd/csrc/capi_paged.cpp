@@ -92,9 +92,9 @@ struct DecodePlan {
 
 // Workgroups resident on the GPU, by registers: 3 (D = 64) or 2 on each of 256 CUs.
 int64_t decode_wgs(int64_t D) { return D == 64 ? 768 : 512; }
-// Sequences of at most this many tiles are not divided: a workgroup each, and no launch
-// that joins (4 sequences of up to 500 keys: 9.5 -> 6.1 us; 8 of 1000, 8 tiles, the other way round
-// 14 -> 26).
+// Where the page table can hold at most this many tiles a sequence (the lengths are not
+// known here), none is divided: a workgroup each, and no launch that joins (4 sequences
+// of up to 500 keys: 9.5 -> 6.1 us; 8 of 1000, 8 tiles, the other way round 14 -> 26).
 constexpr int64_t kDecodeDirect = 4;
 
 int plan_decode(const vafa_paged_cache *c, int64_t H, int64_t window, DecodePlan *p) {

@@ -8,6 +8,10 @@
 //     (token, head) rows that see it, of every query head that shares the key head (or a
 //     part of those blocks, where one workgroup's walk would outlast the launch: fp32
 //     partials, summed in order), and accumulates dV^T += dO^T P, dK^T += Q^T dS.
+// P and dS are rounded to T for the products of dV, dQ and dK, formed from fp32 scores, LSE and
+// delta: gradients 2.4e-3 (bf16) and 3.0e-4 (fp16) off in the 2-norm, where the exact ones
+// rounded are 1.7e-3 and 2.1e-4 off.  Two 16-bit parts each would take half as many products
+// again.
 // With y = cap tanh(z / cap): dz = dx (1 - tanh^2), formed from e of cap_e as 4 e (1 - e).
 #include <algorithm>
 #include <type_traits>

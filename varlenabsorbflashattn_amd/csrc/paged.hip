@@ -488,7 +488,8 @@ __global__ __launch_bounds__(256, D >= 128 ? 2 : 3) void paged_decode_kernel(Dec
 #pragma unroll
       for (int e = 0; e < 4 * KG; ++e) {
         const float x = fast_exp2(y[e] - m_run);
-        // the sum takes the probabilities as rounded for the product
+        // rounded to T, V's type, for the product; the sum takes the rounded values, in fp32
+        // (outputs 0.52 of half a step off in the 2-norm, 0.42 of it their own rounding)
         p[e] = static_cast<T>(x);
         ps += to_f(p[e]);
       }

@@ -496,7 +496,9 @@ int vafa_plan_varlen_balanced(const int64_t *cu_q, const int64_t *cu_k, int64_t 
 //                 and those of its window; between the two ranges nothing of [k0, k1)
 //                 is walked.  pbase as in a varlen plan; owner: 1 for the item that
 //                 holds its rows' first keys.  A tile that sees no key is an item with
-//                 k0 == k1, which writes zeros.
+//                 k0 == k1, which writes zeros.  A tile's range is split where the
+//                 range, gap included, passes the chunk: a part that lies in the gap walks
+//                 nothing and writes partial rows of zeros (lse -inf).
 //   comb section: {q0, q1, pbase, nsplit, seg, 0, 0, 0}.
 //   kv section  : {k0, k1, q0, q1, diag, pre, pbase, part << 16 | parts} key tiles with
 //                 the range of the queries that see some of their keys; a tile's blocks

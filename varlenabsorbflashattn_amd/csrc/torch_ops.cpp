@@ -1,8 +1,10 @@
 // Allocation and launch of one operator pass per call, for the Python layer:
 // each function allocates outputs and workspace with torch's allocator, takes
 // the current stream of the operands' device and calls one entry point of
-// libvafa.so (include/vafa.h).  Autograd, argument checks and the plan cache
-// stay in Python.  With tensor factories, ctypes conversions and stream lookups
+// libvafa.so (include/vafa.h).  The plan cache is in Python, and so are autograd and the
+// argument checks of packed_varlen_attn and packed_target_attn; packed_masked_attn and the
+// paged cache, whose small calls have less time for them, have theirs here.  With tensor
+// factories, ctypes conversions and stream lookups
 // there too, host time held every small call: us a call with cu_seqlens seen before
 // (the plan cached), before -> now, 4 short sequences forward 31 -> 17 (host
 // cu_seqlens), forward + backward 150 -> 93; 16 absorb samples forward 34 -> 25,
