@@ -404,7 +404,8 @@ VAFA_API int vafa_masked_bwd(const void *q, const void *k, const void *v, const 
                              void *workspace, int64_t workspace_bytes, void *stream);
 
 /* ======================================================================== */
-/* Paged key-value cache (bf16 / fp16).  No counterpart in the reference.   */
+/* Paged key-value cache (bf16 / fp16, or codes of 8 bits).  No counterpart */
+/* in the reference.                                                        */
 /* ======================================================================== */
 
 /* Keys and values of n_seq sequences in pages: token p of sequence b is token
@@ -449,6 +450,68 @@ VAFA_API int vafa_paged_decode(const vafa_paged_cache *cache, const void *q, int
                                int64_t q_head, int64_t H, void *out, float scale, float softcap,
                                int64_t window, const float *slopes, int32_t dtype,
                                void *workspace, int64_t workspace_bytes, void *stream);
+
+/* The powers of two of a cache of codes: k and v of the vafa_paged_cache then hold e4m3
+ * (OCP) codes, strides multiples of 16, and the value of a feature is its code times
+ * 2^(byte - 127) with the byte (E8M0) of its (page, token, head) row.  Strides in bytes. */
+typedef struct vafa_row_scales {
+  void *k, *v;
+  int64_t k_page, k_token, k_head;
+  int64_t v_page, v_token, v_head;
+} vafa_row_scales;
+
+/* vafa_paged_append (D in {64, 128, 256}, rot a multiple of 16) of normed rows, into 16 bits
+ * or, with scales, codes: rows of q and k become R(x r w), r = 1 / sqrt(mean x^2 + eps), w =
+ * q_weight / k_weight [D] (NULL: not normed; fp32 where weights_f32, else of dtype), before
+ * the rotation R, whose sine and cosine are multiplied by rot_scale.  dtype is that of k, v,
+ * q.  A row's power of two is the least 2^e with max |x| <= 448 * 2^e (e at most 8 for fp16
+ * and 120 for bf16, where codes end at 240, so that each code's value is finite in dtype);
+ * infinities and NaN become NaN. */
+VAFA_API int vafa_paged_store(const vafa_paged_cache *cache, const vafa_row_scales *scales,
+                              const void *k, int64_t k_token, int64_t k_head, const void *v,
+                              int64_t v_token, int64_t v_head, int64_t T, const int32_t *cu,
+                              const void *q, int64_t q_token, int64_t q_head, int64_t H,
+                              void *q_out, const float *inv_freq, int64_t rot,
+                              int32_t interleaved, float rot_scale, const void *q_weight,
+                              const void *k_weight, int32_t weights_f32, float eps, int32_t dtype,
+                              void *stream);
+
+/* Rows of the cache (codes with scales), as k and v [T, Hk, D] of dtype: row t of sequence b
+ * (cu[b] <= t < cu[b + 1]) is its token at starts[b] + t - cu[b] (starts NULL: from the first
+ * on).  Rows of no sequence or of tokens without a page are zeros.  cache_lens is not read.
+ * D: multiples of 16 up to 1024. */
+VAFA_API int vafa_paged_gather(const vafa_paged_cache *cache, const vafa_row_scales *scales,
+                               const int32_t *cu, const int32_t *starts, int64_t T, void *k,
+                               void *v, int32_t dtype, void *stream);
+
+/* ======================================================================== */
+/* Norms of queries and keys with the position rotation (bf16 / fp16, D in  */
+/* {64, 128, 256}).  No counterpart in the reference.                       */
+/* ======================================================================== */
+
+/* q [T, H, D] and k [T, Hk, D] (strides in elements, multiples of 8) -> q_out [T, H, D] and
+ * k_out [T, Hk, D], normed and rotated as by vafa_paged_store, at positions [T] (device
+ * int32; not read where rot is 0). */
+VAFA_API int vafa_qk_norm_rope_fwd(const void *q, int64_t q_token, int64_t q_head, int64_t H,
+                                   const void *k, int64_t k_token, int64_t k_head, int64_t Hk,
+                                   int64_t T, int64_t D, const int32_t *positions,
+                                   const float *inv_freq, int64_t rot, int32_t interleaved,
+                                   float rot_scale, const void *q_weight, const void *k_weight,
+                                   int32_t weights_f32, float eps, void *q_out, void *k_out,
+                                   int32_t dtype, void *stream);
+/* dq_out [T, H, D], dk_out [T, Hk, D] (contiguous) -> dq, dk (contiguous) and dq_weight,
+ * dk_weight [D] of the weights' type (NULL: not wanted; NULL where there is no weight).
+ * Deterministic (no atomics). */
+VAFA_API int64_t vafa_qk_norm_rope_bwd_workspace(int64_t T, int64_t H, int64_t Hk, int64_t D);
+VAFA_API int vafa_qk_norm_rope_bwd(const void *q, int64_t q_token, int64_t q_head, int64_t H,
+                                   const void *k, int64_t k_token, int64_t k_head, int64_t Hk,
+                                   int64_t T, int64_t D, const int32_t *positions,
+                                   const float *inv_freq, int64_t rot, int32_t interleaved,
+                                   float rot_scale, const void *q_weight, const void *k_weight,
+                                   int32_t weights_f32, float eps, const void *dq_out,
+                                   const void *dk_out, void *dq, void *dk, void *dq_weight,
+                                   void *dk_weight, int32_t dtype, void *workspace,
+                                   int64_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }

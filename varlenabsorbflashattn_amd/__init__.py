@@ -7,8 +7,10 @@ Drop-in replacements for the reference packages' public APIs:
   :func:`target_attn_inner`, :func:`prepare_target_attn_indices`
 
 Beside them, for language models: :func:`packed_masked_attn` (causal, windowed and prefix
-masks, capped scores, distance biases, grouped key heads), :func:`paged_kv_append` and :func:`paged_decode_attn`
-(a paged key-value cache and the attention of one new token over it).
+masks, capped scores, distance biases, grouped key heads), :func:`packed_qk_norm_rope` (norms
+of queries and keys with the position rotation), :func:`paged_kv_append`,
+:func:`paged_kv_gather` and :func:`paged_decode_attn` (a paged key-value cache, in 16 or 8
+bits, and the attention of one new token over it).
 
 All compute runs in the in-tree HIP library ``libvafa.so`` (C ABI in
 ``include/vafa.h``); it is loaded on the first call.
@@ -16,7 +18,8 @@ All compute runs in the in-tree HIP library ``libvafa.so`` (C ABI in
 from .varlen import packed_varlen_attn, set_validate_cu_seqlens
 from .absorb import packed_target_attn, prepare_target_attn_indices, target_attn_inner
 from .masked import packed_masked_attn
-from .paged import paged_decode_attn, paged_kv_append
+from .norm_rope import packed_qk_norm_rope
+from .paged import paged_decode_attn, paged_kv_append, paged_kv_gather
 
 __all__ = [
     "packed_varlen_attn",
@@ -25,7 +28,9 @@ __all__ = [
     "prepare_target_attn_indices",
     "target_attn_inner",
     "packed_masked_attn",
+    "packed_qk_norm_rope",
     "paged_kv_append",
+    "paged_kv_gather",
     "paged_decode_attn",
 ]
 __version__ = "0.1.0"

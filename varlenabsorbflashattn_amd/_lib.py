@@ -52,6 +52,11 @@ class PagedCache(C.Structure):
         ("cache_lens", C.c_void_p), ("n_seq", C.c_int64)]
 
 
+class RowScales(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p)] + [(n, C.c_int64) for n in (
+        "k_page", "k_token", "k_head", "v_page", "v_token", "v_head")]
+
+
 _lib = None
 _lock = threading.Lock()
 
@@ -62,6 +67,8 @@ _PI64 = C.POINTER(C.c_int64)
 _PI32 = C.POINTER(C.c_int32)
 _PINFO = C.POINTER(PlanInfo)
 _PCACHE = C.POINTER(PagedCache)
+_PSCALES = C.POINTER(RowScales)
+_F = C.c_float
 
 _SIGS = {
     "vafa_version": (C.c_char_p, []),
@@ -121,6 +128,16 @@ _SIGS = {
                                               _P, _P, _I64, _P]),
     "vafa_paged_append": (C.c_int, [_PCACHE, _P, _I64, _I64, _P, _I64, _I64, _I64, _P, _P, _I64,
                                     _I64, _I64, _P, _P, _I64, _I32, _I32, _P]),
+    "vafa_paged_store": (C.c_int, [_PCACHE, _PSCALES, _P, _I64, _I64, _P, _I64, _I64, _I64, _P, _P,
+                                   _I64, _I64, _I64, _P, _P, _I64, _I32, _F, _P, _P, _I32, _F,
+                                   _I32, _P]),
+    "vafa_paged_gather": (C.c_int, [_PCACHE, _PSCALES, _P, _P, _I64, _P, _P, _I32, _P]),
+    "vafa_qk_norm_rope_fwd": (C.c_int, [_P, _I64, _I64, _I64, _P, _I64, _I64, _I64, _I64, _I64, _P,
+                                        _P, _I64, _I32, _F, _P, _P, _I32, _F, _P, _P, _I32, _P]),
+    "vafa_qk_norm_rope_bwd_workspace": (C.c_int64, [_I64] * 4),
+    "vafa_qk_norm_rope_bwd": (C.c_int, [_P, _I64, _I64, _I64, _P, _I64, _I64, _I64, _I64, _I64, _P,
+                                        _P, _I64, _I32, _F, _P, _P, _I32, _F] + [_P] * 6 +
+                              [_I32, _P, _I64, _P]),
     "vafa_paged_decode_workspace": (C.c_int64, [_PCACHE, _I64, _I64]),
     "vafa_paged_decode": (C.c_int, [_PCACHE, _P, _I64, _I64, _I64, _P, C.c_float, C.c_float, _I64,
                                     _P, _I32, _P, _I64, _P]),

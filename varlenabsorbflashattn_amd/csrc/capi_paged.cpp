@@ -13,6 +13,7 @@
 
 namespace vafa {
 int fail(int code, const char *fmt, ...);
+int check_head_rows(const char *what, int64_t D, int64_t rot, float eps, float rot_scale);
 
 namespace {
 
@@ -57,6 +58,26 @@ int check_pointers(const char *what, const vafa_paged_cache *c) {
   if (c->n_seq == 0) return VAFA_OK;
   if (int rc = check_given(what, {c->cache_lens})) return rc;
   return c->table_width > 0 ? check_given(what, {c->page_table}) : VAFA_OK;
+}
+
+// The cache and, where it holds codes, their powers of two.
+int check_codes(const char *what, const vafa_paged_cache *c, const vafa_row_scales *s) {
+  if (int rc = check_cache(what, c)) return rc;
+  if (s == nullptr) return VAFA_OK;
+  for (int64_t x : {c->k_page, c->k_token, c->k_head, c->v_page, c->v_token, c->v_head})
+    if (x % 16 != 0)
+      return fail(VAFA_ERR_VALUE, "%s: strides of codes must be multiples of 16, got %lld", what,
+                  (long long)x);
+  for (int64_t x : {s->k_page, s->k_token, s->k_head, s->v_page, s->v_token, s->v_head})
+    if (x < 0)
+      return fail(VAFA_ERR_VALUE, "%s: the scales' strides must not be negative", what);
+  return VAFA_OK;
+}
+
+RowScales scales_of(const vafa_row_scales *s) {
+  if (s == nullptr) return RowScales{};
+  return RowScales{(uint8_t *)s->k, (uint8_t *)s->v, s->k_page, s->k_token, s->k_head,
+                   s->v_page, s->v_token, s->v_head};
 }
 
 int check_dtype(const char *what, int32_t dtype) {
@@ -127,24 +148,12 @@ int plan_decode(const vafa_paged_cache *c, int64_t H, int64_t window, DecodePlan
   return VAFA_OK;
 }
 
-}  // namespace
-}  // namespace vafa
-
-using namespace vafa;
-
-extern "C" {
-
-int vafa_paged_append(const vafa_paged_cache *c, const void *k, int64_t k_token, int64_t k_head,
-                      const void *v, int64_t v_token, int64_t v_head, int64_t T, const int32_t *cu,
-                      const void *q, int64_t q_token, int64_t q_head, int64_t H, void *q_out,
-                      const float *inv_freq, int64_t rot, int32_t interleaved, int32_t dtype,
-                      void *stream) {
-  const char *what = "paged_kv_append";
-  if (int rc = check_dtype(what, dtype)) return rc;
-  if (int rc = check_cache(what, c)) return rc;
-  if (c->D < 8 || c->D > 1024 || c->D % 8 != 0)
-    return fail(VAFA_ERR_ASSERT, "%s: head_dim %lld not supported (multiples of 8 up to 1024)", what,
-                (long long)c->D);
+// The operands of an append, which both kinds of it take.
+int append_args(const char *what, const vafa_paged_cache *c, const void *k, int64_t k_token,
+                int64_t k_head, const void *v, int64_t v_token, int64_t v_head, int64_t T,
+                const int32_t *cu, const void *q, int64_t q_token, int64_t q_head, int64_t H,
+                void *q_out, const float *inv_freq, int64_t rot, int32_t interleaved,
+                AppendArgs *out) {
   if (rot < 0 || rot % 2 != 0 || rot > c->D)
     return fail(VAFA_ERR_VALUE, "%s: %lld rotated features of %lld", what, (long long)rot,
                 (long long)c->D);
@@ -167,7 +176,7 @@ int vafa_paged_append(const vafa_paged_cache *c, const void *k, int64_t k_token,
     if (int rc = check_given(what, {q, q_out})) return rc;
   if (rot > 0)
     if (int rc = check_given(what, {inv_freq})) return rc;
-  AppendArgs a{};
+  AppendArgs &a = *out;
   a.q = q; a.k = k; a.v = v; a.q_out = q_out; a.kc = c->k; a.vc = c->v;
   a.cu = cu; a.lens = c->cache_lens; a.inv_freq = inv_freq;
   a.map = map_of(c);
@@ -177,10 +186,112 @@ int vafa_paged_append(const vafa_paged_cache *c, const void *k, int64_t k_token,
   a.v_page = c->v_page; a.vc_token = c->v_token; a.vc_head = c->v_head;
   a.T = T; a.n_seq = (int)c->n_seq; a.H = (int)H; a.Hk = (int)c->Hk; a.D = (int)c->D;
   a.rot = (int)rot; a.interleaved = interleaved != 0;
+  return VAFA_OK;
+}
+
+}  // namespace
+
+// What norms and rotations of whole rows take, with or without a cache.
+int check_head_rows(const char *what, int64_t D, int64_t rot, float eps, float rot_scale) {
+  if (D != 64 && D != 128 && D != 256)
+    return fail(VAFA_ERR_ASSERT, "%s: head_dim %lld not supported (64, 128, 256)", what,
+                (long long)D);
+  if (rot < 0 || rot % 16 != 0 || rot > D)
+    return fail(VAFA_ERR_VALUE, "%s: %lld rotated features of %lld (multiples of 16)", what,
+                (long long)rot, (long long)D);
+  if (!(eps >= 0.f) || !std::isfinite(eps))
+    return fail(VAFA_ERR_VALUE, "%s: eps must be finite and not negative", what);
+  if (!std::isfinite(rot_scale))
+    return fail(VAFA_ERR_VALUE, "%s: rot_scale must be finite", what);
+  return VAFA_OK;
+}
+
+}  // namespace vafa
+
+using namespace vafa;
+
+extern "C" {
+
+int vafa_paged_append(const vafa_paged_cache *c, const void *k, int64_t k_token, int64_t k_head,
+                      const void *v, int64_t v_token, int64_t v_head, int64_t T, const int32_t *cu,
+                      const void *q, int64_t q_token, int64_t q_head, int64_t H, void *q_out,
+                      const float *inv_freq, int64_t rot, int32_t interleaved, int32_t dtype,
+                      void *stream) {
+  const char *what = "paged_kv_append";
+  if (int rc = check_dtype(what, dtype)) return rc;
+  if (int rc = check_cache(what, c)) return rc;
+  if (c->D < 8 || c->D > 1024 || c->D % 8 != 0)
+    return fail(VAFA_ERR_ASSERT, "%s: head_dim %lld not supported (multiples of 8 up to 1024)", what,
+                (long long)c->D);
+  AppendArgs a{};
+  if (int rc = append_args(what, c, k, k_token, k_head, v, v_token, v_head, T, cu, q, q_token,
+                           q_head, H, q_out, inv_freq, rot, interleaved, &a))
+    return rc;
+  if (T == 0) return VAFA_OK;
   if (dtype == VAFA_BF16)
     launch_paged_append<bf16>(a, (hipStream_t)stream);
   else
     launch_paged_append<f16>(a, (hipStream_t)stream);
+  return check_launch(what);
+}
+
+int vafa_paged_store(const vafa_paged_cache *c, const vafa_row_scales *scales, const void *k,
+                     int64_t k_token, int64_t k_head, const void *v, int64_t v_token,
+                     int64_t v_head, int64_t T, const int32_t *cu, const void *q, int64_t q_token,
+                     int64_t q_head, int64_t H, void *q_out, const float *inv_freq, int64_t rot,
+                     int32_t interleaved, float rot_scale, const void *q_weight,
+                     const void *k_weight, int32_t weights_f32, float eps, int32_t dtype,
+                     void *stream) {
+  const char *what = "paged_kv_append";
+  if (int rc = check_dtype(what, dtype)) return rc;
+  if (int rc = check_codes(what, c, scales)) return rc;
+  if (int rc = check_head_rows(what, c->D, rot, eps, rot_scale)) return rc;
+  HeadRowsArgs s{};
+  if (int rc = append_args(what, c, k, k_token, k_head, v, v_token, v_head, T, cu, q, q_token,
+                           q_head, H, q_out, inv_freq, rot, interleaved, &s.a))
+    return rc;
+  if (T == 0) return VAFA_OK;
+  if (scales != nullptr)
+    if (int rc = check_given(what, {scales->k, scales->v})) return rc;
+  s.scales = scales_of(scales);
+  s.q_weight = q_weight; s.k_weight = k_weight; s.weights_f32 = weights_f32 != 0;
+  s.eps = eps; s.rot_scale = rot_scale;
+  if (dtype == VAFA_BF16)
+    launch_head_rows<bf16>(s, (hipStream_t)stream);
+  else
+    launch_head_rows<f16>(s, (hipStream_t)stream);
+  return check_launch(what);
+}
+
+int vafa_paged_gather(const vafa_paged_cache *c, const vafa_row_scales *scales, const int32_t *cu,
+                      const int32_t *starts, int64_t T, void *k, void *v, int32_t dtype,
+                      void *stream) {
+  const char *what = "paged_kv_gather";
+  if (int rc = check_dtype(what, dtype)) return rc;
+  if (int rc = check_codes(what, c, scales)) return rc;
+  if (c->D < 16 || c->D > 1024 || c->D % 16 != 0)
+    return fail(VAFA_ERR_ASSERT, "%s: head_dim %lld not supported (multiples of 16 up to 1024)",
+                what, (long long)c->D);
+  if (T < 0 || T > INT32_MAX || !grid_ok(T * (2 * c->Hk * (c->D / 16)) / 512 + 1, 256))
+    return fail(VAFA_ERR_VALUE, "%s: %lld rows are too many for a call", what, (long long)T);
+  if (int rc = check_rows(what, "k", k, 0, 0)) return rc;
+  if (int rc = check_rows(what, "v", v, 0, 0)) return rc;
+  if (T == 0) return VAFA_OK;
+  if (int rc = check_given(what, {c->k, c->v, cu, k, v})) return rc;
+  if (c->n_seq > 0 && c->table_width > 0)
+    if (int rc = check_given(what, {c->page_table})) return rc;
+  if (scales != nullptr)
+    if (int rc = check_given(what, {scales->k, scales->v})) return rc;
+  GatherArgs a{};
+  a.kc = c->k; a.vc = c->v; a.scales = scales_of(scales); a.k = k; a.v = v;
+  a.cu = cu; a.starts = starts; a.map = map_of(c);
+  a.k_page = c->k_page; a.kc_token = c->k_token; a.kc_head = c->k_head;
+  a.v_page = c->v_page; a.vc_token = c->v_token; a.vc_head = c->v_head;
+  a.T = T; a.n_seq = (int)c->n_seq; a.Hk = (int)c->Hk; a.D = (int)c->D;
+  if (dtype == VAFA_BF16)
+    launch_paged_gather<bf16>(a, (hipStream_t)stream);
+  else
+    launch_paged_gather<f16>(a, (hipStream_t)stream);
   return check_launch(what);
 }
 

@@ -139,6 +139,52 @@ struct AppendArgs {
   int n_seq, H, Hk, D, rot, interleaved;
 };
 
+// A byte for each row of an 8-bit cache, its power of two (fp8.h); strides in bytes.
+struct RowScales {
+  uint8_t *k, *v;
+  int64_t k_page, k_token, k_head, v_page, v_token, v_head;
+};
+
+// Queries and keys normed and rotated, to a paged cache (values too, all as codes where
+// scales.k is there) or, with kc the keys' rows [T, Hk, D], as packed rows.
+struct HeadRowsArgs {
+  AppendArgs a;
+  RowScales scales;
+  const int32_t *positions;           // packed rows: [T]
+  const void *q_weight, *k_weight;    // [D] or null: not normed
+  int weights_f32;                    // of fp32, not of the rows' type
+  int packed;
+  float eps, rot_scale;
+};
+
+// Backward of packed rows: gradients of q, k and, as partial sums of each block, the weights.
+struct HeadRowsBwdArgs {
+  const void *q, *k, *dq_out, *dk_out;  // the last two contiguous
+  void *dq, *dk;                        // contiguous
+  void *dq_weight, *dk_weight;          // [D] of the weights' type, or null
+  const int32_t *positions;
+  const float *inv_freq;
+  const void *q_weight, *k_weight;
+  float *part;  // [blocks, 2, D]
+  int64_t q_token, q_head, k_token, k_head;
+  int64_t T;
+  int64_t blocks;
+  int H, Hk, D, rot, interleaved, weights_f32;
+  float eps, rot_scale;
+};
+
+// Rows of a paged cache as packed rows [T, Hk, D].
+struct GatherArgs {
+  const void *kc, *vc;
+  RowScales scales;  // of codes, or null
+  void *k, *v;
+  const int32_t *cu, *starts;  // starts: or null (0)
+  PageMap map;
+  int64_t k_page, kc_token, kc_head, v_page, vc_token, vc_head;
+  int64_t T;
+  int n_seq, Hk, D;
+};
+
 // Attention of one new token per sequence over a paged cache.
 struct DecodeArgs {
   const void *q, *kc, *vc;
@@ -222,6 +268,12 @@ void launch_absorb_dax(const AbsorbArgs &, hipStream_t);
 // paged.hip (bf16 / f16)
 template <typename T> void launch_paged_append(const AppendArgs &, hipStream_t);
 template <typename T> void launch_paged_decode(const DecodeArgs &, int D, hipStream_t);
+
+// head_rows.hip (bf16 / f16; D in {64, 128, 256}, gather: multiples of 16)
+template <typename T> void launch_head_rows(const HeadRowsArgs &, hipStream_t);
+int64_t head_rows_bwd_blocks(int64_t T, int64_t heads, int64_t D);
+template <typename T> void launch_head_rows_bwd(const HeadRowsBwdArgs &, hipStream_t);
+template <typename T> void launch_paged_gather(const GatherArgs &, hipStream_t);
 
 // masked_fwd.hip, masked_bwd.hip (bf16 / f16, D in {64, 128, 256})
 template <typename T, int D> void launch_masked_fwd(const MaskedArgs &, hipStream_t);

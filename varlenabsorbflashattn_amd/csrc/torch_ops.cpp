@@ -41,6 +41,8 @@ struct Api {
   X(absorb_project_workspace) X(absorb_project_fwd) X(absorb_project_bwd)                 \
   X(absorb_project_f32_workspace) X(absorb_project_f32_fwd) X(absorb_project_f32_bwd)      \
   X(paged_append) X(paged_decode_workspace) X(paged_decode) X(masked_fwd_workspace)        \
+  X(paged_store) X(paged_gather) X(qk_norm_rope_fwd) X(qk_norm_rope_bwd_workspace)          \
+  X(qk_norm_rope_bwd)                                                                       \
   X(masked_fwd) X(masked_bwd_workspace) X(masked_bwd)
   VAFA_FNS(VAFA_FN)
 #undef VAFA_FN
@@ -284,9 +286,9 @@ int64_t stride_of(const Tensor &t, int64_t dim) { return t.size(dim) > 1 ? t.str
 // dimension (stride 0) holds one element where they would read size of them.
 bool dense(const Tensor &t, int64_t dim) { return t.size(dim) <= 1 || t.stride(dim) == 1; }
 
-bool rows_ok(const Tensor &t) {
+bool rows_ok(const Tensor &t, int64_t step = 8) {
   bool ok = dense(t, t.dim() - 1) && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
-  for (int64_t d = 0; d + 1 < t.dim(); ++d) ok = ok && stride_of(t, d) % 8 == 0;
+  for (int64_t d = 0; d + 1 < t.dim(); ++d) ok = ok && stride_of(t, d) % step == 0;
   return ok;
 }
 
@@ -322,12 +324,32 @@ void on_gpu(const char *what, const Tensor &t) {
   need(t.is_cuda(), what, "requires GPU tensors on one device");
 }
 
-vafa_paged_cache cache_of(const char *what, const Tensor &kc, const Tensor &vc,
-                          const Tensor &table, const Tensor &lens) {
+// A cache as the entry points take it.  With the powers of two of its rows (k_scale and
+// v_scale) it holds codes; `rows` is the type of the rows that go in or come out.
+struct Cache {
+  vafa_paged_cache c{};
+  vafa_row_scales s{};
+  bool codes = false;
+  at::ScalarType rows;
+  const vafa_row_scales *scales() const { return codes ? &s : nullptr; }
+};
+
+Cache cache_of(const char *what, const Tensor &kc, const Tensor &vc, const Tensor &table,
+               const Tensor &lens, const std::optional<Tensor> &ks = std::nullopt,
+               const std::optional<Tensor> &vs = std::nullopt,
+               at::ScalarType rows = at::ScalarType::Undefined) {
   need(kc.dim() == 4 && vc.sizes() == kc.sizes(), what,
        "k_cache and v_cache must be [n_pages, page_size, H_k, D] alike");
+  Cache r;
+  r.codes = ks.has_value();
+  need(ks.has_value() == vs.has_value(), what, "k_scale and v_scale belong together");
   const auto dt = kc.scalar_type();
-  need(dt == at::kHalf || dt == at::kBFloat16, what, "dtype not supported (float16, bfloat16)");
+  r.rows = r.codes ? rows : dt;
+  if (r.codes)
+    need(dt == at::kFloat8_e4m3fn, what, "with k_scale the caches must be float8_e4m3fn");
+  need(dt != at::kFloat8_e4m3fn || r.codes, what, "caches of float8_e4m3fn need k_scale and v_scale");
+  need(r.rows == at::kHalf || r.rows == at::kBFloat16, what,
+       "dtype not supported (float16, bfloat16)");
   need(vc.scalar_type() == dt, what, "k_cache and v_cache must share dtype");
   need(table.dim() == 2 && lens.dim() == 1 && table.size(0) == lens.size(0), what,
        "page_table must be [n_seq, pages] and cache_lens [n_seq]");
@@ -336,18 +358,21 @@ vafa_paged_cache cache_of(const char *what, const Tensor &kc, const Tensor &vc,
   if (!dense(table, 1) || !dense(lens, 0))
     throw py::value_error(std::string(what) +
                           ": the rows of page_table and cache_lens must be contiguous");
-  if (!rows_ok(kc) || !rows_ok(vc))
+  if (!rows_ok(kc, r.codes ? 16 : 8) || !rows_ok(vc, r.codes ? 16 : 8))
     throw py::value_error(std::string(what) +
                           ": the caches must be 16-byte aligned, features contiguous and other "
-                          "strides multiples of 8 elements");
-  for (const Tensor *t : {&kc, &vc})
-    for (int64_t d = 0; d < 4; ++d)
-      if (t->size(d) > 1 && t->stride(d) == 0)
+                          "strides multiples of " + (r.codes ? "16" : "8") + " elements");
+  auto not_expanded = [&](const Tensor &t) {
+    for (int64_t d = 0; d < t.dim(); ++d)
+      if (t.size(d) > 1 && t.stride(d) == 0)
         throw py::value_error(std::string(what) + ": the caches must not be expanded views");
+  };
+  not_expanded(kc);
+  not_expanded(vc);
   need(vc.device() == kc.device() && table.device() == kc.device() &&
            lens.device() == kc.device(),
        what, "requires GPU tensors on one device");
-  vafa_paged_cache c{};
+  vafa_paged_cache &c = r.c;
   c.k = kc.data_ptr(); c.v = vc.data_ptr();
   c.n_pages = kc.size(0); c.page_size = kc.size(1); c.Hk = kc.size(2); c.D = kc.size(3);
   c.k_page = stride_of(kc, 0); c.k_token = stride_of(kc, 1); c.k_head = stride_of(kc, 2);
@@ -355,29 +380,89 @@ vafa_paged_cache cache_of(const char *what, const Tensor &kc, const Tensor &vc,
   c.page_table = table.data_ptr<int32_t>();
   c.table_stride = stride_of(table, 0); c.table_width = table.size(1);
   c.cache_lens = lens.data_ptr<int32_t>(); c.n_seq = lens.size(0);
-  return c;
+  if (r.codes) {
+    for (const Tensor *t : {&*ks, &*vs}) {
+      need(t->scalar_type() == at::kFloat8_e8m0fnu && t->device() == kc.device(), what,
+           "k_scale and v_scale must be float8_e8m0fnu on the cache's device");
+      need(t->dim() == 3 && t->sizes() == kc.sizes().slice(0, 3), what,
+           "k_scale and v_scale must be [n_pages, page_size, H_k]");
+      not_expanded(*t);
+    }
+    r.s.k = ks->data_ptr(); r.s.v = vs->data_ptr();
+    r.s.k_page = stride_of(*ks, 0); r.s.k_token = stride_of(*ks, 1); r.s.k_head = stride_of(*ks, 2);
+    r.s.v_page = stride_of(*vs, 0); r.s.v_token = stride_of(*vs, 1); r.s.v_head = stride_of(*vs, 2);
+  }
+  return r;
 }
 
-// [T, heads, D] of the cache's type and device.
-void check_tokens(const char *what, const char *name, const Tensor &t, const Tensor &kc) {
+// [T, heads, D] of the rows' type and the cache's device.
+void check_tokens(const char *what, const char *name, const Tensor &t, const Tensor &kc,
+                  at::ScalarType rows) {
   if (t.dim() != 3 || t.size(2) != kc.size(3))
     throw AssertionFailed(std::string(what) + ": " + name + " must be [T, heads, " +
                           std::to_string(kc.size(3)) + "]");
-  if (t.scalar_type() != kc.scalar_type() || t.device() != kc.device())
+  if (t.scalar_type() != rows || t.device() != kc.device())
     throw AssertionFailed(std::string(what) + ": " + name +
                           " must have the cache's dtype and device");
 }
 
-std::optional<Tensor> paged_append(const Tensor &k_in, const Tensor &v_in, const Tensor &kc,
-                                   const Tensor &vc, const Tensor &table, const Tensor &lens,
-                                   const std::optional<Tensor> &cu,
-                                   const std::optional<Tensor> &q_in,
-                                   const std::optional<Tensor> &inv_freq, bool interleaved) {
+// An int32 tensor [n] on the device, its elements beside each other.
+const int32_t *ints_of(const char *what, const char *name, const Tensor &t, int64_t n,
+                       const Tensor &like) {
+  if (t.dim() != 1 || t.size(0) != n)
+    throw AssertionFailed(std::string(what) + ": " + name + " must be [" + std::to_string(n) + "]");
+  if (t.scalar_type() != at::kInt || t.device() != like.device())
+    throw AssertionFailed(std::string(what) + ": " + name + " must be int32 on the operands' device");
+  if (!dense(t, 0)) throw py::value_error(std::string(what) + ": " + name + " must be contiguous");
+  return t.data_ptr<int32_t>();
+}
+
+// Rotated features of inv_freq.
+int64_t rot_of(const char *what, const std::optional<Tensor> &inv_freq, int64_t D,
+               const Tensor &like) {
+  if (!inv_freq) return 0;
+  need(inv_freq->dim() == 1 && 2 * inv_freq->size(0) <= D, what,
+       "inv_freq must be [rotated features / 2]");
+  need(inv_freq->scalar_type() == at::kFloat && inv_freq->device() == like.device(), what,
+       "inv_freq must be float32 on the cache's device");
+  if (!dense(*inv_freq, 0))
+    throw py::value_error(std::string(what) + ": inv_freq must be contiguous");
+  return 2 * inv_freq->size(0);
+}
+
+// Weights of the norms: [D] each, both of fp32 or of the rows' type; true for fp32.
+bool weights_of(const char *what, const std::optional<Tensor> &qw, const std::optional<Tensor> &kw,
+                int64_t D, at::ScalarType rows, const Tensor &like) {
+  for (const auto *w : {&qw, &kw}) {
+    if (!*w) continue;
+    const Tensor &t = **w;
+    need(t.dim() == 1 && t.size(0) == D, what, "q_weight and k_weight must be [D]");
+    need((t.scalar_type() == at::kFloat || t.scalar_type() == rows) && t.device() == like.device(),
+         what, "q_weight and k_weight must be float32 or of the rows' dtype, on their device");
+    need(!qw || !kw || qw->scalar_type() == kw->scalar_type(), what,
+         "q_weight and k_weight must share dtype");
+    if (!dense(t, 0))
+      throw py::value_error(std::string(what) + ": q_weight and k_weight must be contiguous");
+  }
+  const auto &w = qw ? qw : kw;
+  return w && w->scalar_type() == at::kFloat;
+}
+
+const void *opt_ptr(const std::optional<Tensor> &t) { return t ? t->data_ptr() : nullptr; }
+
+std::optional<Tensor> paged_append(
+    const Tensor &k_in, const Tensor &v_in, const Tensor &kc, const Tensor &vc, const Tensor &table,
+    const Tensor &lens, const std::optional<Tensor> &cu, const std::optional<Tensor> &q_in,
+    const std::optional<Tensor> &inv_freq, bool interleaved, const std::optional<Tensor> &ks,
+    const std::optional<Tensor> &vs, const std::optional<Tensor> &qw,
+    const std::optional<Tensor> &kw, double eps, double rot_scale) {
   const char *what = "paged_kv_append";
-  no_grad_only(what, {k_in, v_in, kc, vc, q_in.value_or(Tensor()), inv_freq.value_or(Tensor())});
-  const vafa_paged_cache c = cache_of(what, kc, vc, table, lens);
-  check_tokens(what, "k", k_in, kc);
-  check_tokens(what, "v", v_in, kc);
+  no_grad_only(what, {k_in, v_in, kc, vc, q_in.value_or(Tensor()), inv_freq.value_or(Tensor()),
+                      qw.value_or(Tensor()), kw.value_or(Tensor())});
+  const Cache cache = cache_of(what, kc, vc, table, lens, ks, vs, k_in.scalar_type());
+  const vafa_paged_cache &c = cache.c;
+  check_tokens(what, "k", k_in, kc, cache.rows);
+  check_tokens(what, "v", v_in, kc, cache.rows);
   need(k_in.size(1) == c.Hk && v_in.sizes() == k_in.sizes(), what,
        "k and v must be [T, H_k, D] with the cache's heads");
   const int64_t T = k_in.size(0);
@@ -390,38 +475,67 @@ std::optional<Tensor> paged_append(const Tensor &k_in, const Tensor &v_in, const
   } else {
     need(T == c.n_seq, what, "without cu_seqlens there must be one token per sequence");
   }
-  int64_t rot = 0;
-  if (inv_freq) {
-    need(inv_freq->dim() == 1 && 2 * inv_freq->size(0) <= c.D, what,
-         "inv_freq must be [rotated features / 2]");
-    need(inv_freq->scalar_type() == at::kFloat && inv_freq->device() == kc.device(), what,
-         "inv_freq must be float32 on the cache's device");
-    if (!dense(*inv_freq, 0))
-      throw py::value_error(std::string(what) + ": inv_freq must be contiguous");
-    rot = 2 * inv_freq->size(0);
-  }
+  const int64_t rot = rot_of(what, inv_freq, c.D, kc);
+  const bool w_f32 = weights_of(what, qw, kw, c.D, cache.rows, kc);
+  need(!qw || q_in, what, "q_weight needs q");
+  if (!inv_freq && rot_scale != 1.0)
+    throw py::value_error(std::string(what) + ": rot_scale belongs to inv_freq");
   int64_t H = 0;
   if (q_in) {
-    check_tokens(what, "q", *q_in, kc);
+    check_tokens(what, "q", *q_in, kc, cache.rows);
     need(q_in->size(0) == T, what, "q must have as many tokens as k");
     H = q_in->size(1);
   }
   on_gpu(what, kc);
-  Call call(kc);
+  Call call(k_in);
   const Tensor k = rows_in(k_in), v = rows_in(v_in);
   Tensor q, out;
   if (q_in) {
     q = rows_in(*q_in);
     out = call.empty({T, H, c.D});
   }
-  check(api.paged_append(&c, ptr(k), stride_of(k, 0), stride_of(k, 1), ptr(v), stride_of(v, 0),
-                         stride_of(v, 1), T, cu ? cu->data_ptr<int32_t>() : nullptr, ptr(q),
-                         q_in ? stride_of(q, 0) : 0, q_in ? stride_of(q, 1) : 0, H, ptr(out),
-                         inv_freq ? f32(*inv_freq) : nullptr, rot, interleaved, dtype_of(kc),
-                         call.stream));
-  for (const Tensor *t : {&kc, &vc})
-    if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+  const int64_t q_token = q_in ? stride_of(q, 0) : 0, q_head = q_in ? stride_of(q, 1) : 0;
+  const int32_t *cu_ptr = cu ? cu->data_ptr<int32_t>() : nullptr;
+  const float *freq = inv_freq ? f32(*inv_freq) : nullptr;
+  if (cache.codes || qw || kw || rot_scale != 1.0)
+    check(api.paged_store(&c, cache.scales(), ptr(k), stride_of(k, 0), stride_of(k, 1), ptr(v),
+                          stride_of(v, 0), stride_of(v, 1), T, cu_ptr, ptr(q), q_token, q_head, H,
+                          ptr(out), freq, rot, interleaved, (float)rot_scale, opt_ptr(qw),
+                          opt_ptr(kw), w_f32, (float)eps, dtype_of(k), call.stream));
+  else
+    check(api.paged_append(&c, ptr(k), stride_of(k, 0), stride_of(k, 1), ptr(v), stride_of(v, 0),
+                           stride_of(v, 1), T, cu_ptr, ptr(q), q_token, q_head, H, ptr(out), freq,
+                           rot, interleaved, dtype_of(k), call.stream));
+  for (const Tensor &t : {kc, vc, ks.value_or(Tensor()), vs.value_or(Tensor())})
+    if (t.defined() && !t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
   return q_in ? std::optional<Tensor>(out) : std::nullopt;
+}
+
+std::tuple<Tensor, Tensor> paged_gather(const Tensor &kc, const Tensor &vc, const Tensor &table,
+                                        const Tensor &cu, int64_t total,
+                                        const std::optional<Tensor> &starts,
+                                        const std::optional<Tensor> &ks,
+                                        const std::optional<Tensor> &vs,
+                                        std::optional<at::ScalarType> dtype) {
+  const char *what = "paged_kv_gather";
+  no_grad_only(what, {kc, vc});
+  need(table.dim() == 2 && cu.dim() == 1 && cu.size(0) == table.size(0) + 1, what,
+       "page_table must be [n_seq, pages] and cu_seqlens [n_seq + 1]");
+  if (total < 0) throw py::value_error(std::string(what) + ": total must not be negative");
+  need(!ks || dtype, what, "caches of codes need the dtype of the result");
+  // (cache_lens has no part in it: the n_seq first entries of cu_seqlens stand in)
+  const Cache cache = cache_of(what, kc, vc, table, cu.slice(0, 0, table.size(0)), ks, vs,
+                               dtype.value_or(kc.scalar_type()));
+  need(!dtype || *dtype == cache.rows, what, "a 16-bit cache comes back in its dtype");
+  const int32_t *cu_ptr = ints_of(what, "cu_seqlens", cu, table.size(0) + 1, kc);
+  const int32_t *from = starts ? ints_of(what, "starts", *starts, table.size(0), kc) : nullptr;
+  on_gpu(what, kc);
+  Call call(kc);
+  const auto opt = kc.options().dtype(cache.rows);
+  Tensor k = at::empty({total, cache.c.Hk, cache.c.D}, opt), v = at::empty_like(k);
+  check(api.paged_gather(&cache.c, cache.scales(), cu_ptr, from, total, ptr(k), ptr(v),
+                         dtype_of(k), call.stream));
+  return {k, v};
 }
 
 // slopes [H] of the distance bias, float32 on q's device.
@@ -445,8 +559,9 @@ Tensor paged_decode(const Tensor &q_in, const Tensor &kc, const Tensor &vc, cons
   if (softcap && !(*softcap > 0 && (float)*softcap > 0.f))
     throw py::value_error("softcap must be positive");
   if (window && *window < 1) throw py::value_error("window must be positive");
-  const vafa_paged_cache c = cache_of(what, kc, vc, table, lens);
-  check_tokens(what, "q", q_in, kc);
+  const Cache cache = cache_of(what, kc, vc, table, lens);
+  const vafa_paged_cache &c = cache.c;
+  check_tokens(what, "q", q_in, kc, cache.rows);
   need(q_in.size(0) == c.n_seq, what, "q must hold one token per sequence");
   const int64_t H = q_in.size(1);
   const float *sl = slopes_of(what, slopes, H, q_in);
@@ -606,6 +721,125 @@ Tensor masked_attn(const Tensor &q, const Tensor &k, const Tensor &v, const Plan
   return std::get<0>(masked_fwd(q, k, v, p, scale, softcap, window, slopes, false));
 }
 
+// ---- norms of queries and keys with the position rotation --------------------------
+
+struct RowsOptions {
+  int64_t rot;
+  bool interleaved, w_f32;
+  double eps, rot_scale;
+};
+
+std::tuple<Tensor, Tensor> norm_rope_fwd(const Tensor &q, const Tensor &k, const Tensor &pos,
+                                         const Tensor &freq, const Tensor &qw, const Tensor &kw,
+                                         const RowsOptions &o) {
+  Call c(q);
+  const int64_t T = q.size(0), H = q.size(1), Hk = k.size(1), D = q.size(2);
+  Tensor yq = c.empty({T, H, D}), yk = c.empty({T, Hk, D});
+  check(api.qk_norm_rope_fwd(ptr(q), stride_of(q, 0), stride_of(q, 1), H, ptr(k), stride_of(k, 0),
+                             stride_of(k, 1), Hk, T, D, (const int32_t *)ptr(pos), f32(freq), o.rot,
+                             o.interleaved, (float)o.rot_scale, ptr(qw), ptr(kw), o.w_f32,
+                             (float)o.eps, ptr(yq), ptr(yk), dtype_of(q), c.stream));
+  return {yq, yk};
+}
+
+struct QkNormRope : torch::autograd::Function<QkNormRope> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext *ctx,
+                                                const Tensor &q, const Tensor &k,
+                                                const std::optional<Tensor> &qw_in,
+                                                const std::optional<Tensor> &kw_in,
+                                                const std::optional<Tensor> &pos_in,
+                                                const std::optional<Tensor> &freq_in,
+                                                const RowsOptions &o) {
+    const Tensor qw = qw_in.value_or(Tensor()), kw = kw_in.value_or(Tensor()),
+                 pos = pos_in.value_or(Tensor()), freq = freq_in.value_or(Tensor());
+    auto [yq, yk] = norm_rope_fwd(q, k, pos, freq, qw, kw, o);
+    ctx->save_for_backward({q, k, qw, kw, pos, freq});
+    ctx->saved_data["need_qw"] = qw.defined() && qw.requires_grad();
+    ctx->saved_data["need_kw"] = kw.defined() && kw.requires_grad();
+    ctx->saved_data["rot"] = o.rot;
+    ctx->saved_data["interleaved"] = o.interleaved;
+    ctx->saved_data["w_f32"] = o.w_f32;
+    ctx->saved_data["eps"] = o.eps;
+    ctx->saved_data["rot_scale"] = o.rot_scale;
+    return {yq, yk};
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx,
+                                                 torch::autograd::variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &q = saved[0], &k = saved[1], &qw = saved[2], &kw = saved[3];
+    Call c(q);
+    const int64_t T = q.size(0), H = q.size(1), Hk = k.size(1), D = q.size(2);
+    auto dense_grad = [&](const Tensor &g, const Tensor &x) {
+      return g.defined() ? grad_in(g, q) : at::zeros(x.sizes(), q.options());
+    };
+    const Tensor gq = dense_grad(grads[0], q), gk = dense_grad(grads[1], k);
+    Tensor dq = c.empty({T, H, D}), dk = c.empty({T, Hk, D}), dqw, dkw;
+    if (ctx->saved_data["need_qw"].toBool()) dqw = at::empty({D}, qw.options());
+    if (ctx->saved_data["need_kw"].toBool()) dkw = at::empty({D}, kw.options());
+    void *ws = dqw.defined() || dkw.defined()
+                   ? c.workspace(api.qk_norm_rope_bwd_workspace(T, H, Hk, D)) : nullptr;
+    check(api.qk_norm_rope_bwd(
+        ptr(q), stride_of(q, 0), stride_of(q, 1), H, ptr(k), stride_of(k, 0), stride_of(k, 1), Hk,
+        T, D, (const int32_t *)ptr(saved[4]), f32(saved[5]), ctx->saved_data["rot"].toInt(),
+        ctx->saved_data["interleaved"].toBool(), (float)ctx->saved_data["rot_scale"].toDouble(),
+        ptr(qw), ptr(kw), ctx->saved_data["w_f32"].toBool(),
+        (float)ctx->saved_data["eps"].toDouble(), ptr(gq), ptr(gk), ptr(dq), ptr(dk), ptr(dqw),
+        ptr(dkw), dtype_of(q), ws, c.ws_bytes(), c.stream));
+    if (at::GradMode::is_enabled()) {  // create_graph: the gradients depend on these
+      const auto no_second = std::make_shared<torch::autograd::Error>(
+          "packed_qk_norm_rope has no second derivative",
+          torch::autograd::collect_next_edges(q, k, qw, kw, grads[0], grads[1]));
+      for (Tensor *t : {&dq, &dk, &dqw, &dkw})
+        if (t->defined()) torch::autograd::set_history(*t, no_second);
+    }
+    return {dq, dk, dqw, dkw, Tensor(), Tensor(), Tensor()};
+  }
+};
+
+std::tuple<Tensor, Tensor> qk_norm_rope(const Tensor &q_in, const Tensor &k_in,
+                                        const std::optional<Tensor> &positions,
+                                        const std::optional<Tensor> &inv_freq, bool interleaved,
+                                        const std::optional<Tensor> &qw,
+                                        const std::optional<Tensor> &kw, double eps,
+                                        double rot_scale) {
+  const char *what = "packed_qk_norm_rope";
+  direct_only(what, {q_in, k_in, inv_freq.value_or(Tensor()), qw.value_or(Tensor()),
+                     kw.value_or(Tensor())});
+  // [T, heads, D] in a layout that the kernels read; a copy stays in the autograd graph
+  auto rows = [&](const Tensor &x, const char *name) {
+    if (x.dim() != 3 && x.dim() != 4)
+      throw py::value_error(std::string(name) + ": expected 3-D [T,H,D] or 4-D [1,T,H,D], got " +
+                            std::to_string(x.dim()) + "-D");
+    if (x.dim() == 4 && x.size(0) != 1)
+      throw py::value_error(std::string(name) + ": 4-D input must have batch=1 (packed varlen)");
+    return rows_in(x.dim() == 4 ? x.squeeze(0) : x);
+  };
+  const Tensor q = rows(q_in, "q"), k = rows(k_in, "k");
+  const int64_t T = q.size(0), D = q.size(2);
+  const auto dt = q.scalar_type();
+  need(k.size(0) == T && k.size(2) == D, what, "q and k must be [T, H, D] and [T, H_k, D]");
+  need(k.scalar_type() == dt, what, "q and k must share dtype");
+  need(dt == at::kHalf || dt == at::kBFloat16, what, "dtype not supported (float16, bfloat16)");
+  const int64_t rot = rot_of(what, inv_freq, D, q);
+  need(rot == 0 || positions, what, "inv_freq needs positions");
+  if (positions) ints_of(what, "positions", *positions, T, q);
+  if (!inv_freq && rot_scale != 1.0)
+    throw py::value_error(std::string(what) + ": rot_scale belongs to inv_freq");
+  const RowsOptions o{rot, interleaved, weights_of(what, qw, kw, D, dt, q), eps, rot_scale};
+  const bool grad = at::GradMode::is_enabled();
+  if (grad && inv_freq && inv_freq->requires_grad())
+    throw py::value_error(std::string(what) + ": inv_freq gets no gradient: detach it");
+  need(k.device() == q.device(), what, "requires GPU tensors on one device");
+  on_gpu(what, q);
+  auto wants = [&](const std::optional<Tensor> &t) { return t && t->requires_grad(); };
+  if (grad && (wants(q) || wants(k) || wants(qw) || wants(kw))) {
+    auto y = QkNormRope::apply(q, k, qw, kw, positions, inv_freq, o);
+    return {y[0], y[1]};
+  }
+  return norm_rope_fwd(q, k, positions.value_or(Tensor()), inv_freq.value_or(Tensor()),
+                       qw.value_or(Tensor()), kw.value_or(Tensor()), o);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -635,5 +869,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("masked_operands", &masked_operands, no_gil);
   m.def("masked_attn", &masked_attn, no_gil);
   m.def("paged_append", &paged_append, no_gil);
+  m.def("paged_gather", &paged_gather, no_gil);
+  m.def("qk_norm_rope", &qk_norm_rope, no_gil);
   m.def("paged_decode", &paged_decode, no_gil);
 }

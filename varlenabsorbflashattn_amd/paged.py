@@ -1,9 +1,11 @@
-"""A paged key-value cache: appending tokens with the position rotation, and the
-attention of one new token per sequence over the cache.
+"""A paged key-value cache: appending tokens with the position rotation, reading them
+back, and the attention of one new token per sequence over the cache.
 
 The caches are ``[n_pages, page_size, H_k, D]`` (bf16 or fp16), features contiguous and
 other strides any multiple of 8 elements, so views of a joint or head-major allocation
-serve too.  Token ``p`` of sequence ``b`` lies in page ``page_table[b, p // page_size]``
+serve too.  In 8 bits they are ``float8_e4m3fn`` (strides multiples of 16) beside
+``k_scale`` and ``v_scale`` ``[n_pages, page_size, H_k]`` of ``float8_e8m0fnu``: a row (one
+token and key head) is its codes times its power of two.  Token ``p`` of sequence ``b`` lies in page ``page_table[b, p // page_size]``
 at ``p % page_size``.  ``page_table`` and the lengths are int32 tensors on the GPU and
 stay there: no call waits for the GPU, all of them can be captured into a graph and
 replayed with other lengths and pages in the same tensors.  As the host never sees them,
@@ -13,7 +15,7 @@ neither stored nor read.  There is no counterpart in the reference, which has no
 from __future__ import annotations
 
 import math
-from typing import Optional
+from typing import Optional, Tuple
 
 import torch
 
@@ -32,6 +34,12 @@ def paged_kv_append(
     q: Optional[torch.Tensor] = None,
     inv_freq: Optional[torch.Tensor] = None,
     interleaved: bool = False,
+    k_scale: Optional[torch.Tensor] = None,
+    v_scale: Optional[torch.Tensor] = None,
+    q_weight: Optional[torch.Tensor] = None,
+    k_weight: Optional[torch.Tensor] = None,
+    eps: float = 1e-6,
+    rot_scale: float = 1.0,
 ) -> Optional[torch.Tensor]:
     """Appends packed keys and values ``[T, H_k, D]`` to the caches, in place.
 
@@ -45,9 +53,46 @@ def paged_kv_append(
     the result are zeros.  Of two tokens that share a place in the cache, each 16 bytes
     there are of either.  D: multiples of 8 up to 1024.
     Forward only.
+
+    With ``k_scale`` and ``v_scale`` the rows are stored in 8 bits: a row's power of two is
+    the least 2^e with max |x| <= 448 * 2^e (0 for a row of zeros), and x becomes the e4m3
+    number nearest to x / 2^e, halves to even.  Keys are rounded once, from 32 bits.  In the
+    last binade of the type of k and v, where a code would stand for more than the type
+    holds, values end at 240 * 2^8 (fp16) or 240 * 2^120 (bf16); infinities and NaN become NaN.
+    With ``q_weight`` and ``k_weight`` rows of q and k are normed before they turn, and with
+    ``rot_scale`` turned features are scaled, as by :func:`packed_qk_norm_rope`.  These options
+    take D 64, 128 or 256 and a multiple of 16 rotated features.  Of two tokens that share a
+    place in an 8-bit cache, codes and power of two may then not belong together.
     """
     return _lib.ops().paged_append(k, v, k_cache, v_cache, page_table, cache_lens, cu_seqlens, q,
-                                   inv_freq, bool(interleaved))
+                                   inv_freq, bool(interleaved), k_scale, v_scale, q_weight,
+                                   k_weight, eps, rot_scale)
+
+
+def paged_kv_gather(
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    page_table: torch.Tensor,
+    cu_seqlens: torch.Tensor,
+    total: int,
+    *,
+    starts: Optional[torch.Tensor] = None,
+    k_scale: Optional[torch.Tensor] = None,
+    v_scale: Optional[torch.Tensor] = None,
+    dtype: Optional[torch.dtype] = None,
+) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Keys and values of the caches as packed rows ``[total, H_k, D]``, for instance for
+    :func:`packed_masked_attn`.
+
+    Row ``t`` of sequence ``b`` (``cu_seqlens[b] <= t < cu_seqlens[b + 1]``, int32 on the GPU)
+    is its token ``starts[b] + t - cu_seqlens[b]`` (``starts``: int32, default 0); rows of no
+    sequence and tokens without a page are zeros.  An 8-bit cache takes its scales and the
+    ``dtype`` of the result, bf16 or fp16 (fp16 where the rows came from fp16: it rounds
+    values below its smallest step and overflows beyond its largest).  D: multiples of 16
+    up to 1024.  Forward only.
+    """
+    return _lib.ops().paged_gather(k_cache, v_cache, page_table, cu_seqlens, int(total), starts,
+                                   k_scale, v_scale, dtype)
 
 
 def paged_decode_attn(
