@@ -460,6 +460,13 @@ typedef struct vafa_row_scales {
   int64_t v_page, v_token, v_head;
 } vafa_row_scales;
 
+/* vafa_paged_decode over codes (scales NULL: over 16 bits); its workspace. */
+VAFA_API int vafa_paged_decode_codes(const vafa_paged_cache *cache, const vafa_row_scales *scales,
+                                     const void *q, int64_t q_token, int64_t q_head, int64_t H,
+                                     void *out, float scale, float softcap, int64_t window,
+                                     const float *slopes, int32_t dtype, void *workspace,
+                                     int64_t workspace_bytes, void *stream);
+
 /* vafa_paged_append (D in {64, 128, 256}, rot a multiple of 16) of normed rows, into 16 bits
  * or, with scales, codes: rows of q and k become R(x r w), r = 1 / sqrt(mean x^2 + eps), w =
  * q_weight / k_weight [D] (NULL: not normed; fp32 where weights_f32, else of dtype), before

@@ -304,10 +304,20 @@ int vafa_paged_decode(const vafa_paged_cache *c, const void *q, int64_t q_token,
                       int64_t H, void *out, float scale, float softcap, int64_t window,
                       const float *slopes, int32_t dtype, void *workspace, int64_t workspace_bytes,
                       void *stream) {
+  return vafa_paged_decode_codes(c, nullptr, q, q_token, q_head, H, out, scale, softcap, window,
+                                 slopes, dtype, workspace, workspace_bytes, stream);
+}
+
+int vafa_paged_decode_codes(const vafa_paged_cache *c, const vafa_row_scales *scales,
+                            const void *q, int64_t q_token, int64_t q_head, int64_t H, void *out,
+                            float scale, float softcap, int64_t window, const float *slopes,
+                            int32_t dtype, void *workspace, int64_t workspace_bytes,
+                            void *stream) {
   const char *what = "paged_decode_attn";
   if (int rc = check_dtype(what, dtype)) return rc;
   DecodePlan p;
   if (int rc = plan_decode(c, H, window, &p)) return rc;
+  if (int rc = check_codes(what, c, scales)) return rc;
   if (!std::isfinite(scale * kLog2e))
     return fail(VAFA_ERR_VALUE, "%s: scale must be finite", what);
   if (!softcap_ok(softcap))
@@ -324,7 +334,10 @@ int vafa_paged_decode(const vafa_paged_cache *c, const void *q, int64_t q_token,
   if (c->n_seq == 0) return VAFA_OK;
   if (int rc = check_pointers(what, c)) return rc;
   if (int rc = check_given(what, {q, out})) return rc;
+  if (scales != nullptr)
+    if (int rc = check_given(what, {scales->k, scales->v})) return rc;
   DecodeArgs a{};
+  a.scales = scales_of(scales);
   a.q = q; a.kc = c->k; a.vc = c->v; a.out = out; a.lens = c->cache_lens; a.slopes = slopes;
   a.part_o = (float *)workspace;
   a.part_ml = (float *)((char *)workspace + p.ml_off);

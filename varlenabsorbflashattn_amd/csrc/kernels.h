@@ -195,6 +195,7 @@ struct DecodeArgs {
   PageMap map;
   int64_t q_token, q_head;
   int64_t k_page, kc_token, kc_head, v_page, vc_token, vc_head;
+  RowScales scales;  // of codes, or null
   int64_t capacity;  // tokens of a sequence's pages
   int n_seq, H, G, pairs, head_blocks, window;  // window 0: all keys
   int chunks;  // parts of the axis of all sequences' tiles

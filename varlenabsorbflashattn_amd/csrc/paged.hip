@@ -1,7 +1,9 @@
 // Paged key-value cache: appending keys and values with the position rotation,
 // and the attention of one new token over the cache.
 #include <algorithm>
+#include <type_traits>
 
+#include "fp8.h"
 #include "kernels.h"
 #include "mfma.h"
 #include "paged.h"
@@ -276,13 +278,16 @@ __device__ __forceinline__ void find_seq(const DecodeArgs &a, int at, int lane, 
   *base = before;
 }
 
-template <typename T, int D>
+// kCodes: rows of 8-bit codes, which become T on the way into LDS.
+template <typename T, int D, bool kCodes>
 __global__ __launch_bounds__(256, D >= 128 ? 2 : 3) void paged_decode_kernel(DecodeArgs a) {
+  using E = std::conditional_t<kCodes, uint8_t, T>;  // of the cache
   using M = Mfma16<T>;
   using S = DecodeSmem<D>;
   using v8 = typename Mfma<T>::v8;
   constexpr int NC = D / 32, ND = D / 16;
-  constexpr int kLanes = D / 8, kRows = 64 / kLanes;  // of a row, and rows of an instruction
+  constexpr int kPiece = 16 / (int)sizeof(E);         // features of 16 bytes
+  constexpr int kLanes = D / kPiece, kRows = 64 / kLanes;  // of a row, and rows of an instruction
   constexpr int KG = S::kGroups, NI = S::kRows / kRows;  // instructions of a step's K rows
   constexpr int kSteps = 2 / KG;                         // of a tile
   extern __shared__ __align__(16) unsigned char smem[];
@@ -328,8 +333,8 @@ __global__ __launch_bounds__(256, D >= 128 ? 2 : 3) void paged_decode_kernel(Dec
     const int t0 = cur - base;
     const int run = end - cur < nt - t0 ? end - cur : nt - t0;
     const int lo = len - decode_seen(len, a.window);
-    const T *kc = (const T *)a.kc + hk * a.kc_head + lane % kLanes * 8;
-    const T *vc = (const T *)a.vc + hk * a.vc_head + lane % kLanes * 8;
+    const E *kc = (const E *)a.kc + hk * a.kc_head + lane % kLanes * kPiece;
+    const E *vc = (const E *)a.vc + hk * a.vc_head + lane % kLanes * kPiece;
 
     v8 qf[NC];
     {
@@ -366,6 +371,7 @@ __global__ __launch_bounds__(256, D >= 128 ? 2 : 3) void paged_decode_kernel(Dec
     // the step's rows of K and V by whole rows: instruction i takes the rows i * kRows +
     // lane / kLanes, whose places the lanes that looked them up hand over
     u32x4 kr[NI], vr[NI];
+    uint32_t ke[NI], ve[NI];  // kCodes: their powers of two
     auto load = [&](const Keys &k) {
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
@@ -377,6 +383,12 @@ __global__ __launch_bounds__(256, D >= 128 ? 2 : 3) void paged_decode_kernel(Dec
         const int64_t vo = id >= 0 ? id * a.v_page + slot * a.vc_token : 0;
         kr[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(kc + ko));
         vr[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(vc + vo));
+        if constexpr (kCodes) {
+          const RowScales &s = a.scales;
+          const int64_t p = id >= 0 ? id : 0, t = id >= 0 ? slot : 0;
+          ke[i] = s.k[p * s.k_page + t * s.k_token + hk * s.k_head];
+          ve[i] = s.v[p * s.v_page + t * s.v_token + hk * s.v_head];
+        }
       }
     };
 
@@ -399,13 +411,26 @@ __global__ __launch_bounds__(256, D >= 128 ? 2 : 3) void paged_decode_kernel(Dec
         // their zero probabilities do not meet infinities
 #pragma unroll
         for (int i = 0; i < NI; ++i)
-          if (!(ok >> (i * kRows + lane / kLanes) & 1)) vr[i] = u32x4{0, 0, 0, 0};
+          if (!(ok >> (i * kRows + lane / kLanes) & 1)) {
+            vr[i] = u32x4{0, 0, 0, 0};
+            if constexpr (kCodes) ve[i] = 127;
+          }
       }
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
-        const int at = (i * kRows + lane / kLanes) * S::kVS + lane % kLanes * 8;
-        *reinterpret_cast<u32x4 *>(ks + at) = kr[i];
-        *reinterpret_cast<u32x4 *>(vs + at) = vr[i];
+        const int at = (i * kRows + lane / kLanes) * S::kVS + lane % kLanes * kPiece;
+        if constexpr (kCodes) {
+          u32x4 lo, hi;
+          from_codes<T>(kr[i], row_scale(ke[i]), lo, hi);
+          *reinterpret_cast<u32x4 *>(ks + at) = lo;
+          *reinterpret_cast<u32x4 *>(ks + at + 8) = hi;
+          from_codes<T>(vr[i], row_scale(ve[i]), lo, hi);
+          *reinterpret_cast<u32x4 *>(vs + at) = lo;
+          *reinterpret_cast<u32x4 *>(vs + at + 8) = hi;
+        } else {
+          *reinterpret_cast<u32x4 *>(ks + at) = kr[i];
+          *reinterpret_cast<u32x4 *>(vs + at) = vr[i];
+        }
       }
       now = next;
       if (u + 1 < u1) {
@@ -586,15 +611,23 @@ __global__ __launch_bounds__(256) void paged_decode_join_kernel(DecodeArgs a) {
   }
 }
 
-template <typename T, int D>
+template <typename T, int D, bool kCodes>
 void launch_decode_d(const DecodeArgs &a, hipStream_t st) {
   const int smem = DecodeSmem<D>::kBytes;
-  allow_dynamic_lds(reinterpret_cast<const void *>(&paged_decode_kernel<T, D>), smem);
+  allow_dynamic_lds(reinterpret_cast<const void *>(&paged_decode_kernel<T, D, kCodes>), smem);
   const int64_t wgs = (int64_t)(a.chunks + kXcds - 1) / kXcds * kXcds * a.pairs;
-  hipLaunchKernelGGL((paged_decode_kernel<T, D>), dim3((unsigned)wgs), dim3(256), smem, st, a);
+  hipLaunchKernelGGL((paged_decode_kernel<T, D, kCodes>), dim3((unsigned)wgs), dim3(256), smem, st,
+                     a);
   if (a.direct) return;
   hipLaunchKernelGGL((paged_decode_join_kernel<T, D>), dim3((unsigned)((int64_t)a.n_seq * a.H)),
                      dim3(256), 0, st, a);
+}
+
+template <typename T, bool kCodes>
+void launch_decode(const DecodeArgs &a, int D, hipStream_t st) {
+  if (D == 64) return launch_decode_d<T, 64, kCodes>(a, st);
+  if (D == 128) return launch_decode_d<T, 128, kCodes>(a, st);
+  launch_decode_d<T, 256, kCodes>(a, st);
 }
 
 }  // namespace
@@ -618,9 +651,8 @@ void launch_paged_append(const AppendArgs &a, hipStream_t st) {
 
 template <typename T>
 void launch_paged_decode(const DecodeArgs &a, int D, hipStream_t st) {
-  if (D == 64) return launch_decode_d<T, 64>(a, st);
-  if (D == 128) return launch_decode_d<T, 128>(a, st);
-  launch_decode_d<T, 256>(a, st);
+  if (a.scales.k != nullptr) return launch_decode<T, true>(a, D, st);
+  launch_decode<T, false>(a, D, st);
 }
 
 #define VAFA_INST(T)                                              \

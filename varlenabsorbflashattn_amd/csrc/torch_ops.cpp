@@ -40,8 +40,8 @@ struct Api {
   X(absorb_bwd_full_workspace)                                                            \
   X(absorb_project_workspace) X(absorb_project_fwd) X(absorb_project_bwd)                 \
   X(absorb_project_f32_workspace) X(absorb_project_f32_fwd) X(absorb_project_f32_bwd)      \
-  X(paged_append) X(paged_decode_workspace) X(paged_decode) X(masked_fwd_workspace)        \
-  X(paged_store) X(paged_gather) X(qk_norm_rope_fwd) X(qk_norm_rope_bwd_workspace)          \
+  X(paged_append) X(paged_decode_workspace) X(masked_fwd_workspace)        \
+  X(paged_store) X(paged_gather) X(paged_decode_codes) X(qk_norm_rope_fwd) X(qk_norm_rope_bwd_workspace)          \
   X(qk_norm_rope_bwd)                                                                       \
   X(masked_fwd) X(masked_bwd_workspace) X(masked_bwd)
   VAFA_FNS(VAFA_FN)
@@ -552,27 +552,29 @@ const float *slopes_of(const char *what, const std::optional<Tensor> &slopes, in
 
 Tensor paged_decode(const Tensor &q_in, const Tensor &kc, const Tensor &vc, const Tensor &table,
                     const Tensor &lens, double scale, std::optional<double> softcap,
-                    std::optional<int64_t> window, const std::optional<Tensor> &slopes) {
+                    std::optional<int64_t> window, const std::optional<Tensor> &slopes,
+                    const std::optional<Tensor> &ks, const std::optional<Tensor> &vs) {
   const char *what = "paged_decode_attn";
   no_grad_only(what, {q_in, kc, vc, slopes.value_or(Tensor())});
   // (1e-50 would be 0 in 32 bits, which means none)
   if (softcap && !(*softcap > 0 && (float)*softcap > 0.f))
     throw py::value_error("softcap must be positive");
   if (window && *window < 1) throw py::value_error("window must be positive");
-  const Cache cache = cache_of(what, kc, vc, table, lens);
+  const Cache cache = cache_of(what, kc, vc, table, lens, ks, vs, q_in.scalar_type());
   const vafa_paged_cache &c = cache.c;
   check_tokens(what, "q", q_in, kc, cache.rows);
   need(q_in.size(0) == c.n_seq, what, "q must hold one token per sequence");
   const int64_t H = q_in.size(1);
   const float *sl = slopes_of(what, slopes, H, q_in);
   on_gpu(what, kc);
-  Call call(kc);
+  Call call(q_in);
   const Tensor q = rows_in(q_in);
   Tensor out = call.empty({c.n_seq, H, c.D});
   void *ws = call.workspace(api.paged_decode_workspace(&c, H, window.value_or(0)));
-  check(api.paged_decode(&c, ptr(q), stride_of(q, 0), stride_of(q, 1), H, ptr(out), (float)scale,
-                         (float)softcap.value_or(0.0), window.value_or(0), sl, dtype_of(kc), ws,
-                         call.ws_bytes(), call.stream));
+  check(api.paged_decode_codes(&c, cache.scales(), ptr(q), stride_of(q, 0), stride_of(q, 1), H,
+                               ptr(out), (float)scale, (float)softcap.value_or(0.0),
+                               window.value_or(0), sl, dtype_of(q), ws, call.ws_bytes(),
+                               call.stream));
   return out;
 }
 

@@ -106,6 +106,8 @@ def paged_decode_attn(
     softcap: Optional[float] = None,
     window: Optional[int] = None,
     alibi_slopes: Optional[torch.Tensor] = None,
+    k_scale: Optional[torch.Tensor] = None,
+    v_scale: Optional[torch.Tensor] = None,
 ) -> torch.Tensor:
     """Attention of the last token of each sequence, ``q [n_seq, H, D]``, over the first
     ``cache_lens[b]`` tokens of its pages (its own among them).
@@ -114,9 +116,10 @@ def paged_decode_attn(
     ``scale * q.k`` (default 1/sqrt(D)), then ``softcap * tanh(. / softcap)`` (1e-6 to 1e4), then
     minus ``alibi_slopes[h]`` (float32 ``[H]``) times the key's distance; ``window`` keeps
     the last that many keys.  :func:`packed_masked_attn` applies the same to whole sequences.
-    A sequence without keys gets zeros.  Forward only.
+    A sequence without keys gets zeros.  ``k_scale`` and ``v_scale`` belong to an 8-bit cache,
+    whose rows become ``q``'s type (bf16 or fp16).  Forward only.
     """
     if scale is None:
         scale = 1.0 / math.sqrt(q.shape[-1])
     return _lib.ops().paged_decode(q, k_cache, v_cache, page_table, cache_lens, scale, softcap,
-                                   window, alibi_slopes)
+                                   window, alibi_slopes, k_scale, v_scale)
