@@ -80,3 +80,18 @@ def decode(q, k_cache, v_cache, table, lens, scale, softcap=None, window=None, s
             out[b, h], mag[b, h] = P @ v, P @ np.abs(v)
             flat[b, h] = np.abs(v).sum(0) / e.sum()
     return out, mag, flat
+
+
+def chunk(q, k_cache, v_cache, table, lens, cu, scale, softcap=None, window=None, slopes=None):
+    """Several new tokens per sequence: each token as the last of a sequence that ends with
+    it -> what decode gives, by packed row."""
+    out, mag, flat = np.zeros((3,) + q.shape)
+    capacity = table.shape[1] * k_cache.shape[1]
+    for b in range(len(lens)):
+        length = min(max(int(lens[b]), 0), capacity)
+        for t in range(int(cu[b]), int(cu[b + 1])):
+            seen = length - (int(cu[b + 1]) - 1 - t)
+            o = decode(q[t:t + 1], k_cache, v_cache, table[b:b + 1], [seen], scale, softcap, window,
+                       slopes)
+            out[t], mag[t], flat[t] = (x[0] for x in o)
+    return out, mag, flat

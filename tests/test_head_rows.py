@@ -8,8 +8,8 @@ import pytest
 import torch
 
 from oracle import head_rows as hr
-from varlenabsorbflashattn_amd import (_lib, packed_qk_norm_rope, paged_decode_attn,
-                                       paged_kv_append, paged_kv_gather)
+from varlenabsorbflashattn_amd import (_lib, packed_qk_norm_rope, paged_chunk_attn,
+                                       paged_decode_attn, paged_kv_append, paged_kv_gather)
 
 E4M3, E8M0 = torch.float8_e4m3fn, torch.float8_e8m0fnu
 
@@ -87,6 +87,16 @@ def _gather(a):
                            dtype=a["k"].dtype, **kw)
 
 
+def _decode(a):
+    return paged_decode_attn(a["q"], a["k_cache"], a["v_cache"], a["page_table"], a["cache_lens"],
+                             k_scale=a["k_scale"], v_scale=a["v_scale"])
+
+
+def _chunk(a, cu=torch.zeros(4, dtype=torch.int32), **kw):
+    return paged_chunk_attn(a["q"], a["k_cache"], a["v_cache"], a["page_table"], a["cache_lens"],
+                            cu, k_scale=a["k_scale"], v_scale=a["v_scale"], **kw)
+
+
 REFUSED_CODES = [
     ({"k_scale": None, "v_scale": None}, AssertionError, "need k_scale and v_scale"),
     ({"v_scale": None}, AssertionError, "belong together"),
@@ -103,7 +113,7 @@ REFUSED_CODES = [
 ]
 
 
-@pytest.mark.parametrize("call", [_append, _gather])
+@pytest.mark.parametrize("call", [_append, _gather, _decode, _chunk])
 @pytest.mark.parametrize("change,error,text", REFUSED_CODES)
 def test_refused_codes(call, change, error, text):
     a = _cache()
@@ -147,6 +157,25 @@ def test_refused_gather_options():
     refused(AssertionError, "not supported", dtype=torch.float32)
     half = torch.zeros(5, 16, 2, 64, dtype=torch.float16)
     refused(AssertionError, "comes back in its dtype", cache=half, scales=False)
+
+
+def test_refused_chunk_options():
+    def refused(error, text, cu=torch.zeros(4, dtype=torch.int32), change={}, **kw):
+        a = _cache()
+        a.update(change)
+        with pytest.raises(error, match=text):
+            _chunk(a, cu, **kw)
+    refused(AssertionError, "cu_seqlens must be", cu=torch.zeros(3, dtype=torch.int32))
+    refused(AssertionError, "int32", cu=torch.zeros(4, dtype=torch.int64))
+    refused(ValueError, "contiguous", cu=torch.zeros(1, dtype=torch.int32).expand(4))
+    for cap in (0.0, -1.0, float("nan"), 1e-50):
+        refused(ValueError, "softcap must be positive", softcap=cap)
+    refused(ValueError, "window must be positive", window=0)
+    refused(AssertionError, r"alibi_slopes must be \[H\]", alibi_slopes=torch.zeros(3))
+    refused(AssertionError, "q must be", change={"q": torch.zeros(3, 4, 32, dtype=torch.bfloat16)})
+    refused(AssertionError, "not supported", change={"q": torch.zeros(3, 4, 64)})
+    refused(ValueError, "no backward",
+            change={"q": torch.zeros(3, 4, 64, dtype=torch.bfloat16, requires_grad=True)})
 
 
 def test_refused_by_the_c_abi():
@@ -202,7 +231,22 @@ def test_refused_by_the_c_abi():
         (0, None), (15, None), (16, None), (19, None), (20, x + 8), (21, None), (22, x + 2)])
     all_refused(L.vafa_qk_norm_rope_bwd, bwd, [(26, None), (27, need - 1)],
                 _lib.VAFA_ERR_WORKSPACE)
+    wide = cache(table_width=100)
+    need = L.vafa_paged_chunk_workspace(wide, 7, 4, 0)
+    assert need > 0 and L.vafa_paged_chunk_workspace(cache(), 7, 4, 0) == 0
+    for c, T, H, window in ((cache(n_pages=0), 7, 4, 0), (cache(D=96), 7, 4, 0), (wide, -1, 4, 0),
+                            (wide, 1 << 31, 4, 0), (wide, 7, 3, 0), (wide, 7, 8192, 0),
+                            (wide, 7, 4, -1)):
+        assert L.vafa_paged_chunk_workspace(c, T, H, window) == -1
+    chunk = [wide, scales(), x, 256, 64, 7, 4, x, x, 0.125, 0.0, 0, None, BF, x, need, None]
+    all_refused(L.vafa_paged_chunk, chunk, [
+        (0, cache(k_token=136, table_width=100)), (1, scales(k=None)), (2, x + 2), (3, 12), (7, None),
+        (8, None), (9, float("nan")), (10, -1.0), (10, 1e-40), (11, -1)])
+    all_refused(L.vafa_paged_chunk, chunk, [(13, 0), (6, 5)], _lib.VAFA_ERR_ASSERT)
+    all_refused(L.vafa_paged_chunk, chunk, [(14, None), (14, x + 8), (15, need - 1)],
+                _lib.VAFA_ERR_WORKSPACE)
     # no rows: nothing is launched
+    assert L.vafa_paged_chunk(*[0 if i == 5 else y for i, y in enumerate(chunk)]) == 0
     assert L.vafa_qk_norm_rope_fwd(*[0 if i == 8 else y for i, y in enumerate(fwd)]) == 0
     assert L.vafa_paged_gather(*[0 if i == 4 else y for i, y in enumerate(gather)]) == 0
 

@@ -133,6 +133,9 @@ _SIGS = {
                                    _I32, _P]),
     "vafa_paged_decode_codes": (C.c_int, [_PCACHE, _PSCALES, _P, _I64, _I64, _I64, _P, _F, _F, _I64,
                                           _P, _I32, _P, _I64, _P]),
+    "vafa_paged_chunk_workspace": (C.c_int64, [_PCACHE, _I64, _I64, _I64]),
+    "vafa_paged_chunk": (C.c_int, [_PCACHE, _PSCALES, _P, _I64, _I64, _I64, _I64, _P, _P, _F, _F,
+                                   _I64, _P, _I32, _P, _I64, _P]),
     "vafa_paged_gather": (C.c_int, [_PCACHE, _PSCALES, _P, _P, _I64, _P, _P, _I32, _P]),
     "vafa_qk_norm_rope_fwd": (C.c_int, [_P, _I64, _I64, _I64, _P, _I64, _I64, _I64, _I64, _I64, _P,
                                         _P, _I64, _I32, _F, _P, _P, _I32, _F, _P, _P, _I32, _P]),

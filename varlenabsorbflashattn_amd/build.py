@@ -22,7 +22,7 @@ TORCH_MODULE = "_vafa_torch"
 TORCH_LIB_PATH = os.path.join(HERE, TORCH_MODULE + ".so")
 SOURCES = ["plan.cpp", "capi.cpp", "simt.hip", "reduce.hip", "varlen_mfma.hip", "varlen_bwd_mfma.hip",
            "varlen_f32.hip", "masked_fwd.hip", "masked_bwd.hip", "capi_masked.cpp",
-           "paged.hip", "head_rows.hip", "capi_paged.cpp", "capi_rows.cpp",
+           "paged.hip", "paged_chunk.hip", "head_rows.hip", "capi_paged.cpp", "capi_rows.cpp",
            "absorb_mfma.hip", "absorb_bwd_mfma.hip", "absorb_f32.hip",
            "absorb_project.hip"]
 ARCH = os.environ.get("VAFA_OFFLOAD_ARCH", "gfx950")

@@ -148,6 +148,69 @@ int plan_decode(const vafa_paged_cache *c, int64_t H, int64_t window, DecodePlan
   return VAFA_OK;
 }
 
+int check_scores(const char *what, float scale, float softcap) {
+  if (!std::isfinite(scale * kLog2e))
+    return fail(VAFA_ERR_VALUE, "%s: scale must be finite", what);
+  if (!softcap_ok(softcap))
+    return fail(VAFA_ERR_VALUE, "%s: softcap must be positive, from %g to %g", what,
+                (double)kMinSoftcap, (double)kMaxSoftcap);
+  if (softcap > 0.f && !std::isfinite(2.f * kLog2e * scale / softcap))
+    return fail(VAFA_ERR_VALUE, "%s: scale / softcap is not finite", what);
+  return VAFA_OK;
+}
+
+int check_workspace(const void *workspace, int64_t bytes, int64_t needed) {
+  if (needed > 0 && (bytes < needed || workspace == nullptr || (uintptr_t)workspace % 16 != 0))
+    return fail(VAFA_ERR_WORKSPACE, "workspace of %lld bytes, %lld needed (16-byte aligned)",
+                (long long)bytes, (long long)needed);
+  return VAFA_OK;
+}
+
+// The launch of several new tokens per sequence: lengths and cu are device data, so chunks and
+// workspace go by the rows and by what the page table could hold.
+struct ChunkPlan {
+  int lg = 0, lt = 0;
+  int64_t chunks = 0, bytes = 0, lse_off = 0;
+  bool direct = false;
+};
+
+constexpr int64_t kChunkRows = 128;
+// Where no tile can walk more than this many units, none is divided (no launch that joins).
+constexpr int64_t kChunkDirect = 8;
+
+int plan_chunk(const vafa_paged_cache *c, int64_t T, int64_t H, int64_t window, ChunkPlan *p) {
+  const char *what = "paged_chunk_attn";
+  if (int rc = check_cache(what, c)) return rc;
+  if (c->D != 64 && c->D != 128 && c->D != 256)
+    return fail(VAFA_ERR_ASSERT, "%s: head_dim %lld not supported (64, 128, 256)", what,
+                (long long)c->D);
+  if (H < 1 || H % c->Hk != 0 || H > 4096)
+    return fail(VAFA_ERR_ASSERT, "%s: %lld query heads do not divide among %lld key heads", what,
+                (long long)H, (long long)c->Hk);
+  if (T < 0 || T > kMaskedMaxTokens)
+    return fail(VAFA_ERR_VALUE, "%s: %lld tokens are too many for a call", what, (long long)T);
+  if (window < 0) return fail(VAFA_ERR_VALUE, "%s: window must be positive", what);
+  const int64_t G = H / c->Hk;
+  while (p->lg < 5 && G % (int64_t{2} << p->lg) == 0) ++p->lg;
+  while ((kChunkRows >> (p->lt + 1)) >= (int64_t{1} << p->lg)) ++p->lt;
+  const int64_t sets = H >> p->lg, tw = int64_t{1} << p->lt;
+  const int64_t cap = page_capacity(map_of(c));
+  const int64_t keys = window > 0 && window < cap ? std::min(cap, window + tw + kChunkKeys) : cap;
+  const int64_t most = std::max<int64_t>(1, (keys + kChunkKeys - 1) / kChunkKeys);
+  // (a sequence of nq tokens has at most nq / tw + 1 tiles)
+  const int64_t tiles = std::max<int64_t>(1, T / tw + std::min(c->n_seq, T));
+  const int64_t slots = c->D <= 128 ? 512 : 256;  // workgroups that the GPU holds
+  p->direct = most <= kChunkDirect;
+  if (p->direct)
+    p->chunks = std::min<int64_t>(tiles, std::max<int64_t>(slots, 65536 / sets));
+  else
+    p->chunks = std::max<int64_t>(1, std::min(slots / sets, tiles * most));
+  const int64_t rows = p->direct ? 0 : 2 * p->chunks * sets * kChunkRows;
+  p->lse_off = rows * c->D * 4;
+  p->bytes = p->lse_off + rows * 4;
+  return VAFA_OK;
+}
+
 // The operands of an append, which both kinds of it take.
 int append_args(const char *what, const vafa_paged_cache *c, const void *k, int64_t k_token,
                 int64_t k_head, const void *v, int64_t v_token, int64_t v_head, int64_t T,
@@ -318,19 +381,10 @@ int vafa_paged_decode_codes(const vafa_paged_cache *c, const vafa_row_scales *sc
   DecodePlan p;
   if (int rc = plan_decode(c, H, window, &p)) return rc;
   if (int rc = check_codes(what, c, scales)) return rc;
-  if (!std::isfinite(scale * kLog2e))
-    return fail(VAFA_ERR_VALUE, "%s: scale must be finite", what);
-  if (!softcap_ok(softcap))
-    return fail(VAFA_ERR_VALUE, "%s: softcap must be positive, from %g to %g", what,
-                (double)kMinSoftcap, (double)kMaxSoftcap);
-  if (softcap > 0.f && !std::isfinite(2.f * kLog2e * scale / softcap))
-    return fail(VAFA_ERR_VALUE, "%s: scale / softcap is not finite", what);
+  if (int rc = check_scores(what, scale, softcap)) return rc;
   if (int rc = check_rows(what, "q", q, q_token, q_head)) return rc;
   if (int rc = check_rows(what, "out", out, 0, 0)) return rc;
-  if (p.bytes > 0 &&
-      (workspace_bytes < p.bytes || workspace == nullptr || (uintptr_t)workspace % 16 != 0))
-    return fail(VAFA_ERR_WORKSPACE, "workspace of %lld bytes, %lld needed (16-byte aligned)",
-                (long long)workspace_bytes, (long long)p.bytes);
+  if (int rc = check_workspace(workspace, workspace_bytes, p.bytes)) return rc;
   if (c->n_seq == 0) return VAFA_OK;
   if (int rc = check_pointers(what, c)) return rc;
   if (int rc = check_given(what, {q, out})) return rc;
@@ -356,6 +410,57 @@ int vafa_paged_decode_codes(const vafa_paged_cache *c, const vafa_row_scales *sc
     launch_paged_decode<bf16>(a, (int)c->D, (hipStream_t)stream);
   else
     launch_paged_decode<f16>(a, (int)c->D, (hipStream_t)stream);
+  return check_launch(what);
+}
+
+int64_t vafa_paged_chunk_workspace(const vafa_paged_cache *c, int64_t T, int64_t H,
+                                   int64_t window) {
+  ChunkPlan p;
+  return plan_chunk(c, T, H, window, &p) ? -1 : p.bytes;
+}
+
+int vafa_paged_chunk(const vafa_paged_cache *c, const vafa_row_scales *scales, const void *q,
+                     int64_t q_token, int64_t q_head, int64_t T, int64_t H, const int32_t *cu,
+                     void *out, float scale, float softcap, int64_t window, const float *slopes,
+                     int32_t dtype, void *workspace, int64_t workspace_bytes, void *stream) {
+  const char *what = "paged_chunk_attn";
+  if (int rc = check_dtype(what, dtype)) return rc;
+  ChunkPlan p;
+  if (int rc = plan_chunk(c, T, H, window, &p)) return rc;
+  if (int rc = check_codes(what, c, scales)) return rc;
+  if (int rc = check_scores(what, scale, softcap)) return rc;
+  if (int rc = check_rows(what, "q", q, q_token, q_head)) return rc;
+  if (int rc = check_rows(what, "out", out, 0, 0)) return rc;
+  if (int rc = check_workspace(workspace, workspace_bytes, p.bytes)) return rc;
+  if (T == 0) return VAFA_OK;
+  if (int rc = check_pointers(what, c)) return rc;
+  if (int rc = check_given(what, {q, out, cu})) return rc;
+  if (scales != nullptr)
+    if (int rc = check_given(what, {scales->k, scales->v})) return rc;
+  ChunkArgs a{};
+  a.q = q; a.kc = c->k; a.vc = c->v; a.out = out; a.cu = cu; a.lens = c->cache_lens;
+  a.slopes = slopes; a.part_o = (float *)workspace;
+  a.part_lse = (float *)((char *)workspace + p.lse_off);
+  a.map = map_of(c); a.q_token = q_token; a.q_head = q_head;
+  a.k_page = c->k_page; a.kc_token = c->k_token; a.kc_head = c->k_head;
+  a.v_page = c->v_page; a.vc_token = c->v_token; a.vc_head = c->v_head;
+  a.scales = scales_of(scales); a.T = T;
+  // (so that a key behind the last unit still has a number)
+  a.capacity = std::min<int64_t>(page_capacity(a.map), INT32_MAX - 4096);
+  a.n_seq = (int)c->n_seq; a.H = (int)H; a.Hk = (int)c->Hk;
+  a.window = (int)std::min<int64_t>(window, kChunkNoWindow);
+  a.lg = p.lg; a.lt = p.lt; a.chunks = (int)p.chunks; a.direct = p.direct;
+  // (as for one token: tanh(x) = 1 - 2 / (1 + 2^(2 x log2 e)), x = scale q.k / cap)
+  a.c = softcap > 0.f ? 2.f * kLog2e * scale / softcap : scale * kLog2e;
+  a.cap2 = softcap * kLog2e;
+  const hipStream_t st = (hipStream_t)stream;
+  const bool bf = dtype == VAFA_BF16;
+  if (c->D == 64)
+    bf ? launch_paged_chunk<bf16, 64>(a, st) : launch_paged_chunk<f16, 64>(a, st);
+  else if (c->D == 128)
+    bf ? launch_paged_chunk<bf16, 128>(a, st) : launch_paged_chunk<f16, 128>(a, st);
+  else
+    bf ? launch_paged_chunk<bf16, 256>(a, st) : launch_paged_chunk<f16, 256>(a, st);
   return check_launch(what);
 }
 

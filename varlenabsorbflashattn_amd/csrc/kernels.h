@@ -203,6 +203,26 @@ struct DecodeArgs {
   float c, cap2;  // factor on q.k, and cap log2 e (0: none), see paged.hip
 };
 
+// Attention of several new tokens per sequence over a paged cache.
+struct ChunkArgs {
+  const void *q, *kc, *vc;
+  void *out;
+  const int32_t *cu, *lens;
+  const float *slopes;       // or null
+  float *part_o, *part_lse;  // parts of cut tiles: [slots, sets, rows of a tile, D] and [..]
+  PageMap map;
+  int64_t q_token, q_head;
+  int64_t k_page, kc_token, kc_head, v_page, vc_token, vc_head;
+  RowScales scales;  // of codes, or null
+  int64_t capacity;  // tokens of a sequence's pages
+  int64_t T;
+  int n_seq, H, Hk, window;  // window 0: all keys
+  int lg, lt;   // log2 of the heads in a set (masked.h) and of the tokens in a tile
+  int chunks;   // parts of the axis of all units (paged.h)
+  int direct;   // whole tiles, dealt to the chunks in turn: no partial results
+  float c, cap2;
+};
+
 // varlen_f32.hip: fp32 varlen on fp32 matrix cores
 bool f32_varlen_mfma_d(int D);      // D in {32, 64, 128, 256}
 bool f32_varlen_bwd_mfma_d(int D);  // D in {32, 64, 128}
@@ -269,6 +289,9 @@ void launch_absorb_dax(const AbsorbArgs &, hipStream_t);
 // paged.hip (bf16 / f16)
 template <typename T> void launch_paged_append(const AppendArgs &, hipStream_t);
 template <typename T> void launch_paged_decode(const DecodeArgs &, int D, hipStream_t);
+
+// paged_chunk.hip (bf16 / f16, D in {64, 128, 256})
+template <typename T, int D> void launch_paged_chunk(const ChunkArgs &, hipStream_t);
 
 // head_rows.hip (bf16 / f16; D in {64, 128, 256}, gather: multiples of 16)
 template <typename T> void launch_head_rows(const HeadRowsArgs &, hipStream_t);

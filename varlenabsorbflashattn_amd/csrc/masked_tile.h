@@ -1,0 +1,142 @@
+// The forward's step over a tile of keys: scores, online softmax and the product with V for
+// a wave's 32 query rows, under the mask and the score transforms of masked.h.
+//
+// S^T = K Q^T and O^T += V^T P^T over 64 keys in LDS (fwd_tiles.h), with a lazily updated
+// running maximum.
+#pragma once
+#include "fwd_tiles.h"
+#include "masked.h"
+#include "mfma.h"
+
+namespace vafa {
+
+namespace {
+
+// One 64-key tile for the wave's 32 query rows; masked: some (row, key) pair is hidden.  Keys
+// whose bit of `here` is not set are hidden from every row (a masked tile's alone).
+template <typename T, int D, bool kCap, bool kBias>
+__device__ __forceinline__ void masked_tile(const T *ks, const T *vs,
+                                            const typename Mfma<T>::v8 (&qf)[D / 16],
+                                            f32x16 (&acc)[D / 32], float &m_run, float &l_part,
+                                            const ScoreArgs &sa, float slope2, int kbase,
+                                            int k_end, bool masked, int p, int pre, int window,
+                                            int lane, uint64_t here = ~uint64_t{0}) {
+  using M = Mfma<T>;
+  constexpr int NC = D / 16, ND = D / 32;
+  constexpr int KS = FwdSmem<D>::KSK, VS = FwdSmem<D>::KSV;
+  constexpr bool kLog2 = kCap || kBias;  // s holds log2-domain scores after the transform
+  const int lrow = lane & 31, lhalf = lane >> 5;
+  constexpr int kPre = 4;
+  constexpr int NS = 2 * NC;
+  f32x16 s[2];
+#pragma unroll
+  for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[kt][r] = 0.f;
+  const T *kbase_p = ks + lrow * KS + lhalf * 8;
+  auto kop = [&](int i) {  // i = cc * 2 + kt
+    return *reinterpret_cast<const u32x4 *>(kbase_p + (i & 1) * 32 * KS + (i >> 1) * 16);
+  };
+  u32x4 ring[kPre];
+#pragma unroll
+  for (int i = 0; i < kPre; ++i) ring[i] = kop(i);
+  __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+  for (int i = 0; i < NS; ++i) {
+    const u32x4 a = ring[i % kPre];
+    s[i & 1] = M::mma(as_v8<T>(a), qf[i >> 1], s[i & 1]);
+    if (i + kPre < NS) ring[i % kPre] = kop(i + kPre);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  const int k_lane = kbase + lhalf * 4;  // register (kt, r) holds key k_lane + off(kt, r)
+  auto off = [](int kt, int r) { return kt * 32 + (r >> 2) * 8 + (r & 3); };
+  if constexpr (kLog2) {
+    const float back = (float)(p - k_lane);
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        float z = s[kt][r] * sa.c;
+        if constexpr (kCap) z = __builtin_fmaf(-2.f * sa.cap2, cap_e(z), sa.cap2);
+        if constexpr (kBias) z = __builtin_fmaf(-slope2, fabsf(back - (float)off(kt, r)), z);
+        s[kt][r] = z;
+      }
+  }
+  if (masked) {
+    const uint64_t seen =
+        seen_keys(k_lane, k_end, p, pre, window) & (here >> (lhalf * 4));
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        s[kt][r] = where_bit((uint32_t)(seen >> 32 * kt), off(0, r), s[kt][r], kNegInf);
+  }
+  const float c = kLog2 ? 1.f : sa.c;
+  typename M::v8 pb[2][2];
+  float ps4[4];
+  // P is rounded to T, V's type, for the product; its row sum takes the rounded values, in
+  // fp32, so that a constant V comes out as it is (outputs in bf16 1.8e-3 off in the 2-norm,
+  // the exact ones rounded 1.7e-3)
+  auto build_p = [&]() {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) ps4[i] = 0.f;
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+      for (int mm = 0; mm < 2; ++mm) {
+        typename M::v8 x;
+#pragma unroll
+        for (int t = 0; t < 8; ++t) {
+          const float y = s[kt][mm * 8 + t];
+          x[t] = static_cast<T>(
+              fast_exp2(kLog2 ? y - m_run : __builtin_fmaf(y, c, -m_run)));
+        }
+        pb[kt][mm] = x;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) ps4[t] = dot2_ones<T>(x, t, ps4[t]);
+      }
+  };
+  build_p();
+  float ps = (ps4[0] + ps4[1]) + (ps4[2] + ps4[3]);
+  if (wave_any(!(ps <= kLazyMax))) {
+    float m4[4] = {kNegInf, kNegInf, kNegInf, kNegInf};
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) m4[r & 3] = fmaxf(m4[r & 3], s[kt][r]);
+    float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+    mx = max_xor32(mx) * c;
+    const float m_new = fmaxf(m_run, mx);
+    const float alpha = fast_exp2(m_run - m_new);
+    m_run = m_new;
+    l_part *= alpha;
+#pragma unroll
+    for (int i = 0; i < ND; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[i][r] *= alpha;
+    build_p();
+    ps = (ps4[0] + ps4[1]) + (ps4[2] + ps4[3]);
+  }
+  l_part += ps;
+  constexpr int NP = 4 * ND;
+  auto vop = [&](int i) {  // i = km * ND + dt, km = kt * 2 + mm
+    const int km = i / ND, dt = i % ND;
+    return tr_operand<T>(vs, VS, km * 16, dt * 32, lane);
+  };
+  typename M::v8 vring[kPre];
+#pragma unroll
+  for (int i = 0; i < kPre; ++i) vring[i] = vop(i);
+  __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+  for (int i = 0; i < NP; ++i) {
+    const typename M::v8 a = vring[i % kPre];
+    const int km = i / ND, dt = i % ND;
+    acc[dt] = M::mma(a, pb[km >> 1][km & 1], acc[dt]);
+    if (i + kPre < NP) vring[i % kPre] = vop(i + kPre);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
+
+}  // namespace
+
+}  // namespace vafa

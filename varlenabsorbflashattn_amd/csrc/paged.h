@@ -80,4 +80,87 @@ VAFA_HD int64_t decode_slot(int32_t c, int32_t t0, int32_t per) {
   return 2 * (int64_t)c + ((int64_t)c * per < t0 ? 1 : 0);
 }
 
+// ---- attention of a chunk of new tokens: units of kChunkKeys keys ----------------
+// The nq new tokens of a sequence of len cached ones are its last; token t has position
+// diag + t, diag = len - nq, and sees the keys up to its own (the last `window` of them).
+// Tokens go in tiles of 2^lt; tile i walks units of kChunkKeys keys from start(i), a multiple
+// of that, to end(i), one unit at least (a tile without keys writes zeros).  The units of all
+// tiles of all sequences, one after another, form one axis, of which chunk c takes the units
+// [c * per, (c + 1) * per): tiles are cut anywhere, and their parts joined.
+constexpr int kChunkKeys = 64, kChunkShift = 6;
+constexpr int64_t kChunkLeast = 4;  // units of a chunk
+// as a window, every key: no sum with a position or a tile's rows passes 32 bits
+constexpr int32_t kChunkNoWindow = INT32_MAX - 1024;
+
+struct ChunkSeq {
+  int64_t nq, len, diag;
+  int32_t lt, window;  // window 0: all keys
+};
+VAFA_HD ChunkSeq chunk_seq(int64_t nq, int64_t len, int32_t lt, int32_t window) {
+  return ChunkSeq{nq, len, len - nq, lt, window};
+}
+VAFA_HD int64_t chunk_tiles(int64_t nq, int32_t lt) {
+  return (nq + (int64_t{1} << lt) - 1) >> lt;
+}
+VAFA_HD int64_t chunk_end(const ChunkSeq &s, int64_t i) {
+  const int64_t t = (i + 1) << s.lt, e = (t < s.nq ? t : s.nq) + s.diag;
+  return e > 0 ? e : 0;
+}
+VAFA_HD int64_t chunk_start(const ChunkSeq &s, int64_t i) {
+  if (s.window <= 0) return 0;
+  const int64_t b = (i << s.lt) + s.diag - s.window + 1;
+  return b > 0 ? b >> kChunkShift << kChunkShift : 0;
+}
+VAFA_HD int64_t chunk_units(const ChunkSeq &s, int64_t i) {
+  const int64_t e = chunk_end(s, i);
+  return e > 0 ? ((e + kChunkKeys - 1) >> kChunkShift) - (chunk_start(s, i) >> kChunkShift) : 1;
+}
+// sum of floor((c + (j << lt)) / kChunkKeys) over j in [j0, j1), c + (j0 << lt) >= 0
+VAFA_HD int64_t chunk_floors(int64_t c, int32_t lt, int64_t j0, int64_t j1) {
+  if (j1 <= j0) return 0;
+  if (lt >= kChunkShift)
+    return (j1 - j0) * (c >> kChunkShift) +
+           ((j1 * (j1 - 1) - j0 * (j0 - 1)) >> 1 << (lt - kChunkShift));
+  // floor((c + j 2^lt) / 64) = floor((floor(c / 2^lt) + j) / 2^r): below n, whole runs of 2^r
+  const int32_t r = kChunkShift - lt;
+  const int64_t n0 = (c >> lt) + j0, n1 = (c >> lt) + j1, q0 = n0 >> r, q1 = n1 >> r;
+  return ((q1 * (q1 - 1)) >> 1 << r) + (n1 - (q1 << r)) * q1 -
+         (((q0 * (q0 - 1)) >> 1 << r) + (n0 - (q0 << r)) * q0);
+}
+// Units of the tiles in front of tile i (i up to the sequence's tiles: all of them).
+VAFA_HD int64_t chunk_before(const ChunkSeq &s, int64_t i) {
+  const int64_t m = chunk_tiles(s.nq, s.lt);
+  if (s.len <= 0 || i <= 0) return i;
+  // tiles whose end is 0; the last has end len > 0
+  int64_t none = s.diag < 0 ? -s.diag >> s.lt : 0;
+  if (none > m - 1) none = m - 1;
+  if (i <= none) return i;
+  const int64_t last = i < m ? i : m - 1;
+  int64_t n = none + chunk_floors(s.diag + (int64_t{1} << s.lt) + kChunkKeys - 1, s.lt, none, last);
+  if (i == m) n += (s.len + kChunkKeys - 1) >> kChunkShift;
+  if (s.window > 0) {
+    const int64_t back = s.window - 1 - s.diag;  // starts are 0 up to here
+    const int64_t w0 = back <= 0 ? 0 : (back + (int64_t{1} << s.lt) - 1) >> s.lt;
+    n -= chunk_floors(-back, s.lt, w0, i);
+  }
+  return n;
+}
+// The tile that holds unit u of the sequence (u below all of its units).
+VAFA_HD int64_t chunk_tile_of(const ChunkSeq &s, int64_t u) {
+  int64_t lo = 0, hi = chunk_tiles(s.nq, s.lt) - 1;  // chunk_before(lo) <= u
+  while (lo < hi) {
+    const int64_t mid = (lo + hi + 1) >> 1;
+    if (chunk_before(s, mid) <= u)
+      lo = mid;
+    else
+      hi = mid - 1;
+  }
+  return lo;
+}
+// Partial result of the piece that chunk c holds of a tile whose units start at t0 of the
+// axis: its first piece has slot 2 c, its last 2 c + 1 (pieces between them are whole tiles).
+VAFA_HD int64_t chunk_slot(int64_t c, int64_t t0, int64_t per) {
+  return 2 * c + (c * per < t0 ? 1 : 0);
+}
+
 }  // namespace vafa

@@ -41,7 +41,7 @@ struct Api {
   X(absorb_project_workspace) X(absorb_project_fwd) X(absorb_project_bwd)                 \
   X(absorb_project_f32_workspace) X(absorb_project_f32_fwd) X(absorb_project_f32_bwd)      \
   X(paged_append) X(paged_decode_workspace) X(masked_fwd_workspace)        \
-  X(paged_store) X(paged_gather) X(paged_decode_codes) X(qk_norm_rope_fwd) X(qk_norm_rope_bwd_workspace)          \
+  X(paged_store) X(paged_gather) X(paged_decode_codes) X(paged_chunk_workspace) X(paged_chunk) X(qk_norm_rope_fwd) X(qk_norm_rope_bwd_workspace)          \
   X(qk_norm_rope_bwd)                                                                       \
   X(masked_fwd) X(masked_bwd_workspace) X(masked_bwd)
   VAFA_FNS(VAFA_FN)
@@ -578,6 +578,33 @@ Tensor paged_decode(const Tensor &q_in, const Tensor &kc, const Tensor &vc, cons
   return out;
 }
 
+Tensor paged_chunk(const Tensor &q_in, const Tensor &kc, const Tensor &vc, const Tensor &table,
+                   const Tensor &lens, const Tensor &cu, double scale,
+                   std::optional<double> softcap, std::optional<int64_t> window,
+                   const std::optional<Tensor> &slopes, const std::optional<Tensor> &ks,
+                   const std::optional<Tensor> &vs) {
+  const char *what = "paged_chunk_attn";
+  no_grad_only(what, {q_in, kc, vc, slopes.value_or(Tensor())});
+  if (softcap && !(*softcap > 0 && (float)*softcap > 0.f))
+    throw py::value_error("softcap must be positive");
+  if (window && *window < 1) throw py::value_error("window must be positive");
+  const Cache cache = cache_of(what, kc, vc, table, lens, ks, vs, q_in.scalar_type());
+  const vafa_paged_cache &c = cache.c;
+  check_tokens(what, "q", q_in, kc, cache.rows);
+  const int32_t *cu_ptr = ints_of(what, "cu_seqlens", cu, c.n_seq + 1, kc);
+  const int64_t T = q_in.size(0), H = q_in.size(1);
+  const float *sl = slopes_of(what, slopes, H, q_in);
+  on_gpu(what, kc);
+  Call call(q_in);
+  const Tensor q = rows_in(q_in);
+  Tensor out = call.empty({T, H, c.D});
+  void *ws = call.workspace(api.paged_chunk_workspace(&c, T, H, window.value_or(0)));
+  check(api.paged_chunk(&c, cache.scales(), ptr(q), stride_of(q, 0), stride_of(q, 1), T, H, cu_ptr,
+                        ptr(out), (float)scale, (float)softcap.value_or(0.0), window.value_or(0),
+                        sl, dtype_of(q), ws, call.ws_bytes(), call.stream));
+  return out;
+}
+
 // dtype and content of an integer tensor on the host, for a plan's key (tensor.numpy()
 // alone takes 5 to 10 us).
 py::bytes cu_key(const Tensor &t) {
@@ -871,6 +898,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("masked_operands", &masked_operands, no_gil);
   m.def("masked_attn", &masked_attn, no_gil);
   m.def("paged_append", &paged_append, no_gil);
+  m.def("paged_chunk", &paged_chunk, no_gil);
   m.def("paged_gather", &paged_gather, no_gil);
   m.def("qk_norm_rope", &qk_norm_rope, no_gil);
   m.def("paged_decode", &paged_decode, no_gil);

@@ -1,5 +1,5 @@
 """A paged key-value cache: appending tokens with the position rotation, reading them
-back, and the attention of one new token per sequence over the cache.
+back, and the attention of one or several new tokens per sequence over the cache.
 
 The caches are ``[n_pages, page_size, H_k, D]`` (bf16 or fp16), features contiguous and
 other strides any multiple of 8 elements, so views of a joint or head-major allocation
@@ -123,3 +123,36 @@ def paged_decode_attn(
         scale = 1.0 / math.sqrt(q.shape[-1])
     return _lib.ops().paged_decode(q, k_cache, v_cache, page_table, cache_lens, scale, softcap,
                                    window, alibi_slopes, k_scale, v_scale)
+
+
+def paged_chunk_attn(
+    q: torch.Tensor,
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    page_table: torch.Tensor,
+    cache_lens: torch.Tensor,
+    cu_seqlens: torch.Tensor,
+    *,
+    scale: Optional[float] = None,
+    softcap: Optional[float] = None,
+    window: Optional[int] = None,
+    alibi_slopes: Optional[torch.Tensor] = None,
+    k_scale: Optional[torch.Tensor] = None,
+    v_scale: Optional[torch.Tensor] = None,
+) -> torch.Tensor:
+    """Attention of several new tokens per sequence, packed ``q [T, H, D]``, over the caches:
+    a chunk of a prompt, a turn behind a cached prefix, drafted tokens, or any mixture with
+    sequences of one new token.
+
+    Tokens ``cu_seqlens[b] .. cu_seqlens[b + 1] - 1`` (int32 on the GPU, not decreasing) are
+    the last of the ``cache_lens[b]`` tokens of sequence ``b`` (their keys and values are in
+    the cache), and each sees the keys up to its own, with ``window`` the last that many of
+    them.  Scores, heads and 8-bit caches are those of :func:`paged_decode_attn`, the result
+    is what :func:`packed_masked_attn` gives on the gathered keys.  Tokens in front of the
+    first key (more new tokens than the cache holds) and rows of no sequence get zeros.  At
+    most 2^30 tokens and 4096 heads.  Forward only.
+    """
+    if scale is None:
+        scale = 1.0 / math.sqrt(q.shape[-1])
+    return _lib.ops().paged_chunk(q, k_cache, v_cache, page_table, cache_lens, cu_seqlens, scale,
+                                  softcap, window, alibi_slopes, k_scale, v_scale)
