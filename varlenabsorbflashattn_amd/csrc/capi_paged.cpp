@@ -170,11 +170,10 @@ int check_workspace(const void *workspace, int64_t bytes, int64_t needed) {
 // workspace go by the rows and by what the page table could hold.
 struct ChunkPlan {
   int lg = 0, lt = 0;
-  int64_t chunks = 0, bytes = 0, lse_off = 0;
+  int64_t rows = 0, chunks = 0, bytes = 0, lse_off = 0;
   bool direct = false;
 };
 
-constexpr int64_t kChunkRows = 128;
 // Where no tile can walk more than this many units, none is divided (no launch that joins).
 constexpr int64_t kChunkDirect = 8;
 
@@ -192,20 +191,21 @@ int plan_chunk(const vafa_paged_cache *c, int64_t T, int64_t H, int64_t window, 
   if (window < 0) return fail(VAFA_ERR_VALUE, "%s: window must be positive", what);
   const int64_t G = H / c->Hk;
   while (p->lg < 5 && G % (int64_t{2} << p->lg) == 0) ++p->lg;
-  while ((kChunkRows >> (p->lt + 1)) >= (int64_t{1} << p->lg)) ++p->lt;
+  p->rows = c->D <= 128 ? 256 : 128;
+  p->lt = (c->D <= 128 ? 8 : 7) - p->lg;
   const int64_t sets = H >> p->lg, tw = int64_t{1} << p->lt;
   const int64_t cap = page_capacity(map_of(c));
   const int64_t keys = window > 0 && window < cap ? std::min(cap, window + tw + kChunkKeys) : cap;
   const int64_t most = std::max<int64_t>(1, (keys + kChunkKeys - 1) / kChunkKeys);
   // (a sequence of nq tokens has at most nq / tw + 1 tiles)
   const int64_t tiles = std::max<int64_t>(1, T / tw + std::min(c->n_seq, T));
-  const int64_t slots = c->D <= 128 ? 512 : 256;  // workgroups that the GPU holds
+  const int64_t slots = 256;  // workgroups that the GPU holds: one on a CU
   p->direct = most <= kChunkDirect;
   if (p->direct)
     p->chunks = std::min<int64_t>(tiles, std::max<int64_t>(slots, 65536 / sets));
   else
     p->chunks = std::max<int64_t>(1, std::min(slots / sets, tiles * most));
-  const int64_t rows = p->direct ? 0 : 2 * p->chunks * sets * kChunkRows;
+  const int64_t rows = p->direct ? 0 : 2 * p->chunks * sets * p->rows;
   p->lse_off = rows * c->D * 4;
   p->bytes = p->lse_off + rows * 4;
   return VAFA_OK;
@@ -428,6 +428,13 @@ int vafa_paged_chunk(const vafa_paged_cache *c, const vafa_row_scales *scales, c
   ChunkPlan p;
   if (int rc = plan_chunk(c, T, H, window, &p)) return rc;
   if (int rc = check_codes(what, c, scales)) return rc;
+  for (int64_t x : {c->k_page, c->k_token, c->v_page, c->v_token})
+    if (x / 8 > UINT32_MAX)
+      return fail(VAFA_ERR_VALUE, "%s: strides of the cache of %lld elements", what, (long long)x);
+  if (scales != nullptr)
+    for (int64_t x : {scales->k_page, scales->k_token, scales->v_page, scales->v_token})
+      if (x > UINT32_MAX)
+        return fail(VAFA_ERR_VALUE, "%s: strides of the scales of %lld", what, (long long)x);
   if (int rc = check_scores(what, scale, softcap)) return rc;
   if (int rc = check_rows(what, "q", q, q_token, q_head)) return rc;
   if (int rc = check_rows(what, "out", out, 0, 0)) return rc;
@@ -442,8 +449,10 @@ int vafa_paged_chunk(const vafa_paged_cache *c, const vafa_row_scales *scales, c
   a.slopes = slopes; a.part_o = (float *)workspace;
   a.part_lse = (float *)((char *)workspace + p.lse_off);
   a.map = map_of(c); a.q_token = q_token; a.q_head = q_head;
-  a.k_page = c->k_page; a.kc_token = c->k_token; a.kc_head = c->k_head;
-  a.v_page = c->v_page; a.vc_token = c->v_token; a.vc_head = c->v_head;
+  const int64_t piece = scales != nullptr ? 16 : 8;
+  a.kc_head = c->k_head; a.vc_head = c->v_head;
+  a.k_page = (uint32_t)(c->k_page / piece); a.kc_token = (uint32_t)(c->k_token / piece);
+  a.v_page = (uint32_t)(c->v_page / piece); a.vc_token = (uint32_t)(c->v_token / piece);
   a.scales = scales_of(scales); a.T = T;
   // (so that a key behind the last unit still has a number)
   a.capacity = std::min<int64_t>(page_capacity(a.map), INT32_MAX - 4096);

@@ -152,6 +152,14 @@ __device__ __forceinline__ void lds_dma16(u32x4 r, uint32_t lds_base, int32_t vo
                : "memory", "m0");
 }
 
+// The same from an address of each lane's own.
+__device__ __forceinline__ void lds_dma16(const void *p, uint32_t lds_base) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
+               :
+               : "s"(lds_base), "v"(p)
+               : "memory", "m0");
+}
+
 // 4-byte LDS-DMA load: lane l's dword from `rsrc` at byte offset `voff` lands
 // at LDS address lds_base + 4*l (out-of-range offsets write zeros).
 __device__ __forceinline__ void lds_dma4(u32x4 r, uint32_t lds_base, int32_t voff) {
@@ -164,6 +172,19 @@ __device__ __forceinline__ void lds_dma4(u32x4 r, uint32_t lds_base, int32_t vof
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds"
                :
                : "s"(lds_base), "v"(voff), "s"(q)
+               : "memory", "m0");
+}
+// ... of data that nothing reads again: past the caches.
+__device__ __forceinline__ void lds_dma16_once(const void *p, uint32_t lds_base) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off nt"
+               :
+               : "s"(lds_base), "v"(p)
+               : "memory", "m0");
+}
+__device__ __forceinline__ void lds_dma4(const void *p, uint32_t lds_base) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off"
+               :
+               : "s"(lds_base), "v"(p)
                : "memory", "m0");
 }
 #pragma clang diagnostic pop

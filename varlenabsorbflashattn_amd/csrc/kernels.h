@@ -212,8 +212,9 @@ struct ChunkArgs {
   float *part_o, *part_lse;  // parts of cut tiles: [slots, sets, rows of a tile, D] and [..]
   PageMap map;
   int64_t q_token, q_head;
-  int64_t k_page, kc_token, kc_head, v_page, vc_token, vc_head;
-  RowScales scales;  // of codes, or null
+  int64_t kc_head, vc_head;
+  uint32_t k_page, kc_token, v_page, vc_token;  // in pieces of 16 bytes
+  RowScales scales;  // of codes, or null; page and token strides below 2^32
   int64_t capacity;  // tokens of a sequence's pages
   int64_t T;
   int n_seq, H, Hk, window;  // window 0: all keys

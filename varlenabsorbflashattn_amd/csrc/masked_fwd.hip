@@ -96,7 +96,7 @@ __global__ __launch_bounds__(64 * NW, D >= 256 ? 1 : 2) void masked_fwd_kernel(
     const int kl = (kb + kBN < ke ? kb + kBN : ke) - 1;  // last key of the tile
     if (wave_active && !none_visible(kb, kl, p0, p1, pre, window)) {
       const bool masked = kb + kBN > ke || !all_visible(kb, kl, p0, p1, pre, window);
-      masked_tile<T, D, kCap, kBias>(ks, vs, qf, acc, m_run, l_part, sa, slope2, kb, ke, masked, p,
+      masked_tile<T, D, kCap, kBias>(PaddedTile<T, D>(ks, vs, lane), qf, acc, m_run, l_part, sa, slope2, kb, ke, masked, p,
                                      pre, window, lane);
     }
     if (j + 1 < nt) {

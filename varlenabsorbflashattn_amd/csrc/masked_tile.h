@@ -12,31 +12,45 @@ namespace vafa {
 
 namespace {
 
-// One 64-key tile for the wave's 32 query rows; masked: some (row, key) pair is hidden.  Keys
+// A tile's K and V rows in LDS as the operands of its products: k(kt, cc), the A operand of
+// keys 32 kt + l % 32 and features 16 cc + 8 (l / 32) .. + 7, and v(km, dt), that of
+// features 32 dt .. + 31 and keys 16 km .. + 15 in the order of the C layout (mfma.h).
+template <typename T, int D>
+struct PaddedTile {  // rows with FwdSmem's padding
+  static constexpr int kKeys = kBN;
+  const T *kp, *vs;
+  int lane;
+  __device__ __forceinline__ PaddedTile(const T *ks, const T *vs_, int lane_)
+      : kp(ks + (lane_ & 31) * FwdSmem<D>::KSK + (lane_ >> 5) * 8), vs(vs_), lane(lane_) {}
+  __device__ __forceinline__ u32x4 k(int kt, int cc) const {
+    return *reinterpret_cast<const u32x4 *>(kp + kt * 32 * FwdSmem<D>::KSK + cc * 16);
+  }
+  __device__ __forceinline__ typename Mfma<T>::v8 v(int km, int dt) const {
+    return tr_operand<T>(vs, FwdSmem<D>::KSV, km * 16, dt * 32, lane);
+  }
+};
+
+// One tile (64 keys, or 32) for the wave's 32 query rows; masked: some (row, key) pair is hidden.  Keys
 // whose bit of `here` is not set are hidden from every row (a masked tile's alone).
-template <typename T, int D, bool kCap, bool kBias>
-__device__ __forceinline__ void masked_tile(const T *ks, const T *vs,
+template <typename T, int D, bool kCap, bool kBias, typename Tile>
+__device__ __forceinline__ void masked_tile(const Tile &tile,
                                             const typename Mfma<T>::v8 (&qf)[D / 16],
                                             f32x16 (&acc)[D / 32], float &m_run, float &l_part,
                                             const ScoreArgs &sa, float slope2, int kbase,
                                             int k_end, bool masked, int p, int pre, int window,
                                             int lane, uint64_t here = ~uint64_t{0}) {
   using M = Mfma<T>;
-  constexpr int NC = D / 16, ND = D / 32;
-  constexpr int KS = FwdSmem<D>::KSK, VS = FwdSmem<D>::KSV;
+  constexpr int NC = D / 16, ND = D / 32, KT = Tile::kKeys / 32;
   constexpr bool kLog2 = kCap || kBias;  // s holds log2-domain scores after the transform
-  const int lrow = lane & 31, lhalf = lane >> 5;
+  const int lhalf = lane >> 5;
   constexpr int kPre = 4;
-  constexpr int NS = 2 * NC;
-  f32x16 s[2];
+  constexpr int NS = KT * NC;
+  f32x16 s[KT];
 #pragma unroll
-  for (int kt = 0; kt < 2; ++kt)
+  for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
     for (int r = 0; r < 16; ++r) s[kt][r] = 0.f;
-  const T *kbase_p = ks + lrow * KS + lhalf * 8;
-  auto kop = [&](int i) {  // i = cc * 2 + kt
-    return *reinterpret_cast<const u32x4 *>(kbase_p + (i & 1) * 32 * KS + (i >> 1) * 16);
-  };
+  auto kop = [&](int i) { return tile.k(i % KT, i / KT); };
   u32x4 ring[kPre];
 #pragma unroll
   for (int i = 0; i < kPre; ++i) ring[i] = kop(i);
@@ -44,7 +58,7 @@ __device__ __forceinline__ void masked_tile(const T *ks, const T *vs,
 #pragma unroll
   for (int i = 0; i < NS; ++i) {
     const u32x4 a = ring[i % kPre];
-    s[i & 1] = M::mma(as_v8<T>(a), qf[i >> 1], s[i & 1]);
+    s[i % KT] = M::mma(as_v8<T>(a), qf[i / KT], s[i % KT]);
     if (i + kPre < NS) ring[i % kPre] = kop(i + kPre);
     __builtin_amdgcn_sched_barrier(0);
   }
@@ -53,7 +67,7 @@ __device__ __forceinline__ void masked_tile(const T *ks, const T *vs,
   if constexpr (kLog2) {
     const float back = (float)(p - k_lane);
 #pragma unroll
-    for (int kt = 0; kt < 2; ++kt)
+    for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         float z = s[kt][r] * sa.c;
@@ -66,13 +80,13 @@ __device__ __forceinline__ void masked_tile(const T *ks, const T *vs,
     const uint64_t seen =
         seen_keys(k_lane, k_end, p, pre, window) & (here >> (lhalf * 4));
 #pragma unroll
-    for (int kt = 0; kt < 2; ++kt)
+    for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
       for (int r = 0; r < 16; ++r)
         s[kt][r] = where_bit((uint32_t)(seen >> 32 * kt), off(0, r), s[kt][r], kNegInf);
   }
   const float c = kLog2 ? 1.f : sa.c;
-  typename M::v8 pb[2][2];
+  typename M::v8 pb[KT][2];
   float ps4[4];
   // P is rounded to T, V's type, for the product; its row sum takes the rounded values, in
   // fp32, so that a constant V comes out as it is (outputs in bf16 1.8e-3 off in the 2-norm,
@@ -81,7 +95,7 @@ __device__ __forceinline__ void masked_tile(const T *ks, const T *vs,
 #pragma unroll
     for (int i = 0; i < 4; ++i) ps4[i] = 0.f;
 #pragma unroll
-    for (int kt = 0; kt < 2; ++kt)
+    for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
       for (int mm = 0; mm < 2; ++mm) {
         typename M::v8 x;
@@ -101,7 +115,7 @@ __device__ __forceinline__ void masked_tile(const T *ks, const T *vs,
   if (wave_any(!(ps <= kLazyMax))) {
     float m4[4] = {kNegInf, kNegInf, kNegInf, kNegInf};
 #pragma unroll
-    for (int kt = 0; kt < 2; ++kt)
+    for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
       for (int r = 0; r < 16; ++r) m4[r & 3] = fmaxf(m4[r & 3], s[kt][r]);
     float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
@@ -118,10 +132,9 @@ __device__ __forceinline__ void masked_tile(const T *ks, const T *vs,
     ps = (ps4[0] + ps4[1]) + (ps4[2] + ps4[3]);
   }
   l_part += ps;
-  constexpr int NP = 4 * ND;
+  constexpr int NP = 2 * KT * ND;
   auto vop = [&](int i) {  // i = km * ND + dt, km = kt * 2 + mm
-    const int km = i / ND, dt = i % ND;
-    return tr_operand<T>(vs, VS, km * 16, dt * 32, lane);
+    return tile.v(i / ND, i % ND);
   };
   typename M::v8 vring[kPre];
 #pragma unroll

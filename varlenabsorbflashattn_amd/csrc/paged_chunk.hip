@@ -62,17 +62,18 @@ __device__ __forceinline__ int64_t seq_units(const ChunkArgs &a, int b) {
   const int64_t m = chunk_tiles(s.nq, s.lt);
   return a.direct ? m : chunk_before(s, m);
 }
-__device__ __forceinline__ int64_t all_units(const ChunkArgs &a, int lane) {
-  int64_t total = 0;
-  for (int c = 0; c < a.n_seq; c += 64) total += seq_units(a, c + lane);
+// (`mine`: the units of sequence `lane`, which both of these begin with)
+__device__ __forceinline__ int64_t all_units(const ChunkArgs &a, int64_t mine, int lane) {
+  int64_t total = mine;
+  for (int c = 64; c < a.n_seq; c += 64) total += seq_units(a, c + lane);
   return uniform_l(wave_sum_l(total));
 }
 // The sequence that holds unit `at` of the axis, and the units in front of it.
-__device__ __forceinline__ void find_seq(const ChunkArgs &a, int64_t at, int lane, int *b,
-                                         int64_t *base) {
+__device__ __forceinline__ void find_seq(const ChunkArgs &a, int64_t at, int64_t mine, int lane,
+                                         int *b, int64_t *base) {
   int64_t before = 0;
   for (int c = 0; c < a.n_seq; c += 64) {
-    const int64_t t = seq_units(a, c + lane), incl = wave_scan_l(t, lane) + before;
+    const int64_t t = c == 0 ? mine : seq_units(a, c + lane), incl = wave_scan_l(t, lane) + before;
     const uint64_t past = __builtin_amdgcn_ballot_w64(incl > at);
     if (past != 0) {
       const int f = __builtin_ctzll(past);
@@ -90,30 +91,91 @@ __device__ __forceinline__ int64_t units_per(const ChunkArgs &a, int64_t total) 
   return per < kChunkLeast ? kChunkLeast : per;
 }
 
-// Pieces of 16 bytes of a unit's rows, by thread, and the rows' powers of two.
-template <int D, int NT, bool kCodes>
-struct UnitRegs {
-  static constexpr int kPerRow = D / (kCodes ? 16 : 8);
-  static constexpr int kPieces = kChunkKeys * kPerRow / NT;  // of a thread
-  u32x4 k[kPieces], v[kPieces];
-  uint32_t ke, ve;  // of this lane's key
+// A unit's K and V rows in LDS, without padding: 16-byte piece c of row r lies at c ^ f(r), so
+// that rows can come by LDS-DMA, which writes whole lines, and are still read without bank
+// conflicts: K by 16 rows' same piece at a time (their pieces all over the 64 banks), V by
+// transposing reads of 4 rows' 64 bytes.
+template <int D>
+__device__ __forceinline__ int swizzle_k(int row) {
+  return D == 64 ? row >> 1 & 7 : row & 15;
+}
+template <int D>
+__device__ __forceinline__ int swizzle_v(int row) {
+  return D == 64 ? (row >> 1 & 1) << 2 : (row & 3) << 2;
+}
+// Keys of a unit in LDS: the half of an axis unit at D = 256, where 64 leave no room for
+// units on their way.
+template <int D>
+constexpr int kUnitKeys = D == 256 ? 32 : 64;
+template <typename T, int D>
+struct SwizzledTile {
+  static constexpr int kKeys = kUnitKeys<D>;
+  static constexpr int kRow = 2 * D, kHalf = kKeys * kRow;  // bytes
+  typedef const __attribute__((address_space(3))) u32x4 *lds16;
+  typedef __attribute__((address_space(3))) v4s16 *lds8;
+  uint32_t ka, va;  // LDS addresses of this lane's first pieces
+  static __device__ __forceinline__ SwizzledTile at(uint32_t base, int lane) {
+    const int r = lane & 31, i = lane & 15, g = lane >> 4;
+    const int vr = 4 * (g >> 1) + (i >> 2);
+    SwizzledTile t;
+    t.ka = base + r * kRow + (((lane >> 5) ^ swizzle_k<D>(r)) << 4);
+    t.va = base + kHalf + vr * kRow +
+           ((((g & 1) * 2 + ((i & 3) >> 1)) ^ swizzle_v<D>(vr)) << 4) + (i & 1) * 8;
+    return t;
+  }
+  // (units and rows are multiples of what the exclusive or reaches)
+  __device__ __forceinline__ SwizzledTile at_offset(int bytes) const {
+    return SwizzledTile{ka + bytes, va + bytes};
+  }
+  __device__ __forceinline__ u32x4 k(int kt, int cc) const {
+    return *(lds16)(uintptr_t)((ka ^ ((cc & 7) << 5)) + (cc >> 3) * 256 + kt * 32 * kRow);
+  }
+  __device__ __forceinline__ typename Mfma<T>::v8 v(int km, int dt) const {
+    const uint32_t p = (va ^ ((dt & 3) << 6)) + (dt >> 2) * 256 + km * 16 * kRow;
+    const u32x2 lo = __builtin_bit_cast(
+        u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds8)(uintptr_t)p));
+    const u32x2 hi = __builtin_bit_cast(
+        u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds8)(uintptr_t)(p + 8 * kRow)));
+    return as_v8<T>(join(lo, hi));
+  }
 };
 
-template <typename T, int D, int NW>
-constexpr int chunk_lds() {
-  constexpr int kStage = NW * RowStore<T, D / 32>::kBytes;
-  return FwdSmem<D>::kBytes > kStage ? FwdSmem<D>::kBytes : kStage;
-}
+// What absent keys hold, and their page.
+__device__ const u32x4 kZeroRow[32] = {};
+__device__ const int32_t kNoPage = -1;
 
+// Unit u's rows are asked for kAhead units ahead.  16 bits: into one of kAhead + 1 buffers,
+// from which the products read them.  Codes: into a raw buffer; they become T in one of two
+// buffers a unit ahead.  Beside them, for the units of two blocks of NW: the pages on their way,
+// where each key's rows are, which keys there are and, of codes, the words that hold their
+// powers of two.
+template <int D, int NW, bool kCodes>
+struct ChunkSmem {
+  static constexpr int kKeys = kUnitKeys<D>, kAhead = 3, kRing = 2 * NW;  // units
+  static constexpr int kUnit = 2 * kKeys * 2 * D, kRaw = kUnit / 2;       // bytes, K and V
+  static constexpr int kBuffers = kCodes ? 2 : kAhead + 1;
+  static constexpr int kRawAt = kBuffers * kUnit;
+  static constexpr int kRowsAt = kRawAt + (kCodes ? (kAhead + 1) * kRaw : 0);
+  static constexpr int kIdsAt = kRowsAt + kRing * kKeys * 16;
+  static constexpr int kHereAt = kIdsAt + kRing * 256;
+  static constexpr int kWordsAt = kHereAt + kRing * 8;
+  static constexpr int kBytes = kWordsAt + (kCodes ? kRing * 512 : 0);
+  static_assert(kAhead < NW, "a block's rows are looked up before they are asked for");
+};
+
+// 256 rows of 8 waves (D = 256: 128 of 4, which have its registers), one workgroup on a CU.
 template <typename T, int D, int NW, bool kCodes, bool kCap, bool kBias>
 __global__ __launch_bounds__(64 * NW, D >= 256 ? 1 : 2) void paged_chunk_kernel(ChunkArgs a) {
   using M = Mfma<T>;
   using E = std::conditional_t<kCodes, uint8_t, T>;
-  using R = UnitRegs<D, 64 * NW, kCodes>;
+  using Tile = SwizzledTile<T, D>;
+  using S = ChunkSmem<D, NW, kCodes>;
   constexpr int NC = D / 16, ND = D / 32, NT = 64 * NW, BM = 32 * NW;
-  constexpr int kPiece = 16 / (int)sizeof(E);
-  extern __shared__ __align__(16) unsigned char smem_raw[];
-  T *smem = reinterpret_cast<T *>(smem_raw);
+  constexpr int kKeys = S::kKeys, kAhead = S::kAhead;
+  constexpr int kPiece = 16 / (int)sizeof(E), kPerRow = D / kPiece;  // 16-byte pieces of a row
+  constexpr int kHalf = kKeys * kPerRow;                             // of a unit's K
+  constexpr int kPieces = 2 * kHalf / NT;                            // of a thread, K and V
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lrow = lane & 31, lhalf = lane >> 5;
@@ -140,14 +202,15 @@ __global__ __launch_bounds__(64 * NW, D >= 256 ? 1 : 2) void paged_chunk_kernel(
     }
   }
   if (chunk >= a.chunks) return;
-  const int64_t total = all_units(a, lane);
+  const int64_t mine = seq_units(a, lane);
+  const int64_t total = all_units(a, mine, lane);
   const int64_t per = a.direct ? 1 : units_per(a, total);
   int64_t cur = chunk * per;
   const int64_t end = a.direct || total - cur < per ? total : cur + per;
   if (cur >= end) return;
   int b;
   int64_t base;
-  find_seq(a, cur, lane, &b, &base);
+  find_seq(a, cur, mine, lane, &b, &base);
 
   ScoreArgs sa{a.c, a.cap2};
   uint32_t qsign = 0;
@@ -156,8 +219,10 @@ __global__ __launch_bounds__(64 * NW, D >= 256 ? 1 : 2) void paged_chunk_kernel(
     sa.c = score_factor(sa.c);
   }
   const int window = a.window > 0 ? a.window : kChunkNoWindow;
-  const E *kc = (const E *)a.kc + hk * a.kc_head + tid % R::kPerRow * kPiece;
-  const E *vc = (const E *)a.vc + hk * a.vc_head + tid % R::kPerRow * kPiece;
+  const u32x4 *kc = reinterpret_cast<const u32x4 *>((const E *)a.kc + hk * a.kc_head);
+  const u32x4 *vc = reinterpret_cast<const u32x4 *>((const E *)a.vc + hk * a.vc_head);
+  const uint32_t smem = lds_addr(smem_raw);
+  const Tile tile0 = Tile::at(smem, lane);
 
   while (cur < end) {
     if (b >= a.n_seq) break;
@@ -174,10 +239,11 @@ __global__ __launch_bounds__(64 * NW, D >= 256 ? 1 : 2) void paged_chunk_kernel(
     const int64_t t0 = a.direct ? cur : base + chunk_before(s, i);
     const int64_t units = chunk_units(s, i);
     const int64_t u0 = a.direct ? 0 : cur - t0;
-    const int run = (int)uniform_l(a.direct || units - u0 < end - cur ? units - u0 : end - cur);
-    const bool whole = run == units;
+    const int part = (int)uniform_l(a.direct || units - u0 < end - cur ? units - u0 : end - cur);
+    const bool whole = part == units;
+    const int run = part * (kChunkKeys / kKeys);  // in units of LDS
     const int q0 = __builtin_amdgcn_readfirstlane(at.q0 + (int)(i << s.lt));
-    const int qn = (int)(s.nq - (i << s.lt)), q1 = q0 + uniform_clamp(qn, BM >> lg);
+    const int qn = uniform_clamp((int)(s.nq - (i << s.lt)), BM >> lg), q1 = q0 + qn;
     const int diag = __builtin_amdgcn_readfirstlane((int)(s.diag - at.q0));
     const int kb0 = __builtin_amdgcn_readfirstlane((int)(chunk_start(s, i) + u0 * kChunkKeys));
     const int kend = __builtin_amdgcn_readfirstlane((int)chunk_end(s, i));
@@ -211,92 +277,140 @@ __global__ __launch_bounds__(64 * NW, D >= 256 ? 1 : 2) void paged_chunk_kernel(
       for (int r = 0; r < 16; ++r) acc[x][r] = 0.f;
     float m_run = -kHuge, l_part = 0.f;
 
-    struct Key {
-      int id, slot;  // page (-1: none) and token there of this lane's key of a unit
+    // keys that are read once in the whole call pass the caches (one workgroup reads the
+    // tile's keys for one set: none other does if there is one tile and one set a key head)
+    const bool once = tiles == 1 && hs.per_key() == 1;
+
+    // Each wave looks up the rows of one unit of every block of NW.  First their pages:
+    auto ask_ids = [&](int u) {
+      const int key = kb0 + u * kKeys + lane % kKeys;
+      const int32_t *from = &kNoPage;
+      if (u < run && key >= kfirst && key < kend)  // (within the table: kend is)
+        from = a.map.table + b * a.map.row_stride + page_slot(a.map, key).index;
+      lds_dma4(from, smem + S::kIdsAt + u % S::kRing * 256);
     };
-    auto look_up = [&](int j) {
-      const int key = kb0 + j * kChunkKeys + lane;
-      Key k{-1, 0};
-      if (j < run && key >= kfirst && key < kend) {
-        const PageSlot ps = page_slot(a.map, key);
-        k.id = page_of(a.map, b, key, ps);
-        k.slot = ps.slot;
-      }
-      return k;
-    };
-    R regs;
-    // rows of the unit whose keys the lanes looked up -> which of them there are
-    auto load = [&](Key k) {
-      const bool there = k.id >= 0;
-      const int64_t id = there ? k.id : 0, slot = there ? k.slot : 0;
-      const int64_t ko = id * a.k_page + slot * a.kc_token;
-      const int64_t vo = id * a.v_page + slot * a.vc_token;
-#pragma unroll
-      for (int x = 0; x < R::kPieces; ++x) {
-        const int key = (tid + NT * x) / R::kPerRow;
-        regs.k[x] = *reinterpret_cast<const u32x4 *>(kc + __shfl((long long)ko, key, 64));
-      }
-#pragma unroll
-      for (int x = 0; x < R::kPieces; ++x) {
-        const int key = (tid + NT * x) / R::kPerRow;
-        regs.v[x] = *reinterpret_cast<const u32x4 *>(vc + __shfl((long long)vo, key, 64));
+    // then, of each key, where its rows of K and V are, in pieces of 16 bytes from kc and vc
+    // (zeros for absent keys); a factor of 16 drops the highest bits, which hold, of codes, the
+    // byte of the word that is the row's power of two (0 to 3) and whether there is none (4)
+    auto look_up = [&](int u) {
+      const int id = reinterpret_cast<const int32_t *>(smem_raw + S::kIdsAt)[u % S::kRing * 64 + lane];
+      const bool there = (uint32_t)id < (uint32_t)a.map.n_pages;
+      const uint32_t slot = page_slot(a.map, kb0 + u * kKeys + lane % kKeys).slot;
+      // (32-bit factors: one instruction each)
+      uint64_t k = (uint64_t)(uint32_t)id * a.k_page + (uint64_t)slot * a.kc_token;
+      uint64_t v = (uint64_t)(uint32_t)id * a.v_page + (uint64_t)slot * a.vc_token;
+      if (!there) {
+        k = (uint64_t)((uintptr_t)kZeroRow - (uintptr_t)kc) >> 4;
+        v = (uint64_t)((uintptr_t)kZeroRow - (uintptr_t)vc) >> 4;
       }
       if constexpr (kCodes) {
         const RowScales &sc = a.scales;
-        regs.ke = sc.k[id * sc.k_page + slot * sc.k_token + hk * sc.k_head];
-        regs.ve = sc.v[id * sc.v_page + slot * sc.v_token + hk * sc.v_head];
+        const uint32_t i_ = there ? id : 0, s_ = there ? slot : 0;
+        const uintptr_t ks = (uintptr_t)(sc.k + hk * sc.k_head) +
+                             ((uint64_t)i_ * (uint32_t)sc.k_page + (uint64_t)s_ * (uint32_t)sc.k_token);
+        const uintptr_t vs = (uintptr_t)(sc.v + hk * sc.v_head) +
+                             ((uint64_t)i_ * (uint32_t)sc.v_page + (uint64_t)s_ * (uint32_t)sc.v_token);
+        k |= (uint64_t)((ks & 3) | (there ? 0 : 4)) << 60;
+        v |= (uint64_t)((vs & 3) | (there ? 0 : 4)) << 60;
+        const uint32_t words = smem + S::kWordsAt + u % S::kRing * 512;
+        lds_dma4((const void *)(ks & ~uintptr_t{3}), words);
+        lds_dma4((const void *)(vs & ~uintptr_t{3}), words + 256);
       }
-      return __builtin_amdgcn_ballot_w64(there);
+      *reinterpret_cast<u32x4 *>(smem_raw + S::kRowsAt + (u % S::kRing * kKeys + lane % kKeys) * 16) =
+          u32x4{(uint32_t)k, (uint32_t)(k >> 32), (uint32_t)v, (uint32_t)(v >> 32)};
+      const uint64_t here = __builtin_amdgcn_ballot_w64(there);
+      if (lane == 0)
+        *reinterpret_cast<uint64_t *>(smem_raw + S::kHereAt + u % S::kRing * 8) = here;
     };
-    auto store = [&](int buf, uint64_t here) {
-      T *ks = smem + buf * FwdSmem<D>::kBuf, *vs = ks + FwdSmem<D>::kKs;
+    auto present = [&](int u) {  // which keys of unit u there are
+      return uniform_l(*reinterpret_cast<const int64_t *>(smem_raw + S::kHereAt + u % S::kRing * 8));
+    };
+    // where unit u's K and V rows go: 16 bits to where the products read them, piece by piece
+    // swizzled, codes as they are
+    auto unit_at = [&](int u) { return u % S::kBuffers * S::kUnit; };
+    auto raw_at = [&](int u) { return S::kRawAt + u % (kAhead + 1) * S::kRaw; };
+    // this thread's pieces of a unit, K's rows and then V's (for some waves' pieces K's, for
+    // others' V's where a unit has no more)
+    auto row_of = [&](int x) { return (tid + NT * x) % kHalf / kPerRow; };
+    auto of_v = [&](int x) { return wave * 64 + NT * x >= kHalf; };
+    auto place_of = [&](int u, int x) {
+      return smem_raw + S::kRowsAt + (u % S::kRing * kKeys + row_of(x)) * 16 + (of_v(x) ? 8 : 0);
+    };
+    auto ask_rows = [&](int u) {
+      const uint32_t to = smem + (kCodes ? raw_at(u) : unit_at(u)) + wave * 1024;
+      const u32x4 *from[kPieces];
 #pragma unroll
-      for (int x = 0; x < R::kPieces; ++x) {
-        const int key = (tid + NT * x) / R::kPerRow, f = tid % R::kPerRow * kPiece;
-        u32x4 v = regs.v[x];
-        // values of absent keys are whatever the cache holds: zeros, so that their zero
-        // probabilities do not meet infinities
-        if (!(here >> key & 1)) v = u32x4{0, 0, 0, 0};
-        T *kd = ks + key * FwdSmem<D>::KSK + f, *vd = vs + key * FwdSmem<D>::KSV + f;
-        if constexpr (kCodes) {
-          u32x4 lo, hi;
-          from_codes<T>(regs.k[x], row_scale(__shfl(regs.ke, key, 64)), lo, hi);
-          *reinterpret_cast<u32x4 *>(kd) = lo;
-          *reinterpret_cast<u32x4 *>(kd + 8) = hi;
-          const uint32_t ve = __shfl(regs.ve, key, 64);  // (every lane takes part)
-          from_codes<T>(v, row_scale(here >> key & 1 ? ve : 127), lo, hi);
-          *reinterpret_cast<u32x4 *>(vd) = lo;
-          *reinterpret_cast<u32x4 *>(vd + 8) = hi;
-        } else {
-          *reinterpret_cast<u32x4 *>(kd) = regs.k[x];
-          *reinterpret_cast<u32x4 *>(vd) = v;
-        }
+      for (int x = 0; x < kPieces; ++x) {
+        const int piece = tid % kPerRow, row = row_of(x);
+        const int col = kCodes ? piece : piece ^ (of_v(x) ? swizzle_v<D>(row) : swizzle_k<D>(row));
+        from[x] = (of_v(x) ? vc : kc) + col + *reinterpret_cast<const uint64_t *>(place_of(u, x));
+      }
+      if (once) {
+#pragma unroll
+        for (int x = 0; x < kPieces; ++x) lds_dma16_once(from[x], to + x * NT * 16);
+      } else {
+#pragma unroll
+        for (int x = 0; x < kPieces; ++x) lds_dma16(from[x], to + x * NT * 16);
+      }
+    };
+    // codes: unit u's rows, which this thread asked for, become T
+    auto convert = [&](int u) {
+#pragma unroll
+      for (int x = 0; x < kPieces; ++x) {
+        const int row = row_of(x), piece = tid % kPerRow;
+        const bool is_v = of_v(x);
+        const uint32_t top = reinterpret_cast<const uint32_t *>(place_of(u, x))[1] >> 28;
+        const uint32_t e = smem_raw[S::kWordsAt + u % S::kRing * 512 + is_v * 256 + row * 4 + (top & 3)];
+        // (absent keys are zeros, whatever their power of two)
+        const float scale = top < 4 ? row_scale(e) : 1.f;
+        const u32x4 codes =
+            *reinterpret_cast<const u32x4 *>(smem_raw + raw_at(u) + (tid + NT * x) * 16);
+        u32x4 lo, hi;
+        from_codes<T>(codes, scale, lo, hi);
+        const int c = (2 * piece) ^ (is_v ? swizzle_v<D>(row) : swizzle_k<D>(row));
+        unsigned char *to = smem_raw + unit_at(u) + (is_v ? Tile::kHalf : 0) + row * Tile::kRow;
+        *reinterpret_cast<u32x4 *>(to + c * 16) = lo;
+        *reinterpret_cast<u32x4 *>(to + (c ^ 1) * 16) = hi;
       }
     };
 
-    uint64_t here = load(look_up(0)), there = 0;
-    Key next = look_up(1);
-    store(0, here);
+    // Waits count requests, which come in the order they were made: behind unit j + 1's there
+    // are those of the kAhead - 1 units after it, and pages and words now and then (the wait is
+    // then for a little more).  Past the piece's end the requests go on (for zeros).
+    constexpr int kRequests = (kAhead - 1) * kPieces;
+    ask_ids(wave);
+    ask_ids(NW + wave);
+    wait_vmcnt<0>();
+    look_up(wave);
     __syncthreads();
-    auto step = [&](int j, auto buf) {
-      const int B = buf;
-      if (j + 1 < run) {
-        there = load(next);
-        next = look_up(j + 2);
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) ask_rows(u);
+    wait_vmcnt<kRequests>();
+    if constexpr (kCodes) {
+      __syncthreads();  // words that other waves asked for
+      convert(0);
+    }
+    __syncthreads();
+    for (int j = 0; j < run; ++j) {
+      if (j % NW == 0) {  // a block's rows before its first are asked for, pages a block ahead
+        look_up(j + NW + wave);
+        ask_ids(j + 2 * NW + wave);
       }
-      const T *ks = smem + B * FwdSmem<D>::kBuf;
-      const int kb = kb0 + j * kChunkKeys;
-      const int kl = (kb + kChunkKeys < kend ? kb + kChunkKeys : kend) - 1;
+      ask_rows(j + kAhead);
+      const int kb = kb0 + j * kKeys;
+      const int kl = (kb + kKeys < kend ? kb + kKeys : kend) - 1;
       if (wave_active && !none_visible(kb, kl, p0, p1, 0, window)) {
+        const uint64_t here = present(j);
         const bool masked = here != ~uint64_t{0} || !all_visible(kb, kl, p0, p1, 0, window);
-        masked_tile<T, D, kCap, kBias>(ks, ks + FwdSmem<D>::kKs, qf, acc, m_run, l_part, sa, slope2,
-                                       kb, kend, masked, p, 0, window, lane, here);
+        masked_tile<T, D, kCap, kBias>(tile0.at_offset(unit_at(j)), qf, acc, m_run, l_part, sa,
+                                       slope2, kb, kend, masked, p, 0, window, lane, here);
       }
-      if (j + 1 < run) store(1 - B, there);
-      here = there;
+      wait_vmcnt<kRequests>();
+      if constexpr (kCodes) convert(j + 1);
       __syncthreads();
-    };
-    for (int j = 0; j < run; ++j) step(j, j & 1);
+    }
+    wait_vmcnt<0>();  // nothing on its way to what the rows' store takes
+    __syncthreads();
 
     if (wave_active) {
       // a row that sees no key has l = 0 (output 0, lse -inf); NaN scores stay NaN
@@ -320,11 +434,18 @@ __global__ __launch_bounds__(64 * NW, D >= 256 ? 1 : 2) void paged_chunk_kernel(
     __syncthreads();  // the staged rows are read: the next piece may write K and V
     if (a.direct) {
       cur += a.chunks;
-      if (cur < end) find_seq(a, cur, lane, &b, &base);
+      if (cur < end) find_seq(a, cur, mine, lane, &b, &base);
     } else {
-      cur += run;
+      cur += part;
     }
   }
+}
+
+template <typename T, int D, int NW, bool kCodes>
+constexpr int chunk_lds() {
+  constexpr int kStage = NW * RowStore<T, D / 32>::kBytes;
+  static_assert(kStage <= ChunkSmem<D, NW, kCodes>::kBytes, "staged rows");
+  return ChunkSmem<D, NW, kCodes>::kBytes;
 }
 
 // Joins the parts of a tile that chunks cut: a group of workgroups for each border between
@@ -339,11 +460,12 @@ __global__ __launch_bounds__(256) void paged_chunk_join_kernel(ChunkArgs a) {
   const int sets = hs.sets();
   const int part = blockIdx.x % kParts, set = blockIdx.x / kParts % sets;
   const int64_t c = blockIdx.x / kParts / sets + 1;
-  const int64_t total = all_units(a, lane), per = units_per(a, total), u = c * per;
+  const int64_t mine = seq_units(a, lane);
+  const int64_t total = all_units(a, mine, lane), per = units_per(a, total), u = c * per;
   if (u >= total) return;
   int b;
   int64_t base;
-  find_seq(a, u, lane, &b, &base);
+  find_seq(a, u, mine, lane, &b, &base);
   if (b >= a.n_seq) return;
   const SeqAt at = seq_at(a, b);
   const ChunkSeq &s = at.s;
@@ -385,11 +507,10 @@ __global__ __launch_bounds__(256) void paged_chunk_join_kernel(ChunkArgs a) {
   }
 }
 
-template <typename T, int D, bool kCodes, bool kCap, bool kBias>
+template <typename T, int D, int NW, bool kCodes, bool kCap, bool kBias>
 void launch_v(const ChunkArgs &a, hipStream_t st) {
-  constexpr int NW = 4;
   constexpr auto fn = &paged_chunk_kernel<T, D, NW, kCodes, kCap, kBias>;
-  const int smem = chunk_lds<T, D, NW>(), sets = a.H >> a.lg;
+  const int smem = chunk_lds<T, D, NW, kCodes>(), sets = a.H >> a.lg;
   allow_dynamic_lds(reinterpret_cast<const void *>(fn), smem);
   const int64_t wgs = (int64_t)(a.chunks + kXcds - 1) / kXcds * kXcds * sets;
   hipLaunchKernelGGL(fn, dim3((unsigned)wgs), dim3(64 * NW), smem, st, a);
@@ -401,11 +522,12 @@ void launch_v(const ChunkArgs &a, hipStream_t st) {
 
 template <typename T, int D, bool kCodes>
 void launch_d(const ChunkArgs &a, hipStream_t st) {
+  constexpr int NW = D <= 128 ? 8 : 4;
   const bool cap = a.cap2 > 0.f, bias = a.slopes != nullptr;
-  if (cap && bias) return launch_v<T, D, kCodes, true, true>(a, st);
-  if (cap) return launch_v<T, D, kCodes, true, false>(a, st);
-  if (bias) return launch_v<T, D, kCodes, false, true>(a, st);
-  launch_v<T, D, kCodes, false, false>(a, st);
+  if (cap && bias) return launch_v<T, D, NW, kCodes, true, true>(a, st);
+  if (cap) return launch_v<T, D, NW, kCodes, true, false>(a, st);
+  if (bias) return launch_v<T, D, NW, kCodes, false, true>(a, st);
+  launch_v<T, D, NW, kCodes, false, false>(a, st);
 }
 
 }  // namespace
