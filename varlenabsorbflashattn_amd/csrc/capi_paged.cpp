@@ -69,8 +69,14 @@ int check_codes(const char *what, const vafa_paged_cache *c, const vafa_row_scal
       return fail(VAFA_ERR_VALUE, "%s: strides of codes must be multiples of 16, got %lld", what,
                   (long long)x);
   for (int64_t x : {s->k_page, s->k_token, s->k_head, s->v_page, s->v_token, s->v_head})
-    if (x < 0)
-      return fail(VAFA_ERR_VALUE, "%s: the scales' strides must not be negative", what);
+    if (x < 0 || x > UINT32_MAX)
+      return fail(VAFA_ERR_VALUE, "%s: the scales' strides must be below 2^32, got %lld", what,
+                  (long long)x);
+  // (the kernels' factors: strides in pieces of 16 bytes)
+  for (int64_t x : {c->k_page, c->k_token, c->v_page, c->v_token})
+    if (x / 16 > UINT32_MAX)
+      return fail(VAFA_ERR_VALUE, "%s: strides of codes must be below 2^36, got %lld", what,
+                  (long long)x);
   return VAFA_OK;
 }
 
@@ -430,11 +436,8 @@ int vafa_paged_chunk(const vafa_paged_cache *c, const vafa_row_scales *scales, c
   if (int rc = check_codes(what, c, scales)) return rc;
   for (int64_t x : {c->k_page, c->k_token, c->v_page, c->v_token})
     if (x / 8 > UINT32_MAX)
-      return fail(VAFA_ERR_VALUE, "%s: strides of the cache of %lld elements", what, (long long)x);
-  if (scales != nullptr)
-    for (int64_t x : {scales->k_page, scales->k_token, scales->v_page, scales->v_token})
-      if (x > UINT32_MAX)
-        return fail(VAFA_ERR_VALUE, "%s: strides of the scales of %lld", what, (long long)x);
+      return fail(VAFA_ERR_VALUE, "%s: the cache's strides must be below 2^35, got %lld", what,
+                  (long long)x);
   if (int rc = check_scores(what, scale, softcap)) return rc;
   if (int rc = check_rows(what, "q", q, q_token, q_head)) return rc;
   if (int rc = check_rows(what, "out", out, 0, 0)) return rc;

@@ -349,94 +349,17 @@ __global__ __launch_bounds__(256, D >= 128 ? 2 : 3) void paged_decode_kernel(Dec
     float slope2 = 0.f;
     if (a.slopes != nullptr) slope2 = a.slopes[h0 + (l16 < rows ? l16 : 0)] * kLog2e;
 
-    // this lane's key of each group of step u (of the wave's 32 keys in tile u / kSteps):
-    // page and token in it
-    struct Keys {
-      int id[KG], slot[KG];
-    };
-    auto keys_at = [&](int u) {  // the step's first key
+    auto keys_at = [&](int u) {  // the first key of step u (of the wave's 32 in tile u / kSteps)
       return lo + u / kSteps * kDecodeTile + wave * 32 + u % kSteps * S::kRows;
     };
-    auto keys_of = [&](int u) {
-      Keys k;
-#pragma unroll
-      for (int i = 0; i < KG; ++i) {
-        const int t = u / kSteps, key = keys_at(u) + 16 * i + l16;
-        const PageSlot s = page_slot(a.map, key);
-        k.id[i] = t < t0 + run && key < len ? page_of(a.map, b, key, s) : -1;
-        k.slot[i] = s.slot;
-      }
-      return k;
-    };
-    // the step's rows of K and V by whole rows: instruction i takes the rows i * kRows +
-    // lane / kLanes, whose places the lanes that looked them up hand over
-    u32x4 kr[NI], vr[NI];
-    uint32_t ke[NI], ve[NI];  // kCodes: their powers of two
-    auto load = [&](const Keys &k) {
-#pragma unroll
-      for (int i = 0; i < NI; ++i) {
-        const int row = i * kRows + lane / kLanes;
-        // (the rows of one instruction lie in one group)
-        const int id = __shfl(k.id[i * kRows / 16], row & 15, 64);
-        const int slot = __shfl(k.slot[i * kRows / 16], row & 15, 64);
-        const int64_t ko = id >= 0 ? id * a.k_page + slot * a.kc_token : 0;
-        const int64_t vo = id >= 0 ? id * a.v_page + slot * a.vc_token : 0;
-        kr[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(kc + ko));
-        vr[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(vc + vo));
-        if constexpr (kCodes) {
-          const RowScales &s = a.scales;
-          const int64_t p = id >= 0 ? id : 0, t = id >= 0 ? slot : 0;
-          ke[i] = s.k[p * s.k_page + t * s.k_token + hk * s.k_head];
-          ve[i] = s.v[p * s.v_page + t * s.v_token + hk * s.v_head];
-        }
-      }
-    };
-
     f32x4 acc[ND];
 #pragma unroll
     for (int i = 0; i < ND; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
     float m_run = -kHuge, l_run = 0.f;
     const int u0 = t0 * kSteps, u1 = (t0 + run) * kSteps;
-    Keys now = keys_of(u0);
-    load(now);
-    Keys next = keys_of(u0 + 1);
-    for (int u = u0; u < u1; ++u) {
-      // which of the step's keys there are (bit: key)
-      uint32_t ok = 0;
-#pragma unroll
-      for (int i = 0; i < KG; ++i)
-        ok |= (uint32_t)(__builtin_amdgcn_ballot_w64(now.id[i] >= 0) & 0xffffu) << 16 * i;
-      if (ok != 0xffffffffu >> (32 - S::kRows)) {
-        // values of absent keys are whatever the cache holds: zeros instead, so that
-        // their zero probabilities do not meet infinities
-#pragma unroll
-        for (int i = 0; i < NI; ++i)
-          if (!(ok >> (i * kRows + lane / kLanes) & 1)) {
-            vr[i] = u32x4{0, 0, 0, 0};
-            if constexpr (kCodes) ve[i] = 127;
-          }
-      }
-#pragma unroll
-      for (int i = 0; i < NI; ++i) {
-        const int at = (i * kRows + lane / kLanes) * S::kVS + lane % kLanes * kPiece;
-        if constexpr (kCodes) {
-          u32x4 lo, hi;
-          from_codes<T>(kr[i], row_scale(ke[i]), lo, hi);
-          *reinterpret_cast<u32x4 *>(ks + at) = lo;
-          *reinterpret_cast<u32x4 *>(ks + at + 8) = hi;
-          from_codes<T>(vr[i], row_scale(ve[i]), lo, hi);
-          *reinterpret_cast<u32x4 *>(vs + at) = lo;
-          *reinterpret_cast<u32x4 *>(vs + at + 8) = hi;
-        } else {
-          *reinterpret_cast<u32x4 *>(ks + at) = kr[i];
-          *reinterpret_cast<u32x4 *>(vs + at) = vr[i];
-        }
-      }
-      now = next;
-      if (u + 1 < u1) {
-        load(now);
-        next = keys_of(u + 2);
-      }
+    // the scores, softmax and product with V of step u, whose rows are in LDS; ok: which of
+    // its keys there are (bit: key)
+    auto attend = [&](int u, uint32_t ok) {
       f32x4 s[KG];
 #pragma unroll
       for (int i = 0; i < KG; ++i) {
@@ -486,6 +409,138 @@ __global__ __launch_bounds__(256, D >= 128 ? 2 : 3) void paged_decode_kernel(Dec
           acc[i] = M::mma(as_v8<T>(join(lds_tr16(tr), lds_tr16(tr + 16 * S::kVS))), p, acc[i]);
         else
           acc[i] = M::mma4(lds_tr16(tr), p, acc[i]);
+      }
+    };
+    if constexpr (!kCodes) {
+      // this lane's key of each group of a step: page and token in it
+      struct Keys {
+        int id[KG], slot[KG];
+      };
+      auto keys_of = [&](int u) {
+        Keys k;
+#pragma unroll
+        for (int i = 0; i < KG; ++i) {
+          const int t = u / kSteps, key = keys_at(u) + 16 * i + l16;
+          const PageSlot s = page_slot(a.map, key);
+          k.id[i] = t < t0 + run && key < len ? page_of(a.map, b, key, s) : -1;
+          k.slot[i] = s.slot;
+        }
+        return k;
+      };
+      // the step's rows of K and V by whole rows: instruction i takes the rows i * kRows +
+      // lane / kLanes, whose places the lanes that looked them up hand over
+      u32x4 kr[NI], vr[NI];
+      auto load = [&](const Keys &k) {
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+          const int row = i * kRows + lane / kLanes;
+          // (the rows of one instruction lie in one group)
+          const int id = __shfl(k.id[i * kRows / 16], row & 15, 64);
+          const int slot = __shfl(k.slot[i * kRows / 16], row & 15, 64);
+          const int64_t ko = id >= 0 ? id * a.k_page + slot * a.kc_token : 0;
+          const int64_t vo = id >= 0 ? id * a.v_page + slot * a.vc_token : 0;
+          kr[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(kc + ko));
+          vr[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(vc + vo));
+        }
+      };
+      Keys now = keys_of(u0);
+      load(now);
+      Keys next = keys_of(u0 + 1);
+      for (int u = u0; u < u1; ++u) {
+        uint32_t ok = 0;
+#pragma unroll
+        for (int i = 0; i < KG; ++i)
+          ok |= (uint32_t)(__builtin_amdgcn_ballot_w64(now.id[i] >= 0) & 0xffffu) << 16 * i;
+        if (ok != 0xffffffffu >> (32 - S::kRows)) {
+          // values of absent keys are whatever the cache holds: zeros instead, so that
+          // their zero probabilities do not meet infinities
+#pragma unroll
+          for (int i = 0; i < NI; ++i)
+            if (!(ok >> (i * kRows + lane / kLanes) & 1)) vr[i] = u32x4{0, 0, 0, 0};
+        }
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+          const int at = (i * kRows + lane / kLanes) * S::kVS + lane % kLanes * 8;
+          *reinterpret_cast<u32x4 *>(ks + at) = kr[i];
+          *reinterpret_cast<u32x4 *>(vs + at) = vr[i];
+        }
+        now = next;
+        if (u + 1 < u1) {
+          load(now);
+          next = keys_of(u + 2);
+        }
+        attend(u, ok);
+      }
+    } else {
+      // Codes: rows of half the bytes, so those of two steps are on their way.  Lane l looks
+      // up key l % kRows of a step, forms the offsets of its rows, and asks for the power of
+      // two of K's row or V's.
+      struct Key {
+        int id, slot;
+      };
+      auto key_of = [&](int u) {
+        const int key = keys_at(u) + lane % S::kRows;
+        const PageSlot s = page_slot(a.map, key);
+        return Key{u < u1 && key < len ? page_of(a.map, b, key, s) : -1, s.slot};
+      };
+      struct Rows {
+        u32x4 k[NI], v[NI];
+        uint32_t e, ok;
+      };
+      const bool e_of_v = lane / S::kRows % 2;
+      const RowScales &sc = a.scales;
+      const uint8_t *es = e_of_v ? sc.v + hk * sc.v_head : sc.k + hk * sc.k_head;
+      const uint32_t e_page = (uint32_t)(e_of_v ? sc.v_page : sc.k_page);
+      const uint32_t e_token = (uint32_t)(e_of_v ? sc.v_token : sc.k_token);
+      // (strides in 16 bytes, 32-bit factors: one instruction each)
+      const uint32_t kp = (uint32_t)(a.k_page >> 4), kt = (uint32_t)(a.kc_token >> 4);
+      const uint32_t vp = (uint32_t)(a.v_page >> 4), vt = (uint32_t)(a.vc_token >> 4);
+      const bool alike = kp == vp && kt == vt;
+      auto load = [&](Key k, Rows &r) {
+        const bool there = k.id >= 0;
+        const uint32_t id = there ? k.id : 0, slot = there ? k.slot : 0;
+        r.e = es[(uint64_t)id * e_page + (uint64_t)slot * e_token];
+        r.ok = (uint32_t)__builtin_amdgcn_ballot_w64(there) & 0xffffffffu >> (32 - S::kRows);
+        const uint64_t ko = (uint64_t)id * kp + (uint64_t)slot * kt;
+        const uint64_t vo = (uint64_t)id * vp + (uint64_t)slot * vt;
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+          const int row = i * kRows + lane / kLanes;
+          const uint64_t x = __shfl((unsigned long long)ko, row, 64);
+          const uint64_t y = alike ? x : (uint64_t)__shfl((unsigned long long)vo, row, 64);
+          r.k[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(kc) + x);
+          r.v[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(vc) + y);
+        }
+      };
+      Key next = key_of(u0 + 2);
+      auto step = [&](int u, Rows &r) {
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+          const int row = i * kRows + lane / kLanes, at = row * S::kVS + lane % kLanes * kPiece;
+          const float ke = row_scale(__shfl(r.e, row, 64));
+          const float ve = row_scale(__shfl(r.e, S::kRows + row, 64));
+          u32x4 low, high;
+          from_codes<T>(r.k[i], ke, low, high);
+          *reinterpret_cast<u32x4 *>(ks + at) = low;
+          *reinterpret_cast<u32x4 *>(ks + at + 8) = high;
+          from_codes<T>(r.v[i], ve, low, high);
+          if (!(r.ok >> row & 1)) low = high = u32x4{0, 0, 0, 0};  // (as in 16 bits)
+          *reinterpret_cast<u32x4 *>(vs + at) = low;
+          *reinterpret_cast<u32x4 *>(vs + at + 8) = high;
+        }
+        const uint32_t ok = r.ok;
+        if (u + 2 < u1) {
+          load(next, r);
+          next = key_of(u + 3);
+        }
+        attend(u, ok);
+      };
+      Rows one, two;
+      load(key_of(u0), one);
+      load(key_of(u0 + 1), two);
+      for (int u = u0; u < u1; u += 2) {
+        step(u, one);
+        if (u + 1 < u1) step(u + 1, two);
       }
     }
     l_run += __shfl_xor(l_run, 16, 64);
