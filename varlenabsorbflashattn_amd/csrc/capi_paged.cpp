@@ -341,7 +341,7 @@ int vafa_paged_gather(const vafa_paged_cache *c, const vafa_row_scales *scales, 
   if (c->D < 16 || c->D > 1024 || c->D % 16 != 0)
     return fail(VAFA_ERR_ASSERT, "%s: head_dim %lld not supported (multiples of 16 up to 1024)",
                 what, (long long)c->D);
-  if (T < 0 || T > INT32_MAX || !grid_ok(T * (2 * c->Hk * (c->D / 16)) / 512 + 1, 256))
+  if (T < 0 || T > INT32_MAX || !grid_ok(T * (2 * c->Hk * (c->D / 16)) / 256 + 1, 256))
     return fail(VAFA_ERR_VALUE, "%s: %lld rows are too many for a call", what, (long long)T);
   if (int rc = check_rows(what, "k", k, 0, 0)) return rc;
   if (int rc = check_rows(what, "v", v, 0, 0)) return rc;

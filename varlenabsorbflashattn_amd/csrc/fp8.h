@@ -63,16 +63,13 @@ __device__ __forceinline__ float to_code_range(float x, float inv, float limit) 
   const float y = __builtin_amdgcn_fmed3f(x * inv, -limit, limit);
   return fabsf(x) < __builtin_inff() ? y : __builtin_nanf("");
 }
-// Eight values as codes.
-__device__ __forceinline__ u32x2 to_codes(const float *x, float inv, float limit) {
+// Eight values, times inv within 448 (or NaN), as codes.
+__device__ __forceinline__ u32x2 to_codes(const float *x, float inv) {
   u32x2 r;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    float y[4];
-#pragma unroll
-    for (int t = 0; t < 4; ++t) y[t] = to_code_range(x[4 * i + t], inv, limit);
-    int w = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
-    w = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], w, true);
+    int w = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * i] * inv, x[4 * i + 1] * inv, 0, false);
+    w = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * i + 2] * inv, x[4 * i + 3] * inv, w, true);
     r[i] = (uint32_t)w;
   }
   return r;

@@ -26,15 +26,26 @@ __device__ __forceinline__ void load8(const T *p, float *f) {
 #pragma unroll
   for (int e = 0; e < 8; ++e) f[e] = to_f(x[e]);
 }
-// Weights, which need not be aligned.
-template <typename T>
-__device__ __forceinline__ void load_weights(const void *w, bool f32, int at, float *f) {
-  if (f32) {
+// The weights of q and then k in LDS, fp32 (ones where there are none); they need not be
+// aligned.
+template <typename T, int D>
+__device__ __forceinline__ void stage_weights(float *to, const void *q, const void *k, bool f32,
+                                              int tid) {
+  for (int i = tid; i < 2 * D; i += 256) {
+    const void *w = i < D ? q : k;
+    const int at = i < D ? i : i - D;
+    to[i] = w == nullptr ? 1.f
+            : f32        ? static_cast<const float *>(w)[at]
+                         : to_f(static_cast<const T *>(w)[at]);
+  }
+}
+__device__ __forceinline__ void load_weights(const float *w, int at, float *f) {
+  const f32x4 x = *reinterpret_cast<const f32x4 *>(w + at);
+  const f32x4 y = *reinterpret_cast<const f32x4 *>(w + at + 4);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] = static_cast<const float *>(w)[at + e];
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] = to_f(static_cast<const T *>(w)[at + e]);
+  for (int e = 0; e < 4; ++e) {
+    f[e] = x[e];
+    f[4 + e] = y[e];
   }
 }
 template <typename T>
@@ -45,18 +56,28 @@ __device__ __forceinline__ u32x4 pack_row(const float *f) {
   return __builtin_bit_cast(u32x4, x);
 }
 
-// Sum and maximum over the U lanes of a row (U a power of two, rows aligned to it).
-template <int U>
-__device__ __forceinline__ float row_sum(float x) {
-#pragma unroll
-  for (int o = 1; o < U; o <<= 1) x += __shfl_xor(x, o, 64);
+// Sum and maximum over the U lanes of a row (4, 8 or 16, rows aligned to them): neighbours,
+// pairs, then mirrored halves and rows of 16 lanes, whose partial results are alike on both
+// sides; in registers, without the LDS round trip of a shuffle.
+template <int U, typename X, typename F>
+__device__ __forceinline__ X row_reduce(X x, F f) {
+  auto with = [&](auto ctrl) {
+    return f(x, __builtin_bit_cast(X, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x),
+                                                              decltype(ctrl)::value, 0xf, 0xf, true)));
+  };
+  x = with(std::integral_constant<int, 0xb1>{});                        // lanes 1 0 3 2 of 4
+  x = with(std::integral_constant<int, 0x4e>{});                        // lanes 2 3 0 1 of 4
+  if constexpr (U >= 8) x = with(std::integral_constant<int, 0x141>{});   // 8 lanes mirrored
+  if constexpr (U >= 16) x = with(std::integral_constant<int, 0x140>{});  // 16 lanes mirrored
   return x;
 }
 template <int U>
-__device__ __forceinline__ float row_max(float x) {
-#pragma unroll
-  for (int o = 1; o < U; o <<= 1) x = fmaxf(x, __shfl_xor(x, o, 64));
-  return x;
+__device__ __forceinline__ float row_sum(float x) {
+  return row_reduce<U>(x, [](float a, float b) { return a + b; });
+}
+template <int U>
+__device__ __forceinline__ uint32_t row_max(uint32_t x) {
+  return row_reduce<U>(x, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
 }
 
 // The lane's 16 features f: pieces of 8 at 8 c0 and 8 c1.  Of the first `turned` lanes of a
@@ -96,9 +117,9 @@ __device__ __forceinline__ void turn_pieces(float *f, const float2 *cs, bool int
   }
 }
 
-struct RowPlace {  // of a token: places and position
-  int64_t k_off, v_off;
-  int pos, id, slot, ok;  // ok: some sequence holds it
+struct RowPlace {  // of a token: places of its rows and their powers of two, position
+  int64_t k_off, v_off, ks_off, vs_off;
+  int pos, ok;  // ok: some sequence holds it
 };
 
 enum RowsTo { kCache16, kCache8, kPackedRows };
@@ -111,7 +132,8 @@ __global__ __launch_bounds__(256, 4) void head_rows_kernel(HeadRowsArgs s, int s
   constexpr int U = D / 16;
   const AppendArgs &a = s.a;
   extern __shared__ __align__(16) unsigned char smem[];
-  RowPlace *tok = reinterpret_cast<RowPlace *>(smem);
+  float *weights = reinterpret_cast<float *>(smem);  // [2][D]
+  RowPlace *tok = reinterpret_cast<RowPlace *>(weights + 2 * D);
   float2 *turns = reinterpret_cast<float2 *>(tok + span);  // [span][half]
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int heads = a.H + a.Hk + (kTo == kPackedRows ? 0 : a.Hk), per = heads * U;
@@ -150,13 +172,18 @@ __global__ __launch_bounds__(256, 4) void head_rows_kernel(HeadRowsArgs s, int s
   }
   if constexpr (kTo == kPackedRows) {
     for (int i = tid; i < nt; i += 256)
-      tok[i] = RowPlace{(int64_t)(t0 + i) * a.Hk * D, 0, half > 0 ? s.positions[t0 + i] : 0, 0, 0, 1};
+      tok[i] = RowPlace{(int64_t)(t0 + i) * a.Hk * D, 0, 0, 0, half > 0 ? s.positions[t0 + i] : 0, 1};
   } else {
     for (int i = wave; i < nt; i += 4) {
       const TokenAt at = token_at(a, t0 + i, lane);
-      if (lane == 0) tok[i] = RowPlace{at.k_off, at.v_off, at.pos, at.id, at.slot, at.pos >= 0};
+      const int64_t id = at.id, slot = at.slot;
+      if (lane == 0)
+        tok[i] = RowPlace{at.k_off, at.v_off, id * s.scales.k_page + slot * s.scales.k_token,
+                          id * s.scales.v_page + slot * s.scales.v_token, at.pos, at.pos >= 0};
     }
   }
+  const bool normed = s.q_weight != nullptr || s.k_weight != nullptr;
+  if (normed) stage_weights<T, D>(weights, s.q_weight, s.k_weight, s.weights_f32, tid);
   if (half > 0) {
     __syncthreads();
     for (int i = tid; i < nt * half; i += 256) {
@@ -180,17 +207,16 @@ __global__ __launch_bounds__(256, 4) void head_rows_kernel(HeadRowsArgs s, int s
 #pragma unroll
       for (int e = 0; e < 8; ++e) f[8 * h + e] = to_f(v[e]);
     }
-    const void *w = is_q ? s.q_weight : is_k ? s.k_weight : nullptr;
-    if (s.q_weight != nullptr || s.k_weight != nullptr) {
+    if (normed) {
       float ss = 0.f;
 #pragma unroll
       for (int e = 0; e < 16; ++e) ss += f[e] * f[e];
       ss = row_sum<U>(ss);
-      if (w != nullptr) {
+      if ((is_q ? s.q_weight : is_k ? s.k_weight : nullptr) != nullptr) {
         const float rn = rsqrtf(ss * (1.f / D) + s.eps);
         float g[16];
-        load_weights<T>(w, s.weights_f32, 8 * u.x.c0, g);
-        load_weights<T>(w, s.weights_f32, 8 * u.x.c1, g + 8);
+        load_weights(weights + (is_q ? 0 : D), 8 * u.x.c0, g);
+        load_weights(weights + (is_q ? 0 : D), 8 * u.x.c1, g + 8);
 #pragma unroll
         for (int e = 0; e < 16; ++e) f[e] = f[e] * rn * g[e];
       }
@@ -209,24 +235,37 @@ __global__ __launch_bounds__(256, 4) void head_rows_kernel(HeadRowsArgs s, int s
     const int h = is_k ? u.head - a.H : u.head - a.H - a.Hk;
     const int64_t to = is_k ? at.k_off + h * a.kc_head : at.v_off + h * a.vc_head;
     if constexpr (kTo == kCache8) {
-      float amax = 0.f;
+      // |x| as integers, which are ordered alike, infinities and NaN behind all others
+      uint32_t top = 0;
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
-        const float m = fabsf(f[e]);
-        amax = m < __builtin_inff() ? fmaxf(amax, m) : amax;
+        const uint32_t m = __float_as_uint(f[e]) & 0x7fffffffu;
+        top = m > top ? m : top;
       }
-      amax = row_max<U>(amax);
+      top = row_max<U>(top);
       float limit;
-      const int e2 = row_exponent<T>(amax, &limit);
-      const float inv = __uint_as_float((uint32_t)(127 - e2) << 23);
+      int e2 = row_exponent<T>(__uint_as_float(top), &limit);
       uint8_t *dst = (uint8_t *)(is_k ? a.kc : a.vc) + to;
-      *reinterpret_cast<u32x2 *>(dst + 8 * u.x.c0) = to_codes(f, inv, limit);
-      *reinterpret_cast<u32x2 *>(dst + 8 * u.x.c1) = to_codes(f + 8, inv, limit);
+      if (top < 0x7f800000u && limit == 448.f) {
+        const float inv = __uint_as_float((uint32_t)(127 - e2) << 23);
+        *reinterpret_cast<u32x2 *>(dst + 8 * u.x.c0) = to_codes(f, inv);
+        *reinterpret_cast<u32x2 *>(dst + 8 * u.x.c1) = to_codes(f + 8, inv);
+      } else {  // something that is not finite, or the type's last binade
+        float amax = 0.f;
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          amax = fabsf(f[e]) < __builtin_inff() ? fmaxf(amax, fabsf(f[e])) : amax;
+        amax = __uint_as_float(row_max<U>(__float_as_uint(amax)));
+        e2 = row_exponent<T>(amax, &limit);
+        const float inv = __uint_as_float((uint32_t)(127 - e2) << 23);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) f[e] = to_code_range(f[e], inv, limit);
+        *reinterpret_cast<u32x2 *>(dst + 8 * u.x.c0) = to_codes(f, 1.f);
+        *reinterpret_cast<u32x2 *>(dst + 8 * u.x.c1) = to_codes(f + 8, 1.f);
+      }
       if (u.x.p == 0) {
-        uint8_t *sc = is_k ? s.scales.k + at.id * s.scales.k_page + at.slot * s.scales.k_token +
-                                 h * s.scales.k_head
-                           : s.scales.v + at.id * s.scales.v_page + at.slot * s.scales.v_token +
-                                 h * s.scales.v_head;
+        uint8_t *sc = is_k ? s.scales.k + at.ks_off + h * s.scales.k_head
+                           : s.scales.v + at.vs_off + h * s.scales.v_head;
         *sc = (uint8_t)(e2 + 127);
       }
     } else {
@@ -246,8 +285,9 @@ __global__ __launch_bounds__(256, 4) void head_rows_bwd_kernel(HeadRowsBwdArgs a
                                                                int runs) {
   constexpr int U = D / 16;
   extern __shared__ __align__(16) unsigned char smem[];
-  int *pos = reinterpret_cast<int *>(smem);
-  float2 *turns = reinterpret_cast<float2 *>(smem + ((span * 4 + 15) & ~15));
+  float *weights = reinterpret_cast<float *>(smem);  // [2][D]
+  int *pos = reinterpret_cast<int *>(weights + 2 * D);
+  float2 *turns = reinterpret_cast<float2 *>(pos + ((span + 3) & ~3));
   __shared__ __align__(16) float red[256][17];
   const int tid = threadIdx.x;
   const int per = (a.H + a.Hk) * U, half = a.rot / 2, turned = half / 8;
@@ -257,47 +297,76 @@ __global__ __launch_bounds__(256, 4) void head_rows_bwd_kernel(HeadRowsBwdArgs a
 #pragma unroll
   for (int e = 0; e < 16; ++e) sum_q[e] = sum_k[e] = 0.f;
 
-  for (int i = 0; i < runs; ++i) {
-    const int64_t first = ((int64_t)blockIdx.x * runs + i) * 256;
-    if (first >= total) break;
-    const int64_t end = total - first < 256 ? total : first + 256;
-    const int t0 = (int)(first / per), nt = (int)((end - 1) / per) - t0 + 1;
-    const int at = (int)(first - (int64_t)t0 * per) + tid;
-    const int t = at / per, head = (at - t * per) / U;
-    const bool ok = first + tid < end, is_q = head < a.H;
-    float f[16], g[16];
-#pragma unroll
-    for (int e = 0; e < 16; ++e) f[e] = g[e] = 0.f;
-    if (ok) {
-      const int64_t tt = t0 + t;
-      const T *src = is_q ? (const T *)a.q + tt * a.q_token + head * a.q_head
-                          : (const T *)a.k + tt * a.k_token + (head - a.H) * a.k_head;
-      const T *dy = is_q ? (const T *)a.dq_out + (tt * a.H + head) * D
-                         : (const T *)a.dk_out + (tt * a.Hk + head - a.H) * D;
-      load8<T>(dy + 8 * x.c0, g);
-      load8<T>(dy + 8 * x.c1, g + 8);
-      load8<T>(src + 8 * x.c0, f);
-      load8<T>(src + 8 * x.c1, f + 8);
+  const bool normed = a.q_weight != nullptr || a.k_weight != nullptr;
+  if (normed) stage_weights<T, D>(weights, a.q_weight, a.k_weight, a.weights_f32, tid);
+  struct Run {  // of this thread: token of the run's first, head, rows of x and dy
+    int t0, nt, t, head;
+    bool ok;
+    u32x4 x[2], dy[2];
+  };
+  const int64_t first0 = (int64_t)blockIdx.x * runs * 256;
+  auto load = [&](int i) {
+    Run r;
+    const int64_t first = first0 + (int64_t)i * 256;
+    r.ok = i < runs && first + tid < total;
+    if (i >= runs || first >= total) {
+      r.nt = 0;
+      return r;
     }
+    const int64_t end = total - first < 256 ? total : first + 256;
+    r.t0 = (int)(first / per);
+    r.nt = (int)((end - 1) / per) - r.t0 + 1;
+    const int at = (int)(first - (int64_t)r.t0 * per) + tid;
+    r.t = at / per;
+    r.head = (at - r.t * per) / U;
+    if (r.ok) {
+      const int64_t tt = r.t0 + r.t;
+      const bool is_q = r.head < a.H;
+      const T *src = is_q ? (const T *)a.q + tt * a.q_token + r.head * a.q_head
+                          : (const T *)a.k + tt * a.k_token + (r.head - a.H) * a.k_head;
+      const T *dy = is_q ? (const T *)a.dq_out + (tt * a.H + r.head) * D
+                         : (const T *)a.dk_out + (tt * a.Hk + r.head - a.H) * D;
+      r.x[0] = *reinterpret_cast<const u32x4 *>(src + 8 * x.c0);
+      r.x[1] = *reinterpret_cast<const u32x4 *>(src + 8 * x.c1);
+      r.dy[0] = *reinterpret_cast<const u32x4 *>(dy + 8 * x.c0);
+      r.dy[1] = *reinterpret_cast<const u32x4 *>(dy + 8 * x.c1);
+    }
+    return r;
+  };
+  Run next = load(0);
+  for (int i = 0; i < runs && next.nt > 0; ++i) {
+    const Run r = next;
+    next = load(i + 1);
+    __syncthreads();  // the turns of the run before have been read (at first: the weights are there)
     if (half > 0) {
-      __syncthreads();  // the turns of the run before have been read
-      for (int j = tid; j < nt; j += 256) pos[j] = a.positions[t0 + j];
+      for (int j = tid; j < r.nt; j += 256) pos[j] = a.positions[r.t0 + j];
       __syncthreads();
-      for (int j = tid; j < nt * half; j += 256) {
+      for (int j = tid; j < r.nt * half; j += 256) {
         const int tj = j / half;
         const float2 w = turn_of(pos[tj], a.inv_freq[j - tj * half]);
         turns[j] = make_float2(w.x * a.rot_scale, w.y * a.rot_scale);
       }
       __syncthreads();
     }
-    if (!ok) continue;  // (whole rows; the barriers above are met by all)
+    if (!r.ok) continue;  // (whole rows; the barriers above are met by all)
+    const bool is_q = r.head < a.H;
+    float f[16], g[16];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const auto xv = as_v8<T>(r.x[h]), gv = as_v8<T>(r.dy[h]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        f[8 * h + e] = to_f(xv[e]);
+        g[8 * h + e] = to_f(gv[e]);
+      }
+    }
     if (x.turn)
-      turn_pieces(g, turns + t * half + (a.interleaved ? x.c0 / 2 : x.c0) * 8, a.interleaved, -1.f);
-    const void *w = is_q ? a.q_weight : a.k_weight;
-    if (w != nullptr) {
+      turn_pieces(g, turns + r.t * half + (a.interleaved ? x.c0 / 2 : x.c0) * 8, a.interleaved,
+                  -1.f);
+    if ((is_q ? a.q_weight : a.k_weight) != nullptr) {
       float ss = 0.f, gu = 0.f, ws[16];
-      load_weights<T>(w, a.weights_f32, 8 * x.c0, ws);
-      load_weights<T>(w, a.weights_f32, 8 * x.c1, ws + 8);
+      load_weights(weights + (is_q ? 0 : D), 8 * x.c0, ws);
+      load_weights(weights + (is_q ? 0 : D), 8 * x.c1, ws + 8);
 #pragma unroll
       for (int e = 0; e < 16; ++e) ss += f[e] * f[e];
       const float rn = rsqrtf(row_sum<U>(ss) * (1.f / D) + a.eps);
@@ -315,8 +384,9 @@ __global__ __launch_bounds__(256, 4) void head_rows_bwd_kernel(HeadRowsBwdArgs a
 #pragma unroll
       for (int e = 0; e < 16; ++e) g[e] = rn * (g[e] * ws[e] - f[e] * mean);
     }
-    const int64_t tt = t0 + t;
-    T *dst = is_q ? (T *)a.dq + (tt * a.H + head) * D : (T *)a.dk + (tt * a.Hk + head - a.H) * D;
+    const int64_t tt = r.t0 + r.t;
+    T *dst = is_q ? (T *)a.dq + (tt * a.H + r.head) * D
+                  : (T *)a.dk + (tt * a.Hk + r.head - a.H) * D;
     *reinterpret_cast<u32x4 *>(dst + 8 * x.c0) = pack_row<T>(g);
     *reinterpret_cast<u32x4 *>(dst + 8 * x.c1) = pack_row<T>(g + 8);
   }
@@ -422,15 +492,24 @@ int most_tokens(int64_t units, int64_t per, int64_t T) {
   return (int)std::min<int64_t>(T, (units + per - 2) / per + 1);
 }
 
-template <typename T, int D, int kTo>
-void launch_rows_to(const HeadRowsArgs &s, hipStream_t st) {
-  constexpr int R = 2;
-  const int64_t per = (s.a.H + s.a.Hk + (kTo == kPackedRows ? 0 : s.a.Hk)) * (D / 16);
+// Units of a thread: two from 2^19 units on, one below, where twice the blocks fill the GPU
+// sooner (as in the append of 16 bits).
+constexpr int64_t kRowsWide = int64_t{1} << 19;
+
+template <typename T, int D, int R, int kTo>
+void launch_rows_r(const HeadRowsArgs &s, int64_t per, hipStream_t st) {
   const int64_t units = s.a.T * per;
   const int span = most_tokens(256 * R, per, s.a.T);
-  const int smem = span * ((int)sizeof(RowPlace) + s.a.rot / 2 * 8);
-  hipLaunchKernelGGL((head_rows_kernel<T, D, R, kTo>), dim3((unsigned)((units + 256 * R - 1) / (256 * R))),
-                     dim3(256), smem, st, s, span);
+  const int smem = 2 * D * 4 + span * ((int)sizeof(RowPlace) + s.a.rot / 2 * 8);
+  hipLaunchKernelGGL((head_rows_kernel<T, D, R, kTo>),
+                     dim3((unsigned)((units + 256 * R - 1) / (256 * R))), dim3(256), smem, st, s,
+                     span);
+}
+template <typename T, int D, int kTo>
+void launch_rows_to(const HeadRowsArgs &s, hipStream_t st) {
+  const int64_t per = (s.a.H + s.a.Hk + (kTo == kPackedRows ? 0 : s.a.Hk)) * (D / 16);
+  if (s.a.T * per >= kRowsWide) return launch_rows_r<T, D, 2, kTo>(s, per, st);
+  launch_rows_r<T, D, 1, kTo>(s, per, st);
 }
 
 template <typename T, int D>
@@ -444,7 +523,7 @@ template <typename T, int D>
 void launch_rows_bwd_d(const HeadRowsBwdArgs &a, hipStream_t st) {
   const int64_t per = (a.H + a.Hk) * (D / 16), runs = (a.T * per + 255) / 256;
   const int span = most_tokens(256, per, a.T);
-  const int smem = ((span * 4 + 15) & ~15) + span * (a.rot / 2) * 8;
+  const int smem = 2 * (int)a.D * 4 + ((span + 3) & ~3) * 4 + span * (a.rot / 2) * 8;
   const int each = a.blocks > 0 ? (int)((runs + a.blocks - 1) / a.blocks) : 0;
   if (a.blocks > 0)
     hipLaunchKernelGGL((head_rows_bwd_kernel<T, D>), dim3((unsigned)a.blocks), dim3(256), smem, st,
@@ -476,16 +555,22 @@ void launch_head_rows_bwd(const HeadRowsBwdArgs &a, hipStream_t st) {
   launch_rows_bwd_d<T, 256>(a, st);
 }
 
-template <typename T>
-void launch_paged_gather(const GatherArgs &a, hipStream_t st) {
-  constexpr int R = 2;
-  const int64_t per = 2 * (int64_t)a.Hk * (a.D / 16), units = a.T * per;
+template <typename T, int R>
+void launch_gather_r(const GatherArgs &a, int64_t per, hipStream_t st) {
+  const int64_t units = a.T * per;
   const int span = most_tokens(256 * R, per, a.T);
   const dim3 grid((unsigned)((units + 256 * R - 1) / (256 * R)));
   if (a.scales.k != nullptr)
     hipLaunchKernelGGL((paged_gather_kernel<T, R, true>), grid, dim3(256), span * 8, st, a, span);
   else
     hipLaunchKernelGGL((paged_gather_kernel<T, R, false>), grid, dim3(256), span * 8, st, a, span);
+}
+
+template <typename T>
+void launch_paged_gather(const GatherArgs &a, hipStream_t st) {
+  const int64_t per = 2 * (int64_t)a.Hk * (a.D / 16);
+  if (a.T * per >= kRowsWide) return launch_gather_r<T, 2>(a, per, st);
+  launch_gather_r<T, 1>(a, per, st);
 }
 
 #define VAFA_INST(T)                                                          \
