@@ -43,6 +43,8 @@ int check_rows(const char *what, const char *name, const void *p, int64_t token,
     return fail(VAFA_ERR_VALUE,
                 "%s: %s must be 16-byte aligned with strides that are multiples of 8 elements",
                 what, name);
+  if (token > UINT32_MAX || head > UINT32_MAX)
+    return fail(VAFA_ERR_VALUE, "%s: the strides of %s must be below 2^32", what, name);
   return VAFA_OK;
 }
 

@@ -41,9 +41,9 @@ int check_rows(std::initializer_list<const void *> ptrs, std::initializer_list<i
     if ((uintptr_t)p % 16 != 0)
       return fail(VAFA_ERR_VALUE, "%s: operands must be 16-byte aligned", kWhat);
   for (int64_t s : strides)
-    if (s < 0 || s % 8 != 0)
-      return fail(VAFA_ERR_VALUE, "%s: strides must be multiples of 8 elements, got %lld", kWhat,
-                  (long long)s);
+    if (s < 0 || s % 8 != 0 || s > UINT32_MAX)
+      return fail(VAFA_ERR_VALUE, "%s: strides must be multiples of 8 elements below 2^32, got %lld",
+                  kWhat, (long long)s);
   return VAFA_OK;
 }
 

@@ -20,12 +20,6 @@ namespace vafa {
 
 namespace {
 
-template <typename T>
-__device__ __forceinline__ void load8(const T *p, float *f) {
-  const auto x = as_v8<T>(*reinterpret_cast<const u32x4 *>(p));
-#pragma unroll
-  for (int e = 0; e < 8; ++e) f[e] = to_f(x[e]);
-}
 // The weights of q and then k in LDS, fp32 (ones where there are none); they need not be
 // aligned.
 template <typename T, int D>
@@ -122,6 +116,24 @@ struct RowPlace {  // of a token: places of its rows and their powers of two, po
   int pos, ok;  // ok: some sequence holds it
 };
 
+// The row of head `head` (of q's, then k's, then v's) of the token t behind the bases'.  By value
+// and 32-bit factors: a choice between variables or kernel arguments is else made by address,
+// over a copy of them in scratch.
+struct RowStrides {
+  uint32_t token, head;
+};
+template <typename T>
+__device__ __forceinline__ const T *row_source(const T *q, const T *k, const T *v, RowStrides qs,
+                                               RowStrides ks, RowStrides vs, int H, int Hk,
+                                               uint32_t t, uint32_t head) {
+  const bool is_q = head < (uint32_t)H, is_k = head < (uint32_t)(H + Hk);
+  const uint32_t token = is_q ? qs.token + 0 : (is_k ? ks.token + 0 : vs.token + 0);
+  const uint32_t step = is_q ? qs.head + 0 : (is_k ? ks.head + 0 : vs.head + 0);
+  const uint32_t first = is_q ? 0u : (is_k ? (uint32_t)H : (uint32_t)(H + Hk));
+  const uint64_t base = is_q ? (uint64_t)q : (is_k ? (uint64_t)k : (uint64_t)v);
+  return reinterpret_cast<const T *>(base) + ((uint64_t)t * token + (uint64_t)(head - first) * step);
+}
+
 enum RowsTo { kCache16, kCache8, kPackedRows };
 
 // A block takes 256 R neighbouring units of 16 features, heads of q, then k, then v of one
@@ -143,30 +155,33 @@ __global__ __launch_bounds__(256, 4) void head_rows_kernel(HeadRowsArgs s, int s
   const int t0 = (int)(first / per), nt = (int)((end - 1) / per) - t0 + 1;
 
   struct Unit {
-    int t, head;
+    uint32_t t, head;
     Pieces x;
   };
+  const uint32_t at0 = (uint32_t)(first - (int64_t)t0 * per);
   auto unit = [&](int r) {
-    const int at = (int)(first - (int64_t)t0 * per) + r * 256 + tid;
+    const uint32_t at = at0 + r * 256 + tid, p = (uint32_t)per;
     Unit u;
-    u.t = at / per;
-    const int w = at - u.t * per;
-    u.head = w / U;
-    u.x = pieces_of(w % U, turned, a.interleaved);
-    if (u.head >= a.H + a.Hk) u.x = pieces_of(w % U, 0, false);
+    // (below 2 p + 256 R: compared with few tokens' units instead of divided, mostly)
+    u.t = p >= 128 * R ? (uint32_t)(at >= p) + (at >= 2 * p) + (at >= 3 * p) : at / p;
+    u.head = (at - u.t * p) / (uint32_t)U;
+    u.x = pieces_of(tid % U, u.head < (uint32_t)(a.H + a.Hk) ? turned : 0, a.interleaved);
     return u;
   };
+  // (32-bit factors: one instruction each)
+  const T *qb = (const T *)a.q + (int64_t)t0 * a.q_token;
+  const T *kb = (const T *)a.k + (int64_t)t0 * a.k_token;
+  const T *vb = kTo == kPackedRows ? kb : (const T *)a.v + (int64_t)t0 * a.v_token;
+  const RowStrides qs{(uint32_t)a.q_token, (uint32_t)a.q_head};
+  const RowStrides ks{(uint32_t)a.k_token, (uint32_t)a.k_head};
+  const RowStrides vs{(uint32_t)a.v_token, (uint32_t)a.v_head};
   u32x4 x[R][2];
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     x[r][0] = x[r][1] = u32x4{0, 0, 0, 0};
     if (first + r * 256 + tid >= end) continue;
     const Unit u = unit(r);
-    const int64_t t = t0 + u.t;
-    const T *src = u.head < a.H ? (const T *)a.q + t * a.q_token + u.head * a.q_head
-                   : u.head < a.H + a.Hk
-                       ? (const T *)a.k + t * a.k_token + (u.head - a.H) * a.k_head
-                       : (const T *)a.v + t * a.v_token + (u.head - a.H - a.Hk) * a.v_head;
+    const T *src = row_source(qb, kb, vb, qs, ks, vs, a.H, a.Hk, u.t, u.head);
     x[r][0] = *reinterpret_cast<const u32x4 *>(src + 8 * u.x.c0);
     x[r][1] = *reinterpret_cast<const u32x4 *>(src + 8 * u.x.c1);
   }
@@ -199,7 +214,7 @@ __global__ __launch_bounds__(256, 4) void head_rows_kernel(HeadRowsArgs s, int s
     if (first + r * 256 + tid >= end) continue;
     const Unit u = unit(r);
     const RowPlace at = tok[u.t];
-    const bool is_q = u.head < a.H, is_k = !is_q && u.head < a.H + a.Hk;
+    const bool is_q = u.head < (uint32_t)a.H, is_k = !is_q && u.head < (uint32_t)(a.H + a.Hk);
     float f[16];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -277,7 +292,7 @@ __global__ __launch_bounds__(256, 4) void head_rows_kernel(HeadRowsArgs s, int s
 }
 
 // ---- backward of packed rows -------------------------------------------------------
-// A block walks neighbouring runs of 256 units, as the forward does, and sums the weights'
+// A block walks runs of 256 units, all blocks beside each other, and sums the weights'
 // gradients of its rows in registers (a thread's features are the same in every run, which
 // holds whole rows); its sums go to memory as they are, and the blocks' are added in order.
 template <typename T, int D>
@@ -287,7 +302,7 @@ __global__ __launch_bounds__(256, 4) void head_rows_bwd_kernel(HeadRowsBwdArgs a
   extern __shared__ __align__(16) unsigned char smem[];
   float *weights = reinterpret_cast<float *>(smem);  // [2][D]
   int *pos = reinterpret_cast<int *>(weights + 2 * D);
-  float2 *turns = reinterpret_cast<float2 *>(pos + ((span + 3) & ~3));
+  float2 *turns = reinterpret_cast<float2 *>(pos + ((span + 3) & ~3));  // [span][half]
   __shared__ __align__(16) float red[256][17];
   const int tid = threadIdx.x;
   const int per = (a.H + a.Hk) * U, half = a.rot / 2, turned = half / 8;
@@ -304,10 +319,9 @@ __global__ __launch_bounds__(256, 4) void head_rows_bwd_kernel(HeadRowsBwdArgs a
     bool ok;
     u32x4 x[2], dy[2];
   };
-  const int64_t first0 = (int64_t)blockIdx.x * runs * 256;
   auto load = [&](int i) {
     Run r;
-    const int64_t first = first0 + (int64_t)i * 256;
+    const int64_t first = ((int64_t)i * gridDim.x + blockIdx.x) * 256;
     r.ok = i < runs && first + tid < total;
     if (i >= runs || first >= total) {
       r.nt = 0;
@@ -364,12 +378,14 @@ __global__ __launch_bounds__(256, 4) void head_rows_bwd_kernel(HeadRowsBwdArgs a
       turn_pieces(g, turns + r.t * half + (a.interleaved ? x.c0 / 2 : x.c0) * 8, a.interleaved,
                   -1.f);
     if ((is_q ? a.q_weight : a.k_weight) != nullptr) {
-      float ss = 0.f, gu = 0.f, ws[16];
+      float gu = 0.f, ws[16];
       load_weights(weights + (is_q ? 0 : D), 8 * x.c0, ws);
       load_weights(weights + (is_q ? 0 : D), 8 * x.c1, ws + 8);
+      float ss = 0.f;
 #pragma unroll
       for (int e = 0; e < 16; ++e) ss += f[e] * f[e];
-      const float rn = rsqrtf(row_sum<U>(ss) * (1.f / D) + a.eps);
+      ss = row_sum<U>(ss);
+      const float rn = rsqrtf(ss * (1.f / D) + a.eps);
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         f[e] *= rn;
