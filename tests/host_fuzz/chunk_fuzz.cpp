@@ -37,17 +37,18 @@ static void sums(std::mt19937_64 &g) {
   const int64_t m = chunk_tiles(s.nq, lt);
   int64_t total = 0;
   for (int64_t i = 0; i < m; ++i) {
-    CHECK(chunk_before(s, i) == total);
+    CHECK(chunk_units_before(s, i) == total && chunk_before(s, i) == total + i * kChunkBegin);
     const int64_t t0 = i << lt, t1 = (i + 1) << lt < s.nq ? (i + 1) << lt : s.nq;
     const int64_t end = at_least(s.len - s.nq + t1, 0);
     const int64_t first = window ? at_least(s.len - s.nq + t0 - window + 1, 0) : 0;
     const int64_t units = end > 0 ? (end + 63) / 64 - first / 64 : 1;
     CHECK(chunk_end(s, i) == end && chunk_start(s, i) == first / 64 * 64);
     CHECK(chunk_units(s, i) == units && units >= 1);
-    for (int64_t u : {total, total + units / 2, total + units - 1}) CHECK(chunk_tile_of(s, u) == i);
+    const int64_t at = chunk_before(s, i), taken = units + kChunkBegin;
+    for (int64_t u : {at, at + taken / 2, at + taken - 1}) CHECK(chunk_tile_of(s, u) == i);
     total += units;
   }
-  CHECK(chunk_before(s, m) == total);
+  CHECK(chunk_before(s, m) == total + m * kChunkBegin);
 }
 
 static void walks(std::mt19937_64 &g) {
@@ -60,9 +61,9 @@ static void walks(std::mt19937_64 &g) {
   for (int b = 0; b < n; ++b) {
     seqs.push_back(random_seq(g, lt, window));
     for (int64_t i = 0; i < chunk_tiles(seqs[b].nq, lt); ++i) {
-      tile_at.push_back(total);
+      tile_at.push_back(total + kChunkBegin);  // of its own units
       tile_units.push_back(chunk_units(seqs[b], i));
-      total += tile_units.back();
+      total += tile_units.back() + kChunkBegin;
     }
   }
   const int64_t per = at_least((total + chunks - 1) / chunks, kChunkLeast);
@@ -71,7 +72,7 @@ static void walks(std::mt19937_64 &g) {
   std::set<int64_t> slots, joined;
   auto tile_of = [&](int64_t u) {
     size_t t = 0;
-    while (t + 1 < tile_at.size() && tile_at[t + 1] <= u) ++t;
+    while (t + 1 < tile_at.size() && tile_at[t + 1] - kChunkBegin <= u) ++t;
     return t;
   };
   for (int64_t c = 0; c < chunks; ++c) {
@@ -79,16 +80,18 @@ static void walks(std::mt19937_64 &g) {
     const int64_t end = cur + per < total ? cur + per : total;
     while (cur < end) {
       const size_t t = tile_of(cur);
+      const int64_t from = cur > tile_at[t] ? cur : tile_at[t];
       const int64_t stop = tile_at[t] + tile_units[t] < end ? tile_at[t] + tile_units[t] : end;
-      for (int64_t u = cur; u < stop; ++u) ++covered[u];
-      if (stop - cur < tile_units[t]) {
+      if (stop <= from) break;
+      for (int64_t u = from; u < stop; ++u) ++covered[u];
+      if (stop - from < tile_units[t]) {
         const int64_t s = chunk_slot(c, tile_at[t], per);
         CHECK(s >= 0 && s < 2 * chunks && slots.insert(s).second);
       }
       cur = stop;
     }
   }
-  for (int c : covered) CHECK(c == 1);
+  for (int64_t u = 0; u < total; ++u) CHECK(covered[u] == (u >= tile_at[tile_of(u)]));
   for (int64_t c = 1; c < chunks && c * per < total; ++c) {
     const int64_t u = c * per;
     const size_t t = tile_of(u);
@@ -110,7 +113,7 @@ static void ends() {
       CHECK(all >= m && chunk_tile_of(s, 0) == 0 && chunk_tile_of(s, all - 1) == m - 1);
       CHECK(chunk_end(s, m - 1) == s.len);
       const ChunkSeq none = chunk_seq(int64_t{1} << 30, 0, lt, window);
-      CHECK(chunk_before(none, m) == m);
+      CHECK(chunk_before(none, m) == m * (1 + kChunkBegin));
     }
 }
 

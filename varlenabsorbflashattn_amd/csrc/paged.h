@@ -84,11 +84,15 @@ VAFA_HD int64_t decode_slot(int32_t c, int32_t t0, int32_t per) {
 // The nq new tokens of a sequence of len cached ones are its last; token t has position
 // diag + t, diag = len - nq, and sees the keys up to its own (the last `window` of them).
 // Tokens go in tiles of 2^lt; tile i walks units of kChunkKeys keys from start(i), a multiple
-// of that, to end(i), one unit at least (a tile without keys writes zeros).  The units of all
-// tiles of all sequences, one after another, form one axis, of which chunk c takes the units
-// [c * per, (c + 1) * per): tiles are cut anywhere, and their parts joined.
+// of that, to end(i), one unit at least (a tile without keys writes zeros).  Beginning a tile
+// costs as much as kChunkBegin units, which lie in front of its own.  All of them, one tile and
+// one sequence after another, form one axis, of which chunk c takes [c * per, (c + 1) * per):
+// tiles are cut anywhere among their own units, and their parts joined.
 constexpr int kChunkKeys = 64, kChunkShift = 6;
-constexpr int64_t kChunkLeast = 4;  // units of a chunk
+constexpr int64_t kChunkLeast = 8;  // of the axis, a chunk
+// (24 sequences, 1 to 512 new tokens behind 1 to 16k: chunks of many tiles with few keys held
+// the launch; 126 -> 90 us)
+constexpr int64_t kChunkBegin = 4;
 // as a window, every key: no sum with a position or a tile's rows passes 32 bits
 constexpr int32_t kChunkNoWindow = INT32_MAX - 1024;
 
@@ -128,7 +132,7 @@ VAFA_HD int64_t chunk_floors(int64_t c, int32_t lt, int64_t j0, int64_t j1) {
          (((q0 * (q0 - 1)) >> 1 << r) + (n0 - (q0 << r)) * q0);
 }
 // Units of the tiles in front of tile i (i up to the sequence's tiles: all of them).
-VAFA_HD int64_t chunk_before(const ChunkSeq &s, int64_t i) {
+VAFA_HD int64_t chunk_units_before(const ChunkSeq &s, int64_t i) {
   const int64_t m = chunk_tiles(s.nq, s.lt);
   if (s.len <= 0 || i <= 0) return i;
   // tiles whose end is 0; the last has end len > 0
@@ -145,7 +149,11 @@ VAFA_HD int64_t chunk_before(const ChunkSeq &s, int64_t i) {
   }
   return n;
 }
-// The tile that holds unit u of the sequence (u below all of its units).
+// What these tiles take of the axis.
+VAFA_HD int64_t chunk_before(const ChunkSeq &s, int64_t i) {
+  return chunk_units_before(s, i) + i * kChunkBegin;
+}
+// The tile that holds place u of the sequence's part of the axis.
 VAFA_HD int64_t chunk_tile_of(const ChunkSeq &s, int64_t u) {
   int64_t lo = 0, hi = chunk_tiles(s.nq, s.lt) - 1;  // chunk_before(lo) <= u
   while (lo < hi) {
@@ -157,7 +165,7 @@ VAFA_HD int64_t chunk_tile_of(const ChunkSeq &s, int64_t u) {
   }
   return lo;
 }
-// Partial result of the piece that chunk c holds of a tile whose units start at t0 of the
+// Partial result of the piece that chunk c holds of a tile whose own units start at t0 of the
 // axis: its first piece has slot 2 c, its last 2 c + 1 (pieces between them are whole tiles).
 VAFA_HD int64_t chunk_slot(int64_t c, int64_t t0, int64_t per) {
   return 2 * c + (c * per < t0 ? 1 : 0);

@@ -236,10 +236,13 @@ __global__ __launch_bounds__(64 * NW, D >= 256 ? 1 : 2) void paged_chunk_kernel(
       continue;
     }
     const int64_t i = a.direct ? cur - base : chunk_tile_of(s, cur - base);
-    const int64_t t0 = a.direct ? cur : base + chunk_before(s, i);
-    const int64_t units = chunk_units(s, i);
-    const int64_t u0 = a.direct ? 0 : cur - t0;
-    const int part = (int)uniform_l(a.direct || units - u0 < end - cur ? units - u0 : end - cur);
+    // the axis from the tile's own units on, and those that are this chunk's
+    const int64_t t0 = a.direct ? cur : base + chunk_before(s, i) + kChunkBegin;
+    const int64_t units = chunk_units(s, i), from = cur > t0 ? cur : t0;
+    const int64_t till = a.direct || t0 + units < end ? t0 + units : end;
+    if (till <= from) break;  // the chunk ends in front of them
+    const int64_t u0 = from - t0;
+    const int part = (int)uniform_l(till - from);
     const bool whole = part == units;
     const int run = part * (kChunkKeys / kKeys);  // in units of LDS
     const int q0 = __builtin_amdgcn_readfirstlane(at.q0 + (int)(i << s.lt));
@@ -436,7 +439,7 @@ __global__ __launch_bounds__(64 * NW, D >= 256 ? 1 : 2) void paged_chunk_kernel(
       cur += a.chunks;
       if (cur < end) find_seq(a, cur, mine, lane, &b, &base);
     } else {
-      cur += part;
+      cur = till;
     }
   }
 }
@@ -469,8 +472,8 @@ __global__ __launch_bounds__(256) void paged_chunk_join_kernel(ChunkArgs a) {
   if (b >= a.n_seq) return;
   const SeqAt at = seq_at(a, b);
   const ChunkSeq &s = at.s;
-  const int64_t i = chunk_tile_of(s, u - base), t0 = base + chunk_before(s, i);
-  if (t0 >= u || t0 < u - per) return;  // no border within a tile, or not its first
+  const int64_t i = chunk_tile_of(s, u - base), t0 = base + chunk_before(s, i) + kChunkBegin;
+  if (t0 >= u || t0 < u - per) return;  // no border among a tile's units, or not its first
   const int g0 = (int)c - 1, g1 = (int)((t0 + chunk_units(s, i) - 1) / per);
   const int row = part * kRowsOf + tid / (D / 16), f = tid % (D / 16) * 16;
   const int64_t tok = (i << s.lt) + (row >> a.lg);
