@@ -530,8 +530,11 @@ __global__ __launch_bounds__(256, D >= 128 ? 2 : 3) void paged_decode_kernel(Dec
         }
         const uint32_t ok = r.ok;
         if (u + 2 < u1) {
+          // (the page first: loads come back in order, and the next step needs it while these
+          // rows may still be on their way)
+          const Key after = key_of(u + 3);
           load(next, r);
-          next = key_of(u + 3);
+          next = after;
         }
         attend(u, ok);
       };
