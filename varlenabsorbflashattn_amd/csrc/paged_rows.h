@@ -12,7 +12,8 @@ namespace {
 // token lies behind the last one).  Every lane of the wave calls it.
 __device__ __forceinline__ int seq_of(const int32_t *cu, int n, int t, int lane) {
   int b = 0;
-  for (int c = 0; c < n; c += 64) {
+#pragma unroll 4
+  for (int c = 0; c < n; c += 64) {  // (several loads on their way)
     const bool le = c + lane < n && cu[1 + c + lane] <= t;
     b += __popcll(__builtin_amdgcn_ballot_w64(le));
   }
