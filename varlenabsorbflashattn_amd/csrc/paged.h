@@ -89,7 +89,10 @@ VAFA_HD int64_t decode_slot(int32_t c, int32_t t0, int32_t per) {
 // one sequence after another, form one axis, of which chunk c takes [c * per, (c + 1) * per):
 // tiles are cut anywhere among their own units, and their parts joined.
 constexpr int kChunkKeys = 64, kChunkShift = 6;
-constexpr int64_t kChunkLeast = 8;  // of the axis, a chunk
+// Of the axis, a chunk has this many at least (one sequence of 1k keys, 4 and 128 new tokens,
+// D = 128: 2 19 and 32 us, 4 19 and 30, 8 23 and 33, 24 29 and 50; D = 256: 23 and 34, 27 and
+// 36, 37 and 43, 56 and 73)
+constexpr int64_t kChunkLeast = 4;
 // (24 sequences, 1 to 512 new tokens behind 1 to 16k: chunks of many tiles with few keys held
 // the launch; 126 -> 90 us)
 constexpr int64_t kChunkBegin = 4;

@@ -1,13 +1,21 @@
 // Attention of several new tokens per sequence over a paged key-value cache, in 16 bits or
 // in 8-bit codes, on gfx950 matrix cores (bf16 / f16).
 //
-// Tiles and products are those of the packed masked forward (masked_tile.h): 128 rows of a
-// workgroup are tokens of up to 32 query heads that share a key head, keys and values come in
-// units of 64 through LDS, one unit ahead in registers.  What differs: rows of a unit are
-// looked up in the page table, two units ahead; the lengths are device data, so the work is
-// divided here: all units of all tiles form one axis (paged.h), cut into as many even chunks
-// as the GPU holds workgroups for each set of heads, and a second launch joins the tiles that
-// were cut.
+// O_i = sum_j softmax_j(s(q_i k_j)) v_j over the keys that token i sees, s the scale, the cap and
+// the distance bias, in one pass with a running maximum and sum (masked_tile.h, whose products
+// the packed masked forward shares).  A workgroup's 256 rows (128 of 256 features) are tokens of
+// up to 32 query heads that share a key head; of a unit of 64 keys the rows are looked up in the
+// page table and come to LDS three units ahead.  Lengths are device data, so the work is divided
+// here: all units of all tiles form one axis (paged.h), cut into as many even chunks as the GPU
+// holds workgroups for each set of heads, and a second launch joins the tiles that were cut.
+//
+// Few new tokens behind long prefixes are bound by the rows of the cache: 32 sequences of 1 to 8
+// tokens behind 1k to 32k keys of 8 heads of 128, 1.27 GB, 225 us: 5.6 TB/s, all of it read (a
+// large copy, half written, reaches 5.0).  Many are bound by the products and, between them, by the softmax's vector
+// instructions: chunks of 8 prompts, 627 GFLOP, 710 us, 0.88 PFLOP/s, where the packed kernel on
+// gathered keys takes 652 for the same; 18 of them are the join.  256 rows against 128: the
+// chunks 724 us to 962, 24 turns of 1 to 512 tokens over codes 90 to 109, the drafts 214 to 215
+// (each unit is then fetched and, of codes, converted for half as many rows).
 #include <algorithm>
 #include <type_traits>
 
@@ -86,8 +94,13 @@ __device__ __forceinline__ void find_seq(const ChunkArgs &a, int64_t at, int64_t
   *b = a.n_seq;
   *base = uniform_l(before);
 }
+// (By doubles, whose 53 bits hold every axis: the quotient, rounded, is off by one at most.  A
+// division of 64-bit integers becomes a branch of the lanes, at whose end the compiler has put
+// copies of registers where only the branch's lanes were on.)
 __device__ __forceinline__ int64_t units_per(const ChunkArgs &a, int64_t total) {
-  const int64_t per = (total + a.chunks - 1) / a.chunks;
+  int64_t per = (int64_t)((double)total / (double)a.chunks);
+  per -= per * a.chunks >= total;
+  per += per * a.chunks < total;
   return per < kChunkLeast ? kChunkLeast : per;
 }
 
@@ -151,7 +164,7 @@ __device__ const int32_t kNoPage = -1;
 // powers of two.
 template <int D, int NW, bool kCodes>
 struct ChunkSmem {
-  static constexpr int kKeys = kUnitKeys<D>, kAhead = 3, kRing = 2 * NW;  // units
+  static constexpr int kKeys = kUnitKeys<D>, kAhead = D == 64 ? 7 : 3, kRing = 2 * NW;  // units
   static constexpr int kUnit = 2 * kKeys * 2 * D, kRaw = kUnit / 2;       // bytes, K and V
   static constexpr int kBuffers = kCodes ? 2 : kAhead + 1;
   static constexpr int kRawAt = kBuffers * kUnit;
@@ -164,8 +177,8 @@ struct ChunkSmem {
 };
 
 // 256 rows of 8 waves (D = 256: 128 of 4, which have its registers), one workgroup on a CU.
-template <typename T, int D, int NW, bool kCodes, bool kCap, bool kBias>
-__global__ __launch_bounds__(64 * NW, D >= 256 ? 1 : 2) void paged_chunk_kernel(ChunkArgs a) {
+template <typename T, int D, int NW, bool kCodes, bool kCap, bool kBias, bool kOnce>
+__device__ __forceinline__ void chunk_walk(const ChunkArgs &a) {
   using M = Mfma<T>;
   using E = std::conditional_t<kCodes, uint8_t, T>;
   using Tile = SwizzledTile<T, D>;
@@ -188,22 +201,10 @@ __global__ __launch_bounds__(64 * NW, D >= 256 ? 1 : 2) void paged_chunk_kernel(
   const int chunk = group * kXcds + within % kXcds, set = within / kXcds;
   const int h0 = set << lg, hk = set / hs.per_key();
 
-  // rows of no sequence
-  {
-    int lo = a.cu[0], hi = a.cu[a.n_seq];
-    const int T_ = (int)a.T;
-    lo = lo < 0 ? 0 : (lo > T_ ? T_ : lo);
-    hi = hi < lo ? lo : (hi > T_ ? T_ : hi);
-    const int64_t n = lo + (T_ - hi), pieces = n * a.H * D / 8;
-    for (int64_t e = (int64_t)blockIdx.x * NT + tid; e < pieces; e += (int64_t)gridDim.x * NT) {
-      const int64_t at = e * 8, edge = (int64_t)lo * a.H * D;
-      T *p = (T *)a.out + (at < edge ? at : at - edge + (int64_t)hi * a.H * D);
-      *reinterpret_cast<u32x4 *>(p) = u32x4{0, 0, 0, 0};
-    }
-  }
   if (chunk >= a.chunks) return;
   const int64_t mine = seq_units(a, lane);
-  const int64_t total = all_units(a, mine, lane);
+  // (tiles dealt in turn go on until there is no sequence for one)
+  const int64_t total = a.direct ? INT64_MAX : all_units(a, mine, lane);
   const int64_t per = a.direct ? 1 : units_per(a, total);
   int64_t cur = chunk * per;
   const int64_t end = a.direct || total - cur < per ? total : cur + per;
@@ -253,9 +254,18 @@ __global__ __launch_bounds__(64 * NW, D >= 256 ? 1 : 2) void paged_chunk_kernel(
     // keys in front of it are of no row's window, though of the first unit: absent
     const int kfirst = a.window > 0 ? q0 + diag - a.window + 1 : 0;
 
-    const int w0 = q0 + wave * tw;  // the wave's first token
+    // A short piece of a tile of few rows: its units lie in the buffers at once, and each is
+    // another group of waves' (4 sequences of 2 to 8 tokens behind 17 to 500 keys, 16 heads of
+    // 64: 11.8 -> 10.5 us; more features have no room for as many units)
+    constexpr bool kShorts = D == 64 && !kCodes;
+    int lr = 0;  // log2 of a group's waves
+    if (kShorts)
+      while ((tw << lr) < qn) ++lr;
+    const bool is_short = kShorts && run <= kAhead && run <= NW >> lr;
+    const int rw = is_short ? wave & ((1 << lr) - 1) : wave, grp = is_short ? wave >> lr : 0;
+    const int w0 = q0 + rw * tw;  // the wave's first token
     const int tok = w0 + (lrow >> lg), h = h0 + (lrow & ((1 << lg) - 1));
-    const bool row_ok = tok < q1, wave_active = w0 < q1;
+    const bool row_ok = tok < q1, wave_active = w0 < q1 && (!is_short || grp < run);
     const int p = tok + diag;
     const int p0 = w0 + diag, p1 = (w0 + tw < q1 ? w0 + tw : q1) - 1 + diag;
     typename M::v8 qf[NC];
@@ -279,10 +289,6 @@ __global__ __launch_bounds__(64 * NW, D >= 256 ? 1 : 2) void paged_chunk_kernel(
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[x][r] = 0.f;
     float m_run = -kHuge, l_part = 0.f;
-
-    // keys that are read once in the whole call pass the caches (one workgroup reads the
-    // tile's keys for one set: none other does if there is one tile and one set a key head)
-    const bool once = tiles == 1 && hs.per_key() == 1;
 
     // Each wave looks up the rows of one unit of every block of NW.  First their pages:
     auto ask_ids = [&](int u) {
@@ -348,13 +354,12 @@ __global__ __launch_bounds__(64 * NW, D >= 256 ? 1 : 2) void paged_chunk_kernel(
         const int col = kCodes ? piece : piece ^ (of_v(x) ? swizzle_v<D>(row) : swizzle_k<D>(row));
         from[x] = (of_v(x) ? vc : kc) + col + *reinterpret_cast<const uint64_t *>(place_of(u, x));
       }
-      if (once) {
 #pragma unroll
-        for (int x = 0; x < kPieces; ++x) lds_dma16_once(from[x], to + x * NT * 16);
-      } else {
-#pragma unroll
-        for (int x = 0; x < kPieces; ++x) lds_dma16(from[x], to + x * NT * 16);
-      }
+      for (int x = 0; x < kPieces; ++x)
+        if constexpr (kOnce)
+          lds_dma16_once(from[x], to + x * NT * 16);
+        else
+          lds_dma16(from[x], to + x * NT * 16);
     };
     // codes: unit u's rows, which this thread asked for, become T
     auto convert = [&](int u) {
@@ -388,26 +393,33 @@ __global__ __launch_bounds__(64 * NW, D >= 256 ? 1 : 2) void paged_chunk_kernel(
     __syncthreads();
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) ask_rows(u);
-    wait_vmcnt<kRequests>();
+    if (is_short)
+      wait_vmcnt<0>();
+    else
+      wait_vmcnt<kRequests>();
     if constexpr (kCodes) {
       __syncthreads();  // words that other waves asked for
       convert(0);
     }
     __syncthreads();
-    for (int j = 0; j < run; ++j) {
-      if (j % NW == 0) {  // a block's rows before its first are asked for, pages a block ahead
-        look_up(j + NW + wave);
-        ask_ids(j + 2 * NW + wave);
+    const int turns = is_short ? 1 : run;
+    for (int j = 0; j < turns; ++j) {
+      if (!is_short) {
+        if (j % NW == 0) {  // a block's rows before its first are asked for, pages a block ahead
+          look_up(j + NW + wave);
+          ask_ids(j + 2 * NW + wave);
+        }
+        ask_rows(j + kAhead);
       }
-      ask_rows(j + kAhead);
-      const int kb = kb0 + j * kKeys;
+      const int u = j + grp, kb = kb0 + u * kKeys;
       const int kl = (kb + kKeys < kend ? kb + kKeys : kend) - 1;
       if (wave_active && !none_visible(kb, kl, p0, p1, 0, window)) {
-        const uint64_t here = present(j);
+        const uint64_t here = present(u);
         const bool masked = here != ~uint64_t{0} || !all_visible(kb, kl, p0, p1, 0, window);
-        masked_tile<T, D, kCap, kBias>(tile0.at_offset(unit_at(j)), qf, acc, m_run, l_part, sa,
+        masked_tile<T, D, kCap, kBias>(tile0.at_offset(unit_at(u)), qf, acc, m_run, l_part, sa,
                                        slope2, kb, kend, masked, p, 0, window, lane, here);
       }
+      if (is_short) break;
       wait_vmcnt<kRequests>();
       if constexpr (kCodes) convert(j + 1);
       __syncthreads();
@@ -415,7 +427,35 @@ __global__ __launch_bounds__(64 * NW, D >= 256 ? 1 : 2) void paged_chunk_kernel(
     wait_vmcnt<0>();  // nothing on its way to what the rows' store takes
     __syncthreads();
 
-    if (wave_active) {
+    // the groups' rows, each register's 64 lanes beside each other, joined in their order
+    if (kShorts && is_short && run > 1) {
+      constexpr int kRegs = 16 * ND + 2;
+      float *x = reinterpret_cast<float *>(smem_raw) + lane;
+      if (wave_active && grp > 0) {
+        float *to = x + wave * kRegs * 64;
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) to[(d * 16 + r) * 64] = acc[d][r];
+        to[16 * ND * 64] = m_run;
+        to[(16 * ND + 1) * 64] = l_part;
+      }
+      __syncthreads();
+      if (wave_active && grp == 0)
+        for (int g = 1; g < run; ++g) {
+          const float *from = x + ((g << lr) + rw) * kRegs * 64;
+          const float m = from[16 * ND * 64], m_new = fmaxf(m_run, m);
+          const float f = fast_exp2(m_run - m_new), of = fast_exp2(m - m_new);
+          m_run = m_new;
+          l_part = l_part * f + from[(16 * ND + 1) * 64] * of;
+#pragma unroll
+          for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[d][r] = acc[d][r] * f + from[(d * 16 + r) * 64] * of;
+        }
+      __syncthreads();
+    }
+    if (wave_active && grp == 0) {
       // a row that sees no key has l = 0 (output 0, lse -inf); NaN scores stay NaN
       const float l = l_part + __shfl_xor(l_part, 32, 64);
       const float inv = l == 0.f ? 0.f : 1.f / l;
@@ -441,6 +481,23 @@ __global__ __launch_bounds__(64 * NW, D >= 256 ? 1 : 2) void paged_chunk_kernel(
     } else {
       cur = till;
     }
+  }
+}
+
+template <typename T, int D, int NW, bool kCodes, bool kCap, bool kBias, bool kOnce>
+__global__ __launch_bounds__(64 * NW, D >= 256 ? 1 : 2) void paged_chunk_kernel(ChunkArgs a) {
+  chunk_walk<T, D, NW, kCodes, kCap, kBias, kOnce>(a);
+  // rows of no sequence, in front of the first and behind the last
+  const int T_ = (int)a.T;
+  int lo = a.cu[0], hi = a.cu[a.n_seq];
+  lo = lo < 0 ? 0 : (lo > T_ ? T_ : lo);
+  hi = hi < lo ? lo : (hi > T_ ? T_ : hi);
+  const int64_t edge = (int64_t)lo * a.H * D, pieces = (int64_t)(lo + T_ - hi) * a.H * D / 8;
+  for (int64_t e = (int64_t)blockIdx.x * (64 * NW) + threadIdx.x; e < pieces;
+       e += (int64_t)gridDim.x * (64 * NW)) {
+    const int64_t at = e * 8;
+    T *p = (T *)a.out + (at < edge ? at : at - edge + (int64_t)hi * a.H * D);
+    *reinterpret_cast<u32x4 *>(p) = u32x4{0, 0, 0, 0};
   }
 }
 
@@ -510,9 +567,9 @@ __global__ __launch_bounds__(256) void paged_chunk_join_kernel(ChunkArgs a) {
   }
 }
 
-template <typename T, int D, int NW, bool kCodes, bool kCap, bool kBias>
+template <typename T, int D, int NW, bool kCodes, bool kCap, bool kBias, bool kOnce>
 void launch_v(const ChunkArgs &a, hipStream_t st) {
-  constexpr auto fn = &paged_chunk_kernel<T, D, NW, kCodes, kCap, kBias>;
+  constexpr auto fn = &paged_chunk_kernel<T, D, NW, kCodes, kCap, kBias, kOnce>;
   const int smem = chunk_lds<T, D, NW, kCodes>(), sets = a.H >> a.lg;
   allow_dynamic_lds(reinterpret_cast<const void *>(fn), smem);
   const int64_t wgs = (int64_t)(a.chunks + kXcds - 1) / kXcds * kXcds * sets;
@@ -523,22 +580,28 @@ void launch_v(const ChunkArgs &a, hipStream_t st) {
                      st, a);
 }
 
-template <typename T, int D, bool kCodes>
+template <typename T, int D, bool kCodes, bool kOnce>
 void launch_d(const ChunkArgs &a, hipStream_t st) {
   constexpr int NW = D <= 128 ? 8 : 4;
   const bool cap = a.cap2 > 0.f, bias = a.slopes != nullptr;
-  if (cap && bias) return launch_v<T, D, NW, kCodes, true, true>(a, st);
-  if (cap) return launch_v<T, D, NW, kCodes, true, false>(a, st);
-  if (bias) return launch_v<T, D, NW, kCodes, false, true>(a, st);
-  launch_v<T, D, NW, kCodes, false, false>(a, st);
+  if (cap && bias) return launch_v<T, D, NW, kCodes, true, true, kOnce>(a, st);
+  if (cap) return launch_v<T, D, NW, kCodes, true, false, kOnce>(a, st);
+  if (bias) return launch_v<T, D, NW, kCodes, false, true, kOnce>(a, st);
+  launch_v<T, D, NW, kCodes, false, false, kOnce>(a, st);
 }
 
 }  // namespace
 
+// Rows in 16 bits pass the caches where a sequence has no more than a tile's tokens on average
+// and a key head one set, so that most are read once (32 sequences of 1 to 8 tokens behind 1k to
+// 32k keys 250 -> 213 us; of eight prompts' chunks 718 -> 742).  Codes do not: 234 -> 230 us of
+// the same drafts, 708 -> 738 of the chunks.
 template <typename T, int D>
 void launch_paged_chunk(const ChunkArgs &a, hipStream_t st) {
-  if (a.scales.k != nullptr) return launch_d<T, D, true>(a, st);
-  launch_d<T, D, false>(a, st);
+  if (a.scales.k != nullptr) return launch_d<T, D, true, false>(a, st);
+  if (a.T <= (int64_t)a.n_seq << a.lt && a.H == a.Hk << a.lg)
+    return launch_d<T, D, false, true>(a, st);
+  launch_d<T, D, false, false>(a, st);
 }
 
 #define VAFA_INST(T, D) template void launch_paged_chunk<T, D>(const ChunkArgs &, hipStream_t);
