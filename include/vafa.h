@@ -471,7 +471,8 @@ VAFA_API int vafa_paged_decode_codes(const vafa_paged_cache *cache, const vafa_r
  * multiples of 8) -> out [T, H, D]: tokens cu[b] .. cu[b + 1] - 1 (device int32, not
  * decreasing) are the last of the cache_lens[b] tokens of sequence b, and each sees the keys
  * up to its own (the last `window` of them; 0: all).  Else as vafa_paged_decode, over 16 bits
- * or, with scales, codes.  Rows of no sequence, and those that see no key, get zeros. */
+ * or, with scales, codes.  Rows of no sequence, and those that see no key, get zeros.  T at most
+ * 2^30, H at most 4096, strides of pages and tokens below 2^35. */
 VAFA_API int64_t vafa_paged_chunk_workspace(const vafa_paged_cache *cache, int64_t T, int64_t H,
                                             int64_t window);
 VAFA_API int vafa_paged_chunk(const vafa_paged_cache *cache, const vafa_row_scales *scales,
@@ -480,8 +481,8 @@ VAFA_API int vafa_paged_chunk(const vafa_paged_cache *cache, const vafa_row_scal
                               int64_t window, const float *slopes, int32_t dtype, void *workspace,
                               int64_t workspace_bytes, void *stream);
 
-/* vafa_paged_append (D in {64, 128, 256}, rot a multiple of 16) of normed rows, into 16 bits
- * or, with scales, codes: rows of q and k become R(x r w), r = 1 / sqrt(mean x^2 + eps), w =
+/* vafa_paged_append (D in {64, 128, 256}, rot a multiple of 16, strides of rows below 2^32) of
+ * normed rows, into 16 bits or, with scales, codes: rows of q and k become R(x r w), r = 1 / sqrt(mean x^2 + eps), w =
  * q_weight / k_weight [D] (NULL: not normed; fp32 where weights_f32, else of dtype), before
  * the rotation R, whose sine and cosine are multiplied by rot_scale.  dtype is that of k, v,
  * q.  A row's power of two is the least 2^e with max |x| <= 448 * 2^e (e at most 8 for fp16

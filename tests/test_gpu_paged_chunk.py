@@ -3,6 +3,7 @@
 sums take the rounded values), for codes as in test_gpu_paged_codes.py.
 """
 import math
+import threading
 
 import numpy as np
 import pytest
@@ -371,3 +372,67 @@ def test_chunk_past_4_gib(device):
         paged_kv_append(x[:, H:H + Hk], x[:, H + Hk:], kc, vc, table, zero, cu_seqlens=cu)
         outs.append(paged_chunk_attn(x[:, :H], kc, vc, table, zero + 700, cu))
     assert torch.equal(*outs) and outs[0].any()
+
+
+@pytest.mark.parametrize("seed", range(12))
+def test_chunk_random(device, seed):
+    """Drawn shapes, a third of them many short pieces of narrow heads (which groups of waves
+    share)."""
+    rng = np.random.default_rng(seed)
+    D = 64 if seed % 3 == 0 else int(rng.choice([64, 128, 256]))
+    Hk = int(rng.choice([1, 2, 4]))
+    n = int(rng.integers(1, 9))
+    new = [int(x) for x in rng.integers(0, 9 if seed % 3 == 0 else 150, n)]
+    lens = [x + int(rng.integers(0, 1500)) for x in new]
+    codes = bool(rng.integers(0, 2)) and seed % 3 != 0
+    case = (new, lens, Hk * int(rng.choice([1, 3, 4, 8])), Hk, D, int(rng.choice([3, 16, 64])),
+            30.0 if rng.integers(0, 4) == 0 else None,
+            int(rng.integers(1, 600)) if rng.integers(0, 3) == 0 else None,
+            bool(rng.integers(0, 4) == 0), codes,
+            torch.float16 if rng.integers(0, 2) else torch.bfloat16, "plain")
+    print(f"[chunk drawn] {case}", flush=True)
+    args, kw, ref = chunk_case(case, device)
+    out = paged_chunk_attn(*args, **kw)
+    close_decode(out, *ref)
+    assert torch.equal(out, paged_chunk_attn(*args, **kw))
+
+
+def test_threads_with_streams(device):
+    """Two threads, each on its own stream: attention over a cache, and norms with their
+    backward, give what they give alone."""
+    print("[two threads]", flush=True)
+    errors, jobs = [], []
+    for k, case in enumerate((SPLIT[1], SPLIT[2])):
+        args, kw, _ = chunk_case(case, device)
+        g = torch.Generator(device=device).manual_seed(k)
+        x = torch.randn(700, 6, 64, generator=g, device=device).to(torch.bfloat16)
+        pos = torch.arange(700, dtype=torch.int32, device=device)
+        w = torch.rand(64, generator=g, device=device) + 0.5
+
+        def job(args=args, kw=kw, x=x, pos=pos, w=w):
+            q, k_, wq = (t.detach().clone().requires_grad_() for t in (x[:, :4], x[:, 4:], w))
+            yq, yk = packed_qk_norm_rope(q, k_, pos, inv_freq=freqs(64).to(x.device), q_weight=wq,
+                                         k_weight=wq)
+            grads = torch.autograd.grad((yq.float() * x[:, :4]).sum() + yk.float().sum(),
+                                        (q, k_, wq))
+            return [paged_chunk_attn(*args, **kw), yq.detach(), yk.detach(), *grads]
+
+        jobs.append((job, job()))
+    torch.cuda.synchronize()
+
+    def work(job, want):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(5):
+                    got = job()
+                    torch.cuda.current_stream().synchronize()
+                    assert all(torch.equal(a, b) for a, b in zip(got, want))
+        except BaseException as e:
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=j) for j in jobs]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors

@@ -306,3 +306,24 @@ def test_oracle_gradients(rot, inter):
         assert math.isclose((loss(x, w + d) - loss(x, w - d)) / (2 * h), dw[i[2]], rel_tol=1e-6,
                             abs_tol=1e-7)
     assert (np.abs(dx) <= mag + 1e-12).all() and (np.abs(dw) <= wmag + 1e-12).all()
+
+
+def test_row_strides_of_the_c_abi():
+    """Strides past 32 bits: refused by the entry points whose kernels take 32-bit factors, as
+    before no error of the others (no rows: nothing is launched)."""
+    L, x, far, BF = _lib.lib(), 1 << 24, 1 << 33, _lib.DT_BF16
+    c = _lib.PagedCache(k=1 << 20, v=1 << 21, n_pages=5, page_size=16, Hk=2, D=64, k_page=2048,
+                        k_token=128, k_head=64, v_page=2048, v_token=128, v_head=64,
+                        page_table=1 << 22, table_stride=2, table_width=2, cache_lens=1 << 23,
+                        n_seq=0)
+    c = C.byref(c)
+    append = [c, x, far, 64, x, far, far, 0, None, x, far, far, 4, x, x, 64, 0, BF, None]
+    assert L.vafa_paged_append(*append) == 0
+    decode = [c, x, far, far, 4, x, 0.125, 0.0, 0, None, BF, x, 1 << 20, None]
+    assert L.vafa_paged_decode(*decode) == 0
+    store = [c, None, x, 128, 64, x, 128, 64, 0, None, x, 256, 64, 4, x, x, 64, 0, 1.0, x, x, 1,
+             1e-6, BF, None]
+    assert L.vafa_paged_store(*store) == 0
+    for at in (3, 4, 6, 7, 11, 12):
+        assert L.vafa_paged_store(*[far if i == at else y for i, y in enumerate(store)]) == \
+            _lib.VAFA_ERR_VALUE, at

@@ -43,8 +43,6 @@ int check_rows(const char *what, const char *name, const void *p, int64_t token,
     return fail(VAFA_ERR_VALUE,
                 "%s: %s must be 16-byte aligned with strides that are multiples of 8 elements",
                 what, name);
-  if (token > UINT32_MAX || head > UINT32_MAX)
-    return fail(VAFA_ERR_VALUE, "%s: the strides of %s must be below 2^32", what, name);
   return VAFA_OK;
 }
 
@@ -319,6 +317,10 @@ int vafa_paged_store(const vafa_paged_cache *c, const vafa_row_scales *scales, c
   if (int rc = check_dtype(what, dtype)) return rc;
   if (int rc = check_codes(what, c, scales)) return rc;
   if (int rc = check_head_rows(what, c->D, rot, eps, rot_scale)) return rc;
+  for (int64_t x : {q_token, q_head, k_token, k_head, v_token, v_head})  // (the kernel's factors)
+    if (x > UINT32_MAX)
+      return fail(VAFA_ERR_VALUE, "%s: strides of rows must be below 2^32, got %lld", what,
+                  (long long)x);
   HeadRowsArgs s{};
   if (int rc = append_args(what, c, k, k_token, k_head, v, v_token, v_head, T, cu, q, q_token,
                            q_head, H, q_out, inv_freq, rot, interleaved, &s.a))

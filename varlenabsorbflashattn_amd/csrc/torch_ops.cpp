@@ -40,9 +40,10 @@ struct Api {
   X(absorb_bwd_full_workspace)                                                            \
   X(absorb_project_workspace) X(absorb_project_fwd) X(absorb_project_bwd)                 \
   X(absorb_project_f32_workspace) X(absorb_project_f32_fwd) X(absorb_project_f32_bwd)      \
-  X(paged_append) X(paged_decode_workspace) X(masked_fwd_workspace)        \
-  X(paged_store) X(paged_gather) X(paged_decode_codes) X(paged_chunk_workspace) X(paged_chunk) X(qk_norm_rope_fwd) X(qk_norm_rope_bwd_workspace)          \
-  X(qk_norm_rope_bwd)                                                                       \
+  X(paged_append) X(paged_store) X(paged_gather) X(paged_decode_workspace)                \
+  X(paged_decode_codes) X(paged_chunk_workspace) X(paged_chunk)                           \
+  X(qk_norm_rope_fwd) X(qk_norm_rope_bwd_workspace) X(qk_norm_rope_bwd)                   \
+  X(masked_fwd_workspace)                                                                 \
   X(masked_fwd) X(masked_bwd_workspace) X(masked_bwd)
   VAFA_FNS(VAFA_FN)
 #undef VAFA_FN

@@ -36,7 +36,9 @@ def packed_qk_norm_rope(
     be parts of one projection's output.
 
     Gradients for q, k and the weights; the backward is deterministic, a second derivative
-    raises.  At most 2^30 tokens and 4096 heads.  A row that holds an infinity or NaN gives
+    raises.  At most 2^30 tokens and 4096 heads, strides below 2^32 elements.  Forward and
+    backward can be captured into a graph together; no eager graph of the same leaves may be
+    alive then.  A row that holds an infinity or NaN gives
     NaN to itself and to the weights' gradients, and to no other row.
     """
     yq, yk = _lib.ops().qk_norm_rope(q, k, positions, inv_freq, bool(interleaved), q_weight,

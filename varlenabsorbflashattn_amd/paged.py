@@ -5,12 +5,13 @@ The caches are ``[n_pages, page_size, H_k, D]`` (bf16 or fp16), features contigu
 other strides any multiple of 8 elements, so views of a joint or head-major allocation
 serve too.  In 8 bits they are ``float8_e4m3fn`` (strides multiples of 16) beside
 ``k_scale`` and ``v_scale`` ``[n_pages, page_size, H_k]`` of ``float8_e8m0fnu``: a row (one
-token and key head) is its codes times its power of two.  Token ``p`` of sequence ``b`` lies in page ``page_table[b, p // page_size]``
-at ``p % page_size``.  ``page_table`` and the lengths are int32 tensors on the GPU and
-stay there: no call waits for the GPU, all of them can be captured into a graph and
-replayed with other lengths and pages in the same tensors.  As the host never sees them,
-a position outside the table or a page outside the cache is no error: such a token is
-neither stored nor read.  There is no counterpart in the reference, which has no cache.
+token and key head) is its codes times its power of two.  Token ``p`` of sequence ``b`` lies
+in page ``page_table[b, p // page_size]`` at ``p % page_size``.  ``page_table`` and the
+lengths are int32 tensors on the GPU and stay there: no call waits for the GPU, all of them
+can be captured into a graph and replayed with other lengths and pages in the same tensors.
+As the host never sees them, a position outside the table or a page outside the cache is no
+error: such a token is neither stored nor read.  There is no counterpart in the reference,
+which has no cache.
 """
 from __future__ import annotations
 
@@ -61,7 +62,8 @@ def paged_kv_append(
     holds, values end at 240 * 2^8 (fp16) or 240 * 2^120 (bf16); infinities and NaN become NaN.
     With ``q_weight`` and ``k_weight`` rows of q and k are normed before they turn, and with
     ``rot_scale`` turned features are scaled, as by :func:`packed_qk_norm_rope`.  These options
-    take D 64, 128 or 256 and a multiple of 16 rotated features.  Of two tokens that share a
+    take D 64, 128 or 256, a multiple of 16 rotated features, and rows with strides below 2^32
+    elements.  Of two tokens that share a
     place in an 8-bit cache, codes and power of two may then not belong together.
     """
     return _lib.ops().paged_append(k, v, k_cache, v_cache, page_table, cache_lens, cu_seqlens, q,
@@ -150,7 +152,8 @@ def paged_chunk_attn(
     them.  Scores, heads and 8-bit caches are those of :func:`paged_decode_attn`, the result
     is what :func:`packed_masked_attn` gives on the gathered keys.  Tokens in front of the
     first key (more new tokens than the cache holds) and rows of no sequence get zeros.  At
-    most 2^30 tokens and 4096 heads.  Forward only.
+    most 2^30 tokens and 4096 heads; strides of pages and tokens below 2^35 elements (2^36
+    codes, 2^32 powers of two).  Forward only.
     """
     if scale is None:
         scale = 1.0 / math.sqrt(q.shape[-1])
