@@ -176,7 +176,7 @@ int check_workspace(const void *workspace, int64_t bytes, int64_t needed) {
 // workspace go by the rows and by what the page table could hold.
 struct ChunkPlan {
   int lg = 0, lt = 0;
-  int64_t rows = 0, chunks = 0, bytes = 0, lse_off = 0;
+  int64_t rows = 0, chunks = 0, bytes = 0, lse_off = 0, cut_off = 0;
   bool direct = false;
 };
 
@@ -215,7 +215,8 @@ int plan_chunk(const vafa_paged_cache *c, int64_t T, int64_t H, int64_t window, 
     p->chunks = std::max<int64_t>(1, std::min(slots / sets, tiles * most));
   const int64_t rows = p->direct ? 0 : 2 * p->chunks * sets * p->rows;
   p->lse_off = rows * c->D * 4;
-  p->bytes = p->lse_off + rows * 4;
+  p->cut_off = p->lse_off + rows * 4;  // (a multiple of 16: a tile has 128 rows or more)
+  p->bytes = p->cut_off + (p->direct ? 0 : p->chunks * sets * (int64_t)sizeof(ChunkCut));
   return VAFA_OK;
 }
 
@@ -457,6 +458,7 @@ int vafa_paged_chunk(const vafa_paged_cache *c, const vafa_row_scales *scales, c
   a.q = q; a.kc = c->k; a.vc = c->v; a.out = out; a.cu = cu; a.lens = c->cache_lens;
   a.slopes = slopes; a.part_o = (float *)workspace;
   a.part_lse = (float *)((char *)workspace + p.lse_off);
+  a.cuts = (ChunkCut *)((char *)workspace + p.cut_off);
   a.map = map_of(c); a.q_token = q_token; a.q_head = q_head;
   const int64_t piece = scales != nullptr ? 16 : 8;
   a.kc_head = c->k_head; a.vc_head = c->v_head;

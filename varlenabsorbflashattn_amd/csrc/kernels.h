@@ -204,12 +204,18 @@ struct DecodeArgs {
 };
 
 // Attention of several new tokens per sequence over a paged cache.
+// The tile that a chunk's end cuts for the first time: its first token of the packed rows and how
+// many it has (0: none is cut), the chunk that holds its last part, the slot of its first.
+struct ChunkCut {
+  int first, tokens, last, slot;
+};
 struct ChunkArgs {
   const void *q, *kc, *vc;
   void *out;
   const int32_t *cu, *lens;
   const float *slopes;       // or null
   float *part_o, *part_lse;  // parts of cut tiles: [slots, sets, rows of a tile, D] and [..]
+  ChunkCut *cuts;            // [chunks, sets]
   PageMap map;
   int64_t q_token, q_head;
   int64_t kc_head, vc_head;

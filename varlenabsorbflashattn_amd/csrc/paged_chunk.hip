@@ -94,13 +94,16 @@ __device__ __forceinline__ void find_seq(const ChunkArgs &a, int64_t at, int64_t
   *b = a.n_seq;
   *base = uniform_l(before);
 }
-// (By doubles, whose 53 bits hold every axis: the quotient, rounded, is off by one at most.  A
-// division of 64-bit integers becomes a branch of the lanes, at whose end the compiler has put
+// n / d by doubles, whose 53 bits hold every axis: the quotient, rounded, is off by one at most.
+// (A division of 64-bit integers becomes a branch of the lanes, at whose end the compiler has put
 // copies of registers where only the branch's lanes were on.)
+__device__ __forceinline__ int64_t quotient(int64_t n, int64_t d) {
+  int64_t q = (int64_t)((double)n / (double)d);
+  q -= q * d > n;
+  return q + ((q + 1) * d <= n);
+}
 __device__ __forceinline__ int64_t units_per(const ChunkArgs &a, int64_t total) {
-  int64_t per = (int64_t)((double)total / (double)a.chunks);
-  per -= per * a.chunks >= total;
-  per += per * a.chunks < total;
+  const int64_t per = quotient(total + a.chunks - 1, a.chunks);
   return per < kChunkLeast ? kChunkLeast : per;
 }
 
@@ -202,6 +205,8 @@ __device__ __forceinline__ void chunk_walk(const ChunkArgs &a) {
   const int h0 = set << lg, hk = set / hs.per_key();
 
   if (chunk >= a.chunks) return;
+  ChunkCut *cut = a.cuts + (int64_t)chunk * sets + set;  // at this chunk's end
+  if (!a.direct && tid == 0) *cut = ChunkCut{0, 0, 0, 0};
   const int64_t mine = seq_units(a, lane);
   // (tiles dealt in turn go on until there is no sequence for one)
   const int64_t total = a.direct ? INT64_MAX : all_units(a, mine, lane);
@@ -472,6 +477,9 @@ __device__ __forceinline__ void chunk_walk(const ChunkArgs &a) {
         RS::rows32_at(acc, inv, stage, a.part_o + row * D, [&](int r) { return (int64_t)r * D; },
                       rows);
         if (row_ok && lhalf == 0) a.part_lse[row + lrow] = lse;
+        if (tid == 0 && u0 == 0)  // the tile's first part
+          *cut = ChunkCut{q0, qn, (int)quotient(t0 + units - 1, per),
+                          (int)chunk_slot(chunk, t0, per)};
       }
     }
     __syncthreads();  // the staged rows are read: the next piece may write K and V
@@ -508,62 +516,56 @@ constexpr int chunk_lds() {
   return ChunkSmem<D, NW, kCodes>::kBytes;
 }
 
-// Joins the parts of a tile that chunks cut: a group of workgroups for each border between
-// two chunks and each set, of which the tile's first border does the work, 4096 outputs a
-// workgroup, 16 neighbouring features a thread: m = max lse_g, w_g = 2^(lse_g - m),
-// O = sum w_g O_g / sum w_g.
+// Joins the parts of a tile that chunks cut: a group of workgroups for each chunk's end and each
+// set, of which the tile's first has the work, 4096 outputs a workgroup, 16 neighbouring features
+// a thread: m = max lse_g, w_g = 2^(lse_g - m), O = sum w_g O_g / sum w_g.  The first two parts,
+// which are all of most tiles, are asked for at once.
 template <typename T, int D, int BM>
 __global__ __launch_bounds__(256) void paged_chunk_join_kernel(ChunkArgs a) {
   constexpr int kRowsOf = 4096 / D, kParts = BM / kRowsOf;
-  const int tid = threadIdx.x, lane = tid & 63;
-  const HeadSets hs{a.H, a.Hk, a.lg};
-  const int sets = hs.sets();
+  const int tid = threadIdx.x, sets = a.H >> a.lg;
   const int part = blockIdx.x % kParts, set = blockIdx.x / kParts % sets;
-  const int64_t c = blockIdx.x / kParts / sets + 1;
-  const int64_t mine = seq_units(a, lane);
-  const int64_t total = all_units(a, mine, lane), per = units_per(a, total), u = c * per;
-  if (u >= total) return;
-  int b;
-  int64_t base;
-  find_seq(a, u, mine, lane, &b, &base);
-  if (b >= a.n_seq) return;
-  const SeqAt at = seq_at(a, b);
-  const ChunkSeq &s = at.s;
-  const int64_t i = chunk_tile_of(s, u - base), t0 = base + chunk_before(s, i) + kChunkBegin;
-  if (t0 >= u || t0 < u - per) return;  // no border among a tile's units, or not its first
-  const int g0 = (int)c - 1, g1 = (int)((t0 + chunk_units(s, i) - 1) / per);
-  const int row = part * kRowsOf + tid / (D / 16), f = tid % (D / 16) * 16;
-  const int64_t tok = (i << s.lt) + (row >> a.lg);
-  if (tok >= s.nq) return;
-  auto row_of = [&](int g) { return (chunk_slot(g, t0, per) * sets + set) * BM + row; };
-  float m = kNegInf;
-  for (int g = g0; g <= g1; ++g) m = fmaxf(m, a.part_lse[row_of(g)]);
-  const float ms = m == kNegInf ? 0.f : m;  // no part sees a key: zeros
-  float l = 0.f;
-  f32x4 x[4];
-#pragma unroll
-  for (int e = 0; e < 4; ++e) x[e] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll 2
-  for (int g = g0; g <= g1; ++g) {
-    const int64_t r = row_of(g);
-    const float w = fast_exp2(a.part_lse[r] - ms);
-    l += w;
+  const int chunk = blockIdx.x / kParts / sets;
+  const ChunkCut cut = a.cuts[(int64_t)chunk * sets + set];
+  const int row = part * kRowsOf + tid / (D / 16), f = tid % (D / 16) * 16, tok = row >> a.lg;
+  if (tok >= cut.tokens) return;
+  auto row_of = [&](int64_t slot) { return (slot * sets + set) * BM + row; };
+  auto part_of = [&](int64_t r, f32x4 *x) {
     const f32x4 *src = reinterpret_cast<const f32x4 *>(a.part_o + r * D + f);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const f32x4 y = src[e];
+    for (int e = 0; e < 4; ++e) x[e] = src[e];
+    return a.part_lse[r];
+  };
+  f32x4 x[4], y[4];
+  const float m0 = part_of(row_of(cut.slot), x), m1 = part_of(row_of(2 * (int64_t)chunk + 2), y);
+  float m = fmaxf(m0, m1), l = 0.f;
+  auto add = [&](float had, float w) {
+    l = l * had + w;
 #pragma unroll
-      for (int t = 0; t < 4; ++t) x[e][t] += w * y[t];
-    }
+    for (int e = 0; e < 4; ++e)
+#pragma unroll
+      for (int t = 0; t < 4; ++t) x[e][t] = x[e][t] * had + y[e][t] * w;
+  };
+  {
+    const float ms = m == kNegInf ? 0.f : m;  // (a part that sees no key is zeros)
+    const float w0 = fast_exp2(m0 - ms);
+    add(w0, fast_exp2(m1 - ms));
+    l += w0;
+  }
+  for (int g = chunk + 2; g <= cut.last; ++g) {
+    const float mg = part_of(row_of(2 * (int64_t)g), y), top = fmaxf(m, mg);
+    add(m == kNegInf ? 0.f : fast_exp2(m - top), mg == kNegInf ? 0.f : fast_exp2(mg - top));
+    m = top;
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  T *dst = (T *)a.out + ((at.q0 + tok) * a.H + (set << a.lg) + (row & ((1 << a.lg) - 1))) * D + f;
+  const int head = (set << a.lg) + (row & ((1 << a.lg) - 1));
+  T *dst = (T *)a.out + (((int64_t)cut.first + tok) * a.H + head) * D + f;
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
-    typename Mfma<T>::v8 y;
+    typename Mfma<T>::v8 z;
 #pragma unroll
-    for (int t = 0; t < 8; ++t) y[t] = static_cast<T>(x[2 * e + t / 4][t % 4] * inv);
-    *reinterpret_cast<typename Mfma<T>::v8 *>(dst + 8 * e) = y;
+    for (int t = 0; t < 8; ++t) z[t] = static_cast<T>(x[2 * e + t / 4][t % 4] * inv);
+    *reinterpret_cast<typename Mfma<T>::v8 *>(dst + 8 * e) = z;
   }
 }
 
