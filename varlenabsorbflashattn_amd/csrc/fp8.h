@@ -3,7 +3,8 @@
 // The power 2^e of a row is the least whose 448 (the largest code) reaches max |x|; being a
 // power of two it costs no precision (codes of values down to 2^-15 of the largest keep the
 // four bits that e4m3 has), and codes times it are exact in bf16, and in fp16 down to the
-// step of its smallest numbers.
+// step of its smallest numbers.  A conversion makes two features of T of two codes and the
+// power in one instruction: half of one a feature, for half of the bytes.
 #pragma once
 #include "mfma.h"
 

@@ -11,11 +11,11 @@
 //
 // Few new tokens behind long prefixes are bound by the rows of the cache: 32 sequences of 1 to 8
 // tokens behind 1k to 32k keys of 8 heads of 128, 1.27 GB, 225 us: 5.6 TB/s, all of it read (a
-// large copy, half written, reaches 5.0).  Many are bound by the products and, between them, by the softmax's vector
-// instructions: chunks of 8 prompts, 627 GFLOP, 710 us, 0.88 PFLOP/s, where the packed kernel on
-// gathered keys takes 652 for the same; 18 of them are the join.  256 rows against 128: the
-// chunks 724 us to 962, 24 turns of 1 to 512 tokens over codes 90 to 109, the drafts 214 to 215
-// (each unit is then fetched and, of codes, converted for half as many rows).
+// large copy, half written, reaches 5.0).  Many are bound by matrix and vector units in turn
+// (51% and 40% of the cycles, two waves a SIMD): chunks of 8 prompts, 627 GFLOP, 710 us, 0.88
+// PFLOP/s, where the packed kernel on gathered keys takes 652; 14 of them are the join.  256
+// rows against 128: the chunks 724 us to 962, 24 turns of 1 to 512 tokens over codes 90 to 109,
+// the drafts 214 to 215 (a unit is then fetched and, of codes, converted for half the rows).
 #include <algorithm>
 #include <type_traits>
 
@@ -519,7 +519,9 @@ constexpr int chunk_lds() {
 // Joins the parts of a tile that chunks cut: a group of workgroups for each chunk's end and each
 // set, of which the tile's first has the work, 4096 outputs a workgroup, 16 neighbouring features
 // a thread: m = max lse_g, w_g = 2^(lse_g - m), O = sum w_g O_g / sum w_g.  The first two parts,
-// which are all of most tiles, are asked for at once.
+// which are all of most tiles, are asked for at once.  Bound by the parts' bytes where tiles are
+// full (chunks of 8 prompts: 14 us; finding the tiles again here instead of reading where they
+// are cut: 21), else by latency (drafts 7, and 9.5).
 template <typename T, int D, int BM>
 __global__ __launch_bounds__(256) void paged_chunk_join_kernel(ChunkArgs a) {
   constexpr int kRowsOf = 4096 / D, kParts = BM / kRowsOf;
