@@ -58,10 +58,11 @@ struct SeqAt {
 };
 __device__ __forceinline__ SeqAt seq_at(const ChunkArgs &a, int b) {
   const int T = (int)a.T;
-  int q0 = a.cu[b], q1 = a.cu[b + 1];
+  int q0 = a.cu[b], q1 = a.cu[b + 1], len = a.lens[b];
+  asm volatile("" : "+v"(q0), "+v"(q1), "+v"(len));  // (asked for together, used or not)
   q0 = q0 < 0 ? 0 : (q0 > T ? T : q0);
   q1 = q1 < q0 ? q0 : (q1 > T ? T : q1);
-  return SeqAt{q0, chunk_seq(q1 - q0, clip_len(a.lens[b], a.capacity), a.lt, a.window)};
+  return SeqAt{q0, chunk_seq(q1 - q0, clip_len(len, a.capacity), a.lt, a.window)};
 }
 // Units of a sequence (tiles where they are not divided).
 __device__ __forceinline__ int64_t seq_units(const ChunkArgs &a, int b) {
@@ -209,8 +210,12 @@ __device__ __forceinline__ void chunk_walk(const ChunkArgs &a) {
   if (!a.direct && tid == 0) *cut = ChunkCut{0, 0, 0, 0};
   const int64_t mine = seq_units(a, lane);
   // (tiles dealt in turn go on until there is no sequence for one)
-  const int64_t total = a.direct ? INT64_MAX : all_units(a, mine, lane);
-  const int64_t per = a.direct ? 1 : units_per(a, total);
+  int64_t total = INT64_MAX, per = 1;
+  if (!a.direct) {
+    asm volatile("");  // (a branch: not computed aside)
+    total = all_units(a, mine, lane);
+    per = uniform_l(units_per(a, total));
+  }
   int64_t cur = chunk * per;
   const int64_t end = a.direct || total - cur < per ? total : cur + per;
   if (cur >= end) return;
@@ -446,18 +451,27 @@ __device__ __forceinline__ void chunk_walk(const ChunkArgs &a) {
         to[(16 * ND + 1) * 64] = l_part;
       }
       __syncthreads();
-      if (wave_active && grp == 0)
+      if (wave_active && grp == 0) {
+        auto part_of = [&](int g) { return x + ((g << lr) + rw) * kRegs * 64; };
+        float m_new = m_run;
+        for (int g = 1; g < run; ++g) m_new = fmaxf(m_new, part_of(g)[16 * ND * 64]);
+        const float f = fast_exp2(m_run - m_new);
+        m_run = m_new;
+        l_part *= f;
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) acc[d][r] *= f;
         for (int g = 1; g < run; ++g) {
-          const float *from = x + ((g << lr) + rw) * kRegs * 64;
-          const float m = from[16 * ND * 64], m_new = fmaxf(m_run, m);
-          const float f = fast_exp2(m_run - m_new), of = fast_exp2(m - m_new);
-          m_run = m_new;
-          l_part = l_part * f + from[(16 * ND + 1) * 64] * of;
+          const float *from = part_of(g);
+          const float w = fast_exp2(from[16 * ND * 64] - m_new);
+          l_part += from[(16 * ND + 1) * 64] * w;
 #pragma unroll
           for (int d = 0; d < ND; ++d)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) acc[d][r] = acc[d][r] * f + from[(d * 16 + r) * 64] * of;
+            for (int r = 0; r < 16; ++r) acc[d][r] += from[(d * 16 + r) * 64] * w;
         }
+      }
       __syncthreads();
     }
     if (wave_active && grp == 0) {
