@@ -266,7 +266,7 @@ __device__ __forceinline__ void chunk_walk(const ChunkArgs &a) {
 
     // A short piece of a tile of few rows: its units lie in the buffers at once, and each is
     // another group of waves' (4 sequences of 2 to 8 tokens behind 17 to 500 keys, 16 heads of
-    // 64: 11.8 -> 10.5 us; more features have no room for as many units)
+    // 64: 11.8 -> 10.3 us; more features have no room for as many units)
     constexpr bool kShorts = D == 64 && !kCodes;
     int lr = 0;  // log2 of a group's waves
     if (kShorts)
