@@ -327,3 +327,12 @@ def test_row_strides_of_the_c_abi():
     for at in (3, 4, 6, 7, 11, 12):
         assert L.vafa_paged_store(*[far if i == at else y for i, y in enumerate(store)]) == \
             _lib.VAFA_ERR_VALUE, at
+
+
+def test_gather_names_its_argument():
+    """cu_seqlens stands in for lengths inside: errors name it all the same."""
+    kc, table = torch.zeros(4, 16, 2, 64, dtype=torch.bfloat16), torch.zeros(2, 2, dtype=torch.int32)
+    with pytest.raises(AssertionError, match="cu_seqlens must be int32"):
+        paged_kv_gather(kc, kc, table, torch.tensor([0, 1, 2]), 2)
+    with pytest.raises(ValueError, match="cu_seqlens must be contiguous"):
+        paged_kv_gather(kc, kc, table, torch.zeros(6, dtype=torch.int32)[::2], 2)

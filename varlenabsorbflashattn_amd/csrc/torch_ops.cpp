@@ -524,11 +524,11 @@ std::tuple<Tensor, Tensor> paged_gather(const Tensor &kc, const Tensor &vc, cons
        "page_table must be [n_seq, pages] and cu_seqlens [n_seq + 1]");
   if (total < 0) throw py::value_error(std::string(what) + ": total must not be negative");
   need(!ks || dtype, what, "caches of codes need the dtype of the result");
+  const int32_t *cu_ptr = ints_of(what, "cu_seqlens", cu, table.size(0) + 1, kc);
   // (cache_lens has no part in it: the n_seq first entries of cu_seqlens stand in)
   const Cache cache = cache_of(what, kc, vc, table, cu.slice(0, 0, table.size(0)), ks, vs,
                                dtype.value_or(kc.scalar_type()));
   need(!dtype || *dtype == cache.rows, what, "a 16-bit cache comes back in its dtype");
-  const int32_t *cu_ptr = ints_of(what, "cu_seqlens", cu, table.size(0) + 1, kc);
   const int32_t *from = starts ? ints_of(what, "starts", *starts, table.size(0), kc) : nullptr;
   on_gpu(what, kc);
   Call call(kc);
