@@ -623,3 +623,65 @@ def test_codes_streams(device):
     torch.cuda.synchronize()
     for o in outs:
         assert torch.equal(o[0], want[0]) and torch.equal(o[1], want[1])
+
+
+# Rows of bf16 whose squares leave fp32 on either side: eps and the rows' sizes.
+EXTREME = [
+    (1e-6, [1.0, 1e19, 2e20, 1e30, 2.0 ** 126]),
+    (0.0, [1.0, 1e20, 1e-19, 1e-25, 2.0 ** -120, 2.0 ** -131]),
+    (2.0 ** -100, [1e-15, 3e-16, 1e-20, 1e-10, 1e-30, 1e25]),
+]
+
+
+@pytest.mark.parametrize("D,inter", [(64, False), (128, True), (256, False)])
+@pytest.mark.parametrize("eps,sizes", EXTREME)
+def test_rows_of_extreme_sizes(device, D, inter, eps, sizes):
+    """Sums of squares that pass 2^127 or fall below 2^-149 in fp32 are formed of rows scaled by a
+    power of two, which rounds nothing (features of a row are within 2^24 of each other here): the
+    bounds are those of ordinary rows.  dy is scaled so that dx stays a normal number."""
+    print(f"[rows extreme] D {D} eps {eps} {sizes}", flush=True)
+    g = torch.Generator(device=device).manual_seed(D)
+    H, Hk, n = 3, 2, 40
+    size = torch.tensor(sizes, device=device, dtype=torch.float64).repeat(n)
+    T = len(size)
+
+    def rows(h, s):
+        x = torch.randn(T, h, D, generator=g, device=device).clamp(-1.9, 1.9)
+        return (x.double() * s[:, None, None]).to(torch.bfloat16)
+    q, k = rows(H, size), rows(Hk, size)
+    assert q.isfinite().all() and k.isfinite().all()
+    dy = [rows(h, size.clamp(2.0 ** -20, 2.0 ** 20)) for h in (H, Hk)]
+    w = 1 + 0.3 * torch.randn(2, D, generator=g, device=device)
+    pos = torch.arange(T, dtype=torch.int32, device=device)
+    inv = freqs(D).to(device)
+    kw = {"inv_freq": inv, "interleaved": inter, "eps": eps}
+    leaves = [t.detach().requires_grad_(True) for t in (q, k, w[0], w[1])]
+    out = packed_qk_norm_rope(leaves[0], leaves[1], pos, q_weight=leaves[2], k_weight=leaves[3],
+                              **kw)
+    grads = torch.autograd.grad(out, leaves, dy)
+    u, args = U[q.dtype], (pos.cpu().numpy(), f64(inv), inter)
+    for i, x in enumerate((q, k)):
+        ref, mag = hr.forward(f64(x), *args, f64(w[i]), eps)
+        within("qk"[i], out[i], ref, FWD * mag + u * np.abs(ref))
+        dx, dmag, dw, wmag = hr.backward(f64(x), f64(dy[i]), *args, f64(w[i]), eps)
+        within("d" + "qk"[i], grads[i], dx, BWD * dmag + u * np.abs(dx))
+        within("dw", grads[2 + i], dw, DW * wmag + 2.0 ** -24 * np.abs(dw))
+    # the same on the way into caches of both kinds
+    table = torch.zeros(1, 1, dtype=torch.int32, device=device)
+    zero, cu = table[0, :1].clone(), torch.tensor([0, T], dtype=torch.int32, device=device)
+    append = {"cu_seqlens": cu, "q": q, "q_weight": w[0], "k_weight": w[1], **kw}
+    kc, vc = torch.zeros(2, 1, T, Hk, D, device=device, dtype=q.dtype)
+    assert torch.equal(paged_kv_append(k, k, kc, vc, table, zero, **append), out[0])
+    assert torch.equal(kc[0], out[1]) and torch.equal(vc[0], k)
+    kc, vc = (torch.zeros(1, T, Hk, D, device=device).to(E4M3) for _ in "kv")
+    ks, vs = (torch.zeros(1, T, Hk, dtype=torch.uint8, device=device).view(E8M0) for _ in "kv")
+    got = paged_kv_append(k, k, kc, vc, table, zero, k_scale=ks, v_scale=vs, **append)
+    assert torch.equal(got, out[0])
+    y, off = ref, (FWD * mag).max(-1)
+    e = ks.view(torch.uint8).cpu().numpy()[0].astype(np.int64) - 127
+    amax = np.abs(y).max(-1)
+    assert (hr.exponent(np.maximum(amax - off, 0.0), "bf16") <= e).all()
+    assert (e <= hr.exponent(amax + off, "bf16")).all()
+    val = values(kc, ks)[0]
+    assert (val >= hr.to_code(y - FWD * mag, e[..., None], "bf16")).all()
+    assert (val <= hr.to_code(y + FWD * mag, e[..., None], "bf16")).all()

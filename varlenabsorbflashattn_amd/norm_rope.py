@@ -32,8 +32,9 @@ def packed_qk_norm_rope(
     len(inv_freq), turn by ``positions[t] * inv_freq[i]`` (``positions`` int32 ``[T]``), or the
     pairs ``(2i, 2i + 1)`` if ``interleaved``, and are multiplied by ``rot_scale`` (which
     rotations scaled for long contexts carry beside their own frequencies); further features
-    stay.  bf16 or fp16, D 64, 128 or 256; all in 32 bits, rounded once.  ``q`` and ``k`` may
-    be parts of one projection's output.
+    stay.  bf16 or fp16, D 64, 128 or 256; all in 32 bits, rounded once, whatever the size of a
+    finite row (with ``eps`` 0 a row of zeros gives NaN).  ``q`` and ``k`` may be parts of one
+    projection's output.
 
     Gradients for q, k and the weights; the backward is deterministic, a second derivative
     raises.  At most 2^30 tokens and 4096 heads, strides below 2^32 elements.  Forward and
