@@ -685,3 +685,54 @@ def test_rows_of_extreme_sizes(device, D, inter, eps, sizes):
     val = values(kc, ks)[0]
     assert (val >= hr.to_code(y - FWD * mag, e[..., None], "bf16")).all()
     assert (val <= hr.to_code(y + FWD * mag, e[..., None], "bf16")).all()
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rot,inter", [(0, False), (64, False), (64, True), (32, False)])
+def test_rows_with_infinities_and_nan(device, dt, rot, inter):
+    """What an infinity or NaN does to its row: normed, the mean is infinite, so features are 0,
+    and NaN where the infinity stands (inf / inf) and at the other of its pair; a NaN takes the
+    whole row.  Rows without a weight are not normed: pairs that hold neither stay."""
+    print(f"[rows inf] {dt} rot {rot} {inter}", flush=True)
+    D, H, n = 64, 2, rot // 2
+    g = torch.Generator(device=device).manual_seed(rot)
+    x = torch.randn(7, H, D, generator=g, device=device).to(dt)
+    k = torch.randn(7, 1, D, generator=g, device=device).to(dt)
+    w = 1 + 0.1 * torch.rand(D, generator=g, device=device)
+    pos = 3 + torch.arange(7, dtype=torch.int32, device=device)
+    kw = {"inv_freq": dev(freqs(rot), device), "interleaved": inter}
+    plain = packed_qk_norm_rope(x, k, pos, **kw)[0]
+    normed = packed_qk_norm_rope(x, k, pos, q_weight=w, k_weight=w, **kw)
+    bad = x.clone()
+    places = [(1, 0, 5), (2, 1, 40), (4, 0, 63)]
+    for (t, h, i), value in zip(places, (float("inf"), -float("inf"), float("inf"))):
+        bad[t, h, i] = value
+    bad[5, 1, 9] = float("nan")
+
+    def pair(i):
+        if i >= rot:
+            return {i}
+        return {i, i ^ 1} if inter else {i, (i + n) % rot}
+    leaf, weight = bad.detach().requires_grad_(True), w.detach().requires_grad_(True)
+    out, kout = packed_qk_norm_rope(leaf, k, pos, q_weight=weight, k_weight=w, **kw)
+    dx, dw = torch.autograd.grad(out, (leaf, weight), torch.ones_like(out))
+    bare = packed_qk_norm_rope(bad, k, pos, **kw)[0]
+    assert torch.equal(kout, normed[1])
+    good = torch.ones(7, H, dtype=torch.bool, device=device)
+    for t, h, i in places:
+        good[t, h] = False
+        at = torch.zeros(D, dtype=torch.bool, device=device)
+        at[list(pair(i))] = True
+        assert out[t, h][at].isnan().all() and not out[t, h][~at].any()
+        assert torch.equal(bare[t, h][~at], plain[t, h][~at])
+        assert not bare[t, h][at].isfinite().any()
+        assert i < rot or bare[t, h, i] == bad[t, h, i]
+        assert dx[t, h].isnan().all() and dw[i].isnan()
+    good[5, 1] = False
+    assert out[5, 1].isnan().all() and dx[5, 1].isnan().all() and dw.isnan().all()
+    assert torch.equal(out[good], normed[0][good]) and dx[good].isfinite().all()
+    # zeros: eps alone keeps a normed row finite
+    zero = torch.zeros_like(x)
+    for eps, nan in ((1e-45, False), (1e-30, False), (0.0, True)):
+        got = packed_qk_norm_rope(zero, k, pos, q_weight=w, k_weight=w, eps=eps, **kw)[0]
+        assert got.isnan().all() if nan else not got.any()

@@ -39,8 +39,10 @@ def packed_qk_norm_rope(
     Gradients for q, k and the weights; the backward is deterministic, a second derivative
     raises.  At most 2^30 tokens and 4096 heads, strides below 2^32 elements.  Forward and
     backward can be captured into a graph together; no eager graph of the same leaves may be
-    alive then.  A row that holds an infinity or NaN gives
-    NaN to itself and to the weights' gradients, and to no other row.
+    alive then.  An infinity in a normed row gives NaN where it stands and at the other
+    of its pair, and zeros else; a NaN gives NaN to the whole row.  Either gives NaN to the row's
+    gradient and to the weights' gradients (an infinity at its feature alone), and neither
+    touches another row.  Rows without a weight keep both where they stand.
     """
     yq, yk = _lib.ops().qk_norm_rope(q, k, positions, inv_freq, bool(interleaved), q_weight,
                                      k_weight, eps, rot_scale)
