@@ -336,3 +336,17 @@ def test_gather_names_its_argument():
         paged_kv_gather(kc, kc, table, torch.tensor([0, 1, 2]), 2)
     with pytest.raises(ValueError, match="cu_seqlens must be contiguous"):
         paged_kv_gather(kc, kc, table, torch.zeros(6, dtype=torch.int32)[::2], 2)
+
+
+def test_refused_types_name_whose_they_differ_from():
+    """A cache of codes is float8: rows that go into it have to be of k's dtype, not the cache's."""
+    for name in ("q", "v"):
+        a = _cache()
+        a[name] = a[name].to(torch.float16)
+        with pytest.raises(AssertionError, match=f"{name} must have k's dtype and device"):
+            _append(a)
+        for x in ("k_cache", "v_cache"):
+            a[x] = torch.zeros(5, 16, 2, 64, dtype=torch.bfloat16)
+        a["k_scale"] = a["v_scale"] = None
+        with pytest.raises(AssertionError, match=f"{name} must have the cache's dtype and device"):
+            _append(a)

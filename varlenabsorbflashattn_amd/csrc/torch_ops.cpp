@@ -402,9 +402,12 @@ void check_tokens(const char *what, const char *name, const Tensor &t, const Ten
   if (t.dim() != 3 || t.size(2) != kc.size(3))
     throw AssertionFailed(std::string(what) + ": " + name + " must be [T, heads, " +
                           std::to_string(kc.size(3)) + "]");
+  // (a cache of codes has a dtype of its own, and the rows that go into it k's)
+  const char *whose =
+      t.scalar_type() != rows && kc.scalar_type() == at::kFloat8_e4m3fn ? "k's" : "the cache's";
   if (t.scalar_type() != rows || t.device() != kc.device())
-    throw AssertionFailed(std::string(what) + ": " + name +
-                          " must have the cache's dtype and device");
+    throw AssertionFailed(std::string(what) + ": " + name + " must have " + whose +
+                          " dtype and device");
 }
 
 // An int32 tensor [n] on the device, its elements beside each other.
