@@ -2,6 +2,7 @@
 64-bit oracle.  Bounds as in test_gpu_paged.py (probabilities are rounded for the product,
 sums take the rounded values), for codes as in test_gpu_paged_codes.py.
 """
+import ctypes as C
 import math
 import threading
 
@@ -13,8 +14,9 @@ from oracle import paged as op
 from test_gpu_head_rows import E4M3, E8M0, code_caches, freqs, values
 from test_gpu_paged import U, cache_pair, f64, pages_for
 from test_gpu_paged_codes import close_decode
-from varlenabsorbflashattn_amd import (packed_masked_attn, packed_qk_norm_rope, paged_chunk_attn,
-                                       paged_decode_attn, paged_kv_append, paged_kv_gather)
+from varlenabsorbflashattn_amd import (_lib, packed_masked_attn, packed_qk_norm_rope,
+                                       paged_chunk_attn, paged_decode_attn, paged_kv_append,
+                                       paged_kv_gather)
 
 pytestmark = pytest.mark.gpu
 
@@ -436,3 +438,89 @@ def test_threads_with_streams(device):
     for t in threads:
         t.join()
     assert not errors, errors
+
+
+@pytest.mark.parametrize("H,Hk,D,lens,window,cap", [
+    (8, 2, 64, [9000, 3000], None, None), (8, 1, 64, [7000, 5000], 3000, 30.0),
+    (16, 4, 128, [9000, 4000], None, None), (10, 2, 128, [6000, 5000], None, None),
+    (4, 2, 256, [5000, 3000], None, None), (6, 2, 256, [5000, 3000], 2000, 30.0)])
+@pytest.mark.parametrize("new", [[70, 33], [4, 1]])
+def test_chunk_over_codes_cut_anywhere(device, H, Hk, D, lens, window, cap, new):
+    """Ordinary rows stored in 8 bits, which many keys share the softmax of: a unit that a cut
+    tile lost would show in the sequence's 2-norm (bound as in test_chunk_tiles_cut_anywhere)."""
+    print(f"[chunk codes cut] {H}/{Hk} of {D}, {new} behind {lens}", flush=True)
+    dt, page = torch.bfloat16, 64
+    g = torch.Generator(device=device).manual_seed(H + D + sum(new))
+    table, N = pages_for(g, lens, page)
+    kc, vc = (torch.zeros(N, page, Hk, D, device=device).to(E4M3) for _ in "kv")
+    ks, vs = (torch.zeros(N, page, Hk, dtype=torch.uint8, device=device).view(E8M0) for _ in "kv")
+    kv = torch.randn(sum(lens), 2 * Hk, D, generator=g, device=device).to(dt)
+    dev_table = table.to(device)
+    cl = torch.tensor(lens, dtype=torch.int32, device=device)
+    paged_kv_append(kv[:, :Hk], kv[:, Hk:], kc, vc, dev_table, 0 * cl, k_scale=ks, v_scale=vs,
+                    cu_seqlens=torch.tensor(np.cumsum([0] + lens), dtype=torch.int32,
+                                            device=device))
+    q = torch.randn(sum(new), H, D, generator=g, device=device).to(dt)
+    cu = np.cumsum([0] + new)
+    out = paged_chunk_attn(q, kc, vc, dev_table, cl,
+                           torch.tensor(cu, dtype=torch.int32, device=device), window=window,
+                           softcap=cap, k_scale=ks, v_scale=vs)
+    ref = op.chunk(f64(q), values(kc, ks), values(vc, vs), table.numpy(), lens, cu,
+                   1 / math.sqrt(D), cap, window)
+    close_decode(out, *ref)
+    got, u = f64(out), U[dt]
+    for b in range(len(lens)):
+        r = ref[0][cu[b]:cu[b + 1]]
+        off = np.linalg.norm(got[cu[b]:cu[b + 1]] - r) / np.linalg.norm(r) / u
+        print(f"  sequence {b}: {off:.2f} u", flush=True)
+        assert off < 1.0, b
+
+
+@pytest.mark.parametrize("width", [8, 100])  # whole tiles, and tiles that are cut
+@pytest.mark.parametrize("codes", [False, True])
+def test_chunk_bad_cu_writes_only_its_rows(device, width, codes):
+    """cu_seqlens that decrease or leave the rows: nothing in front of or behind the result and
+    the workspace changes, and where the end alone is behind the rows, the sequences in front of
+    it have their values."""
+    H, Hk, D, page, T, G = 4, 2, 64, 16, 30, 4096
+    print(f"[chunk guards] table of {width}, codes {codes}", flush=True)
+    g = torch.Generator(device=device).manual_seed(width)
+    L = _lib.lib()
+    if codes:
+        kc, vc, ks, vs = code_caches(g, width, page, Hk, D, device, "plain")
+        ref_kv = values(kc, ks), values(vc, vs)
+        sc = _lib.RowScales(k=ks.data_ptr(), v=vs.data_ptr(), k_page=page * Hk, k_token=Hk,
+                            k_head=1, v_page=page * Hk, v_token=Hk, v_head=1)
+    else:
+        kc, vc = cache_pair(g, width, page, Hk, D, torch.bfloat16, device, "plain")
+        ref_kv, sc = (f64(kc), f64(vc)), None
+    q = (torch.randn(T, H, D, generator=g, device=device) / 32).to(torch.bfloat16)
+    table = torch.arange(width, dtype=torch.int32, device=device).repeat(2, 1)
+    lens = torch.tensor([16 * width - 9, 100], dtype=torch.int32, device=device)
+    c = _lib.PagedCache(k=kc.data_ptr(), v=vc.data_ptr(), n_pages=width, page_size=page, Hk=Hk,
+                        D=D, k_page=page * Hk * D, k_token=Hk * D, k_head=D,
+                        v_page=page * Hk * D, v_token=Hk * D, v_head=D,
+                        page_table=table.data_ptr(), table_stride=width, table_width=width,
+                        cache_lens=lens.data_ptr(), n_seq=2)
+    need = L.vafa_paged_chunk_workspace(C.byref(c), T, H, 0)
+    assert (need > 0) == (width > 8)
+    far = 2 ** 31 - 1
+    for cu in ([3, 20, far], [0, 12, 5], [0, 30, -far], [-7, 10, 10], [25, 5, 30], [far, -far, 3],
+               [0, 50, 20], [-9, -3, -20]):
+        cu_dev = torch.tensor(cu, dtype=torch.int32, device=device)
+        out = torch.full((2 * G + T * H * D,), 7.0, device=device, dtype=torch.bfloat16)
+        ws = torch.full((2 * G + need,), 0xA5, device=device, dtype=torch.uint8)
+        rc = L.vafa_paged_chunk(C.byref(c), None if sc is None else C.byref(sc), q.data_ptr(),
+                                H * D, D, T, H, cu_dev.data_ptr(), out[G:].data_ptr(), 0.125, 0.0,
+                                0, None, _lib.DT_BF16, ws[G:].data_ptr() if need else None, need,
+                                torch.cuda.current_stream().cuda_stream)
+        torch.cuda.synchronize()
+        assert rc == 0, L.vafa_last_error()
+        assert (out[:G] == 7).all() and (out[-G:] == 7).all(), cu
+        assert (ws[:G] == 0xA5).all() and (ws[G + need:] == 0xA5).all(), cu
+        if cu[2] != far:
+            continue
+        a, b = cu[0], cu[1]
+        ref = op.chunk(f64(q)[a:b], *ref_kv, table.cpu().numpy()[:1], [int(lens[0])], [0, b - a],
+                       0.125)
+        close_decode(out[G:-G].view(T, H, D)[a:b], *ref)
