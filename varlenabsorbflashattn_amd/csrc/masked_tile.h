@@ -4,6 +4,9 @@
 // S^T = K Q^T and O^T += V^T P^T over 64 keys in LDS (fwd_tiles.h), with a lazily updated
 // running maximum.
 #pragma once
+#include <cstddef>
+#include <type_traits>
+
 #include "fwd_tiles.h"
 #include "masked.h"
 #include "mfma.h"
@@ -30,15 +33,16 @@ struct PaddedTile {  // rows with FwdSmem's padding
   }
 };
 
-// One tile (64 keys, or 32) for the wave's 32 query rows; masked: some (row, key) pair is hidden.  Keys
-// whose bit of `here` is not set are hidden from every row (a masked tile's alone).
-template <typename T, int D, bool kCap, bool kBias, typename Tile>
+// One tile (64 keys, or 32) for the wave's 32 query rows; masked: some (row, key) pair is hidden.
+// Keys whose bit of `here` (64 bits, where a tile may lack some) is not set are hidden from every
+// row (a masked tile's alone).
+template <typename T, int D, bool kCap, bool kBias, typename Tile, typename Here = std::nullptr_t>
 __device__ __forceinline__ void masked_tile(const Tile &tile,
                                             const typename Mfma<T>::v8 (&qf)[D / 16],
                                             f32x16 (&acc)[D / 32], float &m_run, float &l_part,
                                             const ScoreArgs &sa, float slope2, int kbase,
                                             int k_end, bool masked, int p, int pre, int window,
-                                            int lane, uint64_t here = ~uint64_t{0}) {
+                                            int lane, Here here = nullptr) {
   using M = Mfma<T>;
   constexpr int NC = D / 16, ND = D / 32, KT = Tile::kKeys / 32;
   constexpr bool kLog2 = kCap || kBias;  // s holds log2-domain scores after the transform
@@ -77,8 +81,8 @@ __device__ __forceinline__ void masked_tile(const Tile &tile,
       }
   }
   if (masked) {
-    const uint64_t seen =
-        seen_keys(k_lane, k_end, p, pre, window) & (here >> (lhalf * 4));
+    uint64_t seen = seen_keys(k_lane, k_end, p, pre, window);
+    if constexpr (!std::is_same_v<Here, std::nullptr_t>) seen &= here >> (lhalf * 4);
 #pragma unroll
     for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
