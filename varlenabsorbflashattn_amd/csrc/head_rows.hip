@@ -505,7 +505,7 @@ __global__ __launch_bounds__(256) void head_rows_dw_kernel(HeadRowsBwdArgs a) {
 // Output row t of sequence b is the token at starts[b] + t - cu[b], zeros where there is
 // none.  256 R units of 16 features, of k's heads, then v's.
 template <typename T, int R, bool kCodes>
-__global__ __launch_bounds__(256) void paged_gather_kernel(GatherArgs a, int span) {
+__global__ __launch_bounds__(256) void paged_gather_kernel(GatherArgs a) {
   extern __shared__ __align__(16) unsigned char smem[];
   int2 *tok = reinterpret_cast<int2 *>(smem);  // page and slot
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -632,9 +632,9 @@ void launch_gather_r(const GatherArgs &a, int64_t per, hipStream_t st) {
   const int span = most_tokens(256 * R, per, a.T);
   const dim3 grid((unsigned)((units + 256 * R - 1) / (256 * R)));
   if (a.scales.k != nullptr)
-    hipLaunchKernelGGL((paged_gather_kernel<T, R, true>), grid, dim3(256), span * 8, st, a, span);
+    hipLaunchKernelGGL((paged_gather_kernel<T, R, true>), grid, dim3(256), span * 8, st, a);
   else
-    hipLaunchKernelGGL((paged_gather_kernel<T, R, false>), grid, dim3(256), span * 8, st, a, span);
+    hipLaunchKernelGGL((paged_gather_kernel<T, R, false>), grid, dim3(256), span * 8, st, a);
 }
 
 template <typename T>
