@@ -472,7 +472,7 @@ VAFA_API int vafa_paged_decode_codes(const vafa_paged_cache *cache, const vafa_r
  * decreasing) are the last of the cache_lens[b] tokens of sequence b, and each sees the keys
  * up to its own (the last `window` of them; 0: all).  Else as vafa_paged_decode, over 16 bits
  * or, with scales, codes.  Rows of no sequence, and those that see no key, get zeros.  T at most
- * 2^30, H at most 4096, strides of pages and tokens below 2^35. */
+ * 2^30, H at most 4096, strides of pages and tokens below 2^35 (codes: 2^36). */
 VAFA_API int64_t vafa_paged_chunk_workspace(const vafa_paged_cache *cache, int64_t T, int64_t H,
                                             int64_t window);
 VAFA_API int vafa_paged_chunk(const vafa_paged_cache *cache, const vafa_row_scales *scales,

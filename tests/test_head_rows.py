@@ -350,3 +350,25 @@ def test_refused_types_name_whose_they_differ_from():
         a["k_scale"] = a["v_scale"] = None
         with pytest.raises(AssertionError, match=f"{name} must have the cache's dtype and device"):
             _append(a)
+
+
+def test_far_strides_of_chunks():
+    """Strides of pages and tokens reach 2^35 elements in 16 bits and 2^36 codes, which are as many
+    pieces of 16 bytes (no rows: nothing is launched)."""
+    L, x = _lib.lib(), 1 << 24
+
+    def rc(codes, **far):
+        c = _lib.PagedCache(k=1 << 20, v=1 << 21, n_pages=5, page_size=16, Hk=2, D=64, k_page=2048,
+                            k_token=128, k_head=64, v_page=2048, v_token=128, v_head=64,
+                            page_table=1 << 22, table_stride=2, table_width=2,
+                            cache_lens=1 << 23, n_seq=3)
+        for n, v in far.items():
+            setattr(c, n, v)
+        s = _lib.RowScales(k=1 << 20, v=1 << 21, k_page=32, k_token=2, k_head=1, v_page=32,
+                           v_token=2, v_head=1)
+        return L.vafa_paged_chunk(C.byref(c), C.byref(s) if codes else None, x, 256, 64, 0, 4, x, x,
+                                  0.125, 0.0, 0, None, _lib.DT_BF16, None, 0, None)
+    for name in ("k_page", "k_token", "v_page", "v_token"):
+        for codes, limit in ((False, 1 << 35), (True, 1 << 36)):
+            assert rc(codes, **{name: limit - 16}) == 0, (name, codes)
+            assert rc(codes, **{name: limit}) == _lib.VAFA_ERR_VALUE, (name, codes)

@@ -441,8 +441,10 @@ int vafa_paged_chunk(const vafa_paged_cache *c, const vafa_row_scales *scales, c
   ChunkPlan p;
   if (int rc = plan_chunk(c, T, H, window, &p)) return rc;
   if (int rc = check_codes(what, c, scales)) return rc;
+  // (codes: as far as check_codes lets them)
+  const int64_t piece = scales != nullptr ? 16 : 8;
   for (int64_t x : {c->k_page, c->k_token, c->v_page, c->v_token})
-    if (x / 8 > UINT32_MAX)
+    if (x / piece > UINT32_MAX)
       return fail(VAFA_ERR_VALUE, "%s: the cache's strides must be below 2^35, got %lld", what,
                   (long long)x);
   if (int rc = check_scores(what, scale, softcap)) return rc;
@@ -460,7 +462,6 @@ int vafa_paged_chunk(const vafa_paged_cache *c, const vafa_row_scales *scales, c
   a.part_lse = (float *)((char *)workspace + p.lse_off);
   a.cuts = (ChunkCut *)((char *)workspace + p.cut_off);
   a.map = map_of(c); a.q_token = q_token; a.q_head = q_head;
-  const int64_t piece = scales != nullptr ? 16 : 8;
   a.kc_head = c->k_head; a.vc_head = c->v_head;
   a.k_page = (uint32_t)(c->k_page / piece); a.kc_token = (uint32_t)(c->k_token / piece);
   a.v_page = (uint32_t)(c->v_page / piece); a.vc_token = (uint32_t)(c->v_token / piece);

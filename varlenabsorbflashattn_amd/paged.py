@@ -5,7 +5,8 @@ The caches are ``[n_pages, page_size, H_k, D]`` (bf16 or fp16), features contigu
 other strides any multiple of 8 elements, so views of a joint or head-major allocation
 serve too.  In 8 bits they are ``float8_e4m3fn`` (strides multiples of 16) beside
 ``k_scale`` and ``v_scale`` ``[n_pages, page_size, H_k]`` of ``float8_e8m0fnu``: a row (one
-token and key head) is its codes times its power of two.  Token ``p`` of sequence ``b`` lies
+token and key head) is its codes times its power of two (page and token strides of the codes
+below 2^36, strides of the powers below 2^32).  Token ``p`` of sequence ``b`` lies
 in page ``page_table[b, p // page_size]`` at ``p % page_size``.  ``page_table`` and the
 lengths are int32 tensors on the GPU and stay there: no call waits for the GPU, all of them
 can be captured into a graph and replayed with other lengths and pages in the same tensors.
@@ -153,7 +154,7 @@ def paged_chunk_attn(
     is what :func:`packed_masked_attn` gives on the gathered keys.  Tokens in front of the
     first key (more new tokens than the cache holds) and rows of no sequence get zeros.  At
     most 2^30 tokens and 4096 heads; strides of pages and tokens below 2^35 elements (2^36
-    codes, 2^32 powers of two).  Forward only.
+    codes).  Forward only.
     """
     if scale is None:
         scale = 1.0 / math.sqrt(q.shape[-1])
