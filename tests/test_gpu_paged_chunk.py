@@ -524,3 +524,30 @@ def test_chunk_bad_cu_writes_only_its_rows(device, width, codes):
         ref = op.chunk(f64(q)[a:b], *ref_kv, table.cpu().numpy()[:1], [int(lens[0])], [0, b - a],
                        0.125)
         close_decode(out[G:-G].view(T, H, D)[a:b], *ref)
+
+
+def test_chunk_bad_rows_stay_in_their_sequence(device):
+    """NaN in a row of q stays in that row, and in the newest key and value of a sequence in that
+    sequence: the others have the bits that they had."""
+    for new, lens in (([3, 40, 5], [900, 64, 33]), ([2, 2, 90], [30, 12, 200])):
+        for D, H, Hk in ((64, 8, 2), (128, 6, 2), (256, 4, 4)):
+            print(f"[chunk bad rows] {new} {lens} D {D}", flush=True)
+            args, kw, _ = chunk_case((new, lens, H, Hk, D, 16, None, None, False, False,
+                                      torch.bfloat16, "plain"), device)
+            q, kc, vc, table, clen, cu = args
+            want = paged_chunk_attn(*args, **kw)
+            rows = cu.tolist()
+            bad = q.clone()
+            bad[rows[1] + 1, 1] = float("nan")
+            got = paged_chunk_attn(bad, *args[1:], **kw)
+            assert got[rows[1] + 1, 1].isnan().all()
+            got[rows[1] + 1, 1] = want[rows[1] + 1, 1]
+            assert torch.equal(got, want)
+            at = op.place(table.cpu().numpy(), kc.shape[0], 16, 1, lens[1] - 1)
+            kb, vb = kc.clone(), vc.clone()
+            kb[at], vb[at] = float("nan"), float("inf")
+            got = paged_chunk_attn(q, kb, vb, *args[3:], **kw)
+            assert got[rows[2] - 1].isnan().all()
+            keep = torch.ones(len(q), dtype=torch.bool, device=device)
+            keep[rows[1]:rows[2]] = False
+            assert torch.equal(got[keep], want[keep])

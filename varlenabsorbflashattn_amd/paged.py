@@ -152,7 +152,10 @@ def paged_chunk_attn(
     the cache), and each sees the keys up to its own, with ``window`` the last that many of
     them.  Scores, heads and 8-bit caches are those of :func:`paged_decode_attn`, the result
     is what :func:`packed_masked_attn` gives on the gathered keys.  Tokens in front of the
-    first key (more new tokens than the cache holds) and rows of no sequence get zeros.  At
+    first key (more new tokens than the cache holds) and rows of no sequence get zeros.  A key
+    that some token of its sequence sees must be finite, also for the tokens that do not see
+    it: they may weigh it with 0.  Query heads that share a key head read it together by the
+    largest power of two in their number; other numbers read the cache several times.  At
     most 2^30 tokens and 4096 heads; strides of pages and tokens below 2^35 elements (2^36
     codes).  Forward only.
     """
