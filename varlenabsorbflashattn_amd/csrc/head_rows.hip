@@ -8,9 +8,11 @@
 //   dw = sum over rows of g u,   dx = r (g w - u mean(g w u)).
 // Each row is read once and written once; D / 16 lanes of a wave hold one, 16 features each, and
 // its sums are exchanges between them.  Memory is the bound where rows stay in 16 bits (35k
-// tokens of 32 + 8 heads of 128: forward 722 MB, 131 us, 5.5 TB/s; backward 1.08 GB, 233 us, 4.6
-// TB/s), the vector instructions (85% of the cycles) where they become codes: with v's 8 heads
-// 794 MB in 171 us, 4.6 TB/s; 41k of such rows back from the cache 251 MB in 49 us, 5.1 TB/s.
+// tokens of 32 + 8 heads of 128: forward 722 MB, 130 us, 5.6 TB/s; backward 1.08 GB, 241 us, 4.5
+// TB/s; with v's 8 heads into a cache 865 MB, 178 us, 4.9 TB/s; those heads back from it 288 MB,
+// 55 us, 5.3 TB/s).  Where they become codes the vector units are busy for 77% of the cycles, of
+// which there are more for a byte: 794 MB in 170 us, 4.7 TB/s; 41k of such rows back 251 MB in 50
+// us, 5.1 TB/s.
 #include <algorithm>
 #include <type_traits>
 

@@ -9,13 +9,23 @@
 // here: all units of all tiles form one axis (paged.h), cut into as many even chunks as the GPU
 // holds workgroups for each set of heads, and a second launch joins the tiles that were cut.
 //
-// Few new tokens behind long prefixes are bound by the rows of the cache: 32 sequences of 1 to 8
-// tokens behind 1k to 32k keys of 8 heads of 128, 1.27 GB, 225 us: 5.6 TB/s, all of it read (a
-// large copy, half written, reaches 5.0).  Many are bound by matrix and vector units in turn
-// (51% and 40% of the cycles, two waves a SIMD): chunks of 8 prompts, 627 GFLOP, 710 us, 0.88
-// PFLOP/s, where the packed kernel on gathered keys takes 652; 14 of them are the join.  256
-// rows against 128: the chunks 724 us to 962, 24 turns of 1 to 512 tokens over codes 90 to 109,
-// the drafts 214 to 215 (a unit is then fetched and, of codes, converted for half the rows).
+// Few new tokens behind long prefixes are bound by the rows of a cache in 16 bits: 32 sequences
+// of 1 to 8 tokens ("drafts" below) behind 1k to 32k keys of 8 heads of 128, 32 query heads, 1.27
+// GB, 228 us: 5.6 TB/s, all of it read (a large copy, half written, reaches 5.0); the same inputs
+// again and again, of which the last cache keeps a part, 213, and so the comparisons below.  Over
+// codes they take 232 for half the bytes, 2.8 TB/s: the units on their way hold half as much, and
+// each is converted before it can be used.  Many new tokens are bound by matrix and vector units
+// in turn (51% and 41% of the cycles, two waves a SIMD): chunks of 8 prompts, 627 GFLOP, 690 to
+// 730 us on different cards, 0.88 PFLOP/s, where the packed kernel on gathered keys takes 652; 14
+// of them are the join.  256 rows against 128: the chunks 724 us to 962, 24 turns of 1 to 512
+// tokens over codes 90 to 109, the drafts 214 to 215 (a unit is then fetched and, of codes,
+// converted for half the rows).
+//
+// Heads that share a key head share a tile by the largest power of two in their number, and each
+// such set walks the keys by itself: the drafts with 16 heads on 4 take 132 us, with 28 on 4, sets
+// of one head, 1160 (1500 over codes), with 40 on 8 1740.  Sets whose number is no power of two
+// lie unevenly on the XCDs, some of whose workgroups then wait for others to end: the drafts with
+// 12 heads on 6 take 275 us for 951 MB, 3.5 TB/s, with 12 on 3 151 for 476, 3.2.
 #include <algorithm>
 #include <type_traits>
 
@@ -611,9 +621,8 @@ void launch_d(const ChunkArgs &a, hipStream_t st) {
 }  // namespace
 
 // Rows in 16 bits pass the caches where a sequence has no more than a tile's tokens on average
-// and a key head one set, so that most are read once (32 sequences of 1 to 8 tokens behind 1k to
-// 32k keys 250 -> 213 us; of eight prompts' chunks 718 -> 742).  Codes do not: 234 -> 230 us of
-// the same drafts, 708 -> 738 of the chunks.
+// and a key head one set, so that most are read once (the drafts 250 -> 213 us; the chunks 718 ->
+// 742).  Codes do not: 234 -> 230 us of the drafts, 708 -> 738 of the chunks.
 template <typename T, int D>
 void launch_paged_chunk(const ChunkArgs &a, hipStream_t st) {
   if (a.scales.k != nullptr) return launch_d<T, D, true, false>(a, st);
